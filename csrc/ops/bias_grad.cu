@@ -4,6 +4,8 @@
 //   tnops_bias_grad:     db[n] = sum_m g[m, n]                   (g bf16, db fp32)
 //   tnops_gelu_bwd_bias: gp[m, n] = bf16(gy[m, n] * gelu'(pre[m, n]))
 //                        db[n]    = sum_m gp[m, n]
+//   tnops_gelu_bwd_bias_int8: the same with pre kept in 8 bits
+//                        (int8_blocks.cuh), read back as it is used.
 //
 // Column sums of an [M, N] row-major bf16 matrix, deterministic: pass 1
 // tiles the matrix into (256-column, rowsPer-row) blocks; each warp of a CTA
@@ -17,6 +19,7 @@
 #include <stdint.h>
 
 #include "common.cuh"
+#include "int8_blocks.cuh"
 #include "tnccl_ops.h"
 
 namespace tnops {
@@ -61,11 +64,17 @@ __device__ __forceinline__ float geluTanhGrad(float x) {
   return fmaf(2.0f * x * r * (e * r), du, r);
 }
 
-template <bool GELU>
+// What the GELU gradient reads pre from: nothing (no GELU), bf16, or 8-bit
+// blocks (whose exponents are `preExp`).
+enum class Pre { kNone, kBf16, kInt8 };
+
+template <Pre PRE>
 __global__ void __launch_bounds__(kWarps * 32)
-    colsumPartial(const uint16_t* __restrict__ gy, const uint16_t* __restrict__ pre,
-                  uint16_t* __restrict__ gout, float* __restrict__ partial, int M, int N,
-                  int rowsPer) {
+    colsumPartial(const uint16_t* __restrict__ gy, const void* __restrict__ pre,
+                  const uint8_t* __restrict__ preExp, uint16_t* __restrict__ gout,
+                  float* __restrict__ partial, int M, int N, int rowsPer) {
+  constexpr bool GELU = PRE != Pre::kNone;
+  const int blocks = (N + kInt8Block - 1) / kInt8Block;
   __shared__ float sAcc[kWarps][kCols];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int col0 = blockIdx.x * kCols + lane * 8;
@@ -76,14 +85,20 @@ __global__ void __launch_bounds__(kWarps * 32)
   for (int e = 0; e < 8; ++e) acc[e] = 0.f;
   if (col0 < N) {
     for (int rb = r0 + w; rb < r1; rb += kWarps * kUnroll) {
-      uint4 g[kUnroll], p[kUnroll];
+      uint4 g[kUnroll], p[kUnroll];  // 8-bit pre: eight values and the exponent
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
         const int r = rb + u * kWarps;
         if (r < r1) {
           const size_t off = (size_t)r * N + col0;
           g[u] = __ldcs(reinterpret_cast<const uint4*>(gy + off));
-          if (GELU) p[u] = __ldcs(reinterpret_cast<const uint4*>(pre + off));
+          if (PRE == Pre::kBf16)
+            p[u] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(pre) + off));
+          if (PRE == Pre::kInt8) {
+            const uint2 q =
+                __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(pre) + off));
+            p[u] = make_uint4(q.x, q.y, preExp[(size_t)r * blocks + col0 / kInt8Block], 0u);
+          }
         }
       }
 #pragma unroll
@@ -94,7 +109,14 @@ __global__ void __launch_bounds__(kWarps * 32)
         bf16x8ToF(g[u], f);
         if (GELU) {
           float x[8];
-          bf16x8ToF(p[u], x);
+          if (PRE == Pre::kInt8) {
+            const float step = int8Step(p[u].z);
+            const float4 a = int8x4(p[u].x, step), b = int8x4(p[u].y, step);
+            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+            x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+          } else {
+            bf16x8ToF(p[u], x);
+          }
           uint32_t o[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -136,21 +158,23 @@ extern "C" int tnops_colsum_parts(int M, int N) {
   return parts < 1 ? 1 : parts > maxParts ? maxParts : parts;
 }
 
-static int launchColsum(const uint16_t* gy, const uint16_t* pre, uint16_t* gout, float* db,
-                        float* partial, int M, int N, bool gelu, cudaStream_t stream) {
+static int launchColsum(Pre kind, const uint16_t* gy, const void* pre, const uint8_t* preExp,
+                        uint16_t* gout, float* db, float* partial, int M, int N,
+                        cudaStream_t stream) {
   if (M <= 0 || N <= 0 || N % 8 != 0) return 1;
-  // 16-byte pieces of every row: N % 8 == 0 keeps the rows on the boundary
-  // when the base pointers are.
-  if ((reinterpret_cast<uintptr_t>(gy) | reinterpret_cast<uintptr_t>(pre) |
-       reinterpret_cast<uintptr_t>(gout)) & 15)
+  // 16-byte pieces of every row (8-byte ones of an 8-bit pre): N % 8 == 0
+  // keeps the rows on the boundary when the base pointers are.
+  const uintptr_t preMask = kind == Pre::kInt8 ? 7 : 15;
+  if (((reinterpret_cast<uintptr_t>(gy) | reinterpret_cast<uintptr_t>(gout)) & 15) ||
+      (reinterpret_cast<uintptr_t>(pre) & preMask))
     return 1;
   const int parts = tnops_colsum_parts(M, N);
   const int rowsPer = (M + parts - 1) / parts;
   const dim3 grid((unsigned)((N + kCols - 1) / kCols), (unsigned)parts);
-  if (gelu)
-    colsumPartial<true><<<grid, kWarps * 32, 0, stream>>>(gy, pre, gout, partial, M, N, rowsPer);
-  else
-    colsumPartial<false><<<grid, kWarps * 32, 0, stream>>>(gy, pre, gout, partial, M, N, rowsPer);
+  auto kernel = kind == Pre::kNone    ? colsumPartial<Pre::kNone>
+                : kind == Pre::kBf16 ? colsumPartial<Pre::kBf16>
+                                     : colsumPartial<Pre::kInt8>;
+  kernel<<<grid, kWarps * 32, 0, stream>>>(gy, pre, preExp, gout, partial, M, N, rowsPer);
   colReduce<<<(N + 31) / 32, kColReduceWarps * 32, 0, stream>>>(partial, parts, N, N, N, db,
                                                                  nullptr);
   gLaunches.fetch_add(2, std::memory_order_relaxed);
@@ -160,10 +184,16 @@ static int launchColsum(const uint16_t* gy, const uint16_t* pre, uint16_t* gout,
 // partial: tnops_colsum_parts(M, N) * N floats of scratch.
 extern "C" int tnops_bias_grad(const uint16_t* g, float* db, float* partial, int M, int N,
                                cudaStream_t stream) {
-  return launchColsum(g, nullptr, nullptr, db, partial, M, N, false, stream);
+  return launchColsum(Pre::kNone, g, nullptr, nullptr, nullptr, db, partial, M, N, stream);
 }
 
 extern "C" int tnops_gelu_bwd_bias(const uint16_t* gy, const uint16_t* pre, uint16_t* gpre,
                                    float* db, float* partial, int M, int N, cudaStream_t stream) {
-  return launchColsum(gy, pre, gpre, db, partial, M, N, true, stream);
+  return launchColsum(Pre::kBf16, gy, pre, nullptr, gpre, db, partial, M, N, stream);
+}
+
+extern "C" int tnops_gelu_bwd_bias_int8(const uint16_t* gy, const uint8_t* pre_q,
+                                        const uint8_t* pre_e, uint16_t* gpre, float* db,
+                                        float* partial, int M, int N, cudaStream_t stream) {
+  return launchColsum(Pre::kInt8, gy, pre_q, pre_e, gpre, db, partial, M, N, stream);
 }

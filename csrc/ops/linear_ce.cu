@@ -1,0 +1,293 @@
+// linear_ce.cu - a linear layer over a large vocabulary and its softmax
+// cross-entropy, without the [rows, classes] logits in memory.
+//
+//   l[r, v] = sum_c x[r, c] w[v, c]
+//   lse[r]  = log sum_v exp(l[r, v]),   loss[r] = lse[r] - l[r, target[r]]
+//   d[r, v] = k[r] (exp(l[r, v] - lse[r]) - [v = target[r]])
+//   dx = d w,   dw = d^T x
+//
+// with k[r] the gradient that arrives at loss[r] (0 for a row whose target is
+// no class). The forward pass is one GEMM whose epilogue keeps, per row and
+// 128 columns, the largest logit and the sum of exponentials below it (fp32,
+// from the fp32 accumulators: no logit is rounded), and a second kernel joins
+// them. The backward pass goes over the vocabulary in pieces: a GEMM forms the
+// piece's logits again and writes d for it (bf16, the operand type of the two
+// products that follow), and one launch of linear_grads.cu forms this piece's
+// rows of dw and adds its share to dx (fp32 between pieces). Beyond its inputs
+// and outputs the backward pass holds one piece of d and, with more than one
+// piece, dx in fp32.
+// 8 rows classes width operations, 2 of them for the logits formed twice.
+#include "linear_grads.h"
+#include "pair_gemm.cuh"
+#include "tnccl_ops.h"
+
+namespace tnops {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Running maximum and sum of exponentials of one row over 128 columns.
+struct StatsEpi {
+  const int64_t* target;
+  float2* partial;  // [2 * tilesN][rows]: (maximum, sum of exp(l - maximum))
+  float* logitOfTarget;
+  int rows, classes;
+
+  struct State {
+    float m, s;
+    int64_t target;
+  };
+  __device__ __forceinline__ State begin(int, int row) const {
+    return {-INFINITY, 0.f, row < rows ? target[row] : -1};
+  }
+  __device__ __forceinline__ void chunk(State& st, const float (&in)[32], int, int lane, int row0,
+                                        int col0, uint32_t) const {
+    if (col0 >= classes) return;
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = col0 + i < classes ? in[i] : -INFINITY;
+    const int64_t at = st.target - col0;
+    if (at >= 0 && at < 32 && st.target < classes) {
+      float t = 0.f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) t = i == (int)at ? v[i] : t;
+      logitOfTarget[row0 + lane] = t;
+    }
+    float top[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int i = 4; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], v[i]);
+    const float m = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), st.m);
+    if (m == -INFINITY) return;
+    const float nm = -m * kLog2e;
+    float s[4] = {st.s * ex2Approx(fmaf(st.m, kLog2e, nm)), 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s[i & 3] += ex2Approx(fmaf(v[i], kLog2e, nm));
+    st.m = m;
+    st.s = (s[0] + s[1]) + (s[2] + s[3]);
+  }
+  __device__ __forceinline__ void end(const State& st, int row, int part) const {
+    if (row < rows) partial[(size_t)part * rows + row] = make_float2(st.m, st.s);
+  }
+};
+
+// d for one piece of the vocabulary, from lse of the whole row.
+struct SoftmaxGradEpi {
+  CUtensorMap mapD;
+  const int64_t* target;
+  const float* lse;
+  const float* grad;   // gradient of each row's loss, or of all with gradStep 0
+  const float* share;  // further factor (1 / rows that count), or null
+  int gradStep, rows, classes, first, width;
+
+  struct State {
+    float nb, k;
+    int at;  // the target's column in this piece (any other value: none)
+    bool counts;
+  };
+  __device__ __forceinline__ State begin(int, int row) const {
+    State st{0.f, 0.f, -1, false};
+    if (row < rows) {
+      const int64_t t = target[row];
+      st.counts = t >= 0 && t < classes;
+      if (st.counts) {
+        st.nb = -lse[row] * kLog2e;
+        st.k = grad[(size_t)row * gradStep];
+        if (share != nullptr) st.k *= *share;
+        st.at = (int)(t - first);
+      }
+    }
+    return st;
+  }
+  __device__ __forceinline__ void chunk(State& st, const float (&in)[32], int, int lane, int row0,
+                                        int col0, uint32_t buf) const {
+    float v[32];
+    // A row that does not count gives zeros whatever its logits are.
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      v[i] = st.counts ? st.k * ex2Approx(fmaf(in[i], kLog2e, st.nb)) : 0.f;
+    const int at = st.at - col0;
+    if (at >= 0 && at < 32) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] -= i == at ? st.k : 0.f;
+    }
+    storeBf16(v, lane, buf, &mapD, row0, col0, row0 < rows && col0 < width);
+  }
+  __device__ __forceinline__ void end(const State&, int, int) const {}
+};
+
+constexpr int kJoinWarps = 8;
+
+// Joins a row's partial statistics: 32 rows per CTA (one per lane), the parts
+// split over the warps; each warp and then the CTA keeps (maximum, sum).
+__global__ void __launch_bounds__(kJoinWarps * 32)
+    joinStats(const float2* __restrict__ partial, const int64_t* __restrict__ target,
+              const float* __restrict__ logitOfTarget, float* __restrict__ lse,
+              float* __restrict__ loss, int parts, int rows, int classes) {
+  __shared__ float2 s[kJoinWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.x * 32 + lane;
+  auto join = [](float2 a, float2 b) {
+    const float m = fmaxf(a.x, b.x);
+    if (m == -INFINITY) return make_float2(m, a.y + b.y);
+    return make_float2(m, a.y * exp2f((a.x - m) * kLog2e) + b.y * exp2f((b.x - m) * kLog2e));
+  };
+  float2 st = make_float2(-INFINITY, 0.f);
+  if (row < rows)
+    for (int p = warp; p < parts; p += kJoinWarps) st = join(st, partial[(size_t)p * rows + row]);
+  s[warp][lane] = st;
+  __syncthreads();
+  if (warp == 0 && row < rows) {
+#pragma unroll
+    for (int w = 1; w < kJoinWarps; ++w) st = join(st, s[w][lane]);
+    const float l = st.x + logf(st.y);
+    const int64_t t = target[row];
+    lse[row] = l;
+    loss[row] = t >= 0 && t < classes ? l - logitOfTarget[row] : 0.f;
+  }
+}
+
+// out[0] = the sum of the losses, or their mean over the rows that count;
+// out[1] = 1 / the number of rows that count (at least one). One CTA, fixed
+// order.
+constexpr int kMeanThreads = 1024;
+__global__ void __launch_bounds__(kMeanThreads)
+    meanLoss(const float* __restrict__ loss, const int64_t* __restrict__ target, int rows,
+             int classes, int mean, float* __restrict__ out) {
+  __shared__ float sSum[32];
+  __shared__ int sCount[32];
+  float sum = 0.f;
+  int count = 0;
+  for (int r = threadIdx.x; r < rows; r += kMeanThreads) {
+    sum += loss[r];
+    const int64_t t = target[r];
+    count += t >= 0 && t < classes;
+  }
+  sum = warpSum(sum);
+  count = __reduce_add_sync(0xffffffffu, count);
+  if ((threadIdx.x & 31) == 0) {
+    sSum[threadIdx.x >> 5] = sum;
+    sCount[threadIdx.x >> 5] = count;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    sum = warpSum(sSum[threadIdx.x]);
+    count = __reduce_add_sync(0xffffffffu, sCount[threadIdx.x]);
+    if (threadIdx.x == 0) {
+      const float share = 1.0f / (float)(count > 0 ? count : 1);
+      out[0] = mean ? sum * share : sum;
+      out[1] = share;
+    }
+  }
+}
+
+__global__ void f32ToBf16(const float* __restrict__ in, uint16_t* __restrict__ out, size_t n4) {
+  const size_t stride = (size_t)gridDim.x * blockDim.x;
+  for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n4; i += stride)
+    reinterpret_cast<uint2*>(out)[i] = tobf4(reinterpret_cast<const float4*>(in)[i]);
+}
+
+int tilesOf(int n) { return (n + 255) / 256; }
+
+// x [rows, width] against w[first .. first + n): the logits' product.
+bool logitsProblem(GemmProblem* p, const void* x, const void* w, int rows, int width, int first,
+                   int n) {
+  p->tilesM = tilesOf(rows);
+  p->tilesN = tilesOf(n);
+  p->kBlocks = (width + kBK - 1) / kBK;
+  p->aMn = p->bMn = 0;
+  return operandMap(&p->mapA, x, rows, width, width, false) &&
+         operandMap(&p->mapB, static_cast<const uint16_t*>(w) + (size_t)first * width, n, width,
+                    width, false);
+}
+
+}  // namespace
+
+unsigned linearCeStatus(int reset) { return readStatus(reset); }
+
+}  // namespace tnops
+
+using namespace tnops;
+
+extern "C" int tnops_linear_ce_parts(int classes) { return 2 * tilesOf(classes); }
+
+extern "C" int tnops_linear_ce_fwd(const void* x, const void* w, const int64_t* target,
+                                   float* loss, float* lse, float* partial, int rows, int width,
+                                   int classes, cudaStream_t stream) {
+  if (rows <= 0 || classes <= 0 || width <= 0 || width % 8 != 0 || !aligned16(x) ||
+      !aligned16(w))
+    return 1;
+  PairGemmArgs<StatsEpi> args{};
+  args.problems = 1;
+  if (!logitsProblem(&args.prob[0], x, w, rows, width, 0, classes)) return 4;
+  args.epi = {target, reinterpret_cast<float2*>(partial), loss, rows, classes};
+  if (int rc = launchPairGemm(args, stream)) return rc;
+  joinStats<<<(rows + 31) / 32, kJoinWarps * 32, 0, stream>>>(
+      args.epi.partial, target, loss, lse, loss, tnops_linear_ce_parts(classes), rows, classes);
+  return launched(cudaGetLastError());
+}
+
+extern "C" int tnops_linear_ce_mean(const float* loss, const int64_t* target, float* out2,
+                                    int rows, int classes, int mean, cudaStream_t stream) {
+  if (rows <= 0) return 1;
+  meanLoss<<<1, kMeanThreads, 0, stream>>>(loss, target, rows, classes, mean, out2);
+  return launched(cudaGetLastError());
+}
+
+extern "C" int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* target,
+                                   const float* lse, const float* grad, int grad_step,
+                                   const float* share, void* d, int piece, float* dx_f32,
+                                   void* dx, void* dw, int dw_f32, int rows, int width,
+                                   int classes, int vocab, cudaStream_t stream) {
+  if (rows <= 0 || classes <= 0 || vocab < classes || width <= 0 || width % 8 != 0 ||
+      piece <= 0 || piece % 8 != 0 || !aligned16(x) || !aligned16(w) || !aligned16(d) ||
+      (dx && !aligned16(dx)) || (dw && !aligned16(dw)))
+    return 1;
+  const bool whole = classes <= piece;
+  if (dx && !whole && (dx_f32 == nullptr || !aligned16(dx_f32))) return 1;
+  const size_t dwSize = dw_f32 ? 4 : 2;
+  if (dw && vocab > classes) {
+    const cudaError_t e = cudaMemsetAsync(static_cast<char*>(dw) + dwSize * width * (size_t)classes,
+                                          0, dwSize * width * (size_t)(vocab - classes), stream);
+    if (e != cudaSuccess) return (int)e;
+  }
+  for (int first = 0; first < classes; first += piece) {
+    const int n = classes - first < piece ? classes - first : piece;
+    PairGemmArgs<SoftmaxGradEpi> args{};
+    args.problems = 1;
+    if (!logitsProblem(&args.prob[0], x, w, rows, width, first, n) ||
+        !bf16OutMap(&args.epi.mapD, d, rows, n, piece))
+      return 4;
+    SoftmaxGradEpi& e = args.epi;
+    e.target = target;
+    e.lse = lse;
+    e.grad = grad;
+    e.share = share;
+    e.gradStep = grad_step;
+    e.rows = rows;
+    e.classes = classes;
+    e.first = first;
+    e.width = n;
+    if (int rc = launchPairGemm(args, stream)) return rc;
+    LinearGrads g{};
+    g.g = d;
+    g.ldg = piece;
+    g.w = static_cast<const uint16_t*>(w) + (size_t)first * width;
+    g.x = x;
+    g.dx = whole ? dx : dx_f32;
+    g.dxStore = !dx ? kStoreNone : whole ? kStoreBf16 : first == 0 ? kStoreF32 : kAddF32;
+    g.dw = dw ? static_cast<char*>(dw) + dwSize * width * (size_t)first : nullptr;
+    g.dwStore = !dw ? kStoreNone : dw_f32 ? kStoreF32 : kStoreBf16;
+    g.rows = rows;
+    g.outs = n;
+    g.ins = width;
+    if (int rc = linearGrads(g, stream)) return rc;
+  }
+  if (dx && !whole) {
+    const size_t n4 = (size_t)rows * width / 4;
+    const size_t blocks = (n4 + 255) / 256;
+    f32ToBf16<<<(unsigned)(blocks < kSMs * 8 ? blocks : kSMs * 8), 256, 0, stream>>>(
+        dx_f32, static_cast<uint16_t*>(dx), n4);
+    return launched(cudaGetLastError());
+  }
+  return 0;
+}

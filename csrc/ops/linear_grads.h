@@ -1,0 +1,34 @@
+// linear_grads.h - the two products of a linear layer's backward pass, for the
+// C++ side of the library (the C launcher is tnops_linear_grads).
+#pragma once
+
+#include <stdint.h>
+
+#include <cuda_runtime_api.h>
+
+namespace tnops {
+
+// How an output is written.
+enum GradStore { kStoreNone = 0, kStoreBf16 = 1, kStoreF32 = 2, kAddF32 = 3 };
+
+// y = x w^T with y [rows, outs], x [rows, ins], w [outs, ins]; g [rows, outs]
+// (rows `ldg` elements apart) is the gradient of y. dx [rows, ins] = g w,
+// dw [outs, ins] = g^T x, each left out with kStoreNone.
+struct LinearGrads {
+  const void* g;
+  int64_t ldg;
+  const void* w;
+  const void* x;
+  void* dx;
+  void* dw;
+  GradStore dxStore, dwStore;
+  int rows, outs, ins;
+};
+
+int linearGrads(const LinearGrads& a, cudaStream_t stream);
+
+// First failure code of the kernels of linear_grads.cu / linear_ce.cu.
+unsigned linearGradsStatus(int reset);
+unsigned linearCeStatus(int reset);
+
+}  // namespace tnops

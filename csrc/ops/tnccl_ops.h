@@ -56,6 +56,11 @@ int tnops_bias_grad(const uint16_t* g, float* db, float* partial, int M, int N,
 int tnops_gelu_bwd_bias(const uint16_t* gy, const uint16_t* pre, uint16_t* gpre, float* db,
                         float* partial, int M, int N, cudaStream_t stream);
 int tnops_colsum_parts(int M, int N);
+// tnops_gelu_bwd_bias with pre in 8-bit blocks (tnops_quantize_int8's form):
+// pre_q [M, N] 8-byte aligned, pre_e [M, ceil(N / 32)].
+int tnops_gelu_bwd_bias_int8(const uint16_t* gy, const uint8_t* pre_q, const uint8_t* pre_e,
+                             uint16_t* gpre, float* db, float* partial, int M, int N,
+                             cudaStream_t stream);
 
 // Multiplies a bf16 tensor by the fp32 scalar *scale (device memory); no-op
 // on the device when *scale == 1.
@@ -94,7 +99,63 @@ int tnops_adamw_dev(const tnops_adamw_list* list, float lr, float beta1, float b
 // N % 8 == 0, x, w, pre, act 16-byte aligned; 1 (invalid argument) otherwise.
 int tnops_gemm_bias_act(const void* x, const void* w, const void* bias, void* pre, void* act,
                         int M, int N, int K, int gelu, int persistent, cudaStream_t stream);
-// First failure code recorded by a tcgen05 GEMM (a bounded wait that expired),
+// Both products of the backward pass of y = x w^T: dx [rows, ins] (bf16) =
+// g w and dw [outs, ins] (fp32 with dw_f32, else bf16) = g^T x, for g
+// [rows, outs] with rows ldg elements apart, w [outs, ins], x [rows, ins],
+// all bf16. A null dx or dw is left out. ins % 8 == 0, ldg % 8 == 0, 16-byte
+// aligned pointers; 1 (invalid argument) without a launch otherwise.
+int tnops_linear_grads(const void* g, int64_t ldg, const void* w, const void* x, void* dx,
+                       void* dw, int dw_f32, int rows, int outs, int ins, cudaStream_t stream);
+
+// Softmax cross-entropy of l = x w^T without the logits in memory: x
+// [rows, width], w [vocab, width] in bf16, of which the first `classes` rows
+// are classes. A row whose target is outside [0, classes) does not count
+// (zero loss, zero gradient). width % 8 == 0, x, w, dx, dw, d 16-byte aligned;
+// 1 (invalid argument) without a launch otherwise.
+//  * fwd: loss[r] and lse[r] (fp32); partial holds
+//    2 * rows * tnops_linear_ce_parts(classes) floats of scratch.
+//  * mean: out2[0] = the losses' sum, or with `mean` their mean over the rows
+//    that count; out2[1] = 1 / max(1, rows that count).
+//  * bwd: dx [rows, width] (bf16) and dw [vocab, width] (fp32 with dw_f32, else
+//    bf16; rows from `classes` on are zero) of sum_r k[r] loss[r], with k[r] =
+//    grad[r * grad_step] (* *share). Works on `piece` classes at a time
+//    (piece % 8 == 0); d holds rows * piece bf16 of scratch, and dx_f32
+//    rows * width floats when piece < classes. A null dx or dw is left out.
+int tnops_linear_ce_parts(int classes);
+int tnops_linear_ce_fwd(const void* x, const void* w, const int64_t* target, float* loss,
+                        float* lse, float* partial, int rows, int width, int classes,
+                        cudaStream_t stream);
+int tnops_linear_ce_mean(const float* loss, const int64_t* target, float* out2, int rows,
+                         int classes, int mean, cudaStream_t stream);
+int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* target, const float* lse,
+                        const float* grad, int grad_step, const float* share, void* d, int piece,
+                        float* dx_f32, void* dx, void* dw, int dw_f32, int rows, int width,
+                        int classes, int vocab, cudaStream_t stream);
+
+// Token and position embedding: y[r] = scale * w[token[r]] + p[position[r]]
+// for w [vocab, cols] and p [context, cols] (both fp32 with w_f32, else bf16;
+// p may be null), y [rows, cols] (fp32 with y_f32, else bf16). A null
+// `position` stands for r % seq. An index outside its table adds nothing.
+int tnops_embedding_fwd(const int64_t* token, const int64_t* position, const void* w,
+                        const void* p, int w_f32, void* y, int y_f32, int64_t rows, int seq,
+                        int vocab, int context, int cols, float scale, cudaStream_t stream);
+// Gradient of a table: dw[v] = scale * sum of g[r] over the rows with
+// token[r] = v, in row order, for every v (rows without a token: zero). A null
+// `token` stands for r % seq.
+int tnops_embedding_grad(const void* g, int g_f32, const int64_t* token, int seq, void* dw,
+                         int dw_f32, int64_t rows, int vocab, int cols, float scale,
+                         cudaStream_t stream);
+
+// x [rows, cols] (fp32 with x_f32, else bf16) in 8-bit blocks: q [rows, cols]
+// signed bytes and one exponent byte per 32 neighbours of a row, e
+// [rows, ceil(cols / 32)]; value = q * 2^(e - 133), 255 marks a block that
+// holds an infinity or a NaN (it reads back as NaN).
+int tnops_quantize_int8(const void* x, int x_f32, uint8_t* q, uint8_t* e, int64_t rows, int cols,
+                        cudaStream_t stream);
+int tnops_dequantize_int8(const uint8_t* q, const uint8_t* e, void* x, int x_f32, int64_t rows,
+                          int cols, cudaStream_t stream);
+
+// First failure code recorded by a tcgen05 kernel (a bounded wait that expired),
 // 0 if none; `reset` clears it. Synchronises the device.
 unsigned tnops_tcgen05_status(int reset);
 

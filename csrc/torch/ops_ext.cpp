@@ -229,6 +229,8 @@ void adamw(const std::vector<at::Tensor>& params, const std::vector<at::Tensor>&
 
 }  // namespace
 
+void registerTrainOps(py::module_& ops);  // train_ext.cpp
+
 void registerOps(py::module_& m) {
   py::module_ ops = m.def_submodule("ops", "fused sm_100a model kernels");
   ops.attr("available") = true;
@@ -253,4 +255,5 @@ void registerOps(py::module_& m) {
           py::arg("step_tensor") = py::none(),
           py::arg("param_bf16") = std::vector<at::Tensor>());
   ops.def("launch_count", []() { return tnops_launch_count(); });
+  registerTrainOps(ops);
 }

@@ -1,0 +1,322 @@
+// train_ext.cpp - PyTorch binding of the training operators: embedding,
+// linear cross-entropy, and linear layers with 8-bit activations (csrc/ops).
+// As in ops_ext.cpp, each entry validates its tensors and calls the C launcher
+// on the current CUDA stream; a launcher error raises.
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/extension.h>
+
+#include <climits>
+#include <vector>
+
+#include "tnccl_ops.h"
+
+namespace py = pybind11;
+
+namespace {
+
+using Opt = c10::optional<at::Tensor>;
+
+cudaStream_t streamOf(const at::Tensor& t) {
+  return c10::cuda::getCurrentCUDAStream(t.get_device()).stream();
+}
+
+void need(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+}
+void need(const at::Tensor& t, at::ScalarType st, const char* name) {
+  need(t, name);
+  TORCH_CHECK(t.scalar_type() == st, name, " has dtype ", t.scalar_type(), ", expected ", st);
+}
+// 1 for fp32, 0 for bf16.
+int f32(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, name,
+              " must be float32 or bfloat16, not ", t.scalar_type());
+  return t.scalar_type() == at::kFloat;
+}
+void sameDevice(const at::Tensor& a, const at::Tensor& b, const char* name) {
+  TORCH_CHECK(a.device() == b.device(), name, " is on ", b.device(), ", expected ", a.device());
+}
+int asInt(int64_t n, const char* what) {
+  TORCH_CHECK(n >= 0 && n <= INT_MAX, what, " (", n, ") is out of range");
+  return (int)n;
+}
+
+void ok(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed (code ", rc, ")"); }
+
+uint8_t* bytes(const at::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
+
+// -- embedding -----------------------------------------------------------------
+
+at::Tensor embeddingFwd(const at::Tensor& token, const Opt& position, const at::Tensor& w,
+                        const Opt& p, int64_t seq, double scale, bool outF32) {
+  need(token, at::kLong, "idx");
+  need(w, "weight");
+  TORCH_CHECK(w.dim() == 2, "weight must be [vocab, width]");
+  const int wF32 = f32(w, "weight");
+  sameDevice(token, w, "weight");
+  if (p) {
+    need(*p, w.scalar_type(), "pos_weight");
+    TORCH_CHECK(p->dim() == 2 && p->size(1) == w.size(1), "pos_weight must be [context, width]");
+    sameDevice(token, *p, "pos_weight");
+  }
+  if (position) {
+    need(*position, at::kLong, "positions");
+    TORCH_CHECK(position->numel() == token.numel(), "positions must have one entry per token");
+    sameDevice(token, *position, "positions");
+  }
+  c10::cuda::CUDAGuard g(token.device());
+  const int64_t rows = token.numel();
+  auto y = at::empty({rows, w.size(1)}, w.options().dtype(outF32 ? at::kFloat : at::kBFloat16));
+  if (y.numel() == 0) return y;
+  ok(tnops_embedding_fwd(token.data_ptr<int64_t>(),
+                         position ? position->data_ptr<int64_t>() : nullptr, w.data_ptr(),
+                         p ? p->data_ptr() : nullptr, wF32, y.data_ptr(), outF32 ? 1 : 0, rows,
+                         asInt(seq, "sequence length"), asInt(w.size(0), "vocabulary"),
+                         p ? asInt(p->size(0), "context") : 0, asInt(w.size(1), "width"),
+                         (float)scale, streamOf(token)),
+     "tnops_embedding_fwd");
+  return y;
+}
+
+// grad [rows, width]; token [rows], or none for row % seq -> the gradient of a
+// [vocab, width] table.
+at::Tensor embeddingGrad(const at::Tensor& grad, const Opt& token, int64_t seq, int64_t vocab,
+                         double scale, bool outF32, const Opt& out) {
+  need(grad, "grad");
+  TORCH_CHECK(grad.dim() == 2, "embedding_grad: want grad [rows, width]");
+  const int gF32 = f32(grad, "grad");
+  if (token) {
+    need(*token, at::kLong, "idx");
+    TORCH_CHECK(token->numel() == grad.size(0), "embedding_grad: one token per row of grad");
+    sameDevice(grad, *token, "idx");
+  }
+  c10::cuda::CUDAGuard g(grad.device());
+  const auto st = outF32 ? at::kFloat : at::kBFloat16;
+  auto dw = out ? *out : at::empty({vocab, grad.size(1)}, grad.options().dtype(st));
+  need(dw, st, "out");
+  TORCH_CHECK(dw.numel() == vocab * grad.size(1), "embedding_grad: out has the wrong size");
+  sameDevice(grad, dw, "out");
+  if (dw.numel() == 0) return dw;
+  if (grad.size(0) == 0) return dw.zero_();
+  ok(tnops_embedding_grad(grad.data_ptr(), gF32, token ? token->data_ptr<int64_t>() : nullptr,
+                          asInt(seq, "sequence length"), dw.data_ptr(), outF32 ? 1 : 0,
+                          grad.size(0), asInt(vocab, "vocabulary"), asInt(grad.size(1), "width"),
+                          (float)scale, streamOf(grad)),
+     "tnops_embedding_grad");
+  return dw;
+}
+
+// -- linear cross-entropy --------------------------------------------------------
+
+struct CeShape {
+  int rows, width, classes, vocab;
+};
+CeShape ceShape(const at::Tensor& x, const at::Tensor& w, const at::Tensor& target,
+                int64_t classes) {
+  need(x, at::kBFloat16, "x");
+  need(w, at::kBFloat16, "weight");
+  need(target, at::kLong, "target");
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1),
+              "linear_cross_entropy: want x [rows, width] and weight [vocab, width]");
+  TORCH_CHECK(x.size(1) > 0 && x.size(1) % 8 == 0,
+              "linear_cross_entropy: width must be a multiple of 8");
+  TORCH_CHECK(target.numel() == x.size(0), "linear_cross_entropy: one target per row");
+  TORCH_CHECK(classes > 0 && classes <= w.size(0),
+              "linear_cross_entropy: classes must be in [1, ", w.size(0), "]");
+  sameDevice(x, w, "weight");
+  sameDevice(x, target, "target");
+  return {asInt(x.size(0), "rows"), asInt(x.size(1), "width"), asInt(classes, "classes"),
+          asInt(w.size(0), "vocabulary")};
+}
+
+// -> per-row loss, lse, and [sum or mean, 1 / rows that count]
+std::vector<at::Tensor> linearCeFwd(const at::Tensor& x, const at::Tensor& w,
+                                    const at::Tensor& target, int64_t classes, bool mean) {
+  const CeShape s = ceShape(x, w, target, classes);
+  c10::cuda::CUDAGuard g(x.device());
+  const auto opt = x.options().dtype(at::kFloat);
+  auto loss = at::empty({s.rows}, opt), lse = at::empty({s.rows}, opt);
+  if (s.rows == 0) {
+    auto out = at::zeros({2}, opt);
+    out.select(0, 1).fill_(1.0);
+    return {loss, lse, out};
+  }
+  auto out = at::empty({2}, opt);
+  auto partial = at::empty({(int64_t)tnops_linear_ce_parts(s.classes), s.rows, 2}, opt);
+  ok(tnops_linear_ce_fwd(x.data_ptr(), w.data_ptr(), target.data_ptr<int64_t>(),
+                         loss.data_ptr<float>(), lse.data_ptr<float>(), partial.data_ptr<float>(),
+                         s.rows, s.width, s.classes, streamOf(x)),
+     "tnops_linear_ce_fwd");
+  ok(tnops_linear_ce_mean(loss.data_ptr<float>(), target.data_ptr<int64_t>(),
+                          out.data_ptr<float>(), s.rows, s.classes, mean ? 1 : 0, streamOf(x)),
+     "tnops_linear_ce_mean");
+  return {loss, lse, out};
+}
+
+// Classes per piece of the backward pass: as many whole 256-wide tiles as fit
+// the scratch budget, spread evenly.
+int64_t cePiece(int64_t rows, int64_t classes, int64_t budget) {
+  const int64_t tiles = (classes + 255) / 256;
+  int64_t most = budget / (rows * 512);
+  if (most < 1) most = 1;
+  const int64_t pieces = (tiles + most - 1) / most;
+  return (tiles + pieces - 1) / pieces * 256;
+}
+
+std::vector<at::Tensor> linearCeBwd(const at::Tensor& x, const at::Tensor& w,
+                                    const at::Tensor& target, const at::Tensor& lse,
+                                    const at::Tensor& grad, const Opt& share, int64_t classes,
+                                    bool wantDx, bool wantDw, bool dwF32, const Opt& dwOut,
+                                    int64_t budget) {
+  const CeShape s = ceShape(x, w, target, classes);
+  need(lse, at::kFloat, "lse");
+  need(grad, at::kFloat, "grad");
+  TORCH_CHECK(grad.numel() == 1 || grad.numel() == s.rows,
+              "linear_cross_entropy: want one gradient, or one per row");
+  TORCH_CHECK(budget > 0, "linear_cross_entropy: the scratch budget must be positive");
+  if (share) need(*share, at::kFloat, "share");
+  c10::cuda::CUDAGuard g(x.device());
+  at::Tensor dx, dw;
+  if (wantDx) dx = at::empty_like(x);
+  if (wantDw) {
+    const auto st = dwF32 ? at::kFloat : at::kBFloat16;
+    dw = dwOut ? *dwOut : at::empty({s.vocab, s.width}, w.options().dtype(st));
+    need(dw, st, "dw_out");
+    TORCH_CHECK(dw.numel() == w.numel(), "linear_cross_entropy: dw_out must match weight");
+    if (s.rows == 0) dw.zero_();
+  }
+  if (s.rows == 0 || (!wantDx && !wantDw)) return {dx, dw};
+  const int64_t piece = cePiece(s.rows, s.classes, budget);
+  auto d = at::empty({(int64_t)s.rows, piece}, x.options());
+  at::Tensor dxF32;
+  if (wantDx && piece < s.classes) dxF32 = at::empty(x.sizes(), x.options().dtype(at::kFloat));
+  ok(tnops_linear_ce_bwd(x.data_ptr(), w.data_ptr(), target.data_ptr<int64_t>(),
+                         lse.data_ptr<float>(), grad.data_ptr<float>(),
+                         grad.numel() == 1 ? 0 : 1, share ? share->data_ptr<float>() : nullptr,
+                         d.data_ptr(), (int)piece,
+                         dxF32.defined() ? dxF32.data_ptr<float>() : nullptr,
+                         wantDx ? dx.data_ptr() : nullptr, wantDw ? dw.data_ptr() : nullptr,
+                         dwF32 ? 1 : 0, s.rows, s.width, s.classes, s.vocab, streamOf(x)),
+     "tnops_linear_ce_bwd");
+  return {dx, dw};
+}
+
+// -- linear layers with 8-bit activations ------------------------------------------
+
+// x [rows, cols] -> (q int8 [rows, cols], e uint8 [rows, ceil(cols / 32)])
+std::vector<at::Tensor> quantizeInt8(const at::Tensor& x) {
+  need(x, "x");
+  TORCH_CHECK(x.dim() == 2, "quantize_int8: want [rows, cols]");
+  const int xF32 = f32(x, "x");
+  c10::cuda::CUDAGuard g(x.device());
+  const int64_t rows = x.size(0), cols = x.size(1);
+  auto q = at::empty({rows, cols}, x.options().dtype(at::kChar));
+  auto e = at::empty({rows, (cols + 31) / 32}, x.options().dtype(at::kByte));
+  if (x.numel() == 0) return {q, e};
+  ok(tnops_quantize_int8(x.data_ptr(), xF32, bytes(q), bytes(e), rows, asInt(cols, "columns"),
+                         streamOf(x)),
+     "tnops_quantize_int8");
+  return {q, e};
+}
+
+void needInt8(const at::Tensor& q, const at::Tensor& e) {
+  need(q, at::kChar, "q");
+  need(e, at::kByte, "e");
+  TORCH_CHECK(q.dim() == 2 && e.dim() == 2 && e.size(0) == q.size(0) &&
+                  e.size(1) == (q.size(1) + 31) / 32,
+              "8-bit blocks: want q [rows, cols] and e [rows, ceil(cols / 32)]");
+  sameDevice(q, e, "e");
+}
+
+at::Tensor dequantizeInt8(const at::Tensor& q, const at::Tensor& e, bool outF32) {
+  needInt8(q, e);
+  c10::cuda::CUDAGuard g(q.device());
+  auto x = at::empty(q.sizes(), q.options().dtype(outF32 ? at::kFloat : at::kBFloat16));
+  if (x.numel() == 0) return x;
+  ok(tnops_dequantize_int8(bytes(q), bytes(e), x.data_ptr(), outF32 ? 1 : 0, q.size(0),
+                           asInt(q.size(1), "columns"), streamOf(q)),
+     "tnops_dequantize_int8");
+  return x;
+}
+
+// gy bf16 [M, N], pre in 8-bit blocks -> (gpre bf16 [M, N], db fp32 [N])
+std::vector<at::Tensor> geluBwdBiasInt8(const at::Tensor& gy, const at::Tensor& q,
+                                        const at::Tensor& e, const Opt& dbOut) {
+  need(gy, at::kBFloat16, "grad_y");
+  needInt8(q, e);
+  TORCH_CHECK(gy.dim() == 2 && gy.sizes() == q.sizes() && gy.size(1) % 8 == 0,
+              "gelu_bwd_bias_int8: want equal [M, N] with N % 8 == 0");
+  sameDevice(gy, q, "q");
+  c10::cuda::CUDAGuard g(gy.device());
+  const int M = asInt(gy.size(0), "rows"), N = asInt(gy.size(1), "columns");
+  auto gpre = at::empty_like(gy);
+  auto db = dbOut ? *dbOut : at::empty({N}, gy.options().dtype(at::kFloat));
+  need(db, at::kFloat, "db_out");
+  TORCH_CHECK(db.numel() == N, "gelu_bwd_bias_int8: db_out needs N elements");
+  auto part = at::empty({(int64_t)tnops_colsum_parts(M, N) * N}, gy.options().dtype(at::kFloat));
+  ok(tnops_gelu_bwd_bias_int8(static_cast<uint16_t*>(gy.data_ptr()), bytes(q), bytes(e),
+                              static_cast<uint16_t*>(gpre.data_ptr()), db.data_ptr<float>(),
+                              part.data_ptr<float>(), M, N, streamOf(gy)),
+     "tnops_gelu_bwd_bias_int8");
+  return {gpre, db};
+}
+
+// g [rows, outs], w [outs, ins], x in 8-bit blocks [rows, ins] -> (dx bf16, dw)
+std::vector<at::Tensor> linearGradsInt8(const at::Tensor& grad, const at::Tensor& w,
+                                        const at::Tensor& q, const at::Tensor& e, bool wantDx,
+                                        bool wantDw, bool dwF32, const Opt& dwOut) {
+  need(grad, at::kBFloat16, "grad");
+  need(w, at::kBFloat16, "weight");
+  needInt8(q, e);
+  TORCH_CHECK(grad.dim() == 2 && w.dim() == 2 && grad.size(1) == w.size(0) &&
+                  q.size(0) == grad.size(0) && q.size(1) == w.size(1),
+              "linear_grads_int8: want grad [rows, outs], weight [outs, ins], q [rows, ins]");
+  TORCH_CHECK(w.size(0) % 8 == 0 && w.size(1) % 8 == 0,
+              "linear_grads_int8: the layer's sizes must be multiples of 8");
+  sameDevice(grad, w, "weight");
+  sameDevice(grad, q, "q");
+  c10::cuda::CUDAGuard g(grad.device());
+  const int rows = asInt(grad.size(0), "rows"), outs = asInt(w.size(0), "outputs"),
+            ins = asInt(w.size(1), "inputs");
+  at::Tensor dx, dw;
+  if (wantDx) dx = at::empty({rows, ins}, grad.options());
+  if (wantDw) {
+    const auto st = dwF32 ? at::kFloat : at::kBFloat16;
+    dw = dwOut ? *dwOut : at::empty({outs, ins}, w.options().dtype(st));
+    need(dw, st, "dw_out");
+    TORCH_CHECK(dw.numel() == w.numel(), "linear_grads_int8: dw_out must match weight");
+  }
+  at::Tensor x;
+  if (wantDw) x = dequantizeInt8(q, e, false);
+  ok(tnops_linear_grads(grad.data_ptr(), outs, w.data_ptr(), wantDw ? x.data_ptr() : nullptr,
+                        wantDx ? dx.data_ptr() : nullptr, wantDw ? dw.data_ptr() : nullptr,
+                        dwF32 ? 1 : 0, rows, outs, ins, streamOf(grad)),
+     "tnops_linear_grads");
+  return {dx, dw};
+}
+
+}  // namespace
+
+void registerTrainOps(py::module_& ops) {
+  ops.def("embedding_fwd", &embeddingFwd, py::arg("idx"), py::arg("positions"),
+          py::arg("weight"), py::arg("pos_weight"), py::arg("seq"), py::arg("scale"),
+          py::arg("out_f32"));
+  ops.def("embedding_grad", &embeddingGrad, py::arg("grad"), py::arg("idx"), py::arg("seq"),
+          py::arg("vocab"), py::arg("scale"), py::arg("out_f32"), py::arg("out") = py::none());
+  ops.def("linear_ce_fwd", &linearCeFwd, py::arg("x"), py::arg("weight"), py::arg("target"),
+          py::arg("classes"), py::arg("mean"));
+  ops.def("linear_ce_piece", &cePiece, py::arg("rows"), py::arg("classes"), py::arg("budget"));
+  ops.def("linear_ce_bwd", &linearCeBwd, py::arg("x"), py::arg("weight"), py::arg("target"),
+          py::arg("lse"), py::arg("grad"), py::arg("share"), py::arg("classes"),
+          py::arg("want_dx"), py::arg("want_dw"), py::arg("dw_f32"),
+          py::arg("dw_out") = py::none(), py::arg("budget") = 512ll << 20);
+  ops.def("quantize_int8", &quantizeInt8, py::arg("x"));
+  ops.def("dequantize_int8", &dequantizeInt8, py::arg("q"), py::arg("e"), py::arg("out_f32"));
+  ops.def("gelu_bwd_bias_int8", &geluBwdBiasInt8, py::arg("grad_y"), py::arg("q"), py::arg("e"),
+          py::arg("db_out") = py::none());
+  ops.def("linear_grads_int8", &linearGradsInt8, py::arg("grad"), py::arg("weight"),
+          py::arg("q"), py::arg("e"), py::arg("want_dx"), py::arg("want_dw"), py::arg("dw_f32"),
+          py::arg("dw_out") = py::none());
+}

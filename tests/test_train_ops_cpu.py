@@ -1,0 +1,118 @@
+"""Host side of the training operators, without a GPU: refusals in Python, in
+the binding and in the C launchers (before any CUDA call), and the piece rule
+of the cross-entropy."""
+import ctypes
+import os
+
+import pytest
+import torch
+
+from conftest import ROOT
+
+P, I, L, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+A = 1 << 20  # an aligned address; never dereferenced on these paths
+
+
+def _launcher(name, *types):
+    f = getattr(ctypes.CDLL(os.path.join(ROOT, "tiny_nccl_b200", "lib", "libtnccl_ops.so")), name)
+    f.argtypes, f.restype = types, I
+    return f
+
+
+def _refuses(f, good, bad):
+    for i, v in bad:
+        args = list(good)
+        args[i] = v
+        assert f(*args) == 1, (i, v)
+
+
+def test_linear_grads_launcher_refuses(built):
+    f = _launcher("tnops_linear_grads", P, L, P, P, P, P, I, I, I, I, P)
+    good = [A, 64, A, A, A, A, 0, 32, 64, 128, None]
+    _refuses(f, good, [(0, None), (0, A + 8), (1, 60), (1, 32), (2, A + 2), (2, None), (3, A + 4),
+                       (3, None), (4, A + 8), (5, A + 8), (7, 0), (8, 0), (9, 0), (9, 132)])
+
+
+def test_linear_ce_launchers_refuse(built):
+    f = _launcher("tnops_linear_ce_fwd", P, P, P, P, P, P, I, I, I, P)
+    good = [A, A, A, A, A, A, 4, 64, 100, None]
+    _refuses(f, good, [(0, A + 8), (1, A + 8), (6, 0), (7, 0), (7, 60), (8, 0)])
+    f = _launcher("tnops_linear_ce_bwd", P, P, P, P, P, I, P, P, I, P, P, P, I, I, I, I, I, P)
+    good = [A, A, A, A, A, 0, A, A, 256, A, A, A, 1, 4, 64, 300, 304, None]
+    _refuses(f, good, [(0, A + 8), (1, A + 8), (7, A + 8), (8, 0), (8, 20), (9, None),
+                       (9, A + 4), (10, A + 8), (11, A + 4), (13, 0), (14, 60), (15, 0),
+                       (16, 299)])
+    f = _launcher("tnops_linear_ce_mean", P, P, P, I, I, I, P)
+    assert f(A, A, A, 0, 5, 1, None) == 1
+
+
+def test_embedding_launchers_refuse(built):
+    f = _launcher("tnops_embedding_fwd", P, P, P, P, I, P, I, L, I, I, I, I, F, P)
+    good = [A, None, A, A, 1, A, 1, 8, 4, 100, 16, 64, 1.0, None]
+    _refuses(f, good, [(7, 0), (7, 1 << 31), (8, 0), (9, 0), (10, 0), (11, 0)])
+    f = _launcher("tnops_embedding_grad", P, I, P, I, P, I, L, I, I, F, P)
+    good = [A, 1, None, 4, A, 1, 8, 100, 64, 1.0, None]
+    _refuses(f, good, [(3, 0), (6, 0), (6, 1 << 31), (7, 0), (8, 0)])
+
+
+def test_int8_launchers_refuse(built):
+    f = _launcher("tnops_quantize_int8", P, I, P, P, L, I, P)
+    _refuses(f, [A, 0, A, A, 4, 64, None], [(4, 0), (5, 0)])
+    f = _launcher("tnops_dequantize_int8", P, P, P, I, L, I, P)
+    _refuses(f, [A, A, A, 0, 4, 64, None], [(4, 0), (5, 0)])
+    f = _launcher("tnops_gelu_bwd_bias_int8", P, P, P, P, P, P, I, I, P)
+    _refuses(f, [A, A, A, A, A, A, 64, 768, None],
+             [(0, A + 8), (1, A + 4), (3, A + 8), (6, 0), (7, 770)])
+
+
+def test_python_refusals(built):
+    from tiny_nccl_b200 import ops
+    w, p = torch.zeros(10, 8), torch.zeros(6, 8)
+    idx = torch.zeros(2, 3, dtype=torch.int64)
+    for error, args, kw in [
+            (TypeError, (idx.float(), w), {}),
+            (TypeError, (idx, w.half()), {}),
+            (TypeError, (idx, w, p.bfloat16()), {}),
+            (TypeError, (idx, w), dict(out_dtype=torch.float16)),
+            (ValueError, (idx, w, torch.zeros(6, 9)), {}),
+            (ValueError, (idx, w[0]), {}),
+            (ValueError, (idx, w), dict(positions=idx)),
+            (ValueError, (idx, w, p), dict(positions=idx[0])),
+            (TypeError, (idx, w, p), dict(positions=idx.float())),
+            (RuntimeError, (idx, w), {})]:  # not on a GPU
+        with pytest.raises(error):
+            ops.embedding(*args, **kw)
+    x, t = torch.zeros(4, 8), torch.zeros(4, dtype=torch.int64)
+    for error, args, kw in [
+            (ValueError, (x, w, t), dict(reduction="max")),
+            (ValueError, (x, torch.zeros(10, 16), t), {}),
+            (ValueError, (x, w, t[:3]), {}),
+            (TypeError, (x, w, t.int()), {}),
+            (TypeError, (x, w.half(), t), {}),
+            (RuntimeError, (x, w, t), {})]:
+        with pytest.raises(error):
+            ops.linear_cross_entropy(*args, **kw)
+    with pytest.raises(TypeError):
+        ops.quantize_int8(x.half())
+    with pytest.raises(TypeError):
+        ops.dequantize_int8(x.to(torch.int8), torch.zeros(4, 1, dtype=torch.uint8), torch.float16)
+    with pytest.raises(RuntimeError):
+        ops.quantize_int8(x)
+    for f in (ops.linear, ops.linear_gelu):
+        with pytest.raises(ValueError):
+            f(x, w, torch.zeros(10), activations="int4")
+
+
+def test_cross_entropy_pieces_cover_the_classes(built):
+    """A piece is a multiple of 256 classes, fits the budget where one tile
+    does, and the pieces are even: the last is at least half of the others
+    where there are few."""
+    from tiny_nccl_b200._native import load
+    piece = load().ops.linear_ce_piece
+    for rows in (1, 7, 200, 8192, 32768, 300000):
+        for classes in (1, 255, 256, 257, 1000, 50257, 200000):
+            for budget in (1 << 12, 1 << 20, 512 << 20):
+                n = piece(rows, classes, budget)
+                assert n > 0 and n % 256 == 0
+                assert n <= (classes + 255) // 256 * 256
+                assert n == 256 or n * rows * 2 <= budget

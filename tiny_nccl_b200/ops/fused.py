@@ -124,6 +124,13 @@ def grad_destination(p: torch.Tensor):
     return d.detach() if d is not None and p.grad is None else None
 
 
+def typed_destination(p: torch.Tensor, dtype: torch.dtype):
+    """grad_destination(p) for a gradient that a kernel writes as ``dtype`` in
+    row-major order; None where p's slice is of another type or layout."""
+    d = grad_destination(p)
+    return d if d is not None and d.dtype == dtype and d.is_contiguous() else None
+
+
 def _wgrad(gy: torch.Tensor, x: torch.Tensor, dest: torch.Tensor | None = None) -> torch.Tensor:
     """dW = gy^T x with bf16 operands and the fp32 result written by the GEMM
     itself (no bf16 rounding, no separate cast to the fp32 parameter),
@@ -139,10 +146,15 @@ class _LinearBias(torch.autograd.Function):
     deterministic column-sum kernel."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias):
+    def compute(x, weight, bias):
+        """(y, the bf16 weight, nothing before an activation)"""
         w16 = bf16_weight(weight)
         with torch.autocast("cuda", enabled=False):
-            y = torch.addmm(bf16_weight(bias), x, w16.t())
+            return torch.addmm(bf16_weight(bias), x, w16.t()), w16, None
+
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        y, w16, _ = _LinearBias.compute(x, weight, bias)
         ctx.save_for_backward(x, w16)
         ctx.params = (weight, bias)
         return y
@@ -173,7 +185,8 @@ class _LinearGelu(torch.autograd.Function):
     that gradient); dX and dW on cuBLAS."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias):
+    def compute(x, weight, bias):
+        """(y, the bf16 weight, the sums before the GELU)"""
         w16 = bf16_weight(weight)
         b16 = bf16_weight(bias)
         if _TCGEN05 != "0":
@@ -182,6 +195,11 @@ class _LinearGelu(torch.autograd.Function):
             with torch.autocast("cuda", enabled=False):
                 pre = torch.addmm(b16, x, w16.t())
                 y = torch.nn.functional.gelu(pre, approximate="tanh")
+        return y, w16, pre
+
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        y, w16, pre = _LinearGelu.compute(x, weight, bias)
         ctx.save_for_backward(x, w16, pre)
         ctx.params = (weight, bias)
         return y
@@ -219,10 +237,55 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return (x if x.dtype == torch.bfloat16 else x.to(torch.bfloat16)).contiguous()
 
 
-def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor) -> torch.Tensor:
-    """bf16 x W^T + b over the last dimension of x (fp32 weight and bias)."""
-    y = _LinearBias.apply(_rows(x), weight, bias)
+class _LinearInt8(torch.autograd.Function):
+    """The linear layers above with what the backward pass needs of the
+    activations kept in 8-bit blocks: x for dW, and the sums before the GELU
+    for its slope. The forward result is the same bit for bit."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, gelu):
+        f = _LinearGelu if gelu else _LinearBias
+        y, w16, pre = f.compute(x, weight, bias)
+        ctx.save_for_backward(w16, *_ops().quantize_int8(x),
+                              *(_ops().quantize_int8(pre) if gelu else ()))
+        ctx.params = (weight, bias)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        w16, q, e, *pre = ctx.saved_tensors
+        pw, pb = ctx.params
+        gy = gy.contiguous()
+        if pre:
+            gy, db = _ops().gelu_bwd_bias_int8(gy, *pre, typed_destination(pb, torch.float32))
+        else:
+            db = _ops().bias_grad(gy, out=typed_destination(pb, torch.float32))
+        dx, dw = _ops().linear_grads_int8(gy, w16, q, e, ctx.needs_input_grad[0],
+                                          ctx.needs_input_grad[1], pw.dtype == torch.float32,
+                                          typed_destination(pw, pw.dtype))
+        return dx, dw, db, None
+
+
+def _linear(x, weight, bias, gelu, activations):
+    if activations not in ("bf16", "int8"):
+        raise ValueError(f"activations must be 'bf16' or 'int8', not {activations!r}")
+    if activations == "int8":
+        y = _LinearInt8.apply(_rows(x), weight, bias, gelu)
+    else:
+        y = (_LinearGelu if gelu else _LinearBias).apply(_rows(x), weight, bias)
     return y.view(*x.shape[:-1], weight.shape[0])
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor,
+           activations: str = "bf16") -> torch.Tensor:
+    """bf16 x W^T + b over the last dimension of x (fp32 weight and bias).
+
+    ``activations="int8"`` keeps x for the backward pass in 8-bit blocks
+    (:func:`quantize_int8`, half the memory): the forward result and dX stay
+    the same, dW = gy^T x is formed from the 8-bit x. Both sizes of the layer
+    must then be multiples of 8."""
+    return _linear(x, weight, bias, False, activations)
 
 
 def linear_nobias(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
@@ -231,11 +294,12 @@ def linear_nobias(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
     return y.view(*x.shape[:-1], weight.shape[0])
 
 
-def linear_gelu(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor) -> torch.Tensor:
+def linear_gelu(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor,
+                activations: str = "bf16") -> torch.Tensor:
     """GELU(tanh)(x W^T + b) in bf16; the backward fuses the GELU gradient
-    with the bias gradient."""
-    y = _LinearGelu.apply(_rows(x), weight, bias)
-    return y.view(*x.shape[:-1], weight.shape[0])
+    with the bias gradient. ``activations="int8"`` keeps x and the sums before
+    the GELU for the backward pass in 8-bit blocks (see :func:`linear`)."""
+    return _linear(x, weight, bias, True, activations)
 
 
 def launch_count() -> int:

@@ -1,0 +1,169 @@
+"""Autograd wrappers of the training operators (csrc/ops): token and position
+embedding, linear layer + softmax cross-entropy in pieces of the vocabulary,
+and 8-bit activation blocks. Like :mod:`.fused`, every function calls the
+native kernels; a missing extension or an unsupported argument raises.
+"""
+from __future__ import annotations
+
+import torch
+
+from .fused import _ops, _rows, bf16_weight, typed_destination
+
+
+def _needs_float(name: str, t: torch.Tensor) -> None:
+    if t.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"{name} must be float32 or bfloat16, not {t.dtype}")
+
+
+class _Embedding(torch.autograd.Function):
+    """y = scale W[idx] + P[positions]. Backward: each table's gradient is the
+    sum of its rows' gradients in row order (deterministic), written once,
+    zeros included."""
+
+    @staticmethod
+    def forward(ctx, idx, weight, pos_weight, positions, seq, scale, out_f32):
+        y = _ops().embedding_fwd(idx, positions, weight.detach(),
+                                 None if pos_weight is None else pos_weight.detach(), seq, scale,
+                                 out_f32)
+        ctx.save_for_backward(idx, positions)
+        ctx.tables = (weight, pos_weight)
+        ctx.seq, ctx.scale = seq, scale
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        idx, positions = ctx.saved_tensors
+        weight, pos_weight = ctx.tables
+        g = g.contiguous()
+        grads = []
+        for table, at, scale, wanted in ((weight, idx, ctx.scale, ctx.needs_input_grad[1]),
+                                         (pos_weight, positions, 1.0, ctx.needs_input_grad[2])):
+            grads.append(_ops().embedding_grad(
+                g, at, ctx.seq, table.shape[0], scale, table.dtype == torch.float32,
+                typed_destination(table, table.dtype)) if wanted else None)
+        return None, grads[0], grads[1], None, None, None, None
+
+
+def embedding(idx: torch.Tensor, weight: torch.Tensor, pos_weight: torch.Tensor | None = None,
+              positions: torch.Tensor | None = None, scale: float = 1.0,
+              out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """scale * weight[idx] + pos_weight[positions], of shape [*idx.shape, width].
+
+    weight [vocab, width] and pos_weight [context, width] (optional) are both
+    float32 or both bfloat16; the sum is formed in fp32 and rounded once to
+    ``out_dtype`` (float32 or bfloat16; the tables' type when None).
+    ``positions`` (idx's shape) gives each token's position, e.g. when single
+    tokens are decoded; None counts along idx's last dimension. idx and
+    positions are int64 (int32 is converted). An index outside its table, such
+    as a negative one for padding, adds nothing and gets no gradient.
+
+    The gradients of both tables are fp32 sums in row order, bit-identical
+    from run to run; a row that no token names gets zero."""
+    for name, t in (("weight", weight), ("pos_weight", pos_weight)):
+        if t is not None:
+            _needs_float(name, t)
+            if t.dim() != 2 or t.shape[1] != weight.shape[1]:
+                raise ValueError(f"{name} must be [rows, {weight.shape[-1]}], not "
+                                 f"{tuple(t.shape)}")
+            if t.dtype != weight.dtype:
+                raise TypeError("weight and pos_weight must have one dtype")
+    out_dtype = weight.dtype if out_dtype is None else out_dtype
+    if out_dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"out_dtype must be float32 or bfloat16, not {out_dtype}")
+    if idx.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"idx must be int64 or int32, not {idx.dtype}")
+    seq = idx.shape[-1] if idx.dim() else 1
+    if positions is not None:
+        if pos_weight is None:
+            raise ValueError("positions without pos_weight")
+        if positions.shape != idx.shape:
+            raise ValueError(f"positions must have idx's shape {tuple(idx.shape)}, not "
+                             f"{tuple(positions.shape)}")
+        if positions.dtype not in (torch.int64, torch.int32):
+            raise TypeError(f"positions must be int64 or int32, not {positions.dtype}")
+        positions = positions.reshape(-1).long().contiguous()
+    y = _Embedding.apply(idx.reshape(-1).long().contiguous(), weight.contiguous(),
+                         None if pos_weight is None else pos_weight.contiguous(), positions, seq,
+                         float(scale), out_dtype == torch.float32)
+    return y.view(*idx.shape, weight.shape[1])
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    """Cross-entropy of x W^T against targets. The forward pass keeps one
+    number per row (the log of the sum of exponentials); the backward pass
+    forms the logits again, a piece of the vocabulary at a time."""
+
+    @staticmethod
+    def forward(ctx, x, weight, target, classes, reduction):
+        w16 = bf16_weight(weight).contiguous()
+        loss, lse, out = _ops().linear_ce_fwd(x, w16, target, classes, reduction == "mean")
+        ctx.save_for_backward(x, w16, target, lse, out)
+        ctx.weight, ctx.classes, ctx.reduction = weight, classes, reduction
+        return loss if reduction == "none" else out[0]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, w16, target, lse, out = ctx.saved_tensors
+        weight = ctx.weight
+        dx, dw = _ops().linear_ce_bwd(
+            x, w16, target, lse, g.reshape(-1).float().contiguous(),
+            out[1:] if ctx.reduction == "mean" else None, ctx.classes, ctx.needs_input_grad[0],
+            ctx.needs_input_grad[1], weight.dtype == torch.float32,
+            typed_destination(weight, weight.dtype))
+        return dx, dw, None, None, None
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor,
+                         classes: int = 0, reduction: str = "mean") -> torch.Tensor:
+    """Softmax cross-entropy of the logits x W^T against int64 targets, without
+    the [rows, vocabulary] logits in memory.
+
+    x [*, width] is taken in bf16, weight [vocab, width] (e.g. the tied token
+    embedding; fp32 or bf16) through its bf16 copy; logits, softmax and losses
+    are fp32. The first ``classes`` rows of weight are classes (all when 0),
+    the rest is padding with zero gradient. A target outside [0, classes) does
+    not count: zero loss, zero gradient, and not part of the mean.
+    ``reduction``: "mean" over the rows that count (0 when none does), "sum",
+    or "none" for fp32 losses of target's shape.
+
+    Backward: the gradient of x is bf16, that of weight has weight's type; the
+    gradient of the logits is rounded to bf16 between the products, a piece of
+    the vocabulary of at most 512 MiB at a time. width must be a multiple of 8."""
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"reduction must be 'mean', 'sum' or 'none', not {reduction!r}")
+    _needs_float("weight", weight)
+    if weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"weight must be [vocab, {x.shape[-1]}], not {tuple(weight.shape)}")
+    if target.dtype != torch.int64:
+        raise TypeError(f"target must be int64, not {target.dtype}")
+    if target.numel() * x.shape[-1] != x.numel():
+        raise ValueError("target must have one entry per row of x")
+    classes = int(classes) or weight.shape[0]
+    loss = _LinearCrossEntropy.apply(_rows(x), weight, target.reshape(-1).contiguous(), classes,
+                                     reduction)
+    return loss.view(target.shape) if reduction == "none" else loss
+
+
+def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """x (float32 or bfloat16) as (q, e): whole numbers in [-127, 127] (int8,
+    x's shape) and one exponent byte for each 32 neighbours of the last
+    dimension (uint8); value = q * 2^(e - 133). Off by at most 2^-7 of the
+    block's largest magnitude; a block with an infinity or a NaN reads back as
+    NaN."""
+    _needs_float("x", x)
+    cols = x.shape[-1]
+    q, e = _ops().quantize_int8(x.reshape(-1, cols).contiguous())
+    return q.view(x.shape), e.view(*x.shape[:-1], e.shape[1])
+
+
+def dequantize_int8(q: torch.Tensor, e: torch.Tensor,
+                    dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values of :func:`quantize_int8`'s blocks (exact in bfloat16 and
+    float32)."""
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"dtype must be float32 or bfloat16, not {dtype}")
+    x = _ops().dequantize_int8(q.reshape(-1, q.shape[-1]).contiguous(),
+                               e.reshape(-1, e.shape[-1]).contiguous(), dtype == torch.float32)
+    return x.view(q.shape)
