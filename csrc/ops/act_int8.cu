@@ -1,6 +1,10 @@
 // act_int8.cu - activations to 8 bits as they are kept for the backward pass,
 // and back (the form: int8_blocks.cuh). Bound by memory: 2 or 4 bytes read and
 // 1 + 1/32 written per value, or the reverse.
+//
+// bf16 rows of a multiple of 8 values take 16-byte pieces: four neighbouring
+// lanes hold a block, each thread several pieces in flight. Other rows and
+// fp32 take one warp per block, one value per lane.
 #include "int8_blocks.cuh"
 #include "tnccl_ops.h"
 
@@ -53,6 +57,96 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+constexpr int kPieces = 4;  // 16-byte pieces in flight per thread
+
+// Piece s of `slots` = rows * blocks * 4 covers values 8 (s mod 4 blocks) ..
+// + 7 of row s / (4 blocks); those past the row's end are skipped.
+struct Piece {
+  int64_t at;  // first value, or -1
+};
+__device__ __forceinline__ Piece pieceAt(uint32_t s, uint32_t slots, uint32_t perRow, int cols) {
+  if (s >= slots) return {-1};
+  const uint32_t row = s / perRow, c = (s - row * perRow) * 8;
+  return {c < (uint32_t)cols ? (int64_t)row * cols + c : -1};
+}
+
+__global__ void __launch_bounds__(kThreads)
+    quantizePieces(const uint16_t* __restrict__ x, uint8_t* __restrict__ q,
+                   uint8_t* __restrict__ e, uint32_t slots, uint32_t perRow, int cols) {
+  const uint32_t s0 = blockIdx.x * (kThreads * kPieces) + threadIdx.x;
+  Piece p[kPieces];
+  uint4 u[kPieces];
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    p[i] = pieceAt(s0 + i * kThreads, slots, perRow, cols);
+    u[i] = p[i].at >= 0 ? __ldcs(reinterpret_cast<const uint4*>(x + p[i].at))
+                        : make_uint4(0u, 0u, 0u, 0u);
+  }
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+    // bf16 magnitudes order like their bits, NaNs above infinity.
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top = __vmaxu2(top, w[k] & 0x7fff7fffu);
+    top = max(top >> 16, top & 0xffffu);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const uint32_t ex = int8Exponent(__uint_as_float(top << 16));
+    const Int8Inverse inv = int8Inverse(ex);
+    uint32_t o[2] = {0u, 0u};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t lo = int8Quantize(__uint_as_float(w[k] << 16), inv);
+      const uint32_t hi = int8Quantize(__uint_as_float(w[k] & 0xffff0000u), inv);
+      o[k >> 1] |= (lo | hi << 8) << ((k & 1) * 16);
+    }
+    if (p[i].at >= 0) *reinterpret_cast<uint2*>(q + p[i].at) = make_uint2(o[0], o[1]);
+    const uint32_t s = s0 + i * kThreads;
+    if ((s & 3) == 0 && s < slots) e[s >> 2] = (uint8_t)ex;
+  }
+}
+
+__global__ void __launch_bounds__(kThreads)
+    dequantizePieces(const uint8_t* __restrict__ q, const uint8_t* __restrict__ e,
+                     uint16_t* __restrict__ x, uint32_t slots, uint32_t perRow, int cols) {
+  const uint32_t s0 = blockIdx.x * (kThreads * kPieces) + threadIdx.x;
+  Piece p[kPieces];
+  uint2 u[kPieces];
+  uint32_t ex[kPieces];
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    p[i] = pieceAt(s0 + i * kThreads, slots, perRow, cols);
+    u[i] = make_uint2(0u, 0u);
+    ex[i] = 0u;
+    if (p[i].at < 0) continue;
+    u[i] = __ldcs(reinterpret_cast<const uint2*>(q + p[i].at));
+    ex[i] = __ldg(e + ((s0 + i * kThreads) >> 2));
+  }
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    if (p[i].at < 0) continue;
+    const float step = int8Step(ex[i]);
+    const uint2 a = tobf4(int8x4(u[i].x, step)), b = tobf4(int8x4(u[i].y, step));
+    *reinterpret_cast<uint4*>(x + p[i].at) = make_uint4(a.x, a.y, b.x, b.y);
+  }
+}
+
+// Whether the piece kernels take these rows, and their piece counts.
+struct PieceGrid {
+  bool fits;
+  uint32_t slots, perRow;
+  unsigned ctas;
+};
+PieceGrid pieceGrid(const void* x, const void* q, int64_t rows, int cols, int blocks) {
+  const int64_t perRow = 4 * (int64_t)blocks, slots = rows * perRow;
+  PieceGrid g{cols % 8 == 0 && slots < (1ll << 31) && (reinterpret_cast<uintptr_t>(x) & 15) == 0 &&
+                  (reinterpret_cast<uintptr_t>(q) & 7) == 0,
+              (uint32_t)slots, (uint32_t)perRow, 0};
+  g.ctas = (unsigned)((slots + kThreads * kPieces - 1) / (kThreads * kPieces));
+  return g;
+}
+
 unsigned gridFor(int64_t blocks) {
   const int64_t ctas = (blocks + kThreads / 32 - 1) / (kThreads / 32);
   return (unsigned)(ctas < kSMs * 8 ? ctas : kSMs * 8);
@@ -67,7 +161,11 @@ extern "C" int tnops_quantize_int8(const void* x, int x_f32, uint8_t* q, uint8_t
                                    int cols, cudaStream_t stream) {
   if (rows <= 0 || cols <= 0) return 1;
   const int blocks = (cols + kInt8Block - 1) / kInt8Block;
-  if (x_f32)
+  const PieceGrid g = pieceGrid(x, q, rows, cols, blocks);
+  if (!x_f32 && g.fits)
+    quantizePieces<<<g.ctas, kThreads, 0, stream>>>(static_cast<const uint16_t*>(x), q, e, g.slots,
+                                                    g.perRow, cols);
+  else if (x_f32)
     quantizeInt8<<<gridFor(rows * blocks), kThreads, 0, stream>>>(static_cast<const float*>(x), q,
                                                                  e, rows, cols, blocks);
   else
@@ -80,7 +178,11 @@ extern "C" int tnops_dequantize_int8(const uint8_t* q, const uint8_t* e, void* x
                                      int64_t rows, int cols, cudaStream_t stream) {
   if (rows <= 0 || cols <= 0) return 1;
   const int blocks = (cols + kInt8Block - 1) / kInt8Block;
-  if (x_f32)
+  const PieceGrid g = pieceGrid(x, q, rows, cols, blocks);
+  if (!x_f32 && g.fits)
+    dequantizePieces<<<g.ctas, kThreads, 0, stream>>>(q, e, static_cast<uint16_t*>(x), g.slots,
+                                                      g.perRow, cols);
+  else if (x_f32)
     dequantizeInt8<<<gridFor(rows * blocks), kThreads, 0, stream>>>(q, e, static_cast<float*>(x),
                                                                    rows, cols, blocks);
   else

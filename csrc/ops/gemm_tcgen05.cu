@@ -698,7 +698,8 @@ extern "C" int tnops_gemm_bias_act(const void* x, const void* w, const void* bia
 // MMA issuer or epilogue timed out; 4-5: a drain after that timed out), 0 if
 // none; `reset` clears it. Synchronises the device.
 extern "C" unsigned tnops_tcgen05_status(int reset) {
-  const unsigned status[3] = {readStatus(reset), linearGradsStatus(reset), linearCeStatus(reset)};
+  const unsigned status[] = {readStatus(reset), linearGradsStatus(reset), linearCeStatus(reset),
+                             geluInt8Status(reset)};
   for (unsigned v : status)
     if (v) return v;
   return 0;

@@ -28,6 +28,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // Running maximum and sum of exponentials of one row over 128 columns.
 struct StatsEpi {
+  static constexpr bool kCuts = false;
   const int64_t* target;
   float2* partial;  // [2 * tilesN][rows]: (maximum, sum of exp(l - maximum))
   float* logitOfTarget;
@@ -72,6 +73,7 @@ struct StatsEpi {
 
 // d for one piece of the vocabulary, from lse of the whole row.
 struct SoftmaxGradEpi {
+  static constexpr bool kCuts = false;
   CUtensorMap mapD;
   const int64_t* target;
   const float* lse;
@@ -220,6 +222,7 @@ extern "C" int tnops_linear_ce_fwd(const void* x, const void* w, const int64_t* 
   args.problems = 1;
   if (!logitsProblem(&args.prob[0], x, w, rows, width, 0, classes)) return 4;
   args.epi = {target, reinterpret_cast<float2*>(partial), loss, rows, classes};
+  planGemm(&args, smPairs(), false);
   if (int rc = launchPairGemm(args, stream)) return rc;
   joinStats<<<(rows + 31) / 32, kJoinWarps * 32, 0, stream>>>(
       args.epi.partial, target, loss, lse, loss, tnops_linear_ce_parts(classes), rows, classes);
@@ -236,13 +239,14 @@ extern "C" int tnops_linear_ce_mean(const float* loss, const int64_t* target, fl
 extern "C" int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* target,
                                    const float* lse, const float* grad, int grad_step,
                                    const float* share, void* d, int piece, float* dx_f32,
-                                   void* dx, void* dw, int dw_f32, int rows, int width,
+                                   void* scratch, void* dx, void* dw, int dw_f32, int rows, int width,
                                    int classes, int vocab, cudaStream_t stream) {
   if (rows <= 0 || classes <= 0 || vocab < classes || width <= 0 || width % 8 != 0 ||
       piece <= 0 || piece % 8 != 0 || !aligned16(x) || !aligned16(w) || !aligned16(d) ||
       (dx && !aligned16(dx)) || (dw && !aligned16(dw)))
     return 1;
   const bool whole = classes <= piece;
+  if (scratch == nullptr || !aligned16(scratch)) return 1;
   if (dx && !whole && (dx_f32 == nullptr || !aligned16(dx_f32))) return 1;
   const size_t dwSize = dw_f32 ? 4 : 2;
   if (dw && vocab > classes) {
@@ -267,8 +271,10 @@ extern "C" int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* 
     e.classes = classes;
     e.first = first;
     e.width = n;
+    planGemm(&args, smPairs(), false);
     if (int rc = launchPairGemm(args, stream)) return rc;
     LinearGrads g{};
+    g.scratch = scratch;
     g.g = d;
     g.ldg = piece;
     g.w = static_cast<const uint16_t*>(w) + (size_t)first * width;

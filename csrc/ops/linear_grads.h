@@ -21,14 +21,17 @@ struct LinearGrads {
   const void* x;
   void* dx;
   void* dw;
+  void* scratch;  // tnops_linear_grads_scratch() bytes, 16-byte aligned
   GradStore dxStore, dwStore;
   int rows, outs, ins;
 };
 
 int linearGrads(const LinearGrads& a, cudaStream_t stream);
 
-// First failure code of the kernels of linear_grads.cu / linear_ce.cu.
+// First failure code of the tensor-core kernels of linear_grads.cu,
+// linear_ce.cu and gelu_int8.cu.
 unsigned linearGradsStatus(int reset);
 unsigned linearCeStatus(int reset);
+unsigned geluInt8Status(int reset);
 
 }  // namespace tnops

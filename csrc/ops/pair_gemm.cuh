@@ -20,11 +20,12 @@
 // each CTA of a pair stages 128 rows of A and of B per 64-wide K block in a
 // six-stage ring, the even CTA issues the MMAs, two accumulators of 256 TMEM
 // columns let the epilogue of a tile run under the next tile's main loop.
-// A launch may hold two products (`GemmProblem`): their tiles share one queue,
-// so that dX and dW of a layer fill the GPU together. Every wait is bounded as
-// there; the first failure is kept in the file's status word.
+// A launch may hold two products (`GemmProblem`), so that dX and dW of a layer
+// fill the GPU together; who computes what is pair_schedule.h's. Every wait is
+// bounded as there; the first failure is kept in the file's status word.
 #pragma once
 
+#include "pair_schedule.h"
 #include "tcgen05.cuh"
 
 namespace tnops {
@@ -46,7 +47,9 @@ struct alignas(64) GemmProblem {
 template <class Epi>
 struct alignas(64) PairGemmArgs {
   GemmProblem prob[2];
+  CUtensorMap mapPartial;  // [2 * pairs * 256, 256] fp32, for an Epi that kCuts
   int problems;
+  PairSchedule schedule;
   Epi epi;
 };
 
@@ -85,163 +88,6 @@ __device__ __forceinline__ void loadHalf(uint32_t dst, const CUtensorMap* map, i
     tmaLoadPair(dst + kHalf / 2, map, mn0 + 64, k0, leaderBar);
   } else {
     tmaLoadPair(dst, map, k0, mn0, leaderBar);
-  }
-}
-
-// Epi: `State begin(problem, row, tileN, half)` once per tile and thread (the
-// thread's row of the output), `chunk(state, v, problem, lane, row0, col0,
-// buf)` for each 32 x 32 block of a warp (v: the row's 32 columns from col0;
-// buf: the warp's 4 KiB of staging), `end(state, ...)` after the last block.
-template <class Epi>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    pairGemmKernel(const __grid_constant__ PairGemmArgs<Epi> args) {
-  __shared__ __align__(8) uint64_t sFull[kPairStages];
-  __shared__ __align__(8) uint64_t sEmpty[kPairStages];
-  __shared__ __align__(8) uint64_t sAccFull[2];
-  __shared__ __align__(8) uint64_t sAccEmpty[2];
-  __shared__ __align__(8) uint64_t sDone;
-  __shared__ uint32_t sTmem;
-  __shared__ int sAbort;
-  extern __shared__ uint8_t dsmem[];
-  const uint32_t base = (smemAddr(dsmem) + 1023u) & ~1023u;
-  const uint32_t stageA0 = base, stageB0 = base + kPairStages * kHalf;
-  const uint32_t epi0 = base + kPairStages * 2 * kHalf;
-
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = clusterRank();
-  const int pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
-  const int tiles0 = args.prob[0].tilesM * args.prob[0].tilesN;
-  const int tiles =
-      tiles0 + (args.problems > 1 ? args.prob[1].tilesM * args.prob[1].tilesN : 0);
-  volatile int* abort = &sAbort;
-
-  if (threadIdx.x == 0) {
-    sAbort = 0;
-    for (int s = 0; s < kPairStages; ++s) {
-      mbarInit(&sFull[s], 1);
-      mbarInit(&sEmpty[s], 1);
-    }
-    for (int b = 0; b < 2; ++b) {
-      mbarInit(&sAccFull[b], 1);
-      mbarInit(&sAccEmpty[b], 2 * kEpiWarps);
-    }
-    mbarInit(&sDone, 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smemAddr(&sTmem)),
-                 "r"(2 * kTmemCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-  }
-  fenceBeforeSync();
-  __syncthreads();
-  clusterSync();  // barriers initialised and TMEM allocated in both CTAs
-  fenceAfterSync();
-  const uint32_t tmem = sTmem;
-
-  if (warp == 0 && lane == 0) {
-    // Producer (both CTAs): this CTA's halves of A and B.
-    uint32_t g = 0;
-    for (int t = pair; t < tiles && !*abort; t += pairs) {
-      const int which = t >= tiles0;
-      const GemmProblem& p = args.prob[which];
-      const int tt = which ? t - tiles0 : t;
-      const int m0 = (tt / p.tilesN) * kPairBM + (int)rank * 128;
-      const int n0 = (tt % p.tilesN) * 256 + (int)rank * 128;
-      const int kBlocks = p.kBlocks, aMn = p.aMn, bMn = p.bMn;
-      for (int kb = 0; kb < kBlocks; ++kb, ++g) {
-        const uint32_t s = g % kPairStages, round = g / kPairStages;
-        if (!mbarWait(&sEmpty[s], (round & 1u) ^ 1u, abort, 1)) break;
-        if (rank == 0) mbarExpectTx(&sFull[s], 4 * kHalf);  // both CTAs' A and B halves
-        const uint32_t bar = inLeader(&sFull[s]);
-        loadHalf(stageA0 + s * kHalf, &p.mapA, aMn, m0, kb * kBK, bar);
-        loadHalf(stageB0 + s * kHalf, &p.mapB, bMn, n0, kb * kBK, bar);
-      }
-    }
-    if (*abort) {
-      if (rank == 0) {
-        for (uint32_t q = g > (uint32_t)kPairStages ? g - kPairStages : 0; q < g; ++q)
-          mbarWait(&sFull[q % kPairStages], (q / kPairStages) & 1u, abort, 4, true);
-      } else {
-        // This CTA's loads complete on the even CTA's barriers: let them land.
-        const uint64_t t0 = globalTimer();
-        while (globalTimer() - t0 < 200000ull) {
-        }
-      }
-    }
-  } else if (warp == 1 && lane == 0 && rank == 0) {
-    // MMA issuer (even CTA only).
-    uint32_t g = 0, local = 0;
-    for (int t = pair; t < tiles && !*abort; t += pairs, ++local) {
-      const GemmProblem& p = args.prob[t >= tiles0];
-      const int kBlocks = p.kBlocks;
-      const uint64_t descA = pairDescBase(p.aMn), descB = pairDescBase(p.bMn);
-      const uint32_t stepA = p.aMn ? 2048 : 32, stepB = p.bMn ? 2048 : 32;
-      const uint32_t instr = pairInstrDesc(p.aMn, p.bMn);
-      const uint32_t b = local & 1u, use = local >> 1;
-      if (!mbarWait(&sAccEmpty[b], (use & 1u) ^ 1u, abort, 2)) break;
-      fenceAfterSync();
-      const uint32_t acc = tmem + b * kTmemCols;
-      bool ok = true;
-      for (int kb = 0; kb < kBlocks; ++kb, ++g) {
-        const uint32_t s = g % kPairStages;
-        if (!(ok = mbarWait(&sFull[s], (g / kPairStages) & 1u, abort, 2))) break;
-        fenceAfterSync();
-        const uint32_t a = stageA0 + s * kHalf, bb = stageB0 + s * kHalf;
-#pragma unroll
-        for (int k = 0; k < kBK / 16; ++k)
-          pairMma(acc, pairDesc(descA, a + k * stepA), pairDesc(descB, bb + k * stepB), instr,
-                  (kb | k) != 0 ? 1u : 0u);
-        commitPair(&sEmpty[s]);
-      }
-      if (!ok) break;
-      commitPair(&sAccFull[b]);
-    }
-    commitPairLocal(&sDone);
-    if (*abort) mbarWait(&sDone, 0, abort, 5, true);
-  } else if (warp >= 2) {
-    // Epilogue (both CTAs): this CTA's 128 rows of the tile; TMEM lane
-    // quarter warp % 4, column half (warp - 2) / 4.
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    const uint32_t buf = epi0 + (uint32_t)(warp - 2) * kEpiBuf;
-    uint32_t local = 0;
-    for (int t = pair; t < tiles; t += pairs, ++local) {
-      const uint32_t b = local & 1u, use = local >> 1;
-      const int which = t >= tiles0;
-      const GemmProblem& p = args.prob[which];
-      const int tt = which ? t - tiles0 : t, tileN = tt % p.tilesN;
-      const int row0 = (tt / p.tilesN) * kPairBM + (int)rank * 128 + quarter * 32;
-      typename Epi::State st = args.epi.begin(which, row0 + lane);
-      const bool ready = mbarWait(&sAccFull[b], use & 1u, abort, 3);
-      if (!__all_sync(0xffffffffu, ready)) break;
-      fenceAfterSync();
-      const uint32_t acc = tmem + b * kTmemCols + ((uint32_t)(quarter * 32) << 16);
-#pragma unroll 1
-      for (int c = half * 128; c < half * 128 + 128; c += 32) {
-        float v[32];
-        tmemLoad32(acc + (uint32_t)c, v);
-        if (c + 32 == half * 128 + 128) {
-          // Last read of this buffer: hand it back before the stores.
-          fenceBeforeSync();
-          __syncwarp();
-          if (lane == 0) mbarArriveRemote(inLeader(&sAccEmpty[b]));
-        }
-        args.epi.chunk(st, v, which, lane, row0, tileN * 256 + c, buf);
-      }
-      args.epi.end(st, row0 + lane, tileN * 2 + half);
-    }
-    epilogueDrain(lane);
-  }
-  fenceBeforeSync();
-  __syncthreads();
-  clusterSync();  // neither CTA leaves while the pair's MMAs or arrivals can reach it
-  if (warp == 1) {
-    fenceAfterSync();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                 "r"(2 * kTmemCols)
-                 : "memory");
   }
 }
 
@@ -302,6 +148,172 @@ __device__ __forceinline__ void storeF32(const float (&v)[32], int lane, uint32_
   }
 }
 
+// Epi: `State begin(problem, row)` once per tile and thread (the thread's row
+// of the output), `chunk(state, v, problem, lane, row0, col0, buf)` for each
+// 32 x 32 block of a warp (v: the row's 32 columns from col0; buf: the warp's
+// 4 KiB of staging), `end(state, row, part)` after the last block (part: the
+// 128 columns' number). With Epi::kCuts, parts of cut tiles go to mapPartial
+// instead.
+template <class Epi>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    pairGemmKernel(const __grid_constant__ PairGemmArgs<Epi> args) {
+  __shared__ __align__(8) uint64_t sFull[kPairStages];
+  __shared__ __align__(8) uint64_t sEmpty[kPairStages];
+  __shared__ __align__(8) uint64_t sAccFull[2];
+  __shared__ __align__(8) uint64_t sAccEmpty[2];
+  __shared__ __align__(8) uint64_t sDone;
+  __shared__ uint32_t sTmem;
+  __shared__ int sAbort;
+  extern __shared__ uint8_t dsmem[];
+  const uint32_t base = (smemAddr(dsmem) + 1023u) & ~1023u;
+  const uint32_t stageA0 = base, stageB0 = base + kPairStages * kHalf;
+  const uint32_t epi0 = base + kPairStages * 2 * kHalf;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = clusterRank();
+  const int pair = (int)(blockIdx.x >> 1);
+  const PairSchedule& schedule = args.schedule;
+  volatile int* abort = &sAbort;
+
+  if (threadIdx.x == 0) {
+    sAbort = 0;
+    for (int s = 0; s < kPairStages; ++s) {
+      mbarInit(&sFull[s], 1);
+      mbarInit(&sEmpty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbarInit(&sAccFull[b], 1);
+      mbarInit(&sAccEmpty[b], 2 * kEpiWarps);
+    }
+    mbarInit(&sDone, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smemAddr(&sTmem)),
+                 "r"(2 * kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  fenceBeforeSync();
+  __syncthreads();
+  clusterSync();  // barriers initialised and TMEM allocated in both CTAs
+  fenceAfterSync();
+  const uint32_t tmem = sTmem;
+
+  if (warp == 0 && lane == 0) {
+    // Producer (both CTAs): this CTA's halves of A and B.
+    uint32_t g = 0;
+    PairWalk walk;
+    PairWork w;
+    walk.init(schedule, pair);
+    while (!*abort && walk.next(schedule, &w)) {
+      const GemmProblem& p = args.prob[w.which];
+      const int m0 = (w.tile / p.tilesN) * kPairBM + (int)rank * 128;
+      const int n0 = (w.tile % p.tilesN) * 256 + (int)rank * 128;
+      const int aMn = p.aMn, bMn = p.bMn;
+      for (int kb = w.kb0; kb < w.kb1; ++kb, ++g) {
+        const uint32_t s = g % kPairStages, round = g / kPairStages;
+        if (!mbarWait(&sEmpty[s], (round & 1u) ^ 1u, abort, 1)) break;
+        if (rank == 0) mbarExpectTx(&sFull[s], 4 * kHalf);  // both CTAs' A and B halves
+        const uint32_t bar = inLeader(&sFull[s]);
+        loadHalf(stageA0 + s * kHalf, &p.mapA, aMn, m0, kb * kBK, bar);
+        loadHalf(stageB0 + s * kHalf, &p.mapB, bMn, n0, kb * kBK, bar);
+      }
+    }
+    if (*abort) {
+      if (rank == 0) {
+        for (uint32_t q = g > (uint32_t)kPairStages ? g - kPairStages : 0; q < g; ++q)
+          mbarWait(&sFull[q % kPairStages], (q / kPairStages) & 1u, abort, 4, true);
+      } else {
+        // This CTA's loads complete on the even CTA's barriers: let them land.
+        const uint64_t t0 = globalTimer();
+        while (globalTimer() - t0 < 200000ull) {
+        }
+      }
+    }
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    // MMA issuer (even CTA only).
+    uint32_t g = 0, local = 0;
+    PairWalk walk;
+    PairWork w;
+    walk.init(schedule, pair);
+    for (; !*abort && walk.next(schedule, &w); ++local) {
+      const GemmProblem& p = args.prob[w.which];
+      const uint64_t descA = pairDescBase(p.aMn), descB = pairDescBase(p.bMn);
+      const uint32_t stepA = p.aMn ? 2048 : 32, stepB = p.bMn ? 2048 : 32;
+      const uint32_t instr = pairInstrDesc(p.aMn, p.bMn);
+      const uint32_t b = local & 1u, use = local >> 1;
+      if (!mbarWait(&sAccEmpty[b], (use & 1u) ^ 1u, abort, 2)) break;
+      fenceAfterSync();
+      const uint32_t acc = tmem + b * kTmemCols;
+      bool ok = true;
+      for (int kb = w.kb0; kb < w.kb1; ++kb, ++g) {
+        const uint32_t s = g % kPairStages;
+        if (!(ok = mbarWait(&sFull[s], (g / kPairStages) & 1u, abort, 2))) break;
+        fenceAfterSync();
+        const uint32_t a = stageA0 + s * kHalf, bb = stageB0 + s * kHalf;
+#pragma unroll
+        for (int k = 0; k < kBK / 16; ++k)
+          pairMma(acc, pairDesc(descA, a + k * stepA), pairDesc(descB, bb + k * stepB), instr,
+                  kb != w.kb0 || k != 0 ? 1u : 0u);
+        commitPair(&sEmpty[s]);
+      }
+      if (!ok) break;
+      commitPair(&sAccFull[b]);
+    }
+    commitPairLocal(&sDone);
+    if (*abort) mbarWait(&sDone, 0, abort, 5, true);
+  } else if (warp >= 2) {
+    // Epilogue (both CTAs): this CTA's 128 rows of the tile; TMEM lane
+    // quarter warp % 4, column half (warp - 2) / 4.
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t buf = epi0 + (uint32_t)(warp - 2) * kEpiBuf;
+    uint32_t local = 0;
+    PairWalk walk;
+    PairWork w;
+    walk.init(schedule, pair);
+    for (; walk.next(schedule, &w); ++local) {
+      const uint32_t b = local & 1u, use = local >> 1;
+      const GemmProblem& p = args.prob[w.which];
+      const int tileN = w.tile % p.tilesN;
+      const int row0 = (w.tile / p.tilesN) * kPairBM + (int)rank * 128 + quarter * 32;
+      typename Epi::State st = args.epi.begin(w.which, row0 + lane);
+      const bool ready = mbarWait(&sAccFull[b], use & 1u, abort, 3);
+      if (!__all_sync(0xffffffffu, ready)) break;
+      fenceAfterSync();
+      const uint32_t acc = tmem + b * kTmemCols + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
+      for (int c = half * 128; c < half * 128 + 128; c += 32) {
+        float v[32];
+        tmemLoad32(acc + (uint32_t)c, v);
+        if (c + 32 == half * 128 + 128) {
+          // Last read of this buffer: hand it back before the stores.
+          fenceBeforeSync();
+          __syncwarp();
+          if (lane == 0) mbarArriveRemote(inLeader(&sAccEmpty[b]));
+        }
+        if (Epi::kCuts && w.slot >= 0)
+          storeF32(v, lane, buf, &args.mapPartial,
+                   (2 * pair + w.slot) * kPairBM + (int)rank * 128 + quarter * 32, c, true, false);
+        else
+          args.epi.chunk(st, v, w.which, lane, row0, tileN * 256 + c, buf);
+      }
+      args.epi.end(st, row0 + lane, tileN * 2 + half);
+    }
+    epilogueDrain(lane);
+  }
+  fenceBeforeSync();
+  __syncthreads();
+  clusterSync();  // neither CTA leaves while the pair's MMAs or arrivals can reach it
+  if (warp == 1) {
+    fenceAfterSync();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(2 * kTmemCols)
+                 : "memory");
+  }
+}
+
 // -- host side -------------------------------------------------------------------
 
 inline bool encode2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t rows,
@@ -335,29 +347,58 @@ inline bool f32OutMap(CUtensorMap* map, const void* base, int64_t rows, int64_t 
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE);
 }
 
-// Launches the products of `args` on every SM pair. Returns 0, or a non-zero
-// code without a launch.
+// SM pairs of the current device (0 on failure), counted once per device.
+inline int smPairs() {
+  static std::atomic<int> known[64];
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 0;
+  if (int n = known[dev].load(std::memory_order_relaxed)) return n;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  known[dev].store(sms / 2, std::memory_order_relaxed);
+  return sms / 2;
+}
+
+// Tile counts and sums of the launch for `pairs` pairs, cut or not.
+template <class Epi>
+void planGemm(PairGemmArgs<Epi>* args, int pairs, bool cut) {
+  PairSchedule& s = args->schedule;
+  s = {};
+  s.pairs = pairs;
+  for (int i = 0; i < 2; ++i) {
+    s.k[i] = 1;
+    if (i >= args->problems) continue;
+    s.tiles[i] = args->prob[i].tilesM * args->prob[i].tilesN;
+    s.k[i] = args->prob[i].kBlocks;
+  }
+  if (cut) {
+    planPairs(&s);
+  } else {
+    s.whole[0] = s.tiles[0];
+    s.whole[1] = s.tiles[1];
+  }
+}
+
+// Launches the products of `args`, whose schedule is planned. Returns 0, or a
+// non-zero code without a launch.
 template <class Epi>
 int launchPairGemm(const PairGemmArgs<Epi>& args, cudaStream_t stream) {
   auto kernel = pairGemmKernel<Epi>;
   // Opt in to the shared memory once per device (bit d of `done`).
   static std::atomic<uint64_t> done{0};
-  static int sms[64] = {};
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 3;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64 || args.schedule.pairs <= 0) return 3;
   const uint64_t bit = 1ull << dev;
   if (!(done.load(std::memory_order_acquire) & bit)) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)kPairSmemBytes) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+                             (int)kPairSmemBytes) != cudaSuccess)
       return 3;
     done.fetch_or(bit, std::memory_order_acq_rel);
   }
-  int tiles = 0;
-  for (int i = 0; i < args.problems; ++i) tiles += args.prob[i].tilesM * args.prob[i].tilesN;
-  const int pairs = sms[dev] > 1 ? sms[dev] / 2 : 74;
-  const unsigned grid = 2u * (unsigned)(tiles < pairs ? tiles : pairs);
-  kernel<<<grid, kThreads, kPairSmemBytes, stream>>>(args);
+  const PairSchedule& s = args.schedule;
+  const int tiles = s.tiles[0] + s.tiles[1];
+  // Without a rest the pairs past the last tile have nothing to do.
+  const int pairs = s.restBlocks() > 0 || tiles > s.pairs ? s.pairs : tiles;
+  kernel<<<2u * (unsigned)pairs, kThreads, kPairSmemBytes, stream>>>(args);
   return launched(cudaGetLastError());
 }
 

@@ -103,9 +103,13 @@ int tnops_gemm_bias_act(const void* x, const void* w, const void* bias, void* pr
 // g w and dw [outs, ins] (fp32 with dw_f32, else bf16) = g^T x, for g
 // [rows, outs] with rows ldg elements apart, w [outs, ins], x [rows, ins],
 // all bf16. A null dx or dw is left out. ins % 8 == 0, ldg % 8 == 0, 16-byte
-// aligned pointers; 1 (invalid argument) without a launch otherwise.
+// aligned pointers; 1 (invalid argument) without a launch otherwise. scratch:
+// tnops_linear_grads_scratch() bytes (partial sums of tiles that several SM
+// pairs share).
+size_t tnops_linear_grads_scratch(void);
 int tnops_linear_grads(const void* g, int64_t ldg, const void* w, const void* x, void* dx,
-                       void* dw, int dw_f32, int rows, int outs, int ins, cudaStream_t stream);
+                       void* dw, int dw_f32, int rows, int outs, int ins, void* scratch,
+                       cudaStream_t stream);
 
 // Softmax cross-entropy of l = x w^T without the logits in memory: x
 // [rows, width], w [vocab, width] in bf16, of which the first `classes` rows
@@ -119,8 +123,9 @@ int tnops_linear_grads(const void* g, int64_t ldg, const void* w, const void* x,
 //  * bwd: dx [rows, width] (bf16) and dw [vocab, width] (fp32 with dw_f32, else
 //    bf16; rows from `classes` on are zero) of sum_r k[r] loss[r], with k[r] =
 //    grad[r * grad_step] (* *share). Works on `piece` classes at a time
-//    (piece % 8 == 0); d holds rows * piece bf16 of scratch, and dx_f32
-//    rows * width floats when piece < classes. A null dx or dw is left out.
+//    (piece % 8 == 0); d holds rows * piece bf16 of scratch, dx_f32
+//    rows * width floats when piece < classes, and scratch
+//    tnops_linear_grads_scratch() bytes. A null dx or dw is left out.
 int tnops_linear_ce_parts(int classes);
 int tnops_linear_ce_fwd(const void* x, const void* w, const int64_t* target, float* loss,
                         float* lse, float* partial, int rows, int width, int classes,
@@ -129,7 +134,7 @@ int tnops_linear_ce_mean(const float* loss, const int64_t* target, float* out2, 
                          int classes, int mean, cudaStream_t stream);
 int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* target, const float* lse,
                         const float* grad, int grad_step, const float* share, void* d, int piece,
-                        float* dx_f32, void* dx, void* dw, int dw_f32, int rows, int width,
+                        float* dx_f32, void* scratch, void* dx, void* dw, int dw_f32, int rows, int width,
                         int classes, int vocab, cudaStream_t stream);
 
 // Token and position embedding: y[r] = scale * w[token[r]] + p[position[r]]
@@ -139,12 +144,18 @@ int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* target, con
 int tnops_embedding_fwd(const int64_t* token, const int64_t* position, const void* w,
                         const void* p, int w_f32, void* y, int y_f32, int64_t rows, int seq,
                         int vocab, int context, int cols, float scale, cudaStream_t stream);
-// Gradient of a table: dw[v] = scale * sum of g[r] over the rows with
-// token[r] = v, in row order, for every v (rows without a token: zero). A null
-// `token` stands for r % seq.
-int tnops_embedding_grad(const void* g, int g_f32, const int64_t* token, int seq, void* dw,
-                         int dw_f32, int64_t rows, int vocab, int cols, float scale,
-                         cudaStream_t stream);
+// Gradients of the tables for g [rows, cols] (fp32 with g_f32, else bf16), dw
+// and dp of one type (fp32 with d_f32, else bf16); a null dw or dp is left
+// out. dw[v] = scale * the sum of g[r] over the rows with token[r] = v, for
+// every v (rows without a token: zero); dp alike over positions, without the
+// scale (a null `position` stands for r % seq; rows must then be a multiple of
+// seq). Bit-identical from run to run. scratch: 16-byte aligned,
+// tnops_embedding_grad_scratch(rows, cols, 1 or 2 tables) bytes. Returns 1
+// (invalid argument) without a launch for anything else.
+size_t tnops_embedding_grad_scratch(int64_t rows, int cols, int tables);
+int tnops_embedding_grad(const void* g, int g_f32, const int64_t* token, void* dw, int vocab,
+                         float scale, const int64_t* position, int seq, void* dp, int context,
+                         int d_f32, int64_t rows, int cols, void* scratch, cudaStream_t stream);
 
 // x [rows, cols] (fp32 with x_f32, else bf16) in 8-bit blocks: q [rows, cols]
 // signed bytes and one exponent byte per 32 neighbours of a row, e
@@ -154,6 +165,14 @@ int tnops_quantize_int8(const void* x, int x_f32, uint8_t* q, uint8_t* e, int64_
                         cudaStream_t stream);
 int tnops_dequantize_int8(const uint8_t* q, const uint8_t* e, void* x, int x_f32, int64_t rows,
                           int cols, cudaStream_t stream);
+
+// act [rows, outs] (bf16) = gelu_tanh(bf16(x w^T + bias)) for x [rows, ins],
+// w [outs, ins], bias [outs] in bf16, and the sums before the GELU in 8-bit
+// blocks (rounded from fp32). ins, outs % 8 == 0, x, w, bias, act 16-byte,
+// pre_q 8-byte, pre_e 4-byte aligned; 1 (invalid argument) otherwise.
+int tnops_linear_gelu_int8(const void* x, const void* w, const void* bias, void* act,
+                           uint8_t* pre_q, uint8_t* pre_e, int rows, int outs, int ins,
+                           cudaStream_t stream);
 
 // First failure code recorded by a tcgen05 kernel (a bounded wait that expired),
 // 0 if none; `reset` clears it. Synchronises the device.

@@ -45,6 +45,10 @@ int asInt(int64_t n, const char* what) {
 
 void ok(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed (code ", rc, ")"); }
 
+at::Tensor gradsScratch(const at::Tensor& like) {
+  return at::empty({(int64_t)tnops_linear_grads_scratch()}, like.options().dtype(at::kByte));
+}
+
 uint8_t* bytes(const at::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
 
 // -- embedding -----------------------------------------------------------------
@@ -80,32 +84,49 @@ at::Tensor embeddingFwd(const at::Tensor& token, const Opt& position, const at::
   return y;
 }
 
-// grad [rows, width]; token [rows], or none for row % seq -> the gradient of a
-// [vocab, width] table.
-at::Tensor embeddingGrad(const at::Tensor& grad, const Opt& token, int64_t seq, int64_t vocab,
-                         double scale, bool outF32, const Opt& out) {
+// grad [rows, width]; token and position (or none for row % seq) [rows] -> the
+// gradients of the [vocab, width] and [context, width] tables; one with no
+// rows (vocab or context 0) is left out.
+std::vector<at::Tensor> embeddingGrad(const at::Tensor& grad, const at::Tensor& token,
+                                      const Opt& position, int64_t seq, int64_t vocab,
+                                      int64_t context, double scale, bool outF32, const Opt& dwOut,
+                                      const Opt& dpOut) {
   need(grad, "grad");
   TORCH_CHECK(grad.dim() == 2, "embedding_grad: want grad [rows, width]");
   const int gF32 = f32(grad, "grad");
-  if (token) {
-    need(*token, at::kLong, "idx");
-    TORCH_CHECK(token->numel() == grad.size(0), "embedding_grad: one token per row of grad");
-    sameDevice(grad, *token, "idx");
+  const int64_t rows = grad.size(0), width = grad.size(1);
+  for (const at::Tensor* t : {&token, position ? &*position : nullptr}) {
+    if (t == nullptr) continue;
+    need(*t, at::kLong, "an index");
+    TORCH_CHECK(t->numel() == rows, "embedding_grad: one index per row of grad");
+    sameDevice(grad, *t, "an index");
   }
+  TORCH_CHECK(seq > 0 ? rows % seq == 0 : rows == 0, "embedding_grad: rows must be whole sequences");
   c10::cuda::CUDAGuard g(grad.device());
-  const auto st = outF32 ? at::kFloat : at::kBFloat16;
-  auto dw = out ? *out : at::empty({vocab, grad.size(1)}, grad.options().dtype(st));
-  need(dw, st, "out");
-  TORCH_CHECK(dw.numel() == vocab * grad.size(1), "embedding_grad: out has the wrong size");
-  sameDevice(grad, dw, "out");
-  if (dw.numel() == 0) return dw;
-  if (grad.size(0) == 0) return dw.zero_();
-  ok(tnops_embedding_grad(grad.data_ptr(), gF32, token ? token->data_ptr<int64_t>() : nullptr,
-                          asInt(seq, "sequence length"), dw.data_ptr(), outF32 ? 1 : 0,
-                          grad.size(0), asInt(vocab, "vocabulary"), asInt(grad.size(1), "width"),
-                          (float)scale, streamOf(grad)),
+  const auto opt = grad.options().dtype(outF32 ? at::kFloat : at::kBFloat16);
+  auto table = [&](int64_t n, const Opt& out) {
+    if (n == 0) return at::Tensor();
+    auto d = out ? *out : at::empty({n, width}, opt);
+    need(d, outF32 ? at::kFloat : at::kBFloat16, "out");
+    TORCH_CHECK(d.numel() == n * width, "embedding_grad: out has the wrong size");
+    sameDevice(grad, d, "out");
+    if (rows == 0) d.zero_();
+    return d;
+  };
+  auto dw = table(vocab, dwOut), dp = table(context, dpOut);
+  if (rows == 0 || width == 0 || (vocab == 0 && context == 0)) return {dw, dp};
+  const int cols = asInt(width, "width");
+  auto scratch = at::empty(
+      {(int64_t)tnops_embedding_grad_scratch(rows, cols, (vocab > 0) + (context > 0))},
+      grad.options().dtype(at::kByte));
+  ok(tnops_embedding_grad(grad.data_ptr(), gF32, token.data_ptr<int64_t>(),
+                          dw.defined() ? dw.data_ptr() : nullptr, asInt(vocab, "vocabulary"),
+                          (float)scale, position ? position->data_ptr<int64_t>() : nullptr,
+                          asInt(seq, "sequence length"), dp.defined() ? dp.data_ptr() : nullptr,
+                          asInt(context, "context"), outF32 ? 1 : 0, rows, cols,
+                          scratch.data_ptr(), streamOf(grad)),
      "tnops_embedding_grad");
-  return dw;
+  return {dw, dp};
 }
 
 // -- linear cross-entropy --------------------------------------------------------
@@ -190,6 +211,7 @@ std::vector<at::Tensor> linearCeBwd(const at::Tensor& x, const at::Tensor& w,
   if (s.rows == 0 || (!wantDx && !wantDw)) return {dx, dw};
   const int64_t piece = cePiece(s.rows, s.classes, budget);
   auto d = at::empty({(int64_t)s.rows, piece}, x.options());
+  auto scratch = gradsScratch(x);
   at::Tensor dxF32;
   if (wantDx && piece < s.classes) dxF32 = at::empty(x.sizes(), x.options().dtype(at::kFloat));
   ok(tnops_linear_ce_bwd(x.data_ptr(), w.data_ptr(), target.data_ptr<int64_t>(),
@@ -197,7 +219,7 @@ std::vector<at::Tensor> linearCeBwd(const at::Tensor& x, const at::Tensor& w,
                          grad.numel() == 1 ? 0 : 1, share ? share->data_ptr<float>() : nullptr,
                          d.data_ptr(), (int)piece,
                          dxF32.defined() ? dxF32.data_ptr<float>() : nullptr,
-                         wantDx ? dx.data_ptr() : nullptr, wantDw ? dw.data_ptr() : nullptr,
+                         scratch.data_ptr(), wantDx ? dx.data_ptr() : nullptr, wantDw ? dw.data_ptr() : nullptr,
                          dwF32 ? 1 : 0, s.rows, s.width, s.classes, s.vocab, streamOf(x)),
      "tnops_linear_ce_bwd");
   return {dx, dw};
@@ -239,6 +261,31 @@ at::Tensor dequantizeInt8(const at::Tensor& q, const at::Tensor& e, bool outF32)
                            asInt(q.size(1), "columns"), streamOf(q)),
      "tnops_dequantize_int8");
   return x;
+}
+
+// x bf16 [rows, ins], w bf16 [outs, ins], bias bf16 [outs] -> (act bf16, and
+// the sums before the GELU in 8-bit blocks)
+std::vector<at::Tensor> linearGeluInt8(const at::Tensor& x, const at::Tensor& w,
+                                       const at::Tensor& bias) {
+  need(x, at::kBFloat16, "x");
+  need(w, at::kBFloat16, "weight");
+  need(bias, at::kBFloat16, "bias");
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1) && bias.numel() == w.size(0),
+              "linear_gelu_int8: want x [rows, ins], weight [outs, ins], bias [outs]");
+  TORCH_CHECK(w.size(0) % 8 == 0 && w.size(1) % 8 == 0,
+              "linear_gelu_int8: the layer's sizes must be multiples of 8");
+  sameDevice(x, w, "weight");
+  sameDevice(x, bias, "bias");
+  c10::cuda::CUDAGuard g(x.device());
+  const int rows = asInt(x.size(0), "rows"), outs = asInt(w.size(0), "outputs"),
+            ins = asInt(w.size(1), "inputs");
+  auto act = at::empty({rows, outs}, x.options());
+  auto q = at::empty({rows, outs}, x.options().dtype(at::kChar));
+  auto e = at::empty({rows, (outs + 31) / 32}, x.options().dtype(at::kByte));
+  ok(tnops_linear_gelu_int8(x.data_ptr(), w.data_ptr(), bias.data_ptr(), act.data_ptr(), bytes(q),
+                            bytes(e), rows, outs, ins, streamOf(x)),
+     "tnops_linear_gelu_int8");
+  return {act, q, e};
 }
 
 // gy bf16 [M, N], pre in 8-bit blocks -> (gpre bf16 [M, N], db fp32 [N])
@@ -290,9 +337,10 @@ std::vector<at::Tensor> linearGradsInt8(const at::Tensor& grad, const at::Tensor
   }
   at::Tensor x;
   if (wantDw) x = dequantizeInt8(q, e, false);
+  auto scratch = gradsScratch(grad);
   ok(tnops_linear_grads(grad.data_ptr(), outs, w.data_ptr(), wantDw ? x.data_ptr() : nullptr,
                         wantDx ? dx.data_ptr() : nullptr, wantDw ? dw.data_ptr() : nullptr,
-                        dwF32 ? 1 : 0, rows, outs, ins, streamOf(grad)),
+                        dwF32 ? 1 : 0, rows, outs, ins, scratch.data_ptr(), streamOf(grad)),
      "tnops_linear_grads");
   return {dx, dw};
 }
@@ -303,8 +351,10 @@ void registerTrainOps(py::module_& ops) {
   ops.def("embedding_fwd", &embeddingFwd, py::arg("idx"), py::arg("positions"),
           py::arg("weight"), py::arg("pos_weight"), py::arg("seq"), py::arg("scale"),
           py::arg("out_f32"));
-  ops.def("embedding_grad", &embeddingGrad, py::arg("grad"), py::arg("idx"), py::arg("seq"),
-          py::arg("vocab"), py::arg("scale"), py::arg("out_f32"), py::arg("out") = py::none());
+  ops.def("embedding_grad", &embeddingGrad, py::arg("grad"), py::arg("idx"),
+          py::arg("positions"), py::arg("seq"), py::arg("vocab"), py::arg("context"),
+          py::arg("scale"), py::arg("out_f32"), py::arg("dw_out") = py::none(),
+          py::arg("dp_out") = py::none());
   ops.def("linear_ce_fwd", &linearCeFwd, py::arg("x"), py::arg("weight"), py::arg("target"),
           py::arg("classes"), py::arg("mean"));
   ops.def("linear_ce_piece", &cePiece, py::arg("rows"), py::arg("classes"), py::arg("budget"));
@@ -314,6 +364,7 @@ void registerTrainOps(py::module_& ops) {
           py::arg("dw_out") = py::none(), py::arg("budget") = 512ll << 20);
   ops.def("quantize_int8", &quantizeInt8, py::arg("x"));
   ops.def("dequantize_int8", &dequantizeInt8, py::arg("q"), py::arg("e"), py::arg("out_f32"));
+  ops.def("linear_gelu_int8", &linearGeluInt8, py::arg("x"), py::arg("weight"), py::arg("bias"));
   ops.def("gelu_bwd_bias_int8", &geluBwdBiasInt8, py::arg("grad_y"), py::arg("q"), py::arg("e"),
           py::arg("db_out") = py::none());
   ops.def("linear_grads_int8", &linearGradsInt8, py::arg("grad"), py::arg("weight"),

@@ -7,7 +7,7 @@ import os
 import pytest
 import torch
 
-from conftest import ROOT
+from conftest import ROOT, run
 
 P, I, L, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
 A = 1 << 20  # an aligned address; never dereferenced on these paths
@@ -27,21 +27,21 @@ def _refuses(f, good, bad):
 
 
 def test_linear_grads_launcher_refuses(built):
-    f = _launcher("tnops_linear_grads", P, L, P, P, P, P, I, I, I, I, P)
-    good = [A, 64, A, A, A, A, 0, 32, 64, 128, None]
+    f = _launcher("tnops_linear_grads", P, L, P, P, P, P, I, I, I, I, P, P)
+    good = [A, 64, A, A, A, A, 0, 32, 64, 128, A, None]
     _refuses(f, good, [(0, None), (0, A + 8), (1, 60), (1, 32), (2, A + 2), (2, None), (3, A + 4),
-                       (3, None), (4, A + 8), (5, A + 8), (7, 0), (8, 0), (9, 0), (9, 132)])
+                       (3, None), (4, A + 8), (5, A + 8), (7, 0), (8, 0), (9, 0), (9, 132), (10, None), (10, A + 8)])
 
 
 def test_linear_ce_launchers_refuse(built):
     f = _launcher("tnops_linear_ce_fwd", P, P, P, P, P, P, I, I, I, P)
     good = [A, A, A, A, A, A, 4, 64, 100, None]
     _refuses(f, good, [(0, A + 8), (1, A + 8), (6, 0), (7, 0), (7, 60), (8, 0)])
-    f = _launcher("tnops_linear_ce_bwd", P, P, P, P, P, I, P, P, I, P, P, P, I, I, I, I, I, P)
-    good = [A, A, A, A, A, 0, A, A, 256, A, A, A, 1, 4, 64, 300, 304, None]
+    f = _launcher("tnops_linear_ce_bwd", P, P, P, P, P, I, P, P, I, P, P, P, P, I, I, I, I, I, P)
+    good = [A, A, A, A, A, 0, A, A, 256, A, A, A, A, 1, 4, 64, 300, 304, None]
     _refuses(f, good, [(0, A + 8), (1, A + 8), (7, A + 8), (8, 0), (8, 20), (9, None),
-                       (9, A + 4), (10, A + 8), (11, A + 4), (13, 0), (14, 60), (15, 0),
-                       (16, 299)])
+                       (9, A + 4), (10, None), (10, A + 8), (11, A + 8), (12, A + 4), (14, 0),
+                       (15, 60), (16, 0), (17, 299)])
     f = _launcher("tnops_linear_ce_mean", P, P, P, I, I, I, P)
     assert f(A, A, A, 0, 5, 1, None) == 1
 
@@ -50,9 +50,20 @@ def test_embedding_launchers_refuse(built):
     f = _launcher("tnops_embedding_fwd", P, P, P, P, I, P, I, L, I, I, I, I, F, P)
     good = [A, None, A, A, 1, A, 1, 8, 4, 100, 16, 64, 1.0, None]
     _refuses(f, good, [(7, 0), (7, 1 << 31), (8, 0), (9, 0), (10, 0), (11, 0)])
-    f = _launcher("tnops_embedding_grad", P, I, P, I, P, I, L, I, I, F, P)
-    good = [A, 1, None, 4, A, 1, 8, 100, 64, 1.0, None]
-    _refuses(f, good, [(3, 0), (6, 0), (6, 1 << 31), (7, 0), (8, 0)])
+    f = _launcher("tnops_embedding_grad", P, I, P, P, I, F, P, I, P, I, I, L, I, P, P)
+    good = [A, 1, A, A, 100, 1.0, None, 4, A, 50, 1, 8, 64, A, None]
+    _refuses(f, good, [(2, None), (4, 0), (7, 0), (7, 3), (9, 0), (11, 0), (11, 1 << 31),
+                       (12, 0), (13, None), (13, A + 8)])
+    assert f(A, 1, A, None, 100, 1.0, None, 4, None, 50, 1, 8, 64, A, None) == 1
+
+
+def test_embedding_scratch_grows_with_its_parts(built):
+    f = _launcher("tnops_embedding_grad_scratch", L, I, I)
+    f.restype = ctypes.c_size_t
+    assert f(0, 64, 2) == 0 and f(1, 1, 1) % 16 == 0
+    # Sort keys and rows of 16 bytes a row, and two rows of fp32 partial sums
+    # for each 16 rows.
+    assert f(65536, 1024, 2) == 2 * (16 * 65536 + 8 * 4096 * 1024)
 
 
 def test_int8_launchers_refuse(built):
@@ -60,9 +71,20 @@ def test_int8_launchers_refuse(built):
     _refuses(f, [A, 0, A, A, 4, 64, None], [(4, 0), (5, 0)])
     f = _launcher("tnops_dequantize_int8", P, P, P, I, L, I, P)
     _refuses(f, [A, A, A, 0, 4, 64, None], [(4, 0), (5, 0)])
+    f = _launcher("tnops_linear_gelu_int8", P, P, P, P, P, P, I, I, I, P)
+    _refuses(f, [A, A, A, A, A, A, 4, 64, 64, None],
+             [(0, A + 8), (1, A + 8), (2, A + 4), (2, None), (3, A + 8), (4, A + 4), (5, A + 2),
+              (6, 0), (7, 0), (7, 60), (8, 0), (8, 60)])
     f = _launcher("tnops_gelu_bwd_bias_int8", P, P, P, P, P, P, I, I, P)
     _refuses(f, [A, A, A, A, A, A, 64, 768, None],
              [(0, A + 8), (1, A + 4), (3, A + 8), (6, 0), (7, 770)])
+
+
+def test_pair_schedule(built):
+    """Every K block of every tile belongs to one SM pair's part, and the
+    joining kernel adds exactly the parts of cut tiles that were written."""
+    r = run([os.path.join(ROOT, "build", "bin", "pair_schedule_test")], timeout=300)
+    assert r.returncode == 0 and "pair schedule ok" in r.stdout, r.stderr
 
 
 def test_python_refusals(built):

@@ -77,7 +77,10 @@ def _embedding_sums(idx, gy, vocab, scale):
     (4, 1024, 50304, 1024, 768, False, ""),
     (2, 999, 300, 1000, 77, True, "few"),   # three tokens share nearly all rows
     (5, 1024, 40, 1024, 132, False, "one"),  # one token has every row
-    (33, 2048, 70000, 2048, 36, False, ""),  # more rows than one sort chunk holds
+    (33, 2048, 70000, 2048, 36, False, ""),  # many chunks of the sort
+    (3, 700, 4200000, 700, 4, True, ""),     # 64-bit sort keys
+    (17, 1024, 1050000, 1024, 4, False, "few"),
+    (16, 4096, 11, 4096, 40, False, "one"),  # a run of thousands of blocks
 ])
 def test_embedding(ops, dtype, batch, seq, vocab, context, width, positions, repeat):
     idx, pos, w, p = _embedding_case(batch, seq, vocab, context, width, dtype, 11, positions,

@@ -186,6 +186,8 @@ PROGRAMS = {
     "gemm_pipeline_model_test": ROOT / "tests" / "cpp" / "gemm_pipeline_model_test.cc",
     # launch geometry and schedule of the row-group LayerNorm backward
     "ln_plan_test": ROOT / "tests" / "cpp" / "ln_plan_test.cc",
+    # which SM pair computes which part of the training operators' products
+    "pair_schedule_test": ROOT / "tests" / "cpp" / "pair_schedule_test.cc",
     # host configuration / partition checks, built with the library's config code
     "config_test": (ROOT / "tests" / "cpp" / "config_test.cc", TNCCL_SRC / "common.cc"),
 }

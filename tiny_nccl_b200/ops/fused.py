@@ -147,14 +147,14 @@ class _LinearBias(torch.autograd.Function):
 
     @staticmethod
     def compute(x, weight, bias):
-        """(y, the bf16 weight, nothing before an activation)"""
+        """(y, the bf16 weight)"""
         w16 = bf16_weight(weight)
         with torch.autocast("cuda", enabled=False):
-            return torch.addmm(bf16_weight(bias), x, w16.t()), w16, None
+            return torch.addmm(bf16_weight(bias), x, w16.t()), w16
 
     @staticmethod
     def forward(ctx, x, weight, bias):
-        y, w16, _ = _LinearBias.compute(x, weight, bias)
+        y, w16 = _LinearBias.compute(x, weight, bias)
         ctx.save_for_backward(x, w16)
         ctx.params = (weight, bias)
         return y
@@ -185,8 +185,7 @@ class _LinearGelu(torch.autograd.Function):
     that gradient); dX and dW on cuBLAS."""
 
     @staticmethod
-    def compute(x, weight, bias):
-        """(y, the bf16 weight, the sums before the GELU)"""
+    def forward(ctx, x, weight, bias):
         w16 = bf16_weight(weight)
         b16 = bf16_weight(bias)
         if _TCGEN05 != "0":
@@ -195,11 +194,6 @@ class _LinearGelu(torch.autograd.Function):
             with torch.autocast("cuda", enabled=False):
                 pre = torch.addmm(b16, x, w16.t())
                 y = torch.nn.functional.gelu(pre, approximate="tanh")
-        return y, w16, pre
-
-    @staticmethod
-    def forward(ctx, x, weight, bias):
-        y, w16, pre = _LinearGelu.compute(x, weight, bias)
         ctx.save_for_backward(x, w16, pre)
         ctx.params = (weight, bias)
         return y
@@ -240,14 +234,17 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 class _LinearInt8(torch.autograd.Function):
     """The linear layers above with what the backward pass needs of the
     activations kept in 8-bit blocks: x for dW, and the sums before the GELU
-    for its slope. The forward result is the same bit for bit."""
+    (rounded from fp32 in the GEMM's epilogue) for its slope."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, gelu):
-        f = _LinearGelu if gelu else _LinearBias
-        y, w16, pre = f.compute(x, weight, bias)
-        ctx.save_for_backward(w16, *_ops().quantize_int8(x),
-                              *(_ops().quantize_int8(pre) if gelu else ()))
+        if gelu:
+            w16 = bf16_weight(weight)
+            y, *pre = _ops().linear_gelu_int8(x, w16, bf16_weight(bias))
+        else:
+            y, w16 = _LinearBias.compute(x, weight, bias)
+            pre = ()
+        ctx.save_for_backward(w16, *_ops().quantize_int8(x), *pre)
         ctx.params = (weight, bias)
         return y
 
@@ -282,9 +279,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor,
     """bf16 x W^T + b over the last dimension of x (fp32 weight and bias).
 
     ``activations="int8"`` keeps x for the backward pass in 8-bit blocks
-    (:func:`quantize_int8`, half the memory): the forward result and dX stay
-    the same, dW = gy^T x is formed from the 8-bit x. Both sizes of the layer
-    must then be multiples of 8."""
+    (:func:`quantize_int8`, half the memory): the forward result stays the
+    same, dW = gy^T x is formed from the 8-bit x. Both sizes of the layer must
+    then be multiples of 8."""
     return _linear(x, weight, bias, False, activations)
 
 
@@ -298,7 +295,8 @@ def linear_gelu(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor,
                 activations: str = "bf16") -> torch.Tensor:
     """GELU(tanh)(x W^T + b) in bf16; the backward fuses the GELU gradient
     with the bias gradient. ``activations="int8"`` keeps x and the sums before
-    the GELU for the backward pass in 8-bit blocks (see :func:`linear`)."""
+    the GELU for the backward pass in 8-bit blocks (see :func:`linear`); the
+    forward then always runs on the tcgen05 GEMM."""
     return _linear(x, weight, bias, True, activations)
 
 

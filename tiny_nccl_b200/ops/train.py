@@ -35,14 +35,14 @@ class _Embedding(torch.autograd.Function):
     def backward(ctx, g):
         idx, positions = ctx.saved_tensors
         weight, pos_weight = ctx.tables
-        g = g.contiguous()
-        grads = []
-        for table, at, scale, wanted in ((weight, idx, ctx.scale, ctx.needs_input_grad[1]),
-                                         (pos_weight, positions, 1.0, ctx.needs_input_grad[2])):
-            grads.append(_ops().embedding_grad(
-                g, at, ctx.seq, table.shape[0], scale, table.dtype == torch.float32,
-                typed_destination(table, table.dtype)) if wanted else None)
-        return None, grads[0], grads[1], None, None, None, None
+        tables = (weight if ctx.needs_input_grad[1] else None,
+                  pos_weight if ctx.needs_input_grad[2] else None)
+        dw, dp = _ops().embedding_grad(
+            g.contiguous(), idx, positions, ctx.seq,
+            *(0 if t is None else t.shape[0] for t in tables), ctx.scale,
+            weight.dtype == torch.float32,
+            *(None if t is None else typed_destination(t, t.dtype) for t in tables))
+        return None, dw, dp, None, None, None, None
 
 
 def embedding(idx: torch.Tensor, weight: torch.Tensor, pos_weight: torch.Tensor | None = None,
