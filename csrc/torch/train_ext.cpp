@@ -176,6 +176,9 @@ std::vector<at::Tensor> linearCeFwd(const at::Tensor& x, const at::Tensor& w,
   return {loss, lse, out};
 }
 
+// Scratch for a piece of the logits' gradient.
+constexpr int64_t kCeBudget = 512ll << 20;
+
 // Classes per piece of the backward pass: as many whole 256-wide tiles as fit
 // the scratch budget, spread evenly.
 int64_t cePiece(int64_t rows, int64_t classes, int64_t budget) {
@@ -288,6 +291,20 @@ std::vector<at::Tensor> linearGeluInt8(const at::Tensor& x, const at::Tensor& w,
   return {act, q, e};
 }
 
+// g bf16 [M, N] -> db fp32 [N] (column sums)
+at::Tensor biasGradient(const at::Tensor& grad, const Opt& out) {
+  need(grad, at::kBFloat16, "grad");
+  TORCH_CHECK(grad.dim() == 2 && grad.size(1) % 8 == 0, "bias_grad: want [M, N] with N % 8 == 0");
+  c10::cuda::CUDAGuard g(grad.device());
+  const int M = asInt(grad.size(0), "rows"), N = asInt(grad.size(1), "columns");
+  auto db = out ? *out : at::empty({N}, grad.options().dtype(at::kFloat));
+  auto part = at::empty({(int64_t)tnops_colsum_parts(M, N) * N}, grad.options().dtype(at::kFloat));
+  ok(tnops_bias_grad(static_cast<uint16_t*>(grad.data_ptr()), db.data_ptr<float>(),
+                     part.data_ptr<float>(), M, N, streamOf(grad)),
+     "tnops_bias_grad");
+  return db;
+}
+
 // gy bf16 [M, N], pre in 8-bit blocks -> (gpre bf16 [M, N], db fp32 [N])
 std::vector<at::Tensor> geluBwdBiasInt8(const at::Tensor& gy, const at::Tensor& q,
                                         const at::Tensor& e, const Opt& dbOut) {
@@ -345,29 +362,200 @@ std::vector<at::Tensor> linearGradsInt8(const at::Tensor& grad, const at::Tensor
   return {dx, dw};
 }
 
+// -- autograd ----------------------------------------------------------------------
+//
+// The operators' autograd functions are C++: a small call's time is the host's,
+// and Python functions take several times as long on both ways.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void onceDifferentiable(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what, " cannot be differentiated twice");
+}
+
+// Where the gradient of parameter p is to be written: its slice of a flat
+// gradient buffer, when it has one (`has`) that the gradient may take now
+// (ops.fused.grad_destination, asked when the backward pass runs: it hands a
+// slice out once per pass, so that a parameter that is used twice gets two
+// gradients to add) and whose type and layout are the gradient's.
+Opt destination(const at::Tensor& p, bool has, at::ScalarType st) {
+  if (!has) return c10::nullopt;
+  py::gil_scoped_acquire gil;
+  const py::object d =
+      py::module_::import("tiny_nccl_b200.ops.fused").attr("grad_destination")(p);
+  if (d.is_none()) return c10::nullopt;
+  const auto t = d.cast<at::Tensor>();
+  if (t.scalar_type() != st || !t.is_contiguous()) return c10::nullopt;
+  return t.detach();
+}
+Opt savedOpt(AutogradContext* ctx, const char* key) {
+  const auto& v = ctx->saved_data[key];
+  return v.isNone() ? Opt() : Opt(v.toTensor());
+}
+at::Tensor bf16Copy(const at::Tensor& p, const Opt& copy) {
+  return (copy ? *copy : p.detach().to(at::kBFloat16)).contiguous();
+}
+
+struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& w, const Opt& p,
+                            const at::Tensor& idx, const Opt& positions, int64_t seq, double scale,
+                            bool outF32, bool dwDest, bool dpDest) {
+    ctx->save_for_backward({idx, positions ? *positions : at::Tensor()});
+    // The parameters themselves, for what their gradients look like: their
+    // values are not needed, so they may change before the backward pass.
+    ctx->saved_data["w"] = w;
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["seq"] = seq;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["dw"] = dwDest;
+    ctx->saved_data["dp"] = dpDest;
+    return embeddingFwd(idx, positions, w, p, seq, scale, outF32);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    onceDifferentiable("embedding");
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor w = ctx->saved_data["w"].toTensor();
+    const Opt p = savedOpt(ctx, "p");
+    const bool wantW = ctx->needs_input_grad(0), wantP = p && ctx->needs_input_grad(1);
+    const auto st = w.scalar_type();
+    const auto g = grads[0].contiguous();
+    const auto d = embeddingGrad(
+        g, saved[0], saved[1].defined() ? Opt(saved[1]) : Opt(), ctx->saved_data["seq"].toInt(),
+        wantW ? w.size(0) : 0, wantP ? p->size(0) : 0, ctx->saved_data["scale"].toDouble(),
+        st == at::kFloat, wantW ? destination(w, ctx->saved_data["dw"].toBool(), st) : Opt(),
+        wantP ? destination(*p, ctx->saved_data["dp"].toBool(), st) : Opt());
+    return {d[0], d[1], {}, {}, {}, {}, {}, {}, {}};
+  }
+};
+
+at::Tensor embedding(const at::Tensor& w, const Opt& p, const at::Tensor& idx,
+                     const Opt& positions, int64_t seq, double scale, bool outF32,
+                     bool dwDest, bool dpDest) {
+  auto flat = [](const at::Tensor& t) { return t.reshape({-1}).to(at::kLong).contiguous(); };
+  auto y = EmbeddingFn::apply(w, p, flat(idx), positions ? Opt(flat(*positions)) : Opt(), seq, scale, outF32, dwDest, dpDest);
+  auto shape = idx.sizes().vec();
+  shape.push_back(w.size(1));
+  return y.view(shape);
+}
+
+enum Reduction { kMean = 0, kSum = 1, kNone = 2 };
+
+struct LinearCeFn : torch::autograd::Function<LinearCeFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
+                            const Opt& w16, const at::Tensor& target, int64_t classes,
+                            int64_t reduction, bool dwDest) {
+    const auto wb = bf16Copy(w, w16);
+    const auto r = linearCeFwd(x, wb, target, classes, reduction == kMean);
+    ctx->save_for_backward({x, wb, target, r[1], r[2]});
+    ctx->saved_data["w"] = w;
+    ctx->saved_data["classes"] = classes;
+    ctx->saved_data["mean"] = reduction == kMean;
+    ctx->saved_data["dw"] = dwDest;
+    return reduction == kNone ? r[0] : r[2].select(0, 0);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    onceDifferentiable("linear_cross_entropy");
+    const auto s = ctx->get_saved_variables();
+    const at::Tensor w = ctx->saved_data["w"].toTensor();
+    const auto st = w.scalar_type();
+    const auto g = grads[0].reshape({-1}).to(at::kFloat).contiguous();
+    const bool wantW = ctx->needs_input_grad(1);
+    const auto d = linearCeBwd(
+        s[0], s[1], s[2], s[3], g, ctx->saved_data["mean"].toBool() ? Opt(s[4].slice(0, 1)) : Opt(),
+        ctx->saved_data["classes"].toInt(), ctx->needs_input_grad(0), wantW, st == at::kFloat,
+        wantW ? destination(w, ctx->saved_data["dw"].toBool(), st) : Opt(), kCeBudget);
+    return {d[0], d[1], {}, {}, {}, {}, {}};
+  }
+};
+
+at::Tensor linearCrossEntropy(const at::Tensor& x, const at::Tensor& w, const Opt& w16,
+                              const at::Tensor& target, int64_t classes, int64_t reduction,
+                              bool dwDest) {
+  auto loss = LinearCeFn::apply(x.reshape({-1, x.size(-1)}).to(at::kBFloat16).contiguous(), w, w16,
+                                target.reshape({-1}).contiguous(), classes, reduction, dwDest);
+  return reduction == kNone ? loss.view(target.sizes()) : loss;
+}
+
+struct LinearInt8Fn : torch::autograd::Function<LinearInt8Fn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
+                            const at::Tensor& b, const Opt& w16, const Opt& b16, bool gelu,
+                            bool dwDest, bool dbDest) {
+    const auto wb = bf16Copy(w, w16), bb = bf16Copy(b, b16);
+    at::Tensor y;
+    variable_list keep{wb};
+    if (gelu) {
+      auto r = linearGeluInt8(x, wb, bb);
+      y = r[0];
+      keep.insert(keep.end(), {r[1], r[2]});
+    } else {
+      c10::impl::ExcludeDispatchKeyGuard guard(c10::DispatchKey::AutocastCUDA);
+      y = at::addmm(bb, x, wb.t());
+    }
+    const auto q = quantizeInt8(x);
+    keep.insert(keep.end(), q.begin(), q.end());
+    ctx->save_for_backward(keep);
+    ctx->saved_data["w"] = w;
+    ctx->saved_data["b"] = b;
+    ctx->saved_data["dw"] = dwDest;
+    ctx->saved_data["db"] = dbDest;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    onceDifferentiable("a linear layer with 8-bit activations");
+    const auto s = ctx->get_saved_variables();
+    const bool gelu = s.size() == 5;
+    const at::Tensor w = ctx->saved_data["w"].toTensor(), b = ctx->saved_data["b"].toTensor();
+    auto g = grads[0].contiguous();
+    const bool wantW = ctx->needs_input_grad(1);
+    const bool wantB = ctx->needs_input_grad(2);
+    const Opt dbOut =
+        wantB ? destination(b, ctx->saved_data["db"].toBool(), at::kFloat) : Opt();
+    at::Tensor db;
+    if (gelu) {
+      auto r = geluBwdBiasInt8(g, s[1], s[2], dbOut);
+      g = r[0];
+      if (wantB) db = r[1];
+    } else if (wantB) {
+      db = biasGradient(g, dbOut);
+    }
+    const auto st = w.scalar_type() == at::kFloat ? at::kFloat : at::kBFloat16;
+    const auto d = linearGradsInt8(g, s[0], s[s.size() - 2], s[s.size() - 1],
+                                   ctx->needs_input_grad(0), wantW, st == at::kFloat,
+                                   wantW ? destination(w, ctx->saved_data["dw"].toBool(), st) : Opt());
+    return {d[0], d[1], db, {}, {}, {}, {}, {}};
+  }
+};
+
+at::Tensor linearInt8(const at::Tensor& x, const at::Tensor& w, const at::Tensor& b,
+                      const Opt& w16, const Opt& b16, bool gelu, bool dwDest,
+                      bool dbDest) {
+  auto y = LinearInt8Fn::apply(x.reshape({-1, x.size(-1)}).to(at::kBFloat16).contiguous(), w, b,
+                               w16, b16, gelu, dwDest, dbDest);
+  auto shape = x.sizes().vec();
+  shape.back() = w.size(0);
+  return y.view(shape);
+}
+
 }  // namespace
 
 void registerTrainOps(py::module_& ops) {
-  ops.def("embedding_fwd", &embeddingFwd, py::arg("idx"), py::arg("positions"),
-          py::arg("weight"), py::arg("pos_weight"), py::arg("seq"), py::arg("scale"),
-          py::arg("out_f32"));
-  ops.def("embedding_grad", &embeddingGrad, py::arg("grad"), py::arg("idx"),
-          py::arg("positions"), py::arg("seq"), py::arg("vocab"), py::arg("context"),
-          py::arg("scale"), py::arg("out_f32"), py::arg("dw_out") = py::none(),
-          py::arg("dp_out") = py::none());
+  ops.def("embedding", &embedding, py::arg("weight"), py::arg("pos_weight"), py::arg("idx"),
+          py::arg("positions"), py::arg("seq"), py::arg("scale"), py::arg("out_f32"),
+          py::arg("has_dw_dest"), py::arg("has_dp_dest"));
+  ops.def("linear_cross_entropy", &linearCrossEntropy, py::arg("x"), py::arg("weight"),
+          py::arg("weight_bf16"), py::arg("target"), py::arg("classes"), py::arg("reduction"),
+          py::arg("has_dw_dest"));
+  ops.def("linear_int8", &linearInt8, py::arg("x"), py::arg("weight"), py::arg("bias"),
+          py::arg("weight_bf16"), py::arg("bias_bf16"), py::arg("gelu"), py::arg("has_dw_dest"),
+          py::arg("has_db_dest"));
   ops.def("linear_ce_fwd", &linearCeFwd, py::arg("x"), py::arg("weight"), py::arg("target"),
           py::arg("classes"), py::arg("mean"));
   ops.def("linear_ce_piece", &cePiece, py::arg("rows"), py::arg("classes"), py::arg("budget"));
   ops.def("linear_ce_bwd", &linearCeBwd, py::arg("x"), py::arg("weight"), py::arg("target"),
           py::arg("lse"), py::arg("grad"), py::arg("share"), py::arg("classes"),
           py::arg("want_dx"), py::arg("want_dw"), py::arg("dw_f32"),
-          py::arg("dw_out") = py::none(), py::arg("budget") = 512ll << 20);
+          py::arg("dw_out") = py::none(), py::arg("budget") = kCeBudget);
   ops.def("quantize_int8", &quantizeInt8, py::arg("x"));
   ops.def("dequantize_int8", &dequantizeInt8, py::arg("q"), py::arg("e"), py::arg("out_f32"));
-  ops.def("linear_gelu_int8", &linearGeluInt8, py::arg("x"), py::arg("weight"), py::arg("bias"));
-  ops.def("gelu_bwd_bias_int8", &geluBwdBiasInt8, py::arg("grad_y"), py::arg("q"), py::arg("e"),
-          py::arg("db_out") = py::none());
-  ops.def("linear_grads_int8", &linearGradsInt8, py::arg("grad"), py::arg("weight"),
-          py::arg("q"), py::arg("e"), py::arg("want_dx"), py::arg("want_dw"), py::arg("dw_f32"),
-          py::arg("dw_out") = py::none());
 }

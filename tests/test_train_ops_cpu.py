@@ -125,6 +125,38 @@ def test_python_refusals(built):
             f(x, w, torch.zeros(10), activations="int4")
 
 
+def test_gradient_slice_is_handed_out_once_per_backward():
+    """A parameter used by two functions in one backward pass: only the first
+    gets its flat slice, so that the two gradients add up; the next pass hands
+    it out again."""
+    from tiny_nccl_b200.ops.fused import grad_destination, has_destination
+    got = []
+
+    class Use(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, p, k):
+            ctx.p, ctx.k = p, k
+            return p.sum() * k
+
+        @staticmethod
+        def backward(ctx, g):
+            d = grad_destination(ctx.p)
+            got.append(d is not None)
+            out = d if d is not None else torch.empty(3)
+            return out.fill_(float(ctx.k)), None
+
+    p = torch.nn.Parameter(torch.zeros(3))
+    assert not has_destination(p) and not has_destination(None)
+    flat = torch.zeros(8)
+    p._tn_grad_dest = flat[4:7]
+    assert has_destination(p)
+    for _ in range(2):
+        (Use.apply(p, 2) + Use.apply(p, 5)).backward()
+        assert torch.equal(p.grad, torch.full((3,), 7.0))
+        p.grad = None
+    assert got == [True, False, True, False]
+
+
 def test_cross_entropy_pieces_cover_the_classes(built):
     """A piece is a multiple of 256 classes, fits the budget where one tile
     does, and the pieces are even: the last is at least half of the others

@@ -471,6 +471,69 @@ def test_operators_together_train_step(ops):
     status_ok()
 
 
+def test_tied_weight_in_a_flat_gradient_buffer(ops):
+    """A weight that is both embedding and head, with its place in a flat
+    gradient buffer: the head's gradient and the embedding's add up there, as
+    without the buffer; a weight used once is written in place."""
+    V, C, R = 700, 64, 90
+    w = torch.nn.Parameter(_normal(V, C, seed=1, std=0.1))
+    p = torch.nn.Parameter(_normal(R, C, seed=2, std=0.1))
+    lw = torch.nn.Parameter(_normal(C, C, seed=3, std=0.1))
+    lb = torch.nn.Parameter(torch.zeros(C, device="cuda"))
+    g = torch.Generator(device="cuda").manual_seed(4)
+    idx = torch.randint(0, V, (2, R), device="cuda", generator=g)
+    leaves = [w, p, lw, lb]
+
+    def backward():
+        for t in leaves:
+            t.grad = None
+        h = ops.embedding(idx, w, p)
+        h = ops.linear(h, lw, lb, activations="int8")
+        ops.linear_cross_entropy(h, w, idx.roll(1, 1)).backward()
+        return [t.grad.clone() for t in leaves]
+
+    want = backward()
+    flat = torch.zeros(sum(t.numel() for t in leaves), device="cuda")
+    at = 0
+    for t in leaves:
+        t._tn_grad_dest = flat[at:at + t.numel()].view_as(t)
+        at += t.numel()
+    for _ in range(2):
+        got = backward()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+        for t in (p, lw, lb):
+            assert t.grad.data_ptr() == t._tn_grad_dest.data_ptr()
+
+
+def test_strided_and_misaligned_inputs(ops):
+    """Rows that are not contiguous, and storage that starts off a 16-byte
+    boundary (copied or read one value at a time)."""
+    w = _normal(50, 12, seed=1)
+    base = torch.empty(50 * 12 + 1, device="cuda")
+    off = base[1:].view(50, 12).copy_(w).requires_grad_()
+    idx = torch.arange(40, device="cuda").view(4, 10)
+    gy = _normal(4, 5, 12, seed=2)
+    wr = w.clone().requires_grad_()
+    y, z = ops.embedding(idx[:, ::2], off), ops.embedding(idx[:, ::2].contiguous(), wr)
+    assert torch.equal(y, z)
+    assert torch.equal(*(torch.autograd.grad(a, [b], gy)[0] for a, b in ((y, off), (z, wr))))
+    x = _normal(64, 128, seed=3, dtype=torch.bfloat16)
+    hw = _normal(100, 64, seed=4, dtype=torch.bfloat16)
+    t = torch.arange(64, device="cuda")
+    a = ops.linear_cross_entropy(x[:, ::2], hw, t)
+    b = ops.linear_cross_entropy(x[:, ::2].contiguous(), hw, t)
+    assert torch.equal(a, b)
+    assert torch.equal(ops.quantize_int8(x.t())[0], ops.quantize_int8(x.t().contiguous())[0])
+
+
+def test_refuses_to_be_differentiated_twice(ops):
+    w = _normal(20, 16, seed=1).requires_grad_()
+    y = ops.embedding(torch.arange(4, device="cuda"), w)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y.sum(), [w], create_graph=True)
+
+
 # -- refusals -----------------------------------------------------------------------
 
 

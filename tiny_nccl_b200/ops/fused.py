@@ -100,14 +100,26 @@ def cross_entropy(logits: torch.Tensor, target: torch.Tensor,
     return _CrossEntropy.apply(logits.contiguous(), target.contiguous(), int(classes))
 
 
-def bf16_weight(p: torch.Tensor) -> torch.Tensor:
-    """The bf16 value of an fp32 parameter for a GEMM operand: the copy the
-    fused AdamW wrote in its last update while it is current (the
-    parameter's version unchanged since), else a cast."""
+def current_copy(p: torch.Tensor):
+    """The bf16 copy of parameter p that the fused AdamW wrote in its last
+    update, while it is current (the parameter's version unchanged since);
+    None otherwise."""
     c = getattr(p, "_tn_bf16", None)
-    if c is not None and c[1] == p._version:
-        return c[0]
-    return p.to(torch.bfloat16)
+    return c[0] if c is not None and c[1] == p._version else None
+
+
+def bf16_weight(p: torch.Tensor) -> torch.Tensor:
+    """The bf16 value of an fp32 parameter for a GEMM operand: the current
+    copy, else a cast."""
+    c = current_copy(p)
+    return c if c is not None else p.to(torch.bfloat16)
+
+
+def has_destination(p: torch.Tensor | None) -> bool:
+    """Whether p's gradient may have a place in a flat gradient buffer. The
+    native backward functions then ask :func:`grad_destination` when they
+    run."""
+    return getattr(p, "_tn_grad_dest", None) is not None
 
 
 def grad_destination(p: torch.Tensor):
@@ -117,18 +129,20 @@ def grad_destination(p: torch.Tensor):
     below write their parameter gradients there and return that slice, which
     autograd then adopts as ``p.grad`` as it is (no copy, no accumulation
     kernel). None otherwise: a new tensor is returned and autograd handles it
-    as usual."""
+    as usual. A slice is handed out once per backward pass: where a parameter
+    is used twice (a head tied to the embedding), the second gradient is a
+    tensor of its own, which autograd adds to the first."""
     d = getattr(p, "_tn_grad_dest", None)
+    if d is None or p.grad is not None:
+        return None
+    task = torch._C._current_graph_task_id()  # -1 outside a backward pass
+    if task >= 0:
+        if getattr(p, "_tn_grad_task", -1) == task:
+            return None
+        p._tn_grad_task = task
     # A new tensor object on the same memory: autograd adopts a gradient
     # without copying only when nothing else holds the object.
-    return d.detach() if d is not None and p.grad is None else None
-
-
-def typed_destination(p: torch.Tensor, dtype: torch.dtype):
-    """grad_destination(p) for a gradient that a kernel writes as ``dtype`` in
-    row-major order; None where p's slice is of another type or layout."""
-    d = grad_destination(p)
-    return d if d is not None and d.dtype == dtype and d.is_contiguous() else None
+    return d.detach()
 
 
 def _wgrad(gy: torch.Tensor, x: torch.Tensor, dest: torch.Tensor | None = None) -> torch.Tensor:
@@ -146,15 +160,10 @@ class _LinearBias(torch.autograd.Function):
     deterministic column-sum kernel."""
 
     @staticmethod
-    def compute(x, weight, bias):
-        """(y, the bf16 weight)"""
+    def forward(ctx, x, weight, bias):
         w16 = bf16_weight(weight)
         with torch.autocast("cuda", enabled=False):
-            return torch.addmm(bf16_weight(bias), x, w16.t()), w16
-
-    @staticmethod
-    def forward(ctx, x, weight, bias):
-        y, w16 = _LinearBias.compute(x, weight, bias)
+            y = torch.addmm(bf16_weight(bias), x, w16.t())
         ctx.save_for_backward(x, w16)
         ctx.params = (weight, bias)
         return y
@@ -231,46 +240,13 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return (x if x.dtype == torch.bfloat16 else x.to(torch.bfloat16)).contiguous()
 
 
-class _LinearInt8(torch.autograd.Function):
-    """The linear layers above with what the backward pass needs of the
-    activations kept in 8-bit blocks: x for dW, and the sums before the GELU
-    (rounded from fp32 in the GEMM's epilogue) for its slope."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, gelu):
-        if gelu:
-            w16 = bf16_weight(weight)
-            y, *pre = _ops().linear_gelu_int8(x, w16, bf16_weight(bias))
-        else:
-            y, w16 = _LinearBias.compute(x, weight, bias)
-            pre = ()
-        ctx.save_for_backward(w16, *_ops().quantize_int8(x), *pre)
-        ctx.params = (weight, bias)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gy):
-        w16, q, e, *pre = ctx.saved_tensors
-        pw, pb = ctx.params
-        gy = gy.contiguous()
-        if pre:
-            gy, db = _ops().gelu_bwd_bias_int8(gy, *pre, typed_destination(pb, torch.float32))
-        else:
-            db = _ops().bias_grad(gy, out=typed_destination(pb, torch.float32))
-        dx, dw = _ops().linear_grads_int8(gy, w16, q, e, ctx.needs_input_grad[0],
-                                          ctx.needs_input_grad[1], pw.dtype == torch.float32,
-                                          typed_destination(pw, pw.dtype))
-        return dx, dw, db, None
-
-
 def _linear(x, weight, bias, gelu, activations):
-    if activations not in ("bf16", "int8"):
-        raise ValueError(f"activations must be 'bf16' or 'int8', not {activations!r}")
     if activations == "int8":
-        y = _LinearInt8.apply(_rows(x), weight, bias, gelu)
-    else:
-        y = (_LinearGelu if gelu else _LinearBias).apply(_rows(x), weight, bias)
+        return _ops().linear_int8(x, weight, bias, current_copy(weight), current_copy(bias), gelu,
+                                  has_destination(weight), has_destination(bias))
+    if activations != "bf16":
+        raise ValueError(f"activations must be 'bf16' or 'int8', not {activations!r}")
+    y = (_LinearGelu if gelu else _LinearBias).apply(_rows(x), weight, bias)
     return y.view(*x.shape[:-1], weight.shape[0])
 
 

@@ -1,48 +1,19 @@
-"""Autograd wrappers of the training operators (csrc/ops): token and position
-embedding, linear layer + softmax cross-entropy in pieces of the vocabulary,
-and 8-bit activation blocks. Like :mod:`.fused`, every function calls the
-native kernels; a missing extension or an unsupported argument raises.
+"""Training operators (csrc/ops): token and position embedding, linear layer +
+softmax cross-entropy in pieces of the vocabulary, and 8-bit activation
+blocks. Their autograd functions are native too (csrc/torch/train_ext.cpp).
+Like :mod:`.fused`, every function calls the native kernels; a missing
+extension or an unsupported argument raises.
 """
 from __future__ import annotations
 
 import torch
 
-from .fused import _ops, _rows, bf16_weight, typed_destination
+from .fused import _ops, current_copy, has_destination
 
 
 def _needs_float(name: str, t: torch.Tensor) -> None:
     if t.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"{name} must be float32 or bfloat16, not {t.dtype}")
-
-
-class _Embedding(torch.autograd.Function):
-    """y = scale W[idx] + P[positions]. Backward: each table's gradient is the
-    sum of its rows' gradients in row order (deterministic), written once,
-    zeros included."""
-
-    @staticmethod
-    def forward(ctx, idx, weight, pos_weight, positions, seq, scale, out_f32):
-        y = _ops().embedding_fwd(idx, positions, weight.detach(),
-                                 None if pos_weight is None else pos_weight.detach(), seq, scale,
-                                 out_f32)
-        ctx.save_for_backward(idx, positions)
-        ctx.tables = (weight, pos_weight)
-        ctx.seq, ctx.scale = seq, scale
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        idx, positions = ctx.saved_tensors
-        weight, pos_weight = ctx.tables
-        tables = (weight if ctx.needs_input_grad[1] else None,
-                  pos_weight if ctx.needs_input_grad[2] else None)
-        dw, dp = _ops().embedding_grad(
-            g.contiguous(), idx, positions, ctx.seq,
-            *(0 if t is None else t.shape[0] for t in tables), ctx.scale,
-            weight.dtype == torch.float32,
-            *(None if t is None else typed_destination(t, t.dtype) for t in tables))
-        return None, dw, dp, None, None, None, None
 
 
 def embedding(idx: torch.Tensor, weight: torch.Tensor, pos_weight: torch.Tensor | None = None,
@@ -82,37 +53,13 @@ def embedding(idx: torch.Tensor, weight: torch.Tensor, pos_weight: torch.Tensor 
                              f"{tuple(positions.shape)}")
         if positions.dtype not in (torch.int64, torch.int32):
             raise TypeError(f"positions must be int64 or int32, not {positions.dtype}")
-        positions = positions.reshape(-1).long().contiguous()
-    y = _Embedding.apply(idx.reshape(-1).long().contiguous(), weight.contiguous(),
-                         None if pos_weight is None else pos_weight.contiguous(), positions, seq,
-                         float(scale), out_dtype == torch.float32)
-    return y.view(*idx.shape, weight.shape[1])
+    return _ops().embedding(weight.contiguous(),
+                            None if pos_weight is None else pos_weight.contiguous(), idx,
+                            positions, seq, scale, out_dtype == torch.float32,
+                            has_destination(weight), has_destination(pos_weight))
 
 
-class _LinearCrossEntropy(torch.autograd.Function):
-    """Cross-entropy of x W^T against targets. The forward pass keeps one
-    number per row (the log of the sum of exponentials); the backward pass
-    forms the logits again, a piece of the vocabulary at a time."""
-
-    @staticmethod
-    def forward(ctx, x, weight, target, classes, reduction):
-        w16 = bf16_weight(weight).contiguous()
-        loss, lse, out = _ops().linear_ce_fwd(x, w16, target, classes, reduction == "mean")
-        ctx.save_for_backward(x, w16, target, lse, out)
-        ctx.weight, ctx.classes, ctx.reduction = weight, classes, reduction
-        return loss if reduction == "none" else out[0]
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        x, w16, target, lse, out = ctx.saved_tensors
-        weight = ctx.weight
-        dx, dw = _ops().linear_ce_bwd(
-            x, w16, target, lse, g.reshape(-1).float().contiguous(),
-            out[1:] if ctx.reduction == "mean" else None, ctx.classes, ctx.needs_input_grad[0],
-            ctx.needs_input_grad[1], weight.dtype == torch.float32,
-            typed_destination(weight, weight.dtype))
-        return dx, dw, None, None, None
+_REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor,
@@ -131,7 +78,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     Backward: the gradient of x is bf16, that of weight has weight's type; the
     gradient of the logits is rounded to bf16 between the products, a piece of
     the vocabulary of at most 512 MiB at a time. width must be a multiple of 8."""
-    if reduction not in ("mean", "sum", "none"):
+    if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', not {reduction!r}")
     _needs_float("weight", weight)
     if weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
@@ -140,10 +87,9 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
         raise TypeError(f"target must be int64, not {target.dtype}")
     if target.numel() * x.shape[-1] != x.numel():
         raise ValueError("target must have one entry per row of x")
-    classes = int(classes) or weight.shape[0]
-    loss = _LinearCrossEntropy.apply(_rows(x), weight, target.reshape(-1).contiguous(), classes,
-                                     reduction)
-    return loss.view(target.shape) if reduction == "none" else loss
+    return _ops().linear_cross_entropy(x, weight, current_copy(weight), target,
+                                       int(classes) or weight.shape[0], _REDUCTIONS[reduction],
+                                       has_destination(weight))
 
 
 def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
