@@ -112,6 +112,6 @@ extern "C" int tnops_linear_gelu_int8(const void* x, const void* w, const void* 
   epi.rows = rows;
   epi.cols = outs;
   epi.blocks = (outs + kInt8Block - 1) / kInt8Block;
-  planGemm(&args, smPairs(), false);
+  planGemm(&args, false);
   return launchPairGemm(args, stream);
 }

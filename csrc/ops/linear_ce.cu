@@ -117,10 +117,18 @@ struct SoftmaxGradEpi {
   __device__ __forceinline__ void end(const State&, int, int) const {}
 };
 
-constexpr int kJoinWarps = 8;
+constexpr int kJoinWarps = 32;
+
+// (maximum, sum) of two sets; -inf and 0 stand for an empty one.
+__device__ __forceinline__ float2 joinSums(float2 a, float2 b) {
+  const float m = fmaxf(a.x, b.x);
+  if (m == -INFINITY) return make_float2(m, a.y + b.y);
+  return make_float2(m, a.y * ex2Approx((a.x - m) * kLog2e) + b.y * ex2Approx((b.x - m) * kLog2e));
+}
 
 // Joins a row's partial statistics: 32 rows per CTA (one per lane), the parts
-// split over the warps; each warp and then the CTA keeps (maximum, sum).
+// split over the warps, four loads in flight each; then the warps' sums in
+// order.
 __global__ void __launch_bounds__(kJoinWarps * 32)
     joinStats(const float2* __restrict__ partial, const int64_t* __restrict__ target,
               const float* __restrict__ logitOfTarget, float* __restrict__ lse,
@@ -128,19 +136,22 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
   __shared__ float2 s[kJoinWarps][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.x * 32 + lane;
-  auto join = [](float2 a, float2 b) {
-    const float m = fmaxf(a.x, b.x);
-    if (m == -INFINITY) return make_float2(m, a.y + b.y);
-    return make_float2(m, a.y * exp2f((a.x - m) * kLog2e) + b.y * exp2f((b.x - m) * kLog2e));
-  };
+  constexpr int U = 4;
   float2 st = make_float2(-INFINITY, 0.f);
   if (row < rows)
-    for (int p = warp; p < parts; p += kJoinWarps) st = join(st, partial[(size_t)p * rows + row]);
+    for (int p = warp; p < parts; p += U * kJoinWarps) {
+      float2 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        v[u] = p + u * kJoinWarps < parts ? partial[(size_t)(p + u * kJoinWarps) * rows + row]
+                                          : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int u = 0; u < U; ++u) st = joinSums(st, v[u]);
+    }
   s[warp][lane] = st;
   __syncthreads();
   if (warp == 0 && row < rows) {
-#pragma unroll
-    for (int w = 1; w < kJoinWarps; ++w) st = join(st, s[w][lane]);
+    for (int w = 1; w < kJoinWarps; ++w) st = joinSums(st, s[w][lane]);
     const float l = st.x + logf(st.y);
     const int64_t t = target[row];
     lse[row] = l;
@@ -222,7 +233,7 @@ extern "C" int tnops_linear_ce_fwd(const void* x, const void* w, const int64_t* 
   args.problems = 1;
   if (!logitsProblem(&args.prob[0], x, w, rows, width, 0, classes)) return 4;
   args.epi = {target, reinterpret_cast<float2*>(partial), loss, rows, classes};
-  planGemm(&args, smPairs(), false);
+  planGemm(&args, false);
   if (int rc = launchPairGemm(args, stream)) return rc;
   joinStats<<<(rows + 31) / 32, kJoinWarps * 32, 0, stream>>>(
       args.epi.partial, target, loss, lse, loss, tnops_linear_ce_parts(classes), rows, classes);
@@ -236,17 +247,27 @@ extern "C" int tnops_linear_ce_mean(const float* loss, const int64_t* target, fl
   return launched(cudaGetLastError());
 }
 
+extern "C" size_t tnops_linear_ce_scratch(int rows, int width, int classes, int piece,
+                                          int want_dx, int want_dw) {
+  if (rows <= 0 || width <= 0 || classes <= 0 || piece <= 0) return 0;
+  const int last = (classes - 1) % piece + 1;
+  const size_t a = tnops_linear_grads_scratch(rows, classes < piece ? classes : piece, width, want_dx,
+                                              want_dw),
+               b = tnops_linear_grads_scratch(rows, last, width, want_dx, want_dw);
+  return a > b ? a : b;
+}
+
 extern "C" int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* target,
                                    const float* lse, const float* grad, int grad_step,
                                    const float* share, void* d, int piece, float* dx_f32,
-                                   void* scratch, void* dx, void* dw, int dw_f32, int rows, int width,
+                                   void* scratch, size_t scratch_bytes, void* dx, void* dw, int dw_f32, int rows, int width,
                                    int classes, int vocab, cudaStream_t stream) {
   if (rows <= 0 || classes <= 0 || vocab < classes || width <= 0 || width % 8 != 0 ||
       piece <= 0 || piece % 8 != 0 || !aligned16(x) || !aligned16(w) || !aligned16(d) ||
       (dx && !aligned16(dx)) || (dw && !aligned16(dw)))
     return 1;
   const bool whole = classes <= piece;
-  if (scratch == nullptr || !aligned16(scratch)) return 1;
+  if (!aligned16(scratch)) return 1;
   if (dx && !whole && (dx_f32 == nullptr || !aligned16(dx_f32))) return 1;
   const size_t dwSize = dw_f32 ? 4 : 2;
   if (dw && vocab > classes) {
@@ -271,10 +292,11 @@ extern "C" int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* 
     e.classes = classes;
     e.first = first;
     e.width = n;
-    planGemm(&args, smPairs(), false);
+    planGemm(&args, false);
     if (int rc = launchPairGemm(args, stream)) return rc;
     LinearGrads g{};
     g.scratch = scratch;
+    g.scratchBytes = scratch_bytes;
     g.g = d;
     g.ldg = piece;
     g.w = static_cast<const uint16_t*>(w) + (size_t)first * width;

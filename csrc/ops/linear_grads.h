@@ -2,6 +2,7 @@
 // C++ side of the library (the C launcher is tnops_linear_grads).
 #pragma once
 
+#include <stddef.h>
 #include <stdint.h>
 
 #include <cuda_runtime_api.h>
@@ -21,7 +22,8 @@ struct LinearGrads {
   const void* x;
   void* dx;
   void* dw;
-  void* scratch;  // tnops_linear_grads_scratch() bytes, 16-byte aligned
+  void* scratch;  // 16-byte aligned, at least tnops_linear_grads_scratch()
+  size_t scratchBytes;
   GradStore dxStore, dwStore;
   int rows, outs, ins;
 };

@@ -47,7 +47,7 @@ struct alignas(64) GemmProblem {
 template <class Epi>
 struct alignas(64) PairGemmArgs {
   GemmProblem prob[2];
-  CUtensorMap mapPartial;  // [2 * pairs * 256, 256] fp32, for an Epi that kCuts
+  CUtensorMap mapPartial;  // [256 slots, 256] fp32, for an Epi that kCuts
   int problems;
   PairSchedule schedule;
   Epi epi;
@@ -295,7 +295,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         if (Epi::kCuts && w.slot >= 0)
           storeF32(v, lane, buf, &args.mapPartial,
-                   (2 * pair + w.slot) * kPairBM + (int)rank * 128 + quarter * 32, c, true, false);
+                   w.slot * kPairBM + (int)rank * 128 + quarter * 32, c, true, false);
         else
           args.epi.chunk(st, v, w.which, lane, row0, tileN * 256 + c, buf);
       }
@@ -347,35 +347,20 @@ inline bool f32OutMap(CUtensorMap* map, const void* base, int64_t rows, int64_t 
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE);
 }
 
-// SM pairs of the current device (0 on failure), counted once per device.
-inline int smPairs() {
-  static std::atomic<int> known[64];
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 0;
-  if (int n = known[dev].load(std::memory_order_relaxed)) return n;
-  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  known[dev].store(sms / 2, std::memory_order_relaxed);
-  return sms / 2;
-}
-
-// Tile counts and sums of the launch for `pairs` pairs, cut or not.
+// Plans the launch for kSMs / 2 pairs; with `cut`, sums may be split. Product
+// 0 must be the one with the longer sum.
 template <class Epi>
-void planGemm(PairGemmArgs<Epi>* args, int pairs, bool cut) {
+void planGemm(PairGemmArgs<Epi>* args, bool cut) {
   PairSchedule& s = args->schedule;
   s = {};
-  s.pairs = pairs;
+  s.pairs = kSMs / 2;
   for (int i = 0; i < 2; ++i) {
     s.k[i] = 1;
     if (i >= args->problems) continue;
     s.tiles[i] = args->prob[i].tilesM * args->prob[i].tilesN;
     s.k[i] = args->prob[i].kBlocks;
   }
-  if (cut) {
-    planPairs(&s);
-  } else {
-    s.whole[0] = s.tiles[0];
-    s.whole[1] = s.tiles[1];
-  }
+  planPairs(&s, cut);
 }
 
 // Launches the products of `args`, whose schedule is planned. Returns 0, or a
@@ -386,7 +371,7 @@ int launchPairGemm(const PairGemmArgs<Epi>& args, cudaStream_t stream) {
   // Opt in to the shared memory once per device (bit d of `done`).
   static std::atomic<uint64_t> done{0};
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64 || args.schedule.pairs <= 0) return 3;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 3;
   const uint64_t bit = 1ull << dev;
   if (!(done.load(std::memory_order_acquire) & bit)) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -395,9 +380,8 @@ int launchPairGemm(const PairGemmArgs<Epi>& args, cudaStream_t stream) {
     done.fetch_or(bit, std::memory_order_acq_rel);
   }
   const PairSchedule& s = args.schedule;
-  const int tiles = s.tiles[0] + s.tiles[1];
-  // Without a rest the pairs past the last tile have nothing to do.
-  const int pairs = s.restBlocks() > 0 || tiles > s.pairs ? s.pairs : tiles;
+  // In a first round, pairs past the last unit have nothing to do.
+  const int units = s.units(0) + s.units(1), pairs = units < s.pairs ? units : s.pairs;
   kernel<<<2u * (unsigned)pairs, kThreads, kPairSmemBytes, stream>>>(args);
   return launched(cudaGetLastError());
 }

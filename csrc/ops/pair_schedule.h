@@ -2,16 +2,20 @@
 // launch (pair_gemm.cuh): shared by the kernels, their launchers and a CPU
 // test.
 //
-// The tiles of the launch's one or two products lie one product after the
-// other; a tile of product i is a sum of k[i] blocks. Whole tiles go to the
-// pairs in turn (tile t to pair t % pairs): neighbouring pairs then read the
-// same rows of an operand at the same time. When the last round of that would
-// leave pairs idle for long, the tiles after the last full rounds (the "rest")
-// are laid out as one line of K blocks and cut evenly: pair p takes blocks
-// [U p / pairs, U (p + 1) / pairs). A pair's share of a cut tile goes to one of
-// its two slots of partial sums (the first part of its range to slot 0, a
-// later one to slot 1: a range can cut a tile only at its two ends), and a
-// second kernel adds the parts of each cut tile in pair order.
+// A launch has one or two products; a tile of product i is a sum of k[i] K
+// blocks, cut into split[i] even parts ("units"; 1: whole tiles). Product 0's
+// units are the longer ones and go to the pairs in turn, unit u to pair
+// u % pairs. Where that leaves `extra` pairs with one more of them, the other
+// pairs begin product 1 with `early` rounds among themselves, and the rest of
+// it goes round all pairs, first to those that then have less behind them.
+// Pairs that work at the same time so have neighbouring units, which read the
+// same rows of an operand in the same order: one read from memory serves them
+// all. (An even cut of the K blocks over the pairs, which also keeps all of
+// them busy, lets every pair read at a place of its own: on a 65536 x 1024 x
+// 4096 layer the two products took 995 us that way and 830 us in turns.)
+//
+// Units of a cut tile leave partial sums, one slot per unit, which a second
+// kernel adds in the order of the sum.
 #pragma once
 
 #include <stdint.h>
@@ -25,125 +29,118 @@
 namespace tnops {
 
 struct PairSchedule {
-  int tiles[2];  // of each product
+  int tiles[2];  // of each product (0: no such product)
   int k[2];      // K blocks of a tile
-  int whole[2];  // tiles that are not part of the rest (the first ones)
+  int split[2];  // parts of a tile
   int pairs;
+  int extra, early;  // pairs with one more unit of product 0; early rounds
+  int lateFirst;     // the late rounds of product 1 begin with this pair
 
-  TNOPS_HD int restTiles(int i) const { return tiles[i] - whole[i]; }
-  TNOPS_HD int64_t restBlocks() const {
-    return (int64_t)restTiles(0) * k[0] + (int64_t)restTiles(1) * k[1];
+  TNOPS_HD int units(int i) const { return tiles[i] * split[i]; }
+  TNOPS_HD int others() const { return pairs - extra; }
+  // First slot of product i.
+  TNOPS_HD int slotBase(int i) const { return i == 1 && split[0] > 1 ? units(0) : 0; }
+  TNOPS_HD int slots() const {
+    return (split[0] > 1 ? units(0) : 0) + (split[1] > 1 ? units(1) : 0);
   }
-  TNOPS_HD int64_t restStart(int p) const { return restBlocks() * p / pairs; }
 };
 
-// A part of a tile: K blocks [kb0, kb1) of `tile` of product `which`; slot -1
-// for a whole tile.
+// K blocks [kb0, kb1) of `tile` of product `which`; slot -1 for a whole tile.
 struct PairWork {
   int which, tile, kb0, kb1, slot;
 };
 
-// The rest's tile that holds block u of the line, and the line's first block
-// of that tile.
-TNOPS_HD void restTileAt(const PairSchedule& s, int64_t u, int* which, int* tile, int64_t* first) {
-  const int64_t line0 = (int64_t)s.restTiles(0) * s.k[0];
-  *which = u >= line0;
-  const int64_t v = *which ? u - line0 : u;
-  const int k = s.k[*which];
-  const int64_t t = v / k;
-  *tile = s.whole[*which] + (int)t;
-  *first = (*which ? line0 : 0) + t * k;
+// Part s of a tile's sum starts at K block k s / split.
+TNOPS_HD PairWork pairUnit(const PairSchedule& s, int which, int unit) {
+  const int part = unit / s.tiles[which], n = s.split[which], k = s.k[which];
+  PairWork w;
+  w.which = which;
+  w.tile = unit - part * s.tiles[which];
+  w.kb0 = (int)((int64_t)k * part / n);
+  w.kb1 = (int)((int64_t)k * (part + 1) / n);
+  w.slot = n > 1 ? s.slotBase(which) + unit : -1;
+  return w;
 }
 
-// Walks a pair's parts in order.
+// Walks a pair's units in order.
 struct PairWalk {
-  int t;          // next whole tile, counted over both products
-  int64_t u, end; // next block of the rest, and the end of this pair's range
-  bool started;   // some of the rest was handed out already
+  int first;          // next unit of product 0
+  int early, earlyEnd;
+  int late;           // next unit of product 1 in the late rounds
 
   TNOPS_HD void init(const PairSchedule& s, int pair) {
-    t = pair;
-    u = s.restStart(pair);
-    end = s.restStart(pair + 1);
-    started = false;
+    first = pair;
+    early = pair >= s.extra ? pair - s.extra : 0;
+    earlyEnd = pair >= s.extra ? s.others() * s.early : 0;
+    const int turn = pair - s.lateFirst;
+    late = s.others() * s.early + (turn < 0 ? turn + s.pairs : turn);
   }
   TNOPS_HD bool next(const PairSchedule& s, PairWork* w) {
-    if (t < s.whole[0] + s.whole[1]) {
-      w->which = t >= s.whole[0];
-      w->tile = w->which ? t - s.whole[0] : t;
-      w->kb0 = 0;
-      w->kb1 = s.k[w->which];
-      w->slot = -1;
-      t += s.pairs;
+    if (first < s.units(0)) {
+      *w = pairUnit(s, 0, first);
+      first += s.pairs;
       return true;
     }
-    if (u >= end) return false;
-    int64_t first;
-    restTileAt(s, u, &w->which, &w->tile, &first);
-    const int k = s.k[w->which];
-    w->kb0 = (int)(u - first);
-    w->kb1 = (int)(end - first < k ? end - first : k);
-    w->slot = w->kb0 == 0 && w->kb1 == k ? -1 : started ? 1 : 0;
-    started = true;
-    u = first + w->kb1;
-    return true;
+    if (early < earlyEnd) {
+      *w = pairUnit(s, 1, early);
+      early += s.others();
+      return true;
+    }
+    if (late < s.units(1)) {
+      *w = pairUnit(s, 1, late);
+      late += s.pairs;
+      return true;
+    }
+    return false;
   }
 };
 
-// The cut tile that begins with pair `p`'s part: false when pair p's range does
-// not end inside a tile, or its tile began with an earlier pair's part.
-// `slotOf` then gives the slot of each later pair's part.
-struct CutTile {
-  int which, tile;
-  int64_t first, end;  // the tile's blocks in the line
-};
-TNOPS_HD bool cutTileOf(const PairSchedule& s, int p, CutTile* c) {
-  if (p + 1 >= s.pairs) return false;
-  const int64_t b = s.restStart(p + 1);
-  if (b <= 0 || b >= s.restBlocks() || b == s.restStart(p)) return false;
-  restTileAt(s, b, &c->which, &c->tile, &c->first);
-  c->end = c->first + s.k[c->which];
-  if (c->first == b) return false;                // a border between tiles
-  return s.restStart(p) <= c->first;
-}
-// Pair q's part of the cut tile: its slot, or -1 when it has none.
-TNOPS_HD int cutSlot(const PairSchedule& s, const CutTile& c, int q) {
-  const int64_t a = s.restStart(q), b = s.restStart(q + 1);
-  if (a >= c.end || b <= c.first || a == b) return -1;
-  return a >= c.first ? 0 : 1;
-}
-
-// Times of the choice below, in K blocks (a block of a 256 x 256 tile takes
-// about 0.3 us): what writing and adding the cut tiles' parts costs.
-constexpr int kCutCost = 32;
-
-// Fills whole[]: everything in turn, or full rounds in turn and the rest cut,
-// whichever takes fewer blocks on the busiest pair. A tile that is longer than
-// a pair's even share is left to the rest entirely.
-inline void planPairs(PairSchedule* s) {
-  const int64_t total = (int64_t)s->tiles[0] * s->k[0] + (int64_t)s->tiles[1] * s->k[1];
-  int64_t busiest = 0;  // in turn
+// The schedule for given splits, and the K blocks of its busiest pair.
+inline int planRounds(PairSchedule* s) {
+  const int len0 = (s->k[0] + s->split[0] - 1) / s->split[0];
+  const int len1 = (s->k[1] + s->split[1] - 1) / s->split[1];
+  s->extra = s->units(0) % s->pairs;
+  s->early = 0;
+  s->lateFirst = 0;
+  if (s->extra > 0 && s->units(1) > 0) {
+    const int most = s->units(1) / s->others();
+    s->early = (len0 + len1 / 2) / len1;
+    if (s->early > most) s->early = most;
+    if (s->early * len1 < len0) s->lateFirst = s->extra;
+  }
+  const int rounds0 = s->units(0) / s->pairs;
+  const int late = s->units(1) - s->others() * s->early;
+  int busiest = 0;
   for (int p = 0; p < s->pairs; ++p) {
-    int64_t n = 0;
-    for (int i = 0, at = 0; i < 2; at += s->tiles[i], ++i) {
-      // Tiles at, at + 1, ... of which pair p has those congruent to p.
-      const int before = (at - p + s->pairs - 1) / s->pairs;
-      const int upTo = (at + s->tiles[i] - p + s->pairs - 1) / s->pairs;
-      n += (int64_t)((upTo > 0 ? upTo : 0) - (before > 0 ? before : 0)) * s->k[i];
-    }
+    const int turn = (p - s->lateFirst + s->pairs) % s->pairs;
+    int n = rounds0 * len0 + (p < s->extra ? len0 : s->early * len1);
+    if (turn < late) n += (late - turn + s->pairs - 1) / s->pairs * len1;
     if (n > busiest) busiest = n;
   }
-  s->whole[0] = s->tiles[0];
-  s->whole[1] = s->tiles[1];
-  const int64_t even = (total + s->pairs - 1) / s->pairs;
-  if (busiest <= even + kCutCost) return;
-  int64_t left = even;
-  for (int i = 0; i < 2; ++i) {
-    if (s->tiles[i] == 0) continue;
-    int64_t rounds = s->tiles[i] / s->pairs;
-    if (rounds > left / s->k[i]) rounds = left / s->k[i];
-    s->whole[i] = (int)rounds * s->pairs;
-    left -= rounds * s->k[i];
+  return busiest;
+}
+
+// Plans the launch: sums stay whole, or with `cut` the longer product's are
+// split in 2 to kMaxSplit where the busiest pair gains more than the partial
+// sums cost. A K block of a tile takes about 0.3 us; partial sums cost one
+// more launch (about 4 us) and about 0.13 us per slot (256 KiB written and
+// read).
+constexpr int kMaxSplit = 8;
+constexpr int kSplitSlots = 296;
+inline void planPairs(PairSchedule* s, bool cut) {
+  s->split[0] = s->split[1] = 1;
+  int best = planRounds(s);
+  if (!cut) return;
+  PairSchedule t = *s;
+  for (int n = 2; n <= kMaxSplit && t.tiles[0] * n <= kSplitSlots; ++n) {
+    if (t.k[0] < 8 * n) break;  // at least 8 K blocks a unit
+    t.split[0] = n;
+    if ((t.k[0] + n - 1) / n < t.k[1] && t.tiles[1] > 0) break;  // product 0's stay the longer
+    const int cost = planRounds(&t) + 14 + t.slots() * 4 / 9;
+    if (cost < best) {
+      best = cost;
+      *s = t;
+    }
   }
 }
 

@@ -103,13 +103,13 @@ int tnops_gemm_bias_act(const void* x, const void* w, const void* bias, void* pr
 // g w and dw [outs, ins] (fp32 with dw_f32, else bf16) = g^T x, for g
 // [rows, outs] with rows ldg elements apart, w [outs, ins], x [rows, ins],
 // all bf16. A null dx or dw is left out. ins % 8 == 0, ldg % 8 == 0, 16-byte
-// aligned pointers; 1 (invalid argument) without a launch otherwise. scratch:
-// tnops_linear_grads_scratch() bytes (partial sums of tiles that several SM
-// pairs share).
-size_t tnops_linear_grads_scratch(void);
+// aligned pointers; 1 (invalid argument) without a launch otherwise. scratch
+// (scratch_bytes, at least tnops_linear_grads_scratch(...), which may be 0):
+// partial sums of tiles that several SM pairs share.
+size_t tnops_linear_grads_scratch(int rows, int outs, int ins, int want_dx, int want_dw);
 int tnops_linear_grads(const void* g, int64_t ldg, const void* w, const void* x, void* dx,
                        void* dw, int dw_f32, int rows, int outs, int ins, void* scratch,
-                       cudaStream_t stream);
+                       size_t scratch_bytes, cudaStream_t stream);
 
 // Softmax cross-entropy of l = x w^T without the logits in memory: x
 // [rows, width], w [vocab, width] in bf16, of which the first `classes` rows
@@ -124,9 +124,11 @@ int tnops_linear_grads(const void* g, int64_t ldg, const void* w, const void* x,
 //    bf16; rows from `classes` on are zero) of sum_r k[r] loss[r], with k[r] =
 //    grad[r * grad_step] (* *share). Works on `piece` classes at a time
 //    (piece % 8 == 0); d holds rows * piece bf16 of scratch, dx_f32
-//    rows * width floats when piece < classes, and scratch
-//    tnops_linear_grads_scratch() bytes. A null dx or dw is left out.
+//    rows * width floats when piece < classes, and scratch scratch_bytes, at
+//    least tnops_linear_ce_scratch(...). A null dx or dw is left out.
 int tnops_linear_ce_parts(int classes);
+size_t tnops_linear_ce_scratch(int rows, int width, int classes, int piece, int want_dx,
+                               int want_dw);
 int tnops_linear_ce_fwd(const void* x, const void* w, const int64_t* target, float* loss,
                         float* lse, float* partial, int rows, int width, int classes,
                         cudaStream_t stream);
@@ -134,7 +136,7 @@ int tnops_linear_ce_mean(const float* loss, const int64_t* target, float* out2, 
                          int classes, int mean, cudaStream_t stream);
 int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* target, const float* lse,
                         const float* grad, int grad_step, const float* share, void* d, int piece,
-                        float* dx_f32, void* scratch, void* dx, void* dw, int dw_f32, int rows, int width,
+                        float* dx_f32, void* scratch, size_t scratch_bytes, void* dx, void* dw, int dw_f32, int rows, int width,
                         int classes, int vocab, cudaStream_t stream);
 
 // Token and position embedding: y[r] = scale * w[token[r]] + p[position[r]]

@@ -45,9 +45,10 @@ int asInt(int64_t n, const char* what) {
 
 void ok(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed (code ", rc, ")"); }
 
-at::Tensor gradsScratch(const at::Tensor& like) {
-  return at::empty({(int64_t)tnops_linear_grads_scratch()}, like.options().dtype(at::kByte));
+at::Tensor scratchOf(size_t n, const at::Tensor& like) {
+  return n ? at::empty({(int64_t)n}, like.options().dtype(at::kByte)) : at::Tensor();
 }
+void* orNull(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 uint8_t* bytes(const at::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
 
@@ -214,15 +215,17 @@ std::vector<at::Tensor> linearCeBwd(const at::Tensor& x, const at::Tensor& w,
   if (s.rows == 0 || (!wantDx && !wantDw)) return {dx, dw};
   const int64_t piece = cePiece(s.rows, s.classes, budget);
   auto d = at::empty({(int64_t)s.rows, piece}, x.options());
-  auto scratch = gradsScratch(x);
+  const size_t scratchBytes =
+      tnops_linear_ce_scratch(s.rows, s.width, s.classes, (int)piece, wantDx, wantDw);
+  auto scratch = scratchOf(scratchBytes, x);
   at::Tensor dxF32;
   if (wantDx && piece < s.classes) dxF32 = at::empty(x.sizes(), x.options().dtype(at::kFloat));
   ok(tnops_linear_ce_bwd(x.data_ptr(), w.data_ptr(), target.data_ptr<int64_t>(),
                          lse.data_ptr<float>(), grad.data_ptr<float>(),
                          grad.numel() == 1 ? 0 : 1, share ? share->data_ptr<float>() : nullptr,
                          d.data_ptr(), (int)piece,
-                         dxF32.defined() ? dxF32.data_ptr<float>() : nullptr,
-                         scratch.data_ptr(), wantDx ? dx.data_ptr() : nullptr, wantDw ? dw.data_ptr() : nullptr,
+                         static_cast<float*>(orNull(dxF32)),
+                         orNull(scratch), scratchBytes, orNull(dx), orNull(dw),
                          dwF32 ? 1 : 0, s.rows, s.width, s.classes, s.vocab, streamOf(x)),
      "tnops_linear_ce_bwd");
   return {dx, dw};
@@ -354,10 +357,11 @@ std::vector<at::Tensor> linearGradsInt8(const at::Tensor& grad, const at::Tensor
   }
   at::Tensor x;
   if (wantDw) x = dequantizeInt8(q, e, false);
-  auto scratch = gradsScratch(grad);
-  ok(tnops_linear_grads(grad.data_ptr(), outs, w.data_ptr(), wantDw ? x.data_ptr() : nullptr,
-                        wantDx ? dx.data_ptr() : nullptr, wantDw ? dw.data_ptr() : nullptr,
-                        dwF32 ? 1 : 0, rows, outs, ins, scratch.data_ptr(), streamOf(grad)),
+  const size_t scratchBytes = tnops_linear_grads_scratch(rows, outs, ins, wantDx, wantDw);
+  auto scratch = scratchOf(scratchBytes, grad);
+  ok(tnops_linear_grads(grad.data_ptr(), outs, w.data_ptr(), orNull(x), orNull(dx), orNull(dw),
+                        dwF32 ? 1 : 0, rows, outs, ins, orNull(scratch), scratchBytes,
+                        streamOf(grad)),
      "tnops_linear_grads");
   return {dx, dw};
 }

@@ -9,7 +9,8 @@ import torch
 
 from conftest import ROOT, run
 
-P, I, L, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+P, I, L, F, S = (ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float,
+                 ctypes.c_size_t)
 A = 1 << 20  # an aligned address; never dereferenced on these paths
 
 
@@ -17,6 +18,12 @@ def _launcher(name, *types):
     f = getattr(ctypes.CDLL(os.path.join(ROOT, "tiny_nccl_b200", "lib", "libtnccl_ops.so")), name)
     f.argtypes, f.restype = types, I
     return f
+
+
+def _scratch(name, *args):
+    f = _launcher(name, *[I] * len(args))
+    f.restype = S
+    return f(*args)
 
 
 def _refuses(f, good, bad):
@@ -27,21 +34,31 @@ def _refuses(f, good, bad):
 
 
 def test_linear_grads_launcher_refuses(built):
-    f = _launcher("tnops_linear_grads", P, L, P, P, P, P, I, I, I, I, P, P)
-    good = [A, 64, A, A, A, A, 0, 32, 64, 128, A, None]
-    _refuses(f, good, [(0, None), (0, A + 8), (1, 60), (1, 32), (2, A + 2), (2, None), (3, A + 4),
-                       (3, None), (4, A + 8), (5, A + 8), (7, 0), (8, 0), (9, 0), (9, 132), (10, None), (10, A + 8)])
+    f = _launcher("tnops_linear_grads", P, L, P, P, P, P, I, I, I, I, P, S, P)
+    # 8192 rows of a 768 -> 768 layer: dW's nine tiles are cut.
+    need = _scratch("tnops_linear_grads_scratch", 8192, 768, 768, 1, 1)
+    assert need > 0 and need % (256 * 256 * 4) == 0
+    good = [A, 768, A, A, A, A, 0, 8192, 768, 768, A, need, None]
+    _refuses(f, good, [(0, None), (0, A + 8), (1, 764), (1, 760), (2, A + 2), (2, None),
+                       (3, A + 4), (3, None), (4, A + 8), (5, A + 8), (7, 0), (8, 0), (9, 0),
+                       (9, 764), (10, None), (10, A + 8), (11, need - 1)])
+    assert _scratch("tnops_linear_grads_scratch", 0, 768, 768, 1, 1) == 0
+    assert _scratch("tnops_linear_grads_scratch", 33, 512, 128, 1, 1) == 0
 
 
 def test_linear_ce_launchers_refuse(built):
     f = _launcher("tnops_linear_ce_fwd", P, P, P, P, P, P, I, I, I, P)
     good = [A, A, A, A, A, A, 4, 64, 100, None]
     _refuses(f, good, [(0, A + 8), (1, A + 8), (6, 0), (7, 0), (7, 60), (8, 0)])
-    f = _launcher("tnops_linear_ce_bwd", P, P, P, P, P, I, P, P, I, P, P, P, P, I, I, I, I, I, P)
-    good = [A, A, A, A, A, 0, A, A, 256, A, A, A, A, 1, 4, 64, 300, 304, None]
+    f = _launcher("tnops_linear_ce_bwd", P, P, P, P, P, I, P, P, I, P, P, S, P, P, I, I, I, I, I, P)
+    good = [A, A, A, A, A, 0, A, A, 256, A, None, 0, A, A, 1, 4, 64, 300, 304, None]
     _refuses(f, good, [(0, A + 8), (1, A + 8), (7, A + 8), (8, 0), (8, 20), (9, None),
-                       (9, A + 4), (10, None), (10, A + 8), (11, A + 8), (12, A + 4), (14, 0),
-                       (15, 60), (16, 0), (17, 299)])
+                       (9, A + 4), (10, A + 8), (12, A + 8), (13, A + 4), (15, 0),
+                       (16, 60), (17, 0), (18, 299)])
+    # The scratch of the first pieces and of the last, shorter one.
+    a, b, c = (_scratch("tnops_linear_grads_scratch", 1024, n, 768, 1, 1) for n in (768, 232, 1000))
+    assert _scratch("tnops_linear_ce_scratch", 1024, 768, 1000, 768, 1, 1) == max(a, b)
+    assert _scratch("tnops_linear_ce_scratch", 1024, 768, 1000, 1024, 1, 1) == c
     f = _launcher("tnops_linear_ce_mean", P, P, P, I, I, I, P)
     assert f(A, A, A, 0, 5, 1, None) == 1
 
