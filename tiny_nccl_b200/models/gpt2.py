@@ -14,6 +14,12 @@ Two implementations share one parameter layout:
 * ``impl="torch"``: the same math in stock PyTorch ops; it is the fp32
   numerics reference for the fused kernels and the path the CPU tests use.
 
+The fused implementation has three options, each the default's math on other
+kernels: ``embedding="fused"`` (token + position embedding and the gradients of
+both tables by sorted tokens), ``head="pieces"`` (LM head and loss without the
+logits in memory), ``activations="int8"`` (the blocks' linear layers keep
+what their backward pass reads in 8 bits).
+
 The reference (tiny-nccl) has no model; this is the workload of the
 "GPT-2 small DP tokens/s" headline metric.
 """
@@ -71,9 +77,10 @@ class Block(nn.Module):
         self.mlp_fc = nn.Linear(d, 4 * d)
         self.mlp_proj = nn.Linear(4 * d, d)
 
-    def attention(self, h: torch.Tensor, ops=None) -> torch.Tensor:
+    def attention(self, h: torch.Tensor, ops=None, activations: str = "bf16") -> torch.Tensor:
         B, T, C = h.shape
-        qkv = ops.linear(h, self.attn_qkv.weight, self.attn_qkv.bias) if ops else self.attn_qkv(h)
+        qkv = (ops.linear(h, self.attn_qkv.weight, self.attn_qkv.bias, activations) if ops
+               else self.attn_qkv(h))
         q, k, v = qkv.split(C, dim=2)
         hd = C // self.n_head
         q = q.view(B, T, self.n_head, hd).transpose(1, 2)
@@ -82,7 +89,7 @@ class Block(nn.Module):
         y = F.scaled_dot_product_attention(q, k, v, is_causal=True)
         y = y.transpose(1, 2).contiguous().view(B, T, C)
         if ops:
-            return ops.linear(y, self.attn_proj.weight, self.attn_proj.bias)
+            return ops.linear(y, self.attn_proj.weight, self.attn_proj.bias, activations)
         return self.attn_proj(y)
 
     def forward_torch(self, x: torch.Tensor) -> torch.Tensor:
@@ -90,18 +97,27 @@ class Block(nn.Module):
         h = F.gelu(self.mlp_fc(self.ln_2(x)), approximate="tanh")
         return x + self.mlp_proj(h)
 
-    def mlp_fused(self, h: torch.Tensor, ops) -> torch.Tensor:
-        g = ops.linear_gelu(h, self.mlp_fc.weight, self.mlp_fc.bias)
-        return ops.linear(g, self.mlp_proj.weight, self.mlp_proj.bias)
+    def mlp_fused(self, h: torch.Tensor, ops, activations: str = "bf16") -> torch.Tensor:
+        g = ops.linear_gelu(h, self.mlp_fc.weight, self.mlp_fc.bias, activations)
+        return ops.linear(g, self.mlp_proj.weight, self.mlp_proj.bias, activations)
 
 
 class GPT2(nn.Module):
-    def __init__(self, cfg: GPT2Config | None = None, impl: str = "fused"):
+    def __init__(self, cfg: GPT2Config | None = None, impl: str = "fused", *,
+                 embedding: str = "torch", head: str = "logits", activations: str = "bf16"):
         super().__init__()
         self.cfg = cfg or GPT2Config()
         if impl not in ("fused", "torch"):
             raise ValueError(f"unknown impl {impl!r}")
+        for name, value, known in (("embedding", embedding, ("torch", "fused")),
+                                   ("head", head, ("logits", "pieces")),
+                                   ("activations", activations, ("bf16", "int8"))):
+            if value not in known:
+                raise ValueError(f"{name} must be one of {known}, not {value!r}")
+            if impl == "torch" and value != known[0]:
+                raise ValueError(f"{name}={value!r} needs impl='fused'")
         self.impl = impl
+        self.embedding, self.head, self.activations = embedding, head, activations
         c = self.cfg
         self.wte = nn.Embedding(c.vocab_padded, c.n_embd)
         self.wpe = nn.Embedding(c.block_size, c.n_embd)
@@ -138,8 +154,13 @@ class GPT2(nn.Module):
         """Returns the mean cross-entropy loss when targets are given, else the
         logits of the last position."""
         B, T = idx.shape
-        pos = torch.arange(T, device=idx.device)
-        x = self.wte(idx) + self.wpe(pos)  # fp32 residual stream
+        if self.embedding == "fused":
+            if T > self.cfg.block_size:
+                raise ValueError(f"{T} tokens exceed the context of {self.cfg.block_size}")
+            x = self._ops().embedding(idx, self.wte.weight, self.wpe.weight)
+        else:
+            pos = torch.arange(T, device=idx.device)
+            x = self.wte(idx) + self.wpe(pos)  # fp32 residual stream
         if self.impl == "fused":
             return self._forward_fused(x, targets)
         for blk in self.blocks:
@@ -161,13 +182,16 @@ class GPT2(nn.Module):
         h = ops.layer_norm(x, first.weight, first.bias)
         L = len(self.blocks)
         for i, blk in enumerate(self.blocks):
-            a = blk.attention(h.view(B, T, C), ops)
+            a = blk.attention(h.view(B, T, C), ops, self.activations)
             x, h = ops.add_layer_norm(x, a.reshape(B * T, C), blk.ln_2.weight, blk.ln_2.bias)
-            m = blk.mlp_fused(h, ops)
+            m = blk.mlp_fused(h, ops, self.activations)
             nxt = self.blocks[i + 1].ln_1 if i + 1 < L else self.ln_f
             x, h = ops.add_layer_norm(x, m, nxt.weight, nxt.bias)
         if targets is None:
             last = h.view(B, T, C)[:, -1]
             return ops.linear_nobias(last, self.wte.weight)[..., :self.cfg.vocab_size]
+        if self.head == "pieces":
+            return ops.linear_cross_entropy(h, self.wte.weight, targets.reshape(-1),
+                                            classes=self.cfg.vocab_size)
         logits = ops.linear_nobias(h, self.wte.weight)
         return ops.cross_entropy(logits, targets.reshape(-1), classes=self.cfg.vocab_size)
