@@ -14,10 +14,10 @@
 //                    chunk (equal ones count in chunks before its own), found
 //                    by binary searches: a stable sort in two launches, one
 //                    when a single chunk holds all rows;
-//   3. tableGrads    the sorted rows in blocks of 16: a group of threads, one
-//                    per four columns, adds the gradients of each run of
-//                    equal tokens in row order and writes the table row of a
-//                    run that lies within its block; runs cut by a block's
+//   3. tableGrads    the sorted rows in blocks of 16 to 64: a group of threads,
+//                    one per 16 bytes of a row, adds the gradients of each run
+//                    of equal tokens in row order and writes the table row of
+//                    a run that lies within its block; runs cut by a block's
 //                    border leave fp32 partial sums. Other CTAs of the launch
 //                    write the rows that no token names: zeros;
 //   4. joinRuns      adds the partial sums of each cut run in block order.
@@ -32,89 +32,160 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Four neighbouring values.
-__device__ __forceinline__ float4 load4(const float* p) {
-  return __ldg(reinterpret_cast<const float4*>(p));
+// N neighbouring values of a row. FAST: whole 8- or 16-byte pieces (cols % N
+// == 0 and aligned rows); else one by one, the ones past the row's end zero.
+template <int N>
+struct Cols {
+  float v[N];
+};
+// N values as they lie in memory: what a load in flight holds in registers.
+template <class T, int N>
+struct Raw {
+  uint32_t w[N * sizeof(T) / 4];
+};
+template <bool FAST, int N, class T>
+__device__ __forceinline__ Raw<T, N> loadRaw(const T* row, int c, int cols) {
+  Raw<T, N> r;
+  constexpr int W = N * sizeof(T) / 4;
+  if (FAST) {
+    if (W == 2) {
+      const uint2 u = __ldg(reinterpret_cast<const uint2*>(row + c));
+      r.w[0] = u.x; r.w[1] = u.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; i += 4) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + c) + i / 4);
+        r.w[i] = u.x; r.w[i + 1] = u.y; r.w[i + 2] = u.z; r.w[i + 3] = u.w;
+      }
+    }
+  } else if (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      r.w[i] = c + i < cols ? *reinterpret_cast<const uint32_t*>(row + c + i) : 0u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const uint32_t lo = c + i < cols ? *reinterpret_cast<const uint16_t*>(row + c + i) : 0u;
+      const uint32_t hi =
+          c + i + 1 < cols ? *reinterpret_cast<const uint16_t*>(row + c + i + 1) : 0u;
+      r.w[i / 2] = lo | hi << 16;
+    }
+  }
+  return r;
 }
-__device__ __forceinline__ float4 load4(const uint16_t* p) {
-  return bf4(__ldg(reinterpret_cast<const uint2*>(p)));
+template <class T, int N>
+__device__ __forceinline__ Raw<T, N> zeroRaw() {
+  Raw<T, N> r;
+#pragma unroll
+  for (int i = 0; i < (int)(N * sizeof(T) / 4); ++i) r.w[i] = 0u;
+  return r;
 }
-__device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
-__device__ __forceinline__ void store4(uint16_t* p, float4 v) {
-  *reinterpret_cast<uint2*>(p) = tobf4(v);
+template <class T, int N>
+__device__ __forceinline__ Cols<N> unpack(const Raw<T, N>& r) {
+  Cols<N> v;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    v.v[i] = __uint_as_float(sizeof(T) == 4 ? r.w[i]
+                             : (i & 1)      ? r.w[i / 2] & 0xffff0000u
+                                            : r.w[i / 2] << 16);
+  return v;
 }
-__device__ __forceinline__ float load1(const float* p) { return *p; }
-__device__ __forceinline__ float load1(const uint16_t* p) { return bf2f(*p); }
+template <int N>
+__device__ __forceinline__ void storeFast(float* p, const float* v) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4)
+    *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+}
+template <int N>
+__device__ __forceinline__ void storeFast(uint16_t* p, const float* v) {
+  const uint2 a = tobf4(make_float4(v[0], v[1], v[2], v[3]));
+  if (N == 8) {
+    const uint2 b = tobf4(make_float4(v[4], v[5], v[6], v[7]));
+    *reinterpret_cast<uint4*>(p) = make_uint4(a.x, a.y, b.x, b.y);
+  } else {
+    *reinterpret_cast<uint2*>(p) = a;
+  }
+}
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store1(uint16_t* p, float v) { *p = f2bf(v); }
 
-// Columns c .. c + 3 of a row of `cols`: whole when VEC (cols % 4 == 0 and
-// aligned rows), else one by one with the missing ones zero.
-template <bool VEC, class T>
-__device__ __forceinline__ float4 loadCols(const T* row, int c, int cols) {
-  if (VEC) return load4(row + c);
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  v.x = load1(row + c);
-  if (c + 1 < cols) v.y = load1(row + c + 1);
-  if (c + 2 < cols) v.z = load1(row + c + 2);
-  if (c + 3 < cols) v.w = load1(row + c + 3);
-  return v;
+template <bool FAST, int N, class T>
+__device__ __forceinline__ Cols<N> loadCols(const T* row, int c, int cols) {
+  return unpack(loadRaw<FAST, N>(row, c, cols));
 }
-template <bool VEC, class T>
-__device__ __forceinline__ void storeCols(T* row, int c, int cols, float4 v) {
-  if (VEC) {
-    store4(row + c, v);
-    return;
+template <bool FAST, int N, class T>
+__device__ __forceinline__ void storeCols(T* row, int c, int cols, const Cols<N>& r) {
+  if (FAST) {
+    storeFast<N>(row + c, r.v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (c + i < cols) store1(row + c + i, r.v[i]);
   }
-  store1(row + c, v.x);
-  if (c + 1 < cols) store1(row + c + 1, v.y);
-  if (c + 2 < cols) store1(row + c + 2, v.z);
-  if (c + 3 < cols) store1(row + c + 3, v.w);
 }
-__device__ __forceinline__ float4 add4(float4 a, float4 b) {
-  return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+template <int N>
+__device__ __forceinline__ Cols<N> zeroCols() {
+  Cols<N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) r.v[i] = 0.f;
+  return r;
 }
-__device__ __forceinline__ float4 scale4(float4 a, float s) {
-  return make_float4(a.x * s, a.y * s, a.z * s, a.w * s);
+template <int N>
+__device__ __forceinline__ void addTo(Cols<N>& a, const Cols<N>& b) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) a.v[i] += b.v[i];
+}
+template <int N>
+__device__ __forceinline__ Cols<N> scaled(const Cols<N>& a, float s) {
+  Cols<N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) r.v[i] = a.v[i] * s;
+  return r;
 }
 
-// A group of `group` threads (a power of two) per row, four columns each and
-// `group * 4` apart, several rows in flight per group. Bound by memory: a row
-// of each table read, one written.
-constexpr int kFwdRows = 4;
-template <class W, class Y, bool VEC>
-__global__ void __launch_bounds__(kThreads)
+// A CTA takes `per` rows: their indices first, then the rows' pieces of N
+// columns in turn, so that several loads per thread are in flight whatever the
+// width. Bound by memory: a row of each table read, one written.
+constexpr int kFwdMaxRows = 16;
+template <class W, class Y, bool FAST, int N>
+__global__ void __launch_bounds__(kThreads, 4)
     embeddingFwd(const int64_t* __restrict__ token, const int64_t* __restrict__ position,
                  const W* __restrict__ w, const W* __restrict__ p, Y* __restrict__ y, int rows,
-                 int seq, int vocab, int context, int cols, float scale, int group) {
-  const int lane = threadIdx.x & (group - 1);
-  const int64_t first =
-      ((int64_t)blockIdx.x * (kThreads / group) + threadIdx.x / group) * kFwdRows;
-  const W* wr[kFwdRows];
-  const W* pr[kFwdRows];
-#pragma unroll
-  for (int i = 0; i < kFwdRows; ++i) {
-    wr[i] = pr[i] = nullptr;
-    const int64_t r = first + i;
-    if (r >= rows) continue;
-    const int64_t t = token[r], at = position ? position[r] : r % seq;
-    if (t >= 0 && t < vocab) wr[i] = w + t * cols;
-    if (p != nullptr && at >= 0 && at < context) pr[i] = p + at * cols;
+                 int seq, int vocab, int context, int cols, float scale, int per) {
+  __shared__ const W* sW[kFwdMaxRows];
+  __shared__ const W* sP[kFwdMaxRows];
+  const int64_t first = (int64_t)blockIdx.x * per;
+  const int n = (int)min((int64_t)per, rows - first);
+  if (threadIdx.x < n) {
+    const int64_t r = first + threadIdx.x, t = token[r];
+    const int64_t at = position ? position[r] : r % seq;
+    sW[threadIdx.x] = t >= 0 && t < vocab ? w + t * cols : nullptr;
+    sP[threadIdx.x] = p != nullptr && at >= 0 && at < context ? p + at * cols : nullptr;
   }
-  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c = lane * 4; c < cols; c += group * 4) {
-    float4 a[kFwdRows], b[kFwdRows];
+  __syncthreads();
+  const uint32_t pieces = (uint32_t)(cols + N - 1) / N, all = pieces * n;
+  constexpr int U = 4;
+  for (uint32_t i0 = threadIdx.x; i0 < all; i0 += U * kThreads) {
+    Raw<W, N> a[U], b[U];
 #pragma unroll
-    for (int i = 0; i < kFwdRows; ++i) {
-      a[i] = wr[i] ? loadCols<VEC>(wr[i], c, cols) : zero;
-      b[i] = pr[i] ? loadCols<VEC>(pr[i], c, cols) : zero;
+    for (int u = 0; u < U; ++u) {
+      const uint32_t i = i0 + u * kThreads;
+      if (i >= all) break;
+      const uint32_t r = i / pieces, c = (i - r * pieces) * N;
+      a[u] = sW[r] ? loadRaw<FAST, N>(sW[r], c, cols) : zeroRaw<W, N>();
+      b[u] = sP[r] ? loadRaw<FAST, N>(sP[r], c, cols) : zeroRaw<W, N>();
     }
 #pragma unroll
-    for (int i = 0; i < kFwdRows; ++i)
-      if (first + i < rows)
-        storeCols<VEC>(y + (first + i) * cols, c, cols,
-                       make_float4(a[i].x * scale + b[i].x, a[i].y * scale + b[i].y,
-                                   a[i].z * scale + b[i].z, a[i].w * scale + b[i].w));
+    for (int u = 0; u < U; ++u) {
+      const uint32_t i = i0 + u * kThreads;
+      if (i >= all) break;
+      const uint32_t r = i / pieces, c = (i - r * pieces) * N;
+      Cols<N> x = unpack(a[u]);
+      const Cols<N> q = unpack(b[u]);
+#pragma unroll
+      for (int k = 0; k < N; ++k) x.v[k] = x.v[k] * scale + q.v[k];
+      storeCols<FAST, N>(y + (first + r) * cols, c, cols, x);
+    }
   }
 }
 
@@ -131,57 +202,89 @@ __device__ __forceinline__ constexpr int chunkBits() {
   return CHUNK == 1024 ? 10 : 12;
 }
 
-// Bitonic sort of CHUNK keys. A thread holds pairs only in shared memory; the
-// steps at distances below 32 pairs need no more than warp order, but a CTA
-// barrier each keeps this short kernel simple. With one chunk the result
-// goes straight to `skey` / `perm`.
+// Bitonic sort of CHUNK keys, CHUNK / 1024 neighbouring ones per thread: steps
+// at a distance inside a thread's keys need no exchange, those inside a warp
+// shuffle, and only the 15 at longer distances go through shared memory. With
+// one chunk the result goes straight to `skey` / `perm`.
 template <class Key, int CHUNK>
 __global__ void __launch_bounds__(kSortThreads)
     sortChunks(const int64_t* __restrict__ token, Key* __restrict__ sorted,
                int* __restrict__ skey, int* __restrict__ perm, int rows, int vocab) {
-  __shared__ Key s[CHUNK];
   constexpr int bits = chunkBits<Key, CHUNK>();
+  constexpr int E = CHUNK / kSortThreads;
+  __shared__ Key s[CHUNK];
   const int64_t base = (int64_t)blockIdx.x * CHUNK;
-  for (int i = threadIdx.x; i < CHUNK; i += kSortThreads) {
-    Key k = ~(Key)0;
-    if (base + i < rows) {
-      const int64_t t = token[base + i];
-      k = ((Key)(t >= 0 && t < vocab ? t : vocab) << bits) | (Key)i;
+  const int t0 = threadIdx.x * E;
+  Key k[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    const int64_t r = base + t0 + j;
+    k[j] = ~(Key)0;
+    if (r < rows) {
+      const int64_t t = token[r];
+      k[j] = ((Key)(t >= 0 && t < vocab ? t : vocab) << bits) | (Key)(t0 + j);
     }
-    s[i] = k;
   }
-  __syncthreads();
-  for (int size = 2; size <= CHUNK; size <<= 1)
+#pragma unroll
+  for (int size = 2; size <= CHUNK; size <<= 1) {
+#pragma unroll
     for (int d = size >> 1; d > 0; d >>= 1) {
-      for (int t = threadIdx.x; t < CHUNK / 2; t += kSortThreads) {
-        const int i = 2 * t - (t & (d - 1)), j = i + d;
-        const Key a = s[i], b = s[j];
-        if ((a > b) == ((i & size) == 0)) {
-          s[i] = b;
-          s[j] = a;
+      if (d < E) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          if (j & d) continue;
+          const bool up = ((t0 + j) & size) == 0;
+          const Key a = k[j], b = k[j | d];
+          const bool swap = (a > b) == up;
+          k[j] = swap ? b : a;
+          k[j | d] = swap ? a : b;
+        }
+      } else {
+        // The partner of key i is key i ^ d, held by thread ^ (d / E).
+        const bool up = (t0 & size) == 0, low = (t0 & d) == 0;
+        if (d >= 32 * E) {
+          __syncthreads();
+#pragma unroll
+          for (int j = 0; j < E; ++j) s[t0 + j] = k[j];
+          __syncthreads();
+        }
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const Key other = d >= 32 * E ? s[(t0 + j) ^ d]
+                                        : __shfl_xor_sync(0xffffffffu, k[j], (d / E) & 31);
+          const bool takeMin = low == up;
+          k[j] = (other < k[j]) == takeMin ? other : k[j];
         }
       }
-      __syncthreads();
     }
-  for (int i = threadIdx.x; i < CHUNK && base + i < rows; i += kSortThreads) {
-    const Key k = s[i];
+  }
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    const int64_t r = base + t0 + j;
+    if (r >= rows) continue;
     if (gridDim.x == 1) {
-      skey[i] = (int)(k >> bits);
-      perm[i] = (int)(k & (CHUNK - 1));
+      skey[r] = (int)(k[j] >> bits);
+      perm[r] = (int)(k[j] & (CHUNK - 1));
     } else {
-      sorted[base + i] = k;
+      sorted[r] = k[j];
     }
   }
 }
 
+// Several chunks at a time in shared memory (128 KiB), one search in each
+// going on side by side.
 constexpr int kMergeThreads = 512;
+constexpr uint32_t kMergeSmem = 128 * 1024;
 
 template <class Key, int CHUNK>
 __global__ void __launch_bounds__(kMergeThreads)
     mergeRanks(const Key* __restrict__ sorted, int* __restrict__ skey, int* __restrict__ perm,
                int rows) {
-  __shared__ Key s[CHUNK];
+  extern __shared__ __align__(16) uint8_t smem[];
+  Key* s = reinterpret_cast<Key*>(smem);
   constexpr int bits = chunkBits<Key, CHUNK>();
+  constexpr int at1 = kMergeSmem / (CHUNK * sizeof(Key));  // chunks at a time
+  constexpr int side = 4;                                  // searches side by side
   const int64_t at = (int64_t)blockIdx.x * kMergeThreads + threadIdx.x;  // CHUNK % 512 == 0
   const int own = (int)((int64_t)blockIdx.x * kMergeThreads / CHUNK);
   const int chunks = (rows + CHUNK - 1) / CHUNK;
@@ -189,19 +292,38 @@ __global__ void __launch_bounds__(kMergeThreads)
   const Key key = has ? sorted[at] : 0;
   const Key token = key >> bits;
   int rank = (int)(at - (int64_t)own * CHUNK);
-  for (int c = 0; c < chunks; ++c) {
-    if (c == own) continue;
-    const int n = min(CHUNK, rows - c * CHUNK);
+  for (int c0 = 0; c0 < chunks; c0 += at1) {
+    const int64_t from = (int64_t)c0 * CHUNK;
+    const int n = (int)min((int64_t)at1 * CHUNK, rows - from);
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kMergeThreads) s[i] = sorted[(int64_t)c * CHUNK + i];
+    // 16-byte pieces; the last may run past n, into scratch that follows.
+    for (int i = threadIdx.x; i < (int)((n * sizeof(Key) + 15) / 16); i += kMergeThreads)
+      reinterpret_cast<uint4*>(smem)[i] =
+          __ldg(reinterpret_cast<const uint4*>(sorted + from) + i);
     __syncthreads();
-    // The keys below `limit` come before this one.
-    const Key limit = (token + (c < own ? 1 : 0)) << bits;
-    int lo = 0;
+    const int here = (n + CHUNK - 1) / CHUNK;
+    for (int c = 0; c < here; c += side) {
+      // lo: how many of the chunk's keys come before this one.
+      int lo[side], len[side];
+      Key limit[side];
 #pragma unroll
-    for (int step = CHUNK; step > 0; step >>= 1)
-      if (lo + step <= n && s[lo + step - 1] < limit) lo += step;
-    rank += lo;
+      for (int u = 0; u < side; ++u) {
+        const int chunk = c0 + c + u;
+        lo[u] = 0;
+        len[u] = c + u < here && chunk != own ? min(CHUNK, n - (c + u) * CHUNK) : 0;
+        limit[u] = (token + (chunk < own ? 1 : 0)) << bits;
+      }
+#pragma unroll 1
+      for (int step = CHUNK; step > 0; step >>= 1) {
+#pragma unroll
+        for (int u = 0; u < side; ++u) {
+          const int next = lo[u] + step;
+          if (next <= len[u] && s[(c + u) * CHUNK + next - 1] < limit[u]) lo[u] = next;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < side; ++u) rank += lo[u];
+    }
   }
   if (has) {
     skey[rank] = (int)token;
@@ -211,7 +333,7 @@ __global__ void __launch_bounds__(kMergeThreads)
 
 // -- gradients of the tables -------------------------------------------------------
 
-constexpr int kBlock = 16;  // sorted rows per block
+constexpr int kMaxBlock = 64;
 
 // A table's gradient. Sorted place i holds token key(i) of row row(i); without
 // arrays the order of r % seq: place i is row (i % batch) * seq + i / batch.
@@ -223,6 +345,8 @@ struct Table {
   int seq, batch;  // used when skey is null
   int vocab;
   float scale;
+  int block, blocks;  // sorted rows per block, blocks
+  int sumCtas, zeroCtas;
 
   __device__ __forceinline__ int key(int i) const { return skey ? skey[i] : i / batch; }
   __device__ __forceinline__ int row(int i) const {
@@ -233,9 +357,7 @@ struct TableGradArgs {
   Table table[2];
   int tables;
   int rows, cols;
-  int blocks;           // ceil(rows / kBlock)
-  int group, sumCtas;   // threads per block of rows, CTAs of them per table
-  int zeroCtas[2];      // CTAs that write rows without a token
+  int group;  // threads per block of rows
 };
 constexpr int kZeroRows = 64;  // table rows per such CTA
 
@@ -256,24 +378,27 @@ __device__ __forceinline__ int lowerBound(const Table& t, int rows, int v) {
   return lo;
 }
 
-template <class G, class W, bool VEC>
-__global__ void __launch_bounds__(kThreads)
+template <class G, class W, bool FAST, int N>
+__global__ void __launch_bounds__(kThreads, 4)
     tableGrads(const G* __restrict__ g, const __grid_constant__ TableGradArgs a) {
-  __shared__ int sKey[kThreads / 8][kBlock + 2];  // with the neighbours' keys
-  __shared__ int sRow[kThreads / 8][kBlock];
+  __shared__ int sKey[kThreads / 8][kMaxBlock + 2];  // with the neighbours' keys
+  __shared__ int sRow[kThreads / 8][kMaxBlock];
   __shared__ uint8_t sEmpty[kZeroRows];
   int cta = blockIdx.x, which = 0;
-  if (cta >= a.sumCtas + a.zeroCtas[0]) {
-    cta -= a.sumCtas + a.zeroCtas[0];
-    which = 1;
-  }
+  // Sums of both tables first, then the rows of zeros.
+  const int sums = a.table[0].sumCtas + (a.tables > 1 ? a.table[1].sumCtas : 0);
+  const bool zeros = cta >= sums;
+  if (zeros) cta -= sums;
+  const int before = zeros ? a.table[0].zeroCtas : a.table[0].sumCtas;
+  which = cta >= before;
+  if (which) cta -= before;
   const Table& t = a.table[which];
   const int cols = a.cols, group = a.group;
   W* out = static_cast<W*>(t.out);
-  const int tile0 = blockIdx.y * group * 4;
-  if (cta >= a.sumCtas) {
+  const int tile0 = blockIdx.y * group * N;
+  if (zeros) {
     // Rows without a token.
-    const int v0 = (cta - a.sumCtas) * kZeroRows;
+    const int v0 = cta * kZeroRows;
     if (threadIdx.x < kZeroRows) {
       const int v = v0 + threadIdx.x;
       bool empty = false;
@@ -284,49 +409,48 @@ __global__ void __launch_bounds__(kThreads)
       sEmpty[threadIdx.x] = empty;
     }
     __syncthreads();
-    const int c = tile0 + (threadIdx.x & (group - 1)) * 4;
+    const int c = tile0 + (threadIdx.x & (group - 1)) * N;
     if (c < cols)
       for (int i = threadIdx.x / group; i < kZeroRows; i += kThreads / group)
-        if (sEmpty[i])
-          storeCols<VEC>(out + (int64_t)(v0 + i) * cols, c, cols,
-                         make_float4(0.f, 0.f, 0.f, 0.f));
+        if (sEmpty[i]) storeCols<FAST, N>(out + (int64_t)(v0 + i) * cols, c, cols, zeroCols<N>());
     return;
   }
   const int slot = threadIdx.x / group, lane = threadIdx.x & (group - 1);
   const int block = cta * (kThreads / group) + slot;
-  const int first = block * kBlock;
-  const int n = min(kBlock, a.rows - first);
-  for (int i = lane; i < kBlock + 2; i += group) {
+  const int first = block * t.block;
+  const int n = min(t.block, a.rows - first);
+  for (int i = lane; i < t.block + 2; i += group) {
     const int at = first + i - 1;
     sKey[slot][i] = at >= 0 && at < a.rows ? t.key(at) : -1;
-    if (i >= 1 && i <= kBlock && at < a.rows) sRow[slot][i - 1] = t.row(at);
+    if (i >= 1 && i <= t.block && at < a.rows) sRow[slot][i - 1] = t.row(at);
   }
   __syncthreads();
-  const int c = tile0 + lane * 4;
+  const int c = tile0 + lane * N;
   if (n <= 0 || c >= cols) return;
   const int* key = sKey[slot] + 1;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  Cols<N> acc = zeroCols<N>();
   bool head = key[0] == key[-1];  // the current run began in a block before
   constexpr int U = 8;
   for (int i0 = 0; i0 < n; i0 += U) {
-    float4 v[U];
+    Raw<G, N> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (i0 + u < n) v[u] = loadCols<VEC>(g + (int64_t)sRow[slot][i0 + u] * cols, c, cols);
+      if (i0 + u < n) v[u] = loadRaw<FAST, N>(g + (int64_t)sRow[slot][i0 + u] * cols, c, cols);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = i0 + u;
       if (i >= n) break;
-      acc = add4(acc, v[u]);
+      addTo(acc, unpack(v[u]));
       const bool ends = key[i + 1] != key[i];
       if (ends || i == n - 1) {
         if (key[i] < t.vocab) {
           if (head || !ends)
-            storeCols<VEC>(t.partial + ((int64_t)block * 2 + (head ? 0 : 1)) * cols, c, cols, acc);
+            storeCols<FAST, N>(t.partial + ((int64_t)block * 2 + (head ? 0 : 1)) * cols, c, cols,
+                               acc);
           else
-            storeCols<VEC>(out + (int64_t)key[i] * cols, c, cols, scale4(acc, t.scale));
+            storeCols<FAST, N>(out + (int64_t)key[i] * cols, c, cols, scaled(acc, t.scale));
         }
-        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        acc = zeroCols<N>();
         head = false;
       }
     }
@@ -338,50 +462,59 @@ __global__ void __launch_bounds__(kThreads)
 // and goes on past it; a long run is added by the whole CTA, each warp an even
 // share of the blocks in order.
 constexpr int kJoinWarps = 16;
-constexpr int kLongRun = 32;  // blocks that one warp still adds by itself
+constexpr int kLongRun = 8;  // blocks that one warp still adds by itself
 
-template <bool VEC>
-__device__ __forceinline__ float4 sumBlocks(const float* partial, int from, int to, int c,
-                                            int cols) {
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+template <bool FAST>
+__device__ __forceinline__ Cols<4> sumBlocks(const float* partial, int from, int to, int c,
+                                             int cols) {
+  Cols<4> acc = zeroCols<4>();
   constexpr int U = 8;
   for (int b0 = from; b0 < to; b0 += U) {
-    float4 v[U];
+    Cols<4> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      v[u] = b0 + u < to ? loadCols<VEC>(partial + (int64_t)(b0 + u) * 2 * cols, c, cols)
-                         : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[u] = b0 + u < to ? loadCols<FAST, 4>(partial + (int64_t)(b0 + u) * 2 * cols, c, cols)
+                         : zeroCols<4>();
 #pragma unroll
-    for (int u = 0; u < U; ++u) acc = add4(acc, v[u]);
+    for (int u = 0; u < U; ++u) addTo(acc, v[u]);
   }
   return acc;
 }
 
-template <class W, bool VEC>
+template <class W, bool FAST>
 __global__ void __launch_bounds__(kJoinWarps * 32)
-    joinRuns(const __grid_constant__ TableGradArgs a) {
-  __shared__ int sLong[kJoinWarps][2];  // first and last + 1 of its later blocks
-  __shared__ float4 sPart[kJoinWarps][32];
-  const Table& t = a.table[blockIdx.z];
+    joinRuns(const __grid_constant__ TableGradArgs a, int firstTable) {
+  __shared__ int sLong[kJoinWarps][2];  // the token, and the last + 1 of its blocks
+  __shared__ Cols<4> sPart[kJoinWarps][32];
+  const Table& t = a.table[firstTable + blockIdx.z];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cols = a.cols, c = blockIdx.y * 128 + lane * 4;
   const int block = blockIdx.x * kJoinWarps + warp;
-  const int first = block * kBlock, last = min(first + kBlock, a.rows) - 1;
+  const int first = block * t.block, last = min(first + t.block, a.rows) - 1;
   W* out = static_cast<W*>(t.out);
   int token = -1, end = 0;  // blocks block + 1 .. end - 1 go on with the run
-  if (block < a.blocks && last + 1 < a.rows) {
-    const int k = t.key(last);
-    const bool begins = t.key(first) != k || first == 0 || t.key(first - 1) != k;
-    if (begins && k < t.vocab && t.key(last + 1) == k) {
+  if (block < t.blocks && last + 1 < a.rows) {
+    // The keys that decide, one per lane: this block's ends and neighbours.
+    const int at = lane == 0 ? last : lane == 1 ? last + 1 : lane == 2 ? first : first - 1;
+    const int k4 = lane < 4 && at >= 0 ? t.key(at) : -1;
+    const int k = __shfl_sync(0xffffffffu, k4, 0), after = __shfl_sync(0xffffffffu, k4, 1);
+    const int begin = __shfl_sync(0xffffffffu, k4, 2), before = __shfl_sync(0xffffffffu, k4, 3);
+    if (k == after && k < t.vocab && (begin != k || before != k)) {
       token = k;
-      end = (lowerBound(t, a.rows, k + 1) - 1) / kBlock + 1;
+      // The run ends with the first of the next 32 blocks whose follower
+      // does not begin with the token; past them, a search.
+      const int b = block + 1 + lane;
+      const bool ends = b >= t.blocks - 1 || t.key((b + 1) * t.block) != k;
+      const uint32_t votes = __ballot_sync(0xffffffffu, ends);
+      end = votes ? block + 1 + __ffs(votes)
+                  : (lowerBound(t, a.rows, k + 1) - 1) / t.block + 1;
     }
   }
   const bool isLong = token >= 0 && end - block > kLongRun;
   if (token >= 0 && !isLong && c < cols) {
-    const float4 head = loadCols<VEC>(t.partial + ((int64_t)block * 2 + 1) * cols, c, cols);
-    const float4 rest = sumBlocks<VEC>(t.partial, block + 1, end, c, cols);
-    storeCols<VEC>(out + (int64_t)token * cols, c, cols, scale4(add4(head, rest), t.scale));
+    Cols<4> sum = loadCols<FAST, 4>(t.partial + ((int64_t)block * 2 + 1) * cols, c, cols);
+    addTo(sum, sumBlocks<FAST>(t.partial, block + 1, end, c, cols));
+    storeCols<FAST, 4>(out + (int64_t)token * cols, c, cols, scaled(sum, t.scale));
   }
   if (lane == 0) {
     sLong[warp][0] = isLong ? token : -1;
@@ -393,14 +526,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
     const int from = blockIdx.x * kJoinWarps + w + 1, to = sLong[w][1];
     const int per = (to - from + kJoinWarps - 1) / kJoinWarps;
     if (c < cols)
-      sPart[warp][lane] = sumBlocks<VEC>(t.partial, min(to, from + warp * per),
-                                         min(to, from + (warp + 1) * per), c, cols);
+      sPart[warp][lane] = sumBlocks<FAST>(t.partial, min(to, from + warp * per),
+                                          min(to, from + (warp + 1) * per), c, cols);
     __syncthreads();
     if (warp == 0 && c < cols) {
-      float4 acc = loadCols<VEC>(t.partial + ((int64_t)(from - 1) * 2 + 1) * cols, c, cols);
+      Cols<4> sum = loadCols<FAST, 4>(t.partial + ((int64_t)(from - 1) * 2 + 1) * cols, c, cols);
 #pragma unroll
-      for (int i = 0; i < kJoinWarps; ++i) acc = add4(acc, sPart[i][lane]);
-      storeCols<VEC>(out + (int64_t)sLong[w][0] * cols, c, cols, scale4(acc, t.scale));
+      for (int i = 0; i < kJoinWarps; ++i) addTo(sum, sPart[i][lane]);
+      storeCols<FAST, 4>(out + (int64_t)sLong[w][0] * cols, c, cols, scaled(sum, t.scale));
     }
     __syncthreads();
   }
@@ -408,34 +541,32 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
 
 // -- launches ----------------------------------------------------------------------
 
-// The least power of two from 8 to `most` that covers cols with four columns
-// per thread.
-int groupFor(int cols, int most) {
+// The least power of two from 8 to 64 that covers cols with n columns per
+// thread.
+int groupFor(int cols, int n) {
   int g = 8;
-  while (g < most && g * 4 < cols) g *= 2;
+  while (g < 64 && g * n < cols) g *= 2;
   return g;
 }
-bool vectorRows(int cols, std::initializer_list<const void*> fp32,
-                std::initializer_list<const void*> bf16) {
-  if (cols % 4 != 0) return false;
-  uintptr_t bits = 0, bits2 = 0;
-  for (const void* p : fp32) bits |= reinterpret_cast<uintptr_t>(p);
-  for (const void* p : bf16) bits2 |= reinterpret_cast<uintptr_t>(p);
-  return (bits & 15) == 0 && (bits2 & 7) == 0;
+// Whether rows of `cols` values from p on divide into aligned pieces of n.
+bool pieces(const void* p, int valueBytes, int cols, int n) {
+  const uintptr_t bytes = (uintptr_t)(n * valueBytes < 16 ? n * valueBytes : 16);
+  return p == nullptr || (cols % n == 0 && reinterpret_cast<uintptr_t>(p) % bytes == 0);
 }
 
 template <class W, class Y>
 int fwd(const int64_t* token, const int64_t* position, const void* w, const void* p, void* y,
         int rows, int seq, int vocab, int context, int cols, float scale, cudaStream_t stream) {
-  const bool wF32 = sizeof(W) == 4, yF32 = sizeof(Y) == 4;
-  const bool vec = vectorRows(cols, {wF32 ? w : nullptr, wF32 ? p : nullptr, yF32 ? y : nullptr},
-                              {wF32 ? nullptr : w, wF32 ? nullptr : p, yF32 ? nullptr : y});
-  const int group = groupFor(cols, kThreads);
-  const int64_t perCta = (int64_t)(kThreads / group) * kFwdRows;
-  auto kernel = vec ? embeddingFwd<W, Y, true> : embeddingFwd<W, Y, false>;
-  kernel<<<(unsigned)((rows + perCta - 1) / perCta), kThreads, 0, stream>>>(
+  constexpr int N = 16 / sizeof(W);  // 16-byte loads
+  const bool fast = pieces(w, sizeof(W), cols, N) && pieces(p, sizeof(W), cols, N) &&
+                    pieces(y, sizeof(Y), cols, N);
+  // Few rows spread over the SMs; many take 16 to a CTA.
+  int per = (rows + kSMs * 4 - 1) / (kSMs * 4);
+  if (per > kFwdMaxRows) per = kFwdMaxRows;
+  auto kernel = fast ? embeddingFwd<W, Y, true, N> : embeddingFwd<W, Y, false, 4>;
+  kernel<<<(unsigned)((rows + per - 1) / per), kThreads, 0, stream>>>(
       token, position, static_cast<const W*>(w), static_cast<const W*>(p), static_cast<Y*>(y),
-      rows, seq, vocab, context, cols, scale, group);
+      rows, seq, vocab, context, cols, scale, per);
   return launched(cudaGetLastError());
 }
 
@@ -447,8 +578,20 @@ int sortTokens(const int64_t* token, void* sorted, int* skey, int* perm, int row
                                                               skey, perm, rows, vocab);
   if (int rc = launched(cudaGetLastError())) return rc;
   if (chunks == 1) return 0;
-  mergeRanks<Key, CHUNK><<<(rows + kMergeThreads - 1) / kMergeThreads, kMergeThreads, 0, stream>>>(
-      static_cast<const Key*>(sorted), skey, perm, rows);
+  auto merge = mergeRanks<Key, CHUNK>;
+  static std::atomic<uint64_t> done{0};  // devices (bit d) with the shared memory opted in
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 3;
+  if (!(done.load(std::memory_order_acquire) & (1ull << dev))) {
+    const cudaError_t e = cudaFuncSetAttribute(
+        merge, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMergeSmem);
+    if (e != cudaSuccess) return (int)e;
+    done.fetch_or(1ull << dev, std::memory_order_acq_rel);
+  }
+  const uint32_t bytes = (uint32_t)chunks * CHUNK * sizeof(Key);
+  merge<<<(rows + kMergeThreads - 1) / kMergeThreads, kMergeThreads,
+          bytes < kMergeSmem ? bytes : kMergeSmem, stream>>>(static_cast<const Key*>(sorted), skey,
+                                                            perm, rows);
   return launched(cudaGetLastError());
 }
 // Chunks of 1024 up to 16384 rows (the sort's one CTA per chunk is what takes
@@ -466,35 +609,53 @@ int sortTokens(const int64_t* token, void* sorted, int* skey, int* perm, int row
   return sortTokens<uint64_t, kLargeChunk>(token, sorted, skey, perm, rows, vocab, stream);
 }
 
+// Sorted rows per block: 16, or 32 where there are many rows (half the partial
+// sums; fewer rows would leave SMs idle). Where every run has `batch` rows,
+// whole runs, as long as they fit.
+int blockRows(int rows, int batch) {
+  if (batch > 0 && batch <= kMaxBlock) return batch <= 16 ? 16 / batch * batch : batch;
+  return rows > 16 * kSmallChunk ? 32 : 16;
+}
+
 template <class G, class W>
 int tableGradients(const void* g, const TableGradArgs& args, cudaStream_t stream) {
   TableGradArgs a = args;
-  const bool gF32 = sizeof(G) == 4, wF32 = sizeof(W) == 4;
-  const void* o0 = a.table[0].out;
-  const void* o1 = a.tables > 1 ? a.table[1].out : nullptr;
-  const bool vec =
-      vectorRows(a.cols,
-                 {gF32 ? g : nullptr, wF32 ? o0 : nullptr, wF32 ? o1 : nullptr,
-                  a.table[0].partial, a.tables > 1 ? a.table[1].partial : nullptr},
-                 {gF32 ? nullptr : g, wF32 ? nullptr : o0, wF32 ? nullptr : o1});
-  a.group = groupFor(a.cols, 64);
-  a.blocks = (a.rows + kBlock - 1) / kBlock;
-  const int perCta = kThreads / a.group;
-  a.sumCtas = (a.blocks + perCta - 1) / perCta;
-  int ctas = 0;
+  constexpr int N = 16 / sizeof(G);  // 16-byte loads
+  bool fast = pieces(g, sizeof(G), a.cols, N), fast4 = true;
   for (int i = 0; i < a.tables; ++i) {
-    a.zeroCtas[i] = (a.table[i].vocab + kZeroRows - 1) / kZeroRows;
-    ctas += a.sumCtas + a.zeroCtas[i];
+    fast = fast && pieces(a.table[i].out, sizeof(W), a.cols, N);
+    fast4 = fast4 && pieces(a.table[i].out, sizeof(W), a.cols, 4);
   }
-  const unsigned tiles = (unsigned)((a.cols + a.group * 4 - 1) / (a.group * 4));
-  auto sum = vec ? tableGrads<G, W, true> : tableGrads<G, W, false>;
+  const int n = fast ? N : 4;
+  a.group = groupFor(a.cols, n);
+  const int perCta = kThreads / a.group;
+  int ctas = 0, joinFrom = a.tables, joinBlocks = 0;
+  for (int i = 0; i < a.tables; ++i) {
+    Table& t = a.table[i];
+    t.block = blockRows(a.rows, t.skey ? 0 : t.batch);
+    t.blocks = (a.rows + t.block - 1) / t.block;
+    t.sumCtas = (t.blocks + perCta - 1) / perCta;
+    t.zeroCtas = (t.vocab + kZeroRows - 1) / kZeroRows;
+    ctas += t.sumCtas + t.zeroCtas;
+    // Blocks of whole runs have nothing to join.
+    if (t.blocks == 1 || (!t.skey && t.block % t.batch == 0)) continue;
+    if (joinFrom == a.tables) joinFrom = i;
+    if (t.blocks > joinBlocks) joinBlocks = t.blocks;
+  }
+  const unsigned tiles = (unsigned)((a.cols + a.group * n - 1) / (a.group * n));
+  auto sum = fast ? tableGrads<G, W, true, N> : tableGrads<G, W, false, 4>;
   sum<<<dim3((unsigned)ctas, tiles), kThreads, 0, stream>>>(static_cast<const G*>(g), a);
   if (int rc = launched(cudaGetLastError())) return rc;
-  if (a.blocks == 1) return 0;  // no border to cross
-  auto join = vec ? joinRuns<W, true> : joinRuns<W, false>;
-  join<<<dim3((unsigned)((a.blocks + kJoinWarps - 1) / kJoinWarps),
-              (unsigned)((a.cols + 127) / 128), (unsigned)a.tables),
-         kJoinWarps * 32, 0, stream>>>(a);
+  if (joinFrom == a.tables) return 0;
+  // Tables joinFrom ... up to the last that has something to join: the first
+  // alone unless the second has too.
+  const Table& last = a.table[a.tables - 1];
+  const bool second = a.tables > 1 && joinFrom == 0 && last.blocks > 1 &&
+                      (last.skey || last.block % last.batch != 0);
+  auto join = fast4 ? joinRuns<W, true> : joinRuns<W, false>;
+  join<<<dim3((unsigned)((joinBlocks + kJoinWarps - 1) / kJoinWarps),
+              (unsigned)((a.cols + 127) / 128), second ? 2u : 1u),
+         kJoinWarps * 32, 0, stream>>>(a, joinFrom);
   return launched(cudaGetLastError());
 }
 
@@ -502,7 +663,7 @@ size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 // Scratch of one table: sort keys, sorted keys and rows, partial sums.
 size_t sortBytes(int64_t rows) { return round16(8 * rows) + 2 * round16(4 * rows); }
 size_t partialBytes(int64_t rows, int cols) {
-  return round16(sizeof(float) * 2 * ((rows + kBlock - 1) / kBlock) * cols);
+  return round16(sizeof(float) * 2 * ((rows + 15) / 16) * cols);
 }
 
 }  // namespace

@@ -110,6 +110,24 @@ def test_embedding(ops, dtype, batch, seq, vocab, context, width, positions, rep
     assert torch.equal(again[0], dw) and torch.equal(again[1], dp)
 
 
+def test_embedding_runs_at_block_borders(ops):
+    """Runs of equal tokens whose lengths put their ends at, before and after
+    every multiple of 16 sorted rows, up to runs of more than 32 blocks."""
+    lengths = torch.tensor([16, 16, 1, 15, 17, 31, 48, 16, 600, 8, 24, 512, 528, 1, 1, 14, 33],
+                           device="cuda")
+    idx = torch.repeat_interleave(torch.arange(len(lengths), device="cuda"), lengths)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for shift in range(17):
+        # `shift` rows of token 0 more move every border.
+        at = torch.cat([idx.new_zeros(shift), idx])
+        at = at[torch.randperm(len(at), device="cuda", generator=g)]
+        w = torch.zeros(len(lengths) + 1, 8, device="cuda", requires_grad=True)
+        gy = torch.randint(-8, 9, (len(at), 8), device="cuda", generator=g).float()
+        (dw,) = torch.autograd.grad(ops.embedding(at, w), [w], gy)
+        want = torch.zeros_like(w).index_add_(0, at, gy)  # whole numbers: exact in any order
+        assert torch.equal(dw, want)
+
+
 def test_embedding_without_positions_and_mixed_types(ops):
     idx = torch.tensor([3, 0, 3], device="cuda", dtype=torch.int32)
     w = _normal(5, 12, seed=1, dtype=torch.bfloat16).requires_grad_()
