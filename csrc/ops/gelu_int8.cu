@@ -5,20 +5,20 @@
 //   act = bf16(gelu_tanh(bf16(pre)))      as tnops_gemm_bias_act gives it
 //   pre_q, pre_e = pre in 8-bit blocks (int8_blocks.cuh)
 //
-// An epilogue of the CTA-pair pipeline (pair_gemm.cuh). A thread of it holds
+// An epilogue of the CTA-pair pipeline of panel_gemm.cuh. A thread of it holds
 // 32 neighbouring sums of one row, which is one 8-bit block: its largest
 // magnitude, its exponent and its bytes need nothing from another thread, and
 // the sums are rounded once, from fp32. A row's 128 columns of a tile half
 // give four exponent bytes, written together where they are aligned.
 #include "int8_blocks.cuh"
-#include "pair_gemm.cuh"
+#include "panel_gemm.cuh"
 #include "tnccl_ops.h"
 
 namespace tnops {
 namespace {
 
 struct GeluInt8Epi {
-  static constexpr bool kCuts = false;
+  static constexpr bool kStages = true;
   CUtensorMap mapAct;
   const uint16_t* bias;
   uint8_t* q;
@@ -28,8 +28,8 @@ struct GeluInt8Epi {
   struct State {
     uint32_t e;
   };
-  __device__ __forceinline__ State begin(int, int) const { return {0u}; }
-  __device__ __forceinline__ void chunk(State& st, const float (&in)[32], int, int lane, int row0,
+  __device__ __forceinline__ State begin(int) const { return {0u}; }
+  __device__ __forceinline__ void chunk(State& st, const float (&in)[32], int lane, int row0,
                                         int col0, uint32_t buf) const {
     float v[32];
     float top = 0.f;
@@ -95,23 +95,14 @@ extern "C" int tnops_linear_gelu_int8(const void* x, const void* w, const void* 
       !aligned16(w) || !aligned16(bias) || !aligned16(act) || bias == nullptr ||
       (reinterpret_cast<uintptr_t>(pre_q) & 7) || (reinterpret_cast<uintptr_t>(pre_e) & 3))
     return 1;
-  PairGemmArgs<GeluInt8Epi> args{};
-  args.problems = 1;
-  GemmProblem& p = args.prob[0];
-  p.tilesM = (rows + 255) / 256;
-  p.tilesN = (outs + 255) / 256;
-  p.kBlocks = (ins + kBK - 1) / kBK;
+  PanelGemmArgs<GeluInt8Epi> args{};
   GeluInt8Epi& epi = args.epi;
-  if (!operandMap(&p.mapA, x, rows, ins, ins, false) ||
-      !operandMap(&p.mapB, w, outs, ins, ins, false) ||
-      !bf16OutMap(&epi.mapAct, act, rows, outs, outs))
-    return 4;
+  if (!bf16OutMap(&epi.mapAct, act, rows, outs, outs)) return 4;
   epi.bias = static_cast<const uint16_t*>(bias);
   epi.q = pre_q;
   epi.e = pre_e;
   epi.rows = rows;
   epi.cols = outs;
   epi.blocks = (outs + kInt8Block - 1) / kInt8Block;
-  planGemm(&args, false);
-  return launchPairGemm(args, stream);
+  return launchPanelGemm(args, x, w, rows, outs, ins, stream);
 }

@@ -18,7 +18,7 @@
 // piece, dx in fp32.
 // 8 rows classes width operations, 2 of them for the logits formed twice.
 #include "linear_grads.h"
-#include "pair_gemm.cuh"
+#include "panel_gemm.cuh"
 #include "tnccl_ops.h"
 
 namespace tnops {
@@ -28,7 +28,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // Running maximum and sum of exponentials of one row over 128 columns.
 struct StatsEpi {
-  static constexpr bool kCuts = false;
+  static constexpr bool kStages = false;
   const int64_t* target;
   float2* partial;  // [2 * tilesN][rows]: (maximum, sum of exp(l - maximum))
   float* logitOfTarget;
@@ -38,10 +38,10 @@ struct StatsEpi {
     float m, s;
     int64_t target;
   };
-  __device__ __forceinline__ State begin(int, int row) const {
+  __device__ __forceinline__ State begin(int row) const {
     return {-INFINITY, 0.f, row < rows ? target[row] : -1};
   }
-  __device__ __forceinline__ void chunk(State& st, const float (&in)[32], int, int lane, int row0,
+  __device__ __forceinline__ void chunk(State& st, const float (&in)[32], int lane, int row0,
                                         int col0, uint32_t) const {
     if (col0 >= classes) return;
     float v[32];
@@ -73,7 +73,7 @@ struct StatsEpi {
 
 // d for one piece of the vocabulary, from lse of the whole row.
 struct SoftmaxGradEpi {
-  static constexpr bool kCuts = false;
+  static constexpr bool kStages = true;
   CUtensorMap mapD;
   const int64_t* target;
   const float* lse;
@@ -86,7 +86,7 @@ struct SoftmaxGradEpi {
     int at;  // the target's column in this piece (any other value: none)
     bool counts;
   };
-  __device__ __forceinline__ State begin(int, int row) const {
+  __device__ __forceinline__ State begin(int row) const {
     State st{0.f, 0.f, -1, false};
     if (row < rows) {
       const int64_t t = target[row];
@@ -100,7 +100,7 @@ struct SoftmaxGradEpi {
     }
     return st;
   }
-  __device__ __forceinline__ void chunk(State& st, const float (&in)[32], int, int lane, int row0,
+  __device__ __forceinline__ void chunk(State& st, const float (&in)[32], int lane, int row0,
                                         int col0, uint32_t buf) const {
     float v[32];
     // A row that does not count gives zeros whatever its logits are.
@@ -201,18 +201,6 @@ __global__ void f32ToBf16(const float* __restrict__ in, uint16_t* __restrict__ o
 
 int tilesOf(int n) { return (n + 255) / 256; }
 
-// x [rows, width] against w[first .. first + n): the logits' product.
-bool logitsProblem(GemmProblem* p, const void* x, const void* w, int rows, int width, int first,
-                   int n) {
-  p->tilesM = tilesOf(rows);
-  p->tilesN = tilesOf(n);
-  p->kBlocks = (width + kBK - 1) / kBK;
-  p->aMn = p->bMn = 0;
-  return operandMap(&p->mapA, x, rows, width, width, false) &&
-         operandMap(&p->mapB, static_cast<const uint16_t*>(w) + (size_t)first * width, n, width,
-                    width, false);
-}
-
 }  // namespace
 
 unsigned linearCeStatus(int reset) { return readStatus(reset); }
@@ -229,12 +217,9 @@ extern "C" int tnops_linear_ce_fwd(const void* x, const void* w, const int64_t* 
   if (rows <= 0 || classes <= 0 || width <= 0 || width % 8 != 0 || !aligned16(x) ||
       !aligned16(w))
     return 1;
-  PairGemmArgs<StatsEpi> args{};
-  args.problems = 1;
-  if (!logitsProblem(&args.prob[0], x, w, rows, width, 0, classes)) return 4;
+  PanelGemmArgs<StatsEpi> args{};
   args.epi = {target, reinterpret_cast<float2*>(partial), loss, rows, classes};
-  planGemm(&args, false);
-  if (int rc = launchPairGemm(args, stream)) return rc;
+  if (int rc = launchPanelGemm(args, x, w, rows, classes, width, stream)) return rc;
   joinStats<<<(rows + 31) / 32, kJoinWarps * 32, 0, stream>>>(
       args.epi.partial, target, loss, lse, loss, tnops_linear_ce_parts(classes), rows, classes);
   return launched(cudaGetLastError());
@@ -277,11 +262,9 @@ extern "C" int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* 
   }
   for (int first = 0; first < classes; first += piece) {
     const int n = classes - first < piece ? classes - first : piece;
-    PairGemmArgs<SoftmaxGradEpi> args{};
-    args.problems = 1;
-    if (!logitsProblem(&args.prob[0], x, w, rows, width, first, n) ||
-        !bf16OutMap(&args.epi.mapD, d, rows, n, piece))
-      return 4;
+    const void* wPiece = static_cast<const uint16_t*>(w) + (size_t)first * width;
+    PanelGemmArgs<SoftmaxGradEpi> args{};
+    if (!bf16OutMap(&args.epi.mapD, d, rows, n, piece)) return 4;
     SoftmaxGradEpi& e = args.epi;
     e.target = target;
     e.lse = lse;
@@ -292,14 +275,13 @@ extern "C" int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* 
     e.classes = classes;
     e.first = first;
     e.width = n;
-    planGemm(&args, false);
-    if (int rc = launchPairGemm(args, stream)) return rc;
+    if (int rc = launchPanelGemm(args, x, wPiece, rows, n, width, stream)) return rc;
     LinearGrads g{};
     g.scratch = scratch;
     g.scratchBytes = scratch_bytes;
     g.g = d;
     g.ldg = piece;
-    g.w = static_cast<const uint16_t*>(w) + (size_t)first * width;
+    g.w = wPiece;
     g.x = x;
     g.dx = whole ? dx : dx_f32;
     g.dxStore = !dx ? kStoreNone : whole ? kStoreBf16 : first == 0 ? kStoreF32 : kAddF32;

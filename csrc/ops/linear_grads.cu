@@ -5,10 +5,10 @@
 //   dW[n, k] = sum_r G[r, n] X[r, k]      A = G (MN-major), B = X (MN-major)
 //
 // G, W and X are read as they lie. 4 rows outs ins operations; each operand
-// is read once per 256 rows or columns of the other side, from L2 when the
-// neighbouring pairs work on the same rows. A layer's dW has few tiles with
-// long sums (27 of 128 K blocks for 8192 rows of a 768 -> 2304 layer, next to
-// 96 of 36 for dX, on 74 pairs): the schedule (pair_schedule.h) lets the pairs
+// is read once per 256 or 512 rows or columns of the other side, from L2 when
+// the neighbouring pairs work on the same rows. A layer's dW has few tiles with
+// long sums (15 of 128 K blocks for 8192 rows of a 768 -> 2304 layer, next to
+// 48 of 36 for dX, on 74 pairs): the schedule (pair_schedule.h) lets the pairs
 // without a long tile begin with the short ones, and where that still leaves
 // pairs idle it cuts the long sums, whose parts a second kernel adds.
 #include "linear_grads.h"
@@ -36,10 +36,9 @@ struct StoreEpi {
   __device__ __forceinline__ void end(const State&, int, int) const {}
 };
 
-int tilesOf(int n) { return (n + 255) / 256; }
 
 struct JoinArgs {
-  const float* partial;  // [split * tiles][256][256]
+  const float* partial;  // [split * tiles][512][256]
   void* out;
   int tiles, tilesN, split, rows, cols, mode;
 };
@@ -55,7 +54,7 @@ __global__ void __launch_bounds__(kJoinThreads)
   if (outCol >= a.cols) return;  // cols % 8 == 0: a thread's four are in or out
   float4 acc[kJoinRows / 4] = {};
   for (int p = 0; p < a.split; ++p) {
-    const float* part = a.partial + ((size_t)p * a.tiles + tile) * 65536;
+    const float* part = a.partial + ((size_t)p * a.tiles + tile) * (kPairBM * 256);
 #pragma unroll
     for (int i = 0; i < kJoinRows / 4; ++i) {
       const float4 v = __ldcs(reinterpret_cast<const float4*>(part + (r0 + 4 * i) * 256 + col));
@@ -64,7 +63,7 @@ __global__ void __launch_bounds__(kJoinThreads)
   }
 #pragma unroll
   for (int i = 0; i < kJoinRows / 4; ++i) {
-    const int row = tile / a.tilesN * 256 + r0 + 4 * i;
+    const int row = tile / a.tilesN * kPairBM + r0 + 4 * i;
     if (row >= a.rows) continue;
     const size_t at = (size_t)row * a.cols + outCol;
     if (a.mode == kStoreBf16) {
@@ -87,8 +86,9 @@ int shapes(int rows, int outs, int ins, bool wantDx, bool wantDw, GemmProblem* p
   int n = 0;
   auto add = [&](bool dx) {
     GemmProblem& p = prob[n];
-    p.tilesM = tilesOf(dx ? rows : outs);
-    p.tilesN = tilesOf(ins);
+    p.rows = dx ? rows : outs;
+    p.tilesM = (p.rows + kPairBM - 1) / kPairBM;
+    p.tilesN = (ins + 255) / 256;
     p.kBlocks = ((dx ? outs : rows) + kBK - 1) / kBK;
     p.aMn = dx ? 0 : 1;
     p.bMn = 1;

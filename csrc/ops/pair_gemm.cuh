@@ -5,35 +5,34 @@
 //
 //   D[m, n] = sum_k A(m, k) B(n, k)
 //
-// An operand is "K-major" when k is contiguous in memory ([m, k] rows) and
-// "MN-major" when m (or n) is contiguous ([k, m] rows): with both, the
+// Either operand may be K-major or MN-major (pair_parts.cuh): with both, the
 // products of a backward pass (dX = G W, dW = G^T X) read G, W and X as they
-// lie, without a transposed copy. In shared memory, with the 128-byte swizzle:
-//   K-major   128 rows of 64 k (128 bytes), 8-row atoms of 1024 bytes; the
-//             descriptor's stride is the 1024 bytes from 8 rows to the next 8,
-//             and a K = 16 slice starts 32 bytes after the one before it;
-//   MN-major  two chunks of 64 m, each 64 rows (one per k) of 128 bytes; the
-//             leading offset is the 8192 bytes from one chunk to the next, the
-//             stride the 1024 bytes from 8 k to the next 8, and a K = 16
-//             slice starts 2048 bytes after the one before it.
-// The pipeline is that of the GEMM with the bias epilogue (gemm_tcgen05.cu):
-// each CTA of a pair stages 128 rows of A and of B per 64-wide K block in a
-// six-stage ring, the even CTA issues the MMAs, two accumulators of 256 TMEM
-// columns let the epilogue of a tile run under the next tile's main loop.
+// lie, without a transposed copy.
+//
+// The pipeline is that of the GEMM with the bias epilogue (gemm_tcgen05.cu)
+// with tiles of 512 x 256: each CTA of a pair stages, per 64-wide K block, 128
+// rows of A for each 256-row half of the tile and 128 rows of B (48 KiB, four
+// stages), the even CTA issues the MMAs, and the two halves' accumulators fill
+// the 512 TMEM columns. An SM then loads 48 bytes per clock of MMA where a
+// 256 x 256 tile takes 64, more than L2 delivers to all SMs at once (8192^3 of
+// zeros, so that power does not limit: 1810 TFLOP/s against 1430). With no
+// accumulator to spare, a tile's epilogue runs before the next tile's first
+// MMA of the same half; these are the products with the long sums.
 // A launch may hold two products (`GemmProblem`), so that dX and dW of a layer
 // fill the GPU together; who computes what is pair_schedule.h's. Every wait is
 // bounded as there; the first failure is kept in the file's status word.
 #pragma once
 
+#include "pair_parts.cuh"
 #include "pair_schedule.h"
-#include "tcgen05.cuh"
 
 namespace tnops {
 namespace {
 
-constexpr int kPairBM = 256;
-constexpr int kPairStages = 6;
-constexpr uint32_t kPairSmemBytes = kPairStages * 2 * kHalf + kEpiBytes + 1024;
+constexpr int kPairBM = 512;
+constexpr int kPairStages = 4;
+constexpr uint32_t kPairStage = 3 * kHalf;  // two halves of A, one of B
+constexpr uint32_t kPairSmemBytes = kPairStages * kPairStage + kEpiBytes + 1024;
 
 // One product of a launch. The tensor maps' boxes are {64 k, 128 rows} for a
 // K-major operand and {64 m, 64 k} for an MN-major one; out-of-range rows and
@@ -41,112 +40,18 @@ constexpr uint32_t kPairSmemBytes = kPairStages * 2 * kHalf + kEpiBytes + 1024;
 struct alignas(64) GemmProblem {
   CUtensorMap mapA, mapB;
   int tilesM, tilesN, kBlocks;
+  int rows;  // m
   int aMn, bMn;
 };
 
 template <class Epi>
 struct alignas(64) PairGemmArgs {
   GemmProblem prob[2];
-  CUtensorMap mapPartial;  // [256 slots, 256] fp32, for an Epi that kCuts
+  CUtensorMap mapPartial;  // [512 slots, 256] fp32, for an Epi that kCuts
   int problems;
   PairSchedule schedule;
   Epi epi;
 };
-
-// Operand descriptor without its start address.
-__device__ __forceinline__ uint64_t pairDescBase(int mn) {
-  uint64_t d = (uint64_t)(mn ? (8192 >> 4) : 1) << 16;  // leading offset, bits [16,30)
-  d |= (uint64_t)(1024 >> 4) << 32;                     // stride, bits [32,46)
-  d |= (uint64_t)1 << 46;                               // descriptor version 1
-  d |= (uint64_t)2 << 61;                               // SWIZZLE_128B
-  return d;
-}
-__device__ __forceinline__ uint64_t pairDesc(uint64_t base, uint32_t addr) {
-  return base | (uint64_t)((addr & 0x3FFFFu) >> 4);
-}
-// kind::f16 instruction descriptor: bf16 x bf16 -> f32, M = N = 256; bits 15
-// and 16 say that A / B is MN-major.
-__device__ __forceinline__ uint32_t pairInstrDesc(int aMn, int bMn) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)aMn << 15) | ((uint32_t)bMn << 16) |
-         ((uint32_t)(256 >> 3) << 17) | ((uint32_t)(kPairBM >> 4) << 24);
-}
-__device__ __forceinline__ void pairMma(uint32_t tmemD, uint64_t a, uint64_t b, uint32_t instr,
-                                        uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, "
-      "{%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}" ::"r"(tmemD),
-      "l"(a), "l"(b), "r"(instr), "r"(accumulate), "r"(0u)
-      : "memory");
-}
-// One CTA's 128 rows (from mn0) of a 64-wide K block (from k0) of an operand.
-__device__ __forceinline__ void loadHalf(uint32_t dst, const CUtensorMap* map, int mn, int mn0,
-                                         int k0, uint32_t leaderBar) {
-  if (mn) {
-    tmaLoadPair(dst, map, mn0, k0, leaderBar);
-    tmaLoadPair(dst + kHalf / 2, map, mn0 + 64, k0, leaderBar);
-  } else {
-    tmaLoadPair(dst, map, k0, mn0, leaderBar);
-  }
-}
-
-// A warp's 32 x 32 block as bf16 (64-byte rows, 64-byte swizzle) or fp32
-// (128-byte rows, 128-byte swizzle) in its staging buffer, then one TMA
-// store; the map clips rows and columns past the output's edge, and a block
-// that starts past it is the caller's to skip (`inside`).
-__device__ __forceinline__ void stageWait(int lane) {
-  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-  __syncwarp();
-}
-__device__ __forceinline__ void stageDone() {
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  __syncwarp();
-}
-__device__ __forceinline__ void storeBf16(const float (&v)[32], int lane, uint32_t buf,
-                                          const CUtensorMap* map, int row0, int col0,
-                                          bool inside) {
-  uint32_t w[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) w[i] = packBf16(v[2 * i], v[2 * i + 1]);
-  stageWait(lane);
-  const uint32_t rowOff = (uint32_t)lane * 64u, sw = ((uint32_t)lane >> 1) & 3u;
-#pragma unroll
-  for (int g = 0; g < 4; ++g)
-    stShared16(buf + rowOff + 16u * ((uint32_t)g ^ sw), w[4 * g], w[4 * g + 1], w[4 * g + 2],
-               w[4 * g + 3]);
-  stageDone();
-  if (lane == 0 && inside) {
-    tmaStore2d(map, col0, row0, buf);
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-  }
-}
-__device__ __forceinline__ void tmaAdd2d(const CUtensorMap* map, int x, int y, uint32_t src) {
-  asm volatile(
-      "cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2}], "
-      "[%3];" ::"l"(reinterpret_cast<uint64_t>(map)),
-      "r"(x), "r"(y), "r"(src)
-      : "memory");
-}
-__device__ __forceinline__ void storeF32(const float (&v)[32], int lane, uint32_t buf,
-                                         const CUtensorMap* map, int row0, int col0, bool inside,
-                                         bool add) {
-  stageWait(lane);
-  const uint32_t rowOff = (uint32_t)lane * 128u, sw = (uint32_t)lane & 7u;
-#pragma unroll
-  for (int g = 0; g < 8; ++g)
-    stShared16(buf + rowOff + 16u * ((uint32_t)g ^ sw), __float_as_uint(v[4 * g]),
-               __float_as_uint(v[4 * g + 1]), __float_as_uint(v[4 * g + 2]),
-               __float_as_uint(v[4 * g + 3]));
-  stageDone();
-  if (lane == 0 && inside) {
-    if (add)
-      tmaAdd2d(map, col0, row0, buf);
-    else
-      tmaStore2d(map, col0, row0, buf);
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-  }
-}
 
 // Epi: `State begin(problem, row)` once per tile and thread (the thread's row
 // of the output), `chunk(state, v, problem, lane, row0, col0, buf)` for each
@@ -166,10 +71,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   __shared__ int sAbort;
   extern __shared__ uint8_t dsmem[];
   const uint32_t base = (smemAddr(dsmem) + 1023u) & ~1023u;
-  const uint32_t stageA0 = base, stageB0 = base + kPairStages * kHalf;
-  const uint32_t epi0 = base + kPairStages * 2 * kHalf;
+  const uint32_t epi0 = base + kPairStages * kPairStage;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = clusterRank();
   const int pair = (int)(blockIdx.x >> 1);
   const PairSchedule& schedule = args.schedule;
@@ -210,15 +114,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     while (!*abort && walk.next(schedule, &w)) {
       const GemmProblem& p = args.prob[w.which];
       const int m0 = (w.tile / p.tilesN) * kPairBM + (int)rank * 128;
+      const bool both = (w.tile / p.tilesN) * kPairBM + 256 < p.rows;  // the second half has rows
       const int n0 = (w.tile % p.tilesN) * 256 + (int)rank * 128;
       const int aMn = p.aMn, bMn = p.bMn;
       for (int kb = w.kb0; kb < w.kb1; ++kb, ++g) {
         const uint32_t s = g % kPairStages, round = g / kPairStages;
         if (!mbarWait(&sEmpty[s], (round & 1u) ^ 1u, abort, 1)) break;
-        if (rank == 0) mbarExpectTx(&sFull[s], 4 * kHalf);  // both CTAs' A and B halves
-        const uint32_t bar = inLeader(&sFull[s]);
-        loadHalf(stageA0 + s * kHalf, &p.mapA, aMn, m0, kb * kBK, bar);
-        loadHalf(stageB0 + s * kHalf, &p.mapB, bMn, n0, kb * kBK, bar);
+        if (rank == 0) mbarExpectTx(&sFull[s], (both ? 6 : 4) * kHalf);  // both CTAs' loads
+        const uint32_t bar = inLeader(&sFull[s]), at = base + s * kPairStage;
+        loadHalf(at, &p.mapA, aMn, m0, kb * kBK, bar);
+        loadHalf(at + 2 * kHalf, &p.mapB, bMn, n0, kb * kBK, bar);
+        if (both) loadHalf(at + kHalf, &p.mapA, aMn, m0 + 256, kb * kBK, bar);
       }
     }
     if (*abort) {
@@ -232,74 +138,93 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
       }
     }
-  } else if (warp == 1 && lane == 0 && rank == 0) {
+  } else if (warp == 1 && rank == 0) {
     // MMA issuer (even CTA only).
+    const bool elected = electOne();
     uint32_t g = 0, local = 0;
     PairWalk walk;
     PairWork w;
     walk.init(schedule, pair);
-    for (; !*abort && walk.next(schedule, &w); ++local) {
+    bool ok = true;
+    for (; ok && walk.next(schedule, &w); ++local) {
       const GemmProblem& p = args.prob[w.which];
       const uint64_t descA = pairDescBase(p.aMn), descB = pairDescBase(p.bMn);
       const uint32_t stepA = p.aMn ? 2048 : 32, stepB = p.bMn ? 2048 : 32;
       const uint32_t instr = pairInstrDesc(p.aMn, p.bMn);
-      const uint32_t b = local & 1u, use = local >> 1;
-      if (!mbarWait(&sAccEmpty[b], (use & 1u) ^ 1u, abort, 2)) break;
-      fenceAfterSync();
-      const uint32_t acc = tmem + b * kTmemCols;
-      bool ok = true;
+      const int halves = (w.tile / p.tilesN) * kPairBM + 256 < p.rows ? 2 : 1;
+      const uint32_t fresh = (local & 1u) ^ 1u;  // phase of an accumulator handed back
       for (int kb = w.kb0; kb < w.kb1; ++kb, ++g) {
         const uint32_t s = g % kPairStages;
-        if (!(ok = mbarWait(&sFull[s], (g / kPairStages) & 1u, abort, 2))) break;
+        if (!(ok = warpWait(&sFull[s], (g / kPairStages) & 1u, abort, 2))) break;
         fenceAfterSync();
-        const uint32_t a = stageA0 + s * kHalf, bb = stageB0 + s * kHalf;
+        const uint32_t at = base + s * kPairStage;
+        for (int h = 0; h < halves; ++h) {
+          if (kb == w.kb0) {
+            if (!(ok = warpWait(&sAccEmpty[h], fresh, abort, 2))) break;
+            fenceAfterSync();
+          }
+          if (elected) {
 #pragma unroll
-        for (int k = 0; k < kBK / 16; ++k)
-          pairMma(acc, pairDesc(descA, a + k * stepA), pairDesc(descB, bb + k * stepB), instr,
-                  kb != w.kb0 || k != 0 ? 1u : 0u);
-        commitPair(&sEmpty[s]);
+            for (int k = 0; k < kBK / 16; ++k)
+              pairMma(tmem + h * kTmemCols, pairDesc(descA, at + h * kHalf + k * stepA),
+                      pairDesc(descB, at + 2 * kHalf + k * stepB), instr,
+                      kb != w.kb0 || k != 0 ? 1u : 0u);
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+        if (elected) commitPair(&sEmpty[s]);
+        __syncwarp();
       }
       if (!ok) break;
-      commitPair(&sAccFull[b]);
+      if (elected) {
+        commitPair(&sAccFull[0]);
+        commitPair(&sAccFull[1]);
+      }
+      __syncwarp();
     }
-    commitPairLocal(&sDone);
+    if (elected) commitPairLocal(&sDone);
+    __syncwarp();
     if (*abort) mbarWait(&sDone, 0, abort, 5, true);
   } else if (warp >= 2) {
-    // Epilogue (both CTAs): this CTA's 128 rows of the tile; TMEM lane
-    // quarter warp % 4, column half (warp - 2) / 4.
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    // Epilogue (both CTAs): this CTA's 128 rows of each half of the tile; TMEM
+    // lane quarter warp % 4, column half (warp - 2) / 4.
+    const int quarter = warp & 3, side = (warp - 2) >> 2;
     const uint32_t buf = epi0 + (uint32_t)(warp - 2) * kEpiBuf;
     uint32_t local = 0;
     PairWalk walk;
     PairWork w;
     walk.init(schedule, pair);
-    for (; walk.next(schedule, &w); ++local) {
-      const uint32_t b = local & 1u, use = local >> 1;
+    bool ok = true;
+    for (; ok && walk.next(schedule, &w); ++local) {
       const GemmProblem& p = args.prob[w.which];
       const int tileN = w.tile % p.tilesN;
-      const int row0 = (w.tile / p.tilesN) * kPairBM + (int)rank * 128 + quarter * 32;
-      typename Epi::State st = args.epi.begin(w.which, row0 + lane);
-      const bool ready = mbarWait(&sAccFull[b], use & 1u, abort, 3);
-      if (!__all_sync(0xffffffffu, ready)) break;
-      fenceAfterSync();
-      const uint32_t acc = tmem + b * kTmemCols + ((uint32_t)(quarter * 32) << 16);
+      for (int h = 0; h < 2; ++h) {
+        const int inTile = h * 256 + (int)rank * 128 + quarter * 32;
+        const int row0 = (w.tile / p.tilesN) * kPairBM + inTile;
+        if (!(ok = warpWait(&sAccFull[h], local & 1u, abort, 3))) break;
+        fenceAfterSync();
+        const uint32_t acc = tmem + h * kTmemCols + ((uint32_t)(quarter * 32) << 16);
+        const bool any = row0 < p.rows;  // the same for the whole warp
+        typename Epi::State st = args.epi.begin(w.which, row0 + lane);
 #pragma unroll 1
-      for (int c = half * 128; c < half * 128 + 128; c += 32) {
-        float v[32];
-        tmemLoad32(acc + (uint32_t)c, v);
-        if (c + 32 == half * 128 + 128) {
-          // Last read of this buffer: hand it back before the stores.
-          fenceBeforeSync();
-          __syncwarp();
-          if (lane == 0) mbarArriveRemote(inLeader(&sAccEmpty[b]));
+        for (int c = side * 128; c < side * 128 + 128; c += 32) {
+          float v[32];
+          if (any) tmemLoad32(acc + (uint32_t)c, v);
+          if (c + 32 == side * 128 + 128) {
+            // Last read of this accumulator: hand it back before the stores.
+            fenceBeforeSync();
+            __syncwarp();
+            if (lane == 0) mbarArriveRemote(inLeader(&sAccEmpty[h]));
+          }
+          if (!any) continue;
+          if (Epi::kCuts && w.slot >= 0)
+            storeF32(v, lane, buf, &args.mapPartial, w.slot * kPairBM + inTile, c, true, false);
+          else
+            args.epi.chunk(st, v, w.which, lane, row0, tileN * 256 + c, buf);
         }
-        if (Epi::kCuts && w.slot >= 0)
-          storeF32(v, lane, buf, &args.mapPartial,
-                   w.slot * kPairBM + (int)rank * 128 + quarter * 32, c, true, false);
-        else
-          args.epi.chunk(st, v, w.which, lane, row0, tileN * 256 + c, buf);
+        if (any) args.epi.end(st, row0 + lane, tileN * 2 + side);
       }
-      args.epi.end(st, row0 + lane, tileN * 2 + half);
     }
     epilogueDrain(lane);
   }
@@ -315,37 +240,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 // -- host side -------------------------------------------------------------------
-
-inline bool encode2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t rows,
-                     int64_t cols, int64_t ldBytes, int boxCols, int boxRows,
-                     CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
-  EncodeTiledFn fn = encodeTiled();
-  if (fn == nullptr) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)ldBytes};
-  const cuuint32_t box[2] = {(cuuint32_t)boxCols, (cuuint32_t)boxRows};
-  const cuuint32_t estr[2] = {1, 1};
-  return fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-// [rows, cols] bf16 operand, rows `ld` elements apart: K-major when cols is
-// the summed index, MN-major when rows is.
-inline bool operandMap(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld,
-                       bool mn) {
-  return encode2d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, rows, cols, ld * 2, 64,
-                  mn ? 64 : 128, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
-}
-inline bool bf16OutMap(CUtensorMap* map, const void* base, int64_t rows, int64_t cols,
-                       int64_t ld) {
-  return encode2d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, rows, cols, ld * 2, 32, 32,
-                  CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE);
-}
-inline bool f32OutMap(CUtensorMap* map, const void* base, int64_t rows, int64_t cols,
-                      int64_t ld) {
-  return encode2d(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base, rows, cols, ld * 4, 32, 32,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE);
-}
 
 // Plans the launch for kSMs / 2 pairs; with `cut`, sums may be split. Product
 // 0 must be the one with the longer sum.

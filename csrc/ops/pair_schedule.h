@@ -122,11 +122,11 @@ inline int planRounds(PairSchedule* s) {
 
 // Plans the launch: sums stay whole, or with `cut` the longer product's are
 // split in 2 to kMaxSplit where the busiest pair gains more than the partial
-// sums cost. A K block of a tile takes about 0.3 us; partial sums cost one
-// more launch (about 4 us) and about 0.13 us per slot (256 KiB written and
-// read).
+// sums cost. A K block of a 512 x 256 tile takes about 0.55 us; partial sums
+// cost one more launch (about 4 us) and about 0.26 us per slot (512 KiB written
+// and read).
 constexpr int kMaxSplit = 8;
-constexpr int kSplitSlots = 296;
+constexpr int kSplitSlots = 148;
 inline void planPairs(PairSchedule* s, bool cut) {
   s->split[0] = s->split[1] = 1;
   int best = planRounds(s);
@@ -136,7 +136,7 @@ inline void planPairs(PairSchedule* s, bool cut) {
     if (t.k[0] < 8 * n) break;  // at least 8 K blocks a unit
     t.split[0] = n;
     if ((t.k[0] + n - 1) / n < t.k[1] && t.tiles[1] > 0) break;  // product 0's stay the longer
-    const int cost = planRounds(&t) + 14 + t.slots() * 4 / 9;
+    const int cost = planRounds(&t) + 7 + t.slots() / 2;
     if (cost < best) {
       best = cost;
       *s = t;
