@@ -18,8 +18,7 @@ namespace tnops {
 namespace {
 
 struct GeluInt8Epi {
-  static constexpr bool kStages = true;
-  CUtensorMap mapAct;
+  uint16_t* act;
   const uint16_t* bias;
   uint8_t* q;
   uint8_t* e;
@@ -29,10 +28,11 @@ struct GeluInt8Epi {
     uint32_t e;
   };
   __device__ __forceinline__ State begin(int) const { return {0u}; }
-  __device__ __forceinline__ void chunk(State& st, const float (&in)[32], int lane, int row0,
-                                        int col0, uint32_t buf) const {
+  __device__ __forceinline__ void chunk(State& st, const float (&in)[32], int row,
+                                        int col0) const {
+    if (row >= rows || col0 >= cols) return;
     float v[32];
-    float top = 0.f;
+    uint32_t top = 0u;  // of the magnitudes' bits: a NaN's are above infinity's
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       uint4 b = make_uint4(0u, 0u, 0u, 0u);
@@ -40,33 +40,61 @@ struct GeluInt8Epi {
       if (in8) b = __ldg(reinterpret_cast<const uint4*>(bias + col0) + g);
       const uint32_t w[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float add = __uint_as_float((i & 1) ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
-        const float s = in8 ? in[8 * g + i] + add : 0.f;
-        v[8 * g + i] = s;
-        // fmaxf drops a NaN: carried as infinity.
-        top = fmaxf(top, __uint_as_float(min(__float_as_uint(s) & 0x7fffffffu, 0x7f800000u)));
+      for (int i = 0; i < 4; ++i) {
+        float* x = v + 8 * g + 2 * i;
+        unpack2(add2(pack2(in[8 * g + 2 * i], in[8 * g + 2 * i + 1]),
+                     pack2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u))),
+                x[0], x[1]);
+        // Columns past the last have zero sums (the weight's rows read zero).
+        top = max(top, max(__float_as_uint(x[0]) & 0x7fffffffu,
+                           __float_as_uint(x[1]) & 0x7fffffffu));
       }
     }
-    const uint32_t ex = int8Exponent(top);
-    const Int8Inverse inv = int8Inverse(ex);
+    const uint32_t ex = int8Exponent(__uint_as_float(top));
     st.e |= ex << (((col0 >> 5) & 3) * 8);
-    const int row = row0 + lane;
-    if (row < rows) {
-      uint8_t* out = q + (size_t)row * cols + col0;
+    const size_t at = (size_t)row * cols + col0;
+    uint32_t o[8];
+    if (ex >= 6u && ex < 254u) {
+      // x 2^(133 - e) + 1.5 2^23: the sum's last byte is the whole number that
+      // x / step rounds to, in two's complement.
+      const float inv = __uint_as_float((260u - ex) << 23);
+      const uint64_t inv2 = pack2(inv, inv), magic = pack2(12582912.f, 12582912.f);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        if (col0 + 8 * g >= cols) break;
-        uint32_t o[2] = {0u, 0u};
+      for (int i = 0; i < 8; ++i) {
+        float r[4];
+        unpack2(fma2(pack2(v[4 * i], v[4 * i + 1]), inv2, magic), r[0], r[1]);
+        unpack2(fma2(pack2(v[4 * i + 2], v[4 * i + 3]), inv2, magic), r[2], r[3]);
+        o[i] = __byte_perm(__byte_perm(__float_as_uint(r[0]), __float_as_uint(r[1]), 0x0040),
+                           __byte_perm(__float_as_uint(r[2]), __float_as_uint(r[3]), 0x0040),
+                           0x5410);
+      }
+    } else {
+      const Int8Inverse inv = int8Inverse(ex);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          o[i >> 2] |= int8Quantize(v[8 * g + i], inv) << ((i & 3) * 8);
-        *reinterpret_cast<uint2*>(out + 8 * g) = make_uint2(o[0], o[1]);
+      for (int i = 0; i < 8; ++i) {
+        o[i] = 0u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i] |= int8Quantize(v[4 * i + j], inv) << (8 * j);
       }
     }
+    if (cols % 32 == 0) {
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(q + at),
+                   "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]),
+                   "r"(o[7])
+                   : "memory");
+    } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = geluTanh(bf2f(f2bf(v[i])));
-    storeBf16(v, lane, buf, &mapAct, row0, col0, row0 < rows && col0 < cols);
+      for (int g = 0; g < 4; ++g)
+        if (col0 + 8 * g < cols)
+          *reinterpret_cast<uint2*>(q + at + 8 * g) = make_uint2(o[2 * g], o[2 * g + 1]);
+    }
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t p = packBf16(v[2 * i], v[2 * i + 1]);
+      w[i] = packBf16(geluTanh(__uint_as_float(p << 16)), geluTanh(__uint_as_float(p & 0xffff0000u)));
+    }
+    storeRow32(act + at, w, cols % 16 == 0, (cols - col0) / 8);
   }
   __device__ __forceinline__ void end(const State& st, int row, int part) const {
     const int b0 = part * 4;  // the first of this thread's exponent bytes
@@ -92,12 +120,12 @@ extern "C" int tnops_linear_gelu_int8(const void* x, const void* w, const void* 
                                       uint8_t* pre_q, uint8_t* pre_e, int rows, int outs, int ins,
                                       cudaStream_t stream) {
   if (rows <= 0 || outs <= 0 || ins <= 0 || outs % 8 != 0 || ins % 8 != 0 || !aligned16(x) ||
-      !aligned16(w) || !aligned16(bias) || !aligned16(act) || bias == nullptr ||
-      (reinterpret_cast<uintptr_t>(pre_q) & 7) || (reinterpret_cast<uintptr_t>(pre_e) & 3))
+      !aligned16(w) || !aligned16(bias) || bias == nullptr ||
+      (reinterpret_cast<uintptr_t>(act) & 31) || (reinterpret_cast<uintptr_t>(pre_q) & 31) || (reinterpret_cast<uintptr_t>(pre_e) & 3))
     return 1;
   PanelGemmArgs<GeluInt8Epi> args{};
   GeluInt8Epi& epi = args.epi;
-  if (!bf16OutMap(&epi.mapAct, act, rows, outs, outs)) return 4;
+  epi.act = static_cast<uint16_t*>(act);
   epi.bias = static_cast<const uint16_t*>(bias);
   epi.q = pre_q;
   epi.e = pre_e;

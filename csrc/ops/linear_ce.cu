@@ -26,9 +26,37 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// v[at], kept in registers (a loop of selects becomes an array in memory).
+__device__ __forceinline__ float valueAt(const float (&v)[32], int at) {
+  float t = 0.f;
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.eq.s32 p, %1, %2;\n\t"
+        "@p mov.f32 %0, %3;\n\t}"
+        : "+f"(t)
+        : "r"(at), "r"(i), "f"(v[i]));
+  return t;
+}
+
+// The bf16 number `bits` in place of number `at` of 16 pairs, likewise.
+__device__ __forceinline__ void putBf16(uint32_t (&w)[16], int at, uint32_t bits) {
+  const uint32_t order = (at & 1) ? 0x5410u : 0x3254u;  // bytes of (pair, bits)
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t with = __byte_perm(w[i], bits, order);
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.eq.s32 p, %1, %2;\n\t"
+        "@p mov.b32 %0, %3;\n\t}"
+        : "+r"(w[i])
+        : "r"(at >> 1), "r"(i), "r"(with));
+  }
+}
+
 // Running maximum and sum of exponentials of one row over 128 columns.
 struct StatsEpi {
-  static constexpr bool kStages = false;
   const int64_t* target;
   float2* partial;  // [2 * tilesN][rows]: (maximum, sum of exp(l - maximum))
   float* logitOfTarget;
@@ -41,30 +69,39 @@ struct StatsEpi {
   __device__ __forceinline__ State begin(int row) const {
     return {-INFINITY, 0.f, row < rows ? target[row] : -1};
   }
-  __device__ __forceinline__ void chunk(State& st, const float (&in)[32], int lane, int row0,
-                                        int col0, uint32_t) const {
+  // 32 logits: their maximum, then one packed FMA for two, one ex2 for each
+  // and one packed addition for two.
+  __device__ __forceinline__ void chunk(State& st, const float (&in)[32], int row,
+                                        int col0) const {
     if (col0 >= classes) return;
     float v[32];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = col0 + i < classes ? in[i] : -INFINITY;
-    const int64_t at = st.target - col0;
-    if (at >= 0 && at < 32 && st.target < classes) {
-      float t = 0.f;
+    for (int i = 0; i < 32; ++i) v[i] = in[i];
+    if (col0 + 32 > classes) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) t = i == (int)at ? v[i] : t;
-      logitOfTarget[row0 + lane] = t;
+      for (int i = 0; i < 32; ++i) v[i] = col0 + i < classes ? in[i] : -INFINITY;
     }
+    const int64_t at = st.target - col0;
+    if (at >= 0 && at < 32 && st.target < classes)
+      logitOfTarget[row] = valueAt(v, (int)at);
     float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
     for (int i = 4; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], v[i]);
     const float m = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), st.m);
     if (m == -INFINITY) return;
     const float nm = -m * kLog2e;
-    float s[4] = {st.s * ex2Approx(fmaf(st.m, kLog2e, nm)), 0.f, 0.f, 0.f};
+    const uint64_t scale = pack2(kLog2e, kLog2e), shift = pack2(nm, nm);
+    uint64_t s[4] = {pack2(st.s * ex2Approx(fmaf(st.m, kLog2e, nm)), 0.f), 0ull, 0ull, 0ull};
 #pragma unroll
-    for (int i = 0; i < 32; ++i) s[i & 3] += ex2Approx(fmaf(v[i], kLog2e, nm));
+    for (int i = 0; i < 16; ++i) {
+      float a, b;
+      unpack2(fma2(pack2(v[2 * i], v[2 * i + 1]), scale, shift), a, b);
+      s[i & 3] = add2(s[i & 3], pack2(ex2Approx(a), ex2Approx(b)));
+    }
+    float a, b;
+    unpack2(add2(add2(s[0], s[1]), add2(s[2], s[3])), a, b);
     st.m = m;
-    st.s = (s[0] + s[1]) + (s[2] + s[3]);
+    st.s = a + b;
   }
   __device__ __forceinline__ void end(const State& st, int row, int part) const {
     if (row < rows) partial[(size_t)part * rows + row] = make_float2(st.m, st.s);
@@ -73,46 +110,57 @@ struct StatsEpi {
 
 // d for one piece of the vocabulary, from lse of the whole row.
 struct SoftmaxGradEpi {
-  static constexpr bool kStages = true;
-  CUtensorMap mapD;
+  uint16_t* d;  // [rows, ld]
   const int64_t* target;
   const float* lse;
   const float* grad;   // gradient of each row's loss, or of all with gradStep 0
   const float* share;  // further factor (1 / rows that count), or null
-  int gradStep, rows, classes, first, width;
+  int ld, gradStep, rows, classes, first, width;
 
+  // |k| exp(l - lse) = 2^(l log2e + nb) with nb = log2 |k| - lse log2e: the
+  // factor costs nothing per logit; k's sign goes on the packed results.
   struct State {
-    float nb, k;
-    int at;  // the target's column in this piece (any other value: none)
-    bool counts;
+    float nb, nl, k;      // nl = -lse log2e
+    int at;               // the target's column in this piece (any other value: none)
+    uint32_t keep, sign;  // masks of a pair of bf16: all or nothing, k's sign
   };
   __device__ __forceinline__ State begin(int row) const {
-    State st{0.f, 0.f, -1, false};
+    State st{0.f, 0.f, 0.f, -1, 0u, 0u};
     if (row < rows) {
       const int64_t t = target[row];
-      st.counts = t >= 0 && t < classes;
-      if (st.counts) {
-        st.nb = -lse[row] * kLog2e;
+      if (t >= 0 && t < classes) {
         st.k = grad[(size_t)row * gradStep];
         if (share != nullptr) st.k *= *share;
+        st.nl = -lse[row] * kLog2e;
+        st.nb = st.nl + log2f(fabsf(st.k));
         st.at = (int)(t - first);
+        st.keep = 0xffffffffu;
+        st.sign = st.k < 0.f ? 0x80008000u : 0u;
       }
     }
     return st;
   }
-  __device__ __forceinline__ void chunk(State& st, const float (&in)[32], int lane, int row0,
-                                        int col0, uint32_t buf) const {
-    float v[32];
-    // A row that does not count gives zeros whatever its logits are.
+  __device__ __forceinline__ void chunk(State& st, const float (&v)[32], int row,
+                                        int col0) const {
+    if (row >= rows || col0 >= width) return;
+    const uint64_t scale = pack2(kLog2e, kLog2e), shift = pack2(st.nb, st.nb);
+    uint32_t w[16];
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      v[i] = st.counts ? st.k * ex2Approx(fmaf(in[i], kLog2e, st.nb)) : 0.f;
+    for (int i = 0; i < 16; ++i) {
+      float a, b;
+      unpack2(fma2(pack2(v[2 * i], v[2 * i + 1]), scale, shift), a, b);
+      // A row that does not count gives zeros whatever its logits are.
+      w[i] = (packBf16(ex2Approx(a), ex2Approx(b)) & st.keep) ^ st.sign;
+    }
     const int at = st.at - col0;
     if (at >= 0 && at < 32) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] -= i == at ? st.k : 0.f;
+      // The target's own: k (p - 1), rounded once.
+      const float l = valueAt(v, at);
+      const float d = st.k * (ex2Approx(fmaf(l, kLog2e, st.nl)) - 1.f);
+      putBf16(w, at, f2bf(d));
     }
-    storeBf16(v, lane, buf, &mapD, row0, col0, row0 < rows && col0 < width);
+    // Whole: d's rows are `ld` apart, a multiple of 32 at or past the width.
+    storeRow32(d + (size_t)row * ld + col0, w, true, 4);
   }
   __device__ __forceinline__ void end(const State&, int, int) const {}
 };
@@ -248,7 +296,8 @@ extern "C" int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* 
                                    void* scratch, size_t scratch_bytes, void* dx, void* dw, int dw_f32, int rows, int width,
                                    int classes, int vocab, cudaStream_t stream) {
   if (rows <= 0 || classes <= 0 || vocab < classes || width <= 0 || width % 8 != 0 ||
-      piece <= 0 || piece % 8 != 0 || !aligned16(x) || !aligned16(w) || !aligned16(d) ||
+      piece <= 0 || piece % 32 != 0 || !aligned16(x) || !aligned16(w) ||
+      (reinterpret_cast<uintptr_t>(d) & 31) ||
       (dx && !aligned16(dx)) || (dw && !aligned16(dw)))
     return 1;
   const bool whole = classes <= piece;
@@ -264,8 +313,9 @@ extern "C" int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* 
     const int n = classes - first < piece ? classes - first : piece;
     const void* wPiece = static_cast<const uint16_t*>(w) + (size_t)first * width;
     PanelGemmArgs<SoftmaxGradEpi> args{};
-    if (!bf16OutMap(&args.epi.mapD, d, rows, n, piece)) return 4;
     SoftmaxGradEpi& e = args.epi;
+    e.d = static_cast<uint16_t*>(d);
+    e.ld = piece;
     e.target = target;
     e.lse = lse;
     e.grad = grad;

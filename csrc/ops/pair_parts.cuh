@@ -30,6 +30,32 @@ __device__ __forceinline__ bool electOne() {
       : "=r"(p));
   return p != 0;
 }
+// Two fp32 numbers in one 64-bit register and the packed arithmetic on them
+// (one instruction for both).
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // mbarWait by a whole warp, with one answer for all of it: a warp leaves its
 // loop together.
 __device__ __forceinline__ bool warpWait(uint64_t* bar, uint32_t parity, volatile int* abort,
@@ -86,12 +112,10 @@ __device__ __forceinline__ void stageDone() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncwarp();
 }
-__device__ __forceinline__ void storeBf16(const float (&v)[32], int lane, uint32_t buf,
-                                          const CUtensorMap* map, int row0, int col0,
-                                          bool inside) {
-  uint32_t w[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) w[i] = packBf16(v[2 * i], v[2 * i + 1]);
+// w: the row's 32 columns as 16 pairs of bf16.
+__device__ __forceinline__ void storePacked(const uint32_t (&w)[16], int lane, uint32_t buf,
+                                            const CUtensorMap* map, int row0, int col0,
+                                            bool inside) {
   stageWait(lane);
   const uint32_t rowOff = (uint32_t)lane * 64u, sw = ((uint32_t)lane >> 1) & 3u;
 #pragma unroll
@@ -103,6 +127,14 @@ __device__ __forceinline__ void storeBf16(const float (&v)[32], int lane, uint32
     tmaStore2d(map, col0, row0, buf);
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
   }
+}
+__device__ __forceinline__ void storeBf16(const float (&v)[32], int lane, uint32_t buf,
+                                          const CUtensorMap* map, int row0, int col0,
+                                          bool inside) {
+  uint32_t w[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i] = packBf16(v[2 * i], v[2 * i + 1]);
+  storePacked(w, lane, buf, map, row0, col0, inside);
 }
 __device__ __forceinline__ void tmaAdd2d(const CUtensorMap* map, int x, int y, uint32_t src) {
   asm volatile(

@@ -12,7 +12,7 @@
 // delivers to all SMs at once; so the first K blocks of A (up to kResident of
 // them) stay in shared memory while a pair goes along n through its share of a
 // 256-row panel, and only B and the rest of A stream through a ring of 16 KiB
-// slots. With seven blocks of twelve resident (k = 768) that is 45 bytes per
+// slots. With eight blocks of twelve resident (k = 768) that is 43 bytes per
 // clock.
 //
 // A pair's tiles are consecutive (n fastest), so A is loaded again only where
@@ -24,7 +24,7 @@
 namespace tnops {
 namespace {
 
-constexpr int kPanelSlots = 14;   // of kHalf bytes, without an epilogue's staging
+constexpr int kPanelSlots = 14;   // of kHalf bytes
 constexpr int kPanelRing = 6;     // at least this many slots stream
 constexpr uint32_t kPanelSmem = kPanelSlots * kHalf + 1024;
 
@@ -38,14 +38,14 @@ struct alignas(64) PanelGemmArgs {
 };
 
 // Epi: `State begin(row)` once per tile and thread (the thread's row of the
-// output), `chunk(state, v, lane, row0, col0, buf)` for each 32 x 32 block of a
-// warp (v: the row's 32 columns from col0; buf: the warp's 2 KiB of staging if
-// Epi::kStages), `end(state, row, part)` after the last block (part: the 128
-// columns' number).
+// output), `chunk(state, v, row, col0)` for its 32 columns from col0 of each
+// block, `end(state, row, part)` after the last block (part: the 128 columns'
+// number). What an epilogue writes goes straight from registers: operands in
+// and out of shared memory take its whole bandwidth here (107 of 128 bytes per
+// clock), and a staged copy of the result cost a fifth of the time.
 template <class Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     panelGemmKernel(const __grid_constant__ PanelGemmArgs<Epi> args) {
-  constexpr int kSlots = Epi::kStages ? kPanelSlots - 1 : kPanelSlots;
   __shared__ __align__(8) uint64_t sFull[kPanelSlots];
   __shared__ __align__(8) uint64_t sEmpty[kPanelSlots];
   __shared__ __align__(8) uint64_t sPanelFull;   // the resident blocks of A are there
@@ -58,9 +58,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t dsmem[];
   const uint32_t base = (smemAddr(dsmem) + 1023u) & ~1023u;
   const int resident = args.resident;
-  const uint32_t slots = (uint32_t)(kSlots - resident);  // of the ring
+  const uint32_t slots = (uint32_t)(kPanelSlots - resident);  // of the ring
   const uint32_t ring = base + resident * kHalf;
-  const uint32_t epi0 = base + kSlots * kHalf;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = clusterRank();
@@ -192,7 +191,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // Epilogue (both CTAs): this CTA's 128 rows of the tile; TMEM lane
     // quarter warp % 4, column half (warp - 2) / 4.
     const int quarter = warp & 3, half = (warp - 2) >> 2;
-    const uint32_t buf = epi0 + (uint32_t)(warp - 2) * (kEpiBuf / 2);
     uint32_t local = 0;
     for (int t = first; t < end; ++t, ++local) {
       const uint32_t b = local & 1u, use = local >> 1;
@@ -212,11 +210,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (lane == 0) mbarArriveRemote(inLeader(&sAccEmpty[b]));
         }
-        args.epi.chunk(st, v, lane, row0, tileN * 256 + c, buf);
+        args.epi.chunk(st, v, row0 + lane, tileN * 256 + c);
       }
       args.epi.end(st, row0 + lane, tileN * 2 + half);
     }
-    if (Epi::kStages) epilogueDrain(lane);
   }
   fenceBeforeSync();
   __syncthreads();
@@ -226,6 +223,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "r"(2 * kTmemCols)
                  : "memory");
+  }
+}
+
+// 32 columns of a row as 16 pairs of bf16, straight to memory in 32-byte (`wide`:
+// the row's address is a multiple of 32), or 16-byte pieces of which the first
+// `pieces` 16-byte ones are inside the row.
+__device__ __forceinline__ void storeRow32(uint16_t* out, const uint32_t (&w)[16], bool wide,
+                                           int pieces) {
+  if (wide && pieces >= 4) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 8)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + 2 * i),
+                   "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]),
+                   "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+                   : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < pieces)
+        reinterpret_cast<uint4*>(out)[i] =
+            make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   }
 }
 
@@ -257,7 +275,7 @@ int launchPanelGemm(PanelGemmArgs<Epi>& args, const void* a, const void* b, int 
   if (tiles > (1 << 30)) return 1;
   args.tiles = (int)tiles;
   args.pairs = tiles < kSMs / 2 ? (int)tiles : kSMs / 2;
-  const int most = (Epi::kStages ? kPanelSlots - 1 : kPanelSlots) - kPanelRing;
+  const int most = kPanelSlots - kPanelRing;
   args.resident = args.kBlocks < most ? args.kBlocks : most;
   kernel<<<2u * (unsigned)args.pairs, kThreads, kPanelSmem, stream>>>(args);
   return launched(cudaGetLastError());

@@ -114,7 +114,7 @@ int tnops_linear_grads(const void* g, int64_t ldg, const void* w, const void* x,
 // Softmax cross-entropy of l = x w^T without the logits in memory: x
 // [rows, width], w [vocab, width] in bf16, of which the first `classes` rows
 // are classes. A row whose target is outside [0, classes) does not count
-// (zero loss, zero gradient). width % 8 == 0, x, w, dx, dw, d 16-byte aligned;
+// (zero loss, zero gradient). width % 8 == 0, x, w, dx, dw 16-byte, d 32-byte aligned;
 // 1 (invalid argument) without a launch otherwise.
 //  * fwd: loss[r] and lse[r] (fp32); partial holds
 //    2 * rows * tnops_linear_ce_parts(classes) floats of scratch.
@@ -123,7 +123,7 @@ int tnops_linear_grads(const void* g, int64_t ldg, const void* w, const void* x,
 //  * bwd: dx [rows, width] (bf16) and dw [vocab, width] (fp32 with dw_f32, else
 //    bf16; rows from `classes` on are zero) of sum_r k[r] loss[r], with k[r] =
 //    grad[r * grad_step] (* *share). Works on `piece` classes at a time
-//    (piece % 8 == 0); d holds rows * piece bf16 of scratch, dx_f32
+//    (piece % 32 == 0); d holds rows * piece bf16 of scratch, dx_f32
 //    rows * width floats when piece < classes, and scratch scratch_bytes, at
 //    least tnops_linear_ce_scratch(...). A null dx or dw is left out.
 int tnops_linear_ce_parts(int classes);
@@ -170,8 +170,8 @@ int tnops_dequantize_int8(const uint8_t* q, const uint8_t* e, void* x, int x_f32
 
 // act [rows, outs] (bf16) = gelu_tanh(bf16(x w^T + bias)) for x [rows, ins],
 // w [outs, ins], bias [outs] in bf16, and the sums before the GELU in 8-bit
-// blocks (rounded from fp32). ins, outs % 8 == 0, x, w, bias, act 16-byte,
-// pre_q 8-byte, pre_e 4-byte aligned; 1 (invalid argument) otherwise.
+// blocks (rounded from fp32). ins, outs % 8 == 0, x, w, bias 16-byte, act
+// and pre_q 32-byte, pre_e 4-byte aligned; 1 (invalid argument) otherwise.
 int tnops_linear_gelu_int8(const void* x, const void* w, const void* bias, void* act,
                            uint8_t* pre_q, uint8_t* pre_e, int rows, int outs, int ins,
                            cudaStream_t stream);

@@ -284,6 +284,22 @@ def test_linear_cross_entropy_rows_that_do_not_count(ops):
     assert torch.equal(res[0][0], res[1][0]) and torch.equal(res[0][1], res[1][1])
 
 
+def test_linear_cross_entropy_gradients_of_any_sign(ops):
+    """reduction="none" with positive, negative, zero and very small gradients
+    of the rows' losses."""
+    x, w, target = _ce_case(64, 64, 300, 300, seed=14, ignored=0.1)
+    g = _normal(64, seed=15)
+    g[::4] = 0.0
+    g[1::8] *= -1e-20
+    xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = ops.linear_cross_entropy(xr, wr, target, reduction="none")
+    dx, dw = torch.autograd.grad(loss, [xr, wr], g)
+    _, ex, ew, sx, sw = _ce_exact(x, w, target, 300, g)
+    _within(dx, ex, (BF16 + 2e-5) * sx + BF16 * ex.abs() * 1.01)
+    _within(dw, ew, (BF16 + 2e-5) * sw + BF16 * ew.abs() * 1.01 + 1e-30)
+    assert bool((dx[::4] == 0).all())
+
+
 def test_linear_cross_entropy_large_logits(ops):
     """Logits in the hundreds: the running maximum keeps every exponential
     finite."""
