@@ -215,7 +215,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             // Last read of this accumulator: hand it back before the stores.
             fenceBeforeSync();
             __syncwarp();
-            if (lane == 0) mbarArriveRemote(inLeader(&sAccEmpty[h]));
+            if (lane == 0) arriveInLeader(&sAccEmpty[h]);
           }
           if (!any) continue;
           if (Epi::kCuts && w.slot >= 0)

@@ -200,16 +200,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!warpWait(&sAccFull[b], use & 1u, abort, 3)) break;
       fenceAfterSync();
       const uint32_t acc = tmem + b * kTmemCols + ((uint32_t)(quarter * 32) << 16);
-#pragma unroll 1
-      for (int c = half * 128; c < half * 128 + 128; c += 32) {
-        float v[32];
-        tmemLoad32(acc + (uint32_t)c, v);
-        if (c + 32 == half * 128 + 128) {
-          // Last read of this buffer: hand it back before the stores.
+      // The next 32 columns are on their way while these are worked on.
+      uint32_t r[2][32];
+      tmemIssue32(acc + (uint32_t)(half * 128), r[0]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = half * 128 + i * 32;
+        tmemWait(r[i & 1]);
+        if (i < 3) {
+          tmemIssue32(acc + (uint32_t)(c + 32), r[(i + 1) & 1]);
+        } else {
+          // Everything is read: the accumulator goes back before the stores.
           fenceBeforeSync();
           __syncwarp();
-          if (lane == 0) mbarArriveRemote(inLeader(&sAccEmpty[b]));
+          if (lane == 0) arriveInLeader(&sAccEmpty[b]);
         }
+        float v[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(r[i & 1][k]);
         args.epi.chunk(st, v, row0 + lane, tileN * 256 + c);
       }
       args.epi.end(st, row0 + lane, tileN * 2 + half);
