@@ -93,13 +93,26 @@ __global__ void __launch_bounds__(kThreads)
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const uint32_t ex = int8Exponent(__uint_as_float(top << 16));
-    const Int8Inverse inv = int8Inverse(ex);
-    uint32_t o[2] = {0u, 0u};
+    float v[8];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const uint32_t lo = int8Quantize(__uint_as_float(w[k] << 16), inv);
-      const uint32_t hi = int8Quantize(__uint_as_float(w[k] & 0xffff0000u), inv);
-      o[k >> 1] |= (lo | hi << 8) << ((k & 1) * 16);
+      v[2 * k] = __uint_as_float(w[k] << 16);
+      v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+    }
+    uint32_t o[2];
+    if (int8Plain(ex)) {
+      const float inv = int8Inverse(ex).a;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        o[k] = int8Quantize4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3], inv);
+    } else {
+      const Int8Inverse inv = int8Inverse(ex);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        o[k] = 0u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[k] |= int8Quantize(v[4 * k + j], inv) << (8 * j);
+      }
     }
     if (p[i].at >= 0) *reinterpret_cast<uint2*>(q + p[i].at) = make_uint2(o[0], o[1]);
     const uint32_t s = s0 + i * kThreads;

@@ -20,6 +20,7 @@
 
 #include "common.cuh"
 #include "int8_blocks.cuh"
+#include "packed_f32.cuh"
 #include "tnccl_ops.h"
 
 namespace tnops {
@@ -64,6 +65,36 @@ __device__ __forceinline__ float geluTanhGrad(float x) {
   return fmaf(2.0f * x * r * (e * r), du, r);
 }
 
+// The same derivative of two numbers at once, for finite ones. Only the lower
+// end of u is held: there e^(-2u) would pass the fp32 range; at the other
+// e is 0, r is 1 and the slope 1.
+__device__ __forceinline__ uint64_t geluTanhGrad2(uint64_t x) {
+  const float k0 = 0.7978845608028654f, k0k1 = 0.7978845608028654f * 0.044715f;
+  const float m2log2e = -2.0f * 1.4426950408889634f;
+  const uint64_t x2 = mul2(x, x);
+  const uint64_t du = fma2(pack2(3.0f * k0k1, 3.0f * k0k1), x2, pack2(k0, k0));
+  float a, b;
+  unpack2(mul2(x, fma2(pack2(k0k1, k0k1), x2, pack2(k0, k0))), a, b);
+  unpack2(mul2(pack2(fmaxf(a, -40.0f), fmaxf(b, -40.0f)), pack2(m2log2e, m2log2e)), a, b);
+  const uint64_t e = pack2(ex2Approx(a), ex2Approx(b));
+  unpack2(add2(e, pack2(1.0f, 1.0f)), a, b);
+  float ra, rb;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(ra) : "f"(a));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rb) : "f"(b));
+  const uint64_t r = pack2(ra, rb);
+  const uint64_t t = mul2(mul2(x, r), mul2(e, r));
+  return fma2(add2(t, t), du, r);
+}
+// Four 8-bit values as two pairs.
+__device__ __forceinline__ void int8x4Pairs(uint32_t q, uint64_t step, uint64_t& lo,
+                                            uint64_t& hi) {
+  const uint32_t u = q ^ 0x80808080u;
+  const uint64_t off = pack2(-8388736.f, -8388736.f);
+  auto at = [&](uint32_t bytes) { return __uint_as_float(__byte_perm(u, 0x4b000000u, bytes)); };
+  lo = mul2(add2(pack2(at(0x7650), at(0x7651)), off), step);
+  hi = mul2(add2(pack2(at(0x7652), at(0x7653)), off), step);
+}
+
 // What the GELU gradient reads pre from: nothing (no GELU), bf16, or 8-bit
 // blocks (whose exponents are `preExp`).
 enum class Pre { kNone, kBf16, kInt8 };
@@ -73,7 +104,6 @@ __global__ void __launch_bounds__(kWarps * 32)
     colsumPartial(const uint16_t* __restrict__ gy, const void* __restrict__ pre,
                   const uint8_t* __restrict__ preExp, uint16_t* __restrict__ gout,
                   float* __restrict__ partial, int M, int N, int rowsPer) {
-  constexpr bool GELU = PRE != Pre::kNone;
   const int blocks = (N + kInt8Block - 1) / kInt8Block;
   __shared__ float sAcc[kWarps][kCols];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -107,16 +137,26 @@ __global__ void __launch_bounds__(kWarps * 32)
         if (r >= r1) continue;
         float f[8];
         bf16x8ToF(g[u], f);
-        if (GELU) {
-          float x[8];
-          if (PRE == Pre::kInt8) {
-            const float step = int8Step(p[u].z);
-            const float4 a = int8x4(p[u].x, step), b = int8x4(p[u].y, step);
-            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-            x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-          } else {
-            bf16x8ToF(p[u], x);
+        if (PRE == Pre::kInt8) {
+          const float s1 = int8Step(p[u].z);
+          const uint64_t step = pack2(s1, s1);
+          uint64_t x[4];
+          int8x4Pairs(p[u].x, step, x[0], x[1]);
+          int8x4Pairs(p[u].y, step, x[2], x[3]);
+          uint32_t o[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float a, b;
+            unpack2(mul2(pack2(f[2 * i], f[2 * i + 1]), geluTanhGrad2(x[i])), a, b);
+            const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+            o[i] = *reinterpret_cast<const uint32_t*>(&h);
+            f[2 * i] = __uint_as_float(o[i] << 16);
+            f[2 * i + 1] = __uint_as_float(o[i] & 0xffff0000u);
           }
+          *reinterpret_cast<uint4*>(gout + (size_t)r * N + col0) = make_uint4(o[0], o[1], o[2], o[3]);
+        } else if (PRE == Pre::kBf16) {
+          float x[8];
+          bf16x8ToF(p[u], x);
           uint32_t o[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {

@@ -54,7 +54,7 @@ struct GeluInt8Epi {
     st.e |= ex << (((col0 >> 5) & 3) * 8);
     const size_t at = (size_t)row * cols + col0;
     uint32_t o[8];
-    if (ex >= 6u && ex < 254u) {
+    if (int8Plain(ex)) {
       // x 2^(133 - e) + 1.5 2^23: the sum's last byte is the whole number that
       // x / step rounds to, in two's complement.
       const float inv = __uint_as_float((260u - ex) << 23);

@@ -37,20 +37,36 @@ __device__ __forceinline__ Int8Inverse int8Inverse(uint32_t e) {
   const uint32_t c = e < 6u ? 6u : e > 254u ? 254u : e;
   return {__uint_as_float((260u - c) << 23), __uint_as_float((127u + c - (e < 6u ? e : c)) << 23)};
 }
-// q as a two's complement byte. Only fp32 values above 127.5 2^121 can reach
-// 128 (e stops at 254): they keep 127.
+// q as a two's complement byte. x / step + 1.5 2^23 is a whole number whose
+// last byte is q (one FMA, where a conversion takes the special-function
+// unit). Only fp32 values above 127.5 2^121 can reach 128 (e stops at 254):
+// they keep 127.
 __device__ __forceinline__ uint32_t int8Quantize(float x, Int8Inverse inv) {
-  const int q = __float2int_rn(x * inv.a * inv.b);
-  return (uint32_t)max(-127, min(127, q)) & 0xffu;
+  const float y = fminf(fmaxf(x * inv.a * inv.b, -127.f), 127.f);
+  return __float_as_uint(y + 12582912.f) & 0xffu;
+}
+// Four values to four bytes, for an exponent in [6, 254): one factor, and
+// nothing to clamp.
+__device__ __forceinline__ bool int8Plain(uint32_t e) { return e - 6u < 248u; }
+__device__ __forceinline__ uint32_t int8Quantize4(float a, float b, float c, float d, float inv) {
+  const uint32_t x = __float_as_uint(fmaf(a, inv, 12582912.f)),
+                 y = __float_as_uint(fmaf(b, inv, 12582912.f)),
+                 z = __float_as_uint(fmaf(c, inv, 12582912.f)),
+                 w = __float_as_uint(fmaf(d, inv, 12582912.f));
+  return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
 }
 __device__ __forceinline__ float int8Step(uint32_t e) {
   if (e == 255u) return __uint_as_float(0x7fc00000u);
   return __uint_as_float(e >= 7u ? (e - 6u) << 23 : 1u << (e + 16u));
 }
-// Four bytes to four values.
+// Four bytes to four values: q + 128 is put in the last byte of 2^23, from
+// which 2^23 + 128 is taken; both steps are exact.
 __device__ __forceinline__ float4 int8x4(uint32_t q, float step) {
-  return make_float4((float)(int8_t)(q & 0xff) * step, (float)(int8_t)((q >> 8) & 0xff) * step,
-                     (float)(int8_t)((q >> 16) & 0xff) * step, (float)(int8_t)(q >> 24) * step);
+  const uint32_t u = q ^ 0x80808080u;
+  auto value = [&](uint32_t bytes) {
+    return (__uint_as_float(__byte_perm(u, 0x4b000000u, bytes)) - 8388736.f) * step;
+  };
+  return make_float4(value(0x7650), value(0x7651), value(0x7652), value(0x7653));
 }
 
 }  // namespace

@@ -3,7 +3,8 @@
 // warp stores a block of the result.
 //
 // An operand is "K-major" when k is contiguous in memory ([m, k] rows) and
-// "MN-major" when m (or n) is contiguous ([k, m] rows). In shared memory, with the 128-byte swizzle:
+// "MN-major" when m (or n) is contiguous ([k, m] rows). In shared memory, with
+// the 128-byte swizzle:
 //   K-major   128 rows of 64 k (128 bytes), 8-row atoms of 1024 bytes; the
 //             descriptor's stride is the 1024 bytes from 8 rows to the next 8,
 //             and a K = 16 slice starts 32 bytes after the one before it;
@@ -13,6 +14,7 @@
 //             slice starts 2048 bytes after the one before it.
 #pragma once
 
+#include "packed_f32.cuh"
 #include "tcgen05.cuh"
 
 namespace tnops {
@@ -30,32 +32,6 @@ __device__ __forceinline__ bool electOne() {
       : "=r"(p));
   return p != 0;
 }
-// Two fp32 numbers in one 64-bit register and the packed arithmetic on them
-// (one instruction for both).
-__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
-  return d;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 // tcgen05.ld of 32 columns in two steps: the load is issued, and its registers
 // may be read after tmemWait (which names them, so that no use moves ahead).
 __device__ __forceinline__ void tmemIssue32(uint32_t taddr, uint32_t (&r)[32]) {
