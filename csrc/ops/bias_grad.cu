@@ -11,12 +11,14 @@
 // tiles the matrix into (256-column, rowsPer-row) blocks; each warp of a CTA
 // owns 256 columns (8 per lane, one 16-byte load per row) and every 8th row
 // of the block, 4 rows in flight; the 8 warp sums are added in warp order
-// into one fp32 partial per block. Pass 2 adds the partials of a column in
+// into one fp32 partial per block (the result, where one block is all). Pass 2 adds the partials of a column in
 // block order (colReduce, common.cuh). The summation order depends only on
 // (M, N), never on scheduling. Rounding of the GELU gradient to bf16 happens before it is
 // summed, as when the gradient tensor is materialised and then reduced.
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "int8_blocks.cuh"
@@ -99,11 +101,13 @@ __device__ __forceinline__ void int8x4Pairs(uint32_t q, uint64_t step, uint64_t&
 // blocks (whose exponents are `preExp`).
 enum class Pre { kNone, kBf16, kInt8 };
 
-template <Pre PRE>
+// T: what the sums are written as (fp32 partial sums, or the result itself
+// where one block of rows is all).
+template <Pre PRE, class T>
 __global__ void __launch_bounds__(kWarps * 32)
     colsumPartial(const uint16_t* __restrict__ gy, const void* __restrict__ pre,
                   const uint8_t* __restrict__ preExp, uint16_t* __restrict__ gout,
-                  float* __restrict__ partial, int M, int N, int rowsPer) {
+                  T* __restrict__ partial, int M, int N, int rowsPer) {
   const int blocks = (N + kInt8Block - 1) / kInt8Block;
   __shared__ float sAcc[kWarps][kCols];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -181,7 +185,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     float s = sAcc[0][threadIdx.x];
 #pragma unroll
     for (int k = 1; k < kWarps; ++k) s += sAcc[k][threadIdx.x];
-    partial[(size_t)blockIdx.y * N + c] = s;
+    putSum(partial + (size_t)blockIdx.y * N + c, s);
   }
 }
 
@@ -198,8 +202,9 @@ extern "C" int tnops_colsum_parts(int M, int N) {
   return parts < 1 ? 1 : parts > maxParts ? maxParts : parts;
 }
 
+template <class T>
 static int launchColsum(Pre kind, const uint16_t* gy, const void* pre, const uint8_t* preExp,
-                        uint16_t* gout, float* db, float* partial, int M, int N,
+                        uint16_t* gout, T* db, float* partial, int M, int N,
                         cudaStream_t stream) {
   if (M <= 0 || N <= 0 || N % 8 != 0) return 1;
   // 16-byte pieces of every row (8-byte ones of an 8-bit pre): N % 8 == 0
@@ -211,12 +216,20 @@ static int launchColsum(Pre kind, const uint16_t* gy, const void* pre, const uin
   const int parts = tnops_colsum_parts(M, N);
   const int rowsPer = (M + parts - 1) / parts;
   const dim3 grid((unsigned)((N + kCols - 1) / kCols), (unsigned)parts);
-  auto kernel = kind == Pre::kNone    ? colsumPartial<Pre::kNone>
-                : kind == Pre::kBf16 ? colsumPartial<Pre::kBf16>
-                                     : colsumPartial<Pre::kInt8>;
-  kernel<<<grid, kWarps * 32, 0, stream>>>(gy, pre, preExp, gout, partial, M, N, rowsPer);
-  colReduce<<<(N + 31) / 32, kColReduceWarps * 32, 0, stream>>>(partial, parts, N, N, N, db,
-                                                                 nullptr);
+  auto run = [&](auto* sums) {
+    using S = std::remove_pointer_t<decltype(sums)>;
+    auto kernel = kind == Pre::kNone    ? colsumPartial<Pre::kNone, S>
+                  : kind == Pre::kBf16 ? colsumPartial<Pre::kBf16, S>
+                                       : colsumPartial<Pre::kInt8, S>;
+    kernel<<<grid, kWarps * 32, 0, stream>>>(gy, pre, preExp, gout, sums, M, N, rowsPer);
+  };
+  if (parts == 1) {
+    run(db);
+    return launched(cudaGetLastError()) == 0 ? 0 : 2;
+  }
+  run(partial);
+  colReduce<T><<<(N + 31) / 32, kColReduceWarps * 32, 0, stream>>>(partial, parts, N, N, N, db,
+                                                                   static_cast<T*>(nullptr));
   gLaunches.fetch_add(2, std::memory_order_relaxed);
   return cudaGetLastError() == cudaSuccess ? 0 : 2;
 }
@@ -232,8 +245,17 @@ extern "C" int tnops_gelu_bwd_bias(const uint16_t* gy, const uint16_t* pre, uint
   return launchColsum(Pre::kBf16, gy, pre, nullptr, gpre, db, partial, M, N, stream);
 }
 
+extern "C" int tnops_bias_grad_bf16(const uint16_t* g, uint16_t* db, float* partial, int M, int N,
+                                    cudaStream_t stream) {
+  return launchColsum(Pre::kNone, g, nullptr, nullptr, nullptr, db, partial, M, N, stream);
+}
+
 extern "C" int tnops_gelu_bwd_bias_int8(const uint16_t* gy, const uint8_t* pre_q,
-                                        const uint8_t* pre_e, uint16_t* gpre, float* db,
-                                        float* partial, int M, int N, cudaStream_t stream) {
-  return launchColsum(Pre::kInt8, gy, pre_q, pre_e, gpre, db, partial, M, N, stream);
+                                        const uint8_t* pre_e, uint16_t* gpre, void* db,
+                                        int db_f32, float* partial, int M, int N,
+                                        cudaStream_t stream) {
+  return db_f32 ? launchColsum(Pre::kInt8, gy, pre_q, pre_e, gpre, static_cast<float*>(db),
+                               partial, M, N, stream)
+                : launchColsum(Pre::kInt8, gy, pre_q, pre_e, gpre, static_cast<uint16_t*>(db),
+                               partial, M, N, stream);
 }

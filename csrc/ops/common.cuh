@@ -56,9 +56,12 @@ constexpr int kSMs = 148;
 // count of 100-300 rows is common).
 constexpr int kColReduceWarps = 32;
 namespace {  // one copy per translation unit
+__device__ __forceinline__ void putSum(float* p, float v) { *p = v; }
+__device__ __forceinline__ void putSum(uint16_t* p, float v) { *p = f2bf(v); }
+template <class T = float>
 __global__ void __launch_bounds__(kColReduceWarps * 32)
     colReduce(const float* __restrict__ in, int nparts, int ld, int ncols, int split,
-              float* __restrict__ out0, float* __restrict__ out1) {
+              T* __restrict__ out0, T* __restrict__ out1) {
   __shared__ float s[kColReduceWarps][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = blockIdx.x * 32 + lane;
@@ -82,9 +85,9 @@ __global__ void __launch_bounds__(kColReduceWarps * 32)
 #pragma unroll
     for (int w = 0; w < kColReduceWarps; ++w) t += s[w][lane];
     if (col < split)
-      out0[col] = t;
+      putSum(out0 + col, t);
     else
-      out1[col - split] = t;
+      putSum(out1 + col - split, t);
   }
 }
 }  // namespace

@@ -280,13 +280,20 @@ extern "C" int tnops_linear_ce_mean(const float* loss, const int64_t* target, fl
   return launched(cudaGetLastError());
 }
 
-extern "C" size_t tnops_linear_ce_scratch(int rows, int width, int classes, int piece,
+// Rows of padding after the classes that the last piece's product writes; more
+// of them are left to a memset.
+static int paddedRows(int classes, int vocab) {
+  return vocab - classes < 256 ? vocab - classes : 0;
+}
+
+extern "C" size_t tnops_linear_ce_scratch(int rows, int width, int classes, int vocab, int piece,
                                           int want_dx, int want_dw) {
-  if (rows <= 0 || width <= 0 || classes <= 0 || piece <= 0) return 0;
+  if (rows <= 0 || width <= 0 || classes <= 0 || vocab < classes || piece <= 0) return 0;
   const int last = (classes - 1) % piece + 1;
-  const size_t a = tnops_linear_grads_scratch(rows, classes < piece ? classes : piece, width, want_dx,
-                                              want_dw),
-               b = tnops_linear_grads_scratch(rows, last, width, want_dx, want_dw);
+  const size_t a = last == classes ? 0
+                                   : linearGradsScratch(rows, piece, 0, width, want_dx, want_dw),
+               b = linearGradsScratch(rows, last, paddedRows(classes, vocab), width, want_dx,
+                                      want_dw);
   return a > b ? a : b;
 }
 
@@ -304,7 +311,8 @@ extern "C" int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* 
   if (!aligned16(scratch)) return 1;
   if (dx && !whole && (dx_f32 == nullptr || !aligned16(dx_f32))) return 1;
   const size_t dwSize = dw_f32 ? 4 : 2;
-  if (dw && vocab > classes) {
+  const int padded = paddedRows(classes, vocab);
+  if (dw && vocab > classes + padded) {
     const cudaError_t e = cudaMemsetAsync(static_cast<char*>(dw) + dwSize * width * (size_t)classes,
                                           0, dwSize * width * (size_t)(vocab - classes), stream);
     if (e != cudaSuccess) return (int)e;
@@ -340,6 +348,7 @@ extern "C" int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* 
     g.rows = rows;
     g.outs = n;
     g.ins = width;
+    g.padded = first + n == classes ? padded : 0;
     if (int rc = linearGrads(g, stream)) return rc;
   }
   if (dx && !whole) {

@@ -12,30 +12,12 @@
 // without a long tile begin with the short ones, and where that still leaves
 // pairs idle it cuts the long sums, whose parts a second kernel adds.
 #include "linear_grads.h"
+
 #include "pair_gemm.cuh"
 #include "tnccl_ops.h"
 
 namespace tnops {
 namespace {
-
-struct StoreEpi {
-  static constexpr bool kCuts = true;
-  CUtensorMap mapOut[2];
-  int rows[2], cols[2], mode[2];
-
-  struct State {};
-  __device__ __forceinline__ State begin(int, int) const { return {}; }
-  __device__ __forceinline__ void chunk(State&, const float (&v)[32], int which, int lane,
-                                        int row0, int col0, uint32_t buf) const {
-    const bool inside = row0 < rows[which] && col0 < cols[which];
-    if (mode[which] == kStoreBf16)
-      storeBf16(v, lane, buf, &mapOut[which], row0, col0, inside);
-    else
-      storeF32(v, lane, buf, &mapOut[which], row0, col0, inside, mode[which] == kAddF32);
-  }
-  __device__ __forceinline__ void end(const State&, int, int) const {}
-};
-
 
 struct JoinArgs {
   const float* partial;  // [split * tiles][512][256]
@@ -81,12 +63,12 @@ __global__ void __launch_bounds__(kJoinThreads)
 
 // Tile counts and sums of the launch: the product with the longer sum first.
 // kinds[i]: whether product i is dX.
-int shapes(int rows, int outs, int ins, bool wantDx, bool wantDw, GemmProblem* prob,
+int shapes(int rows, int outs, int padded, int ins, bool wantDx, bool wantDw, GemmProblem* prob,
            bool* isDx) {
   int n = 0;
   auto add = [&](bool dx) {
     GemmProblem& p = prob[n];
-    p.rows = dx ? rows : outs;
+    p.rows = dx ? rows : outs + padded;  // past the last of g's columns A reads zero
     p.tilesM = (p.rows + kPairBM - 1) / kPairBM;
     p.tilesN = (ins + 255) / 256;
     p.kBlocks = ((dx ? outs : rows) + kBK - 1) / kBK;
@@ -108,34 +90,33 @@ size_t scratchFor(const PairSchedule& s) {
 }  // namespace
 
 int linearGrads(const LinearGrads& a, cudaStream_t stream) {
-  if (a.rows <= 0 || a.outs <= 0 || a.ins <= 0 || a.ldg < a.outs) return 1;
+  if (a.rows <= 0 || a.outs <= 0 || a.ins <= 0 || a.padded < 0 || a.ldg < a.outs) return 1;
   if (a.ldg % 8 != 0 || a.ins % 8 != 0) return 1;  // 16-byte rows (TMA)
   if (!aligned16(a.g) || (a.dxStore && (!aligned16(a.w) || !aligned16(a.dx))) ||
       (a.dwStore && (!aligned16(a.x) || !aligned16(a.dw))) || !aligned16(a.scratch))
     return 1;
-  PairGemmArgs<StoreEpi> args{};
+  PairGemmArgs args{};
   bool isDx[2] = {};
-  args.problems = shapes(a.rows, a.outs, a.ins, a.dxStore != kStoreNone,
+  args.problems = shapes(a.rows, a.outs, a.padded, a.ins, a.dxStore != kStoreNone,
                          a.dwStore != kStoreNone, args.prob, isDx);
   if (args.problems == 0) return 0;
-  planGemm(&args, true);
+  planGemm(&args);
   const PairSchedule& plan = args.schedule;
   if (scratchFor(plan) > a.scratchBytes || (plan.slots() > 0 && a.scratch == nullptr)) return 1;
   JoinArgs join[2] = {};
   for (int i = 0; i < args.problems; ++i) {
     GemmProblem& p = args.prob[i];
-    const int m = isDx[i] ? a.rows : a.outs, sum = isDx[i] ? a.outs : a.rows;
+    const int m = p.rows, sum = isDx[i] ? a.outs : a.rows;
     const int mode = isDx[i] ? a.dxStore : a.dwStore;
     void* out = isDx[i] ? a.dx : a.dw;
-    args.epi.rows[i] = m;
-    args.epi.cols[i] = a.ins;
-    args.epi.mode[i] = mode;
+    args.cols[i] = a.ins;
+    args.mode[i] = mode;
     join[i] = {static_cast<const float*>(a.scratch) + (size_t)plan.slotBase(i) * kPairBM * 256,
                out, plan.tiles[i], p.tilesN, plan.split[i], m, a.ins, mode};
     if (!operandMap(&p.mapA, a.g, a.rows, a.outs, a.ldg, !isDx[i]) ||
         !operandMap(&p.mapB, isDx[i] ? a.w : a.x, sum, a.ins, a.ins, true) ||
-        !(mode == kStoreBf16 ? bf16OutMap(&args.epi.mapOut[i], out, m, a.ins, a.ins)
-                             : f32OutMap(&args.epi.mapOut[i], out, m, a.ins, a.ins)))
+        !(mode == kStoreBf16 ? bf16OutMap(&args.mapOut[i], out, m, a.ins, a.ins)
+                             : f32OutMap(&args.mapOut[i], out, m, a.ins, a.ins)))
       return 4;
   }
   if (plan.slots() > 0 &&
@@ -151,6 +132,16 @@ int linearGrads(const LinearGrads& a, cudaStream_t stream) {
   return 0;
 }
 
+size_t linearGradsScratch(int rows, int outs, int padded, int ins, bool wantDx, bool wantDw) {
+  if (rows <= 0 || outs <= 0 || padded < 0 || ins <= 0) return 0;
+  PairGemmArgs args{};
+  bool isDx[2];
+  args.problems = shapes(rows, outs, padded, ins, wantDx, wantDw, args.prob, isDx);
+  if (args.problems == 0) return 0;
+  planGemm(&args);
+  return scratchFor(args.schedule);
+}
+
 unsigned linearGradsStatus(int reset) { return readStatus(reset); }
 
 }  // namespace tnops
@@ -159,13 +150,7 @@ using namespace tnops;
 
 extern "C" size_t tnops_linear_grads_scratch(int rows, int outs, int ins, int want_dx,
                                              int want_dw) {
-  if (rows <= 0 || outs <= 0 || ins <= 0) return 0;
-  PairGemmArgs<StoreEpi> args{};
-  bool isDx[2];
-  args.problems = shapes(rows, outs, ins, want_dx != 0, want_dw != 0, args.prob, isDx);
-  if (args.problems == 0) return 0;
-  planGemm(&args, true);
-  return scratchFor(args.schedule);
+  return linearGradsScratch(rows, outs, 0, ins, want_dx != 0, want_dw != 0);
 }
 
 extern "C" int tnops_linear_grads(const void* g, int64_t ldg, const void* w, const void* x,
@@ -173,6 +158,6 @@ extern "C" int tnops_linear_grads(const void* g, int64_t ldg, const void* w, con
                                   void* scratch, size_t scratch_bytes, cudaStream_t stream) {
   if (g == nullptr || (dx && !w) || (dw && !x)) return 1;
   LinearGrads a{g, ldg, w, x, dx, dw, scratch, scratch_bytes, dx ? kStoreBf16 : kStoreNone,
-                dw ? (dw_f32 ? kStoreF32 : kStoreBf16) : kStoreNone, rows, outs, ins};
+                dw ? (dw_f32 ? kStoreF32 : kStoreBf16) : kStoreNone, rows, outs, ins, 0};
   return linearGrads(a, stream);
 }

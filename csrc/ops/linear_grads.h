@@ -14,7 +14,8 @@ enum GradStore { kStoreNone = 0, kStoreBf16 = 1, kStoreF32 = 2, kAddF32 = 3 };
 
 // y = x w^T with y [rows, outs], x [rows, ins], w [outs, ins]; g [rows, outs]
 // (rows `ldg` elements apart) is the gradient of y. dx [rows, ins] = g w,
-// dw [outs, ins] = g^T x, each left out with kStoreNone.
+// dw [outs, ins] = g^T x, each left out with kStoreNone. dw may have `padded`
+// more rows, which get zeros.
 struct LinearGrads {
   const void* g;
   int64_t ldg;
@@ -25,10 +26,11 @@ struct LinearGrads {
   void* scratch;  // 16-byte aligned, at least tnops_linear_grads_scratch()
   size_t scratchBytes;
   GradStore dxStore, dwStore;
-  int rows, outs, ins;
+  int rows, outs, ins, padded;
 };
 
 int linearGrads(const LinearGrads& a, cudaStream_t stream);
+size_t linearGradsScratch(int rows, int outs, int padded, int ins, bool wantDx, bool wantDw);
 
 // First failure code of the tensor-core kernels of linear_grads.cu,
 // linear_ce.cu and gelu_int8.cu.

@@ -16,13 +16,14 @@
 // the 512 TMEM columns. An SM then loads 48 bytes per clock of MMA where a
 // 256 x 256 tile takes 64, more than L2 delivers to all SMs at once (8192^3 of
 // zeros, so that power does not limit: 1810 TFLOP/s against 1430). With no
-// accumulator to spare, a tile's epilogue runs before the next tile's first
-// MMA of the same half; these are the products with the long sums.
+// accumulator to spare, an epilogue warp reads all that it has of a half into
+// registers and hands the accumulator back before it stores any of it.
 // A launch may hold two products (`GemmProblem`), so that dX and dW of a layer
 // fill the GPU together; who computes what is pair_schedule.h's. Every wait is
 // bounded as there; the first failure is kept in the file's status word.
 #pragma once
 
+#include "linear_grads.h"
 #include "pair_parts.cuh"
 #include "pair_schedule.h"
 
@@ -44,24 +45,18 @@ struct alignas(64) GemmProblem {
   int aMn, bMn;
 };
 
-template <class Epi>
 struct alignas(64) PairGemmArgs {
   GemmProblem prob[2];
-  CUtensorMap mapPartial;  // [512 slots, 256] fp32, for an Epi that kCuts
+  CUtensorMap mapOut[2];
+  CUtensorMap mapPartial;  // [512 slots, 256] fp32: parts of cut tiles
   int problems;
+  int cols[2];             // n
+  int mode[2];             // GradStore
   PairSchedule schedule;
-  Epi epi;
 };
 
-// Epi: `State begin(problem, row)` once per tile and thread (the thread's row
-// of the output), `chunk(state, v, problem, lane, row0, col0, buf)` for each
-// 32 x 32 block of a warp (v: the row's 32 columns from col0; buf: the warp's
-// 4 KiB of staging), `end(state, row, part)` after the last block (part: the
-// 128 columns' number). With Epi::kCuts, parts of cut tiles go to mapPartial
-// instead.
-template <class Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    pairGemmKernel(const __grid_constant__ PairGemmArgs<Epi> args) {
+    pairGemmKernel(const __grid_constant__ PairGemmArgs args) {
   __shared__ __align__(8) uint64_t sFull[kPairStages];
   __shared__ __align__(8) uint64_t sEmpty[kPairStages];
   __shared__ __align__(8) uint64_t sAccFull[2];
@@ -206,24 +201,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         fenceAfterSync();
         const uint32_t acc = tmem + h * kTmemCols + ((uint32_t)(quarter * 32) << 16);
         const bool any = row0 < p.rows;  // the same for the whole warp
-        typename Epi::State st = args.epi.begin(w.which, row0 + lane);
-#pragma unroll 1
-        for (int c = side * 128; c < side * 128 + 128; c += 32) {
-          float v[32];
-          if (any) tmemLoad32(acc + (uint32_t)c, v);
-          if (c + 32 == side * 128 + 128) {
-            // Last read of this accumulator: hand it back before the stores.
-            fenceBeforeSync();
-            __syncwarp();
-            if (lane == 0) arriveInLeader(&sAccEmpty[h]);
-          }
-          if (!any) continue;
-          if (Epi::kCuts && w.slot >= 0)
-            storeF32(v, lane, buf, &args.mapPartial, w.slot * kPairBM + inTile, c, true, false);
-          else
-            args.epi.chunk(st, v, w.which, lane, row0, tileN * 256 + c, buf);
+        // All of the warp's 32 x 128 first: the accumulator goes back before
+        // anything is stored.
+        uint32_t r[4][32];
+        if (any) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tmemIssue32(acc + (uint32_t)(side * 128 + 32 * i), r[i]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tmemWait(r[i]);
         }
-        if (any) args.epi.end(st, row0 + lane, tileN * 2 + side);
+        fenceBeforeSync();
+        __syncwarp();
+        if (lane == 0) arriveInLeader(&sAccEmpty[h]);
+        if (!any) continue;
+        const int mode = args.mode[w.which], cols = args.cols[w.which];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(r[i][k]);
+          const int c = side * 128 + 32 * i, col0 = tileN * 256 + c;
+          if (w.slot >= 0)
+            storeF32(v, lane, buf, &args.mapPartial, w.slot * kPairBM + inTile, c, true, false);
+          else if (mode == kStoreBf16)
+            storeBf16(v, lane, buf, &args.mapOut[w.which], row0, col0, col0 < cols);
+          else
+            storeF32(v, lane, buf, &args.mapOut[w.which], row0, col0, col0 < cols,
+                     mode == kAddF32);
+        }
       }
     }
     epilogueDrain(lane);
@@ -241,10 +246,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 // -- host side -------------------------------------------------------------------
 
-// Plans the launch for kSMs / 2 pairs; with `cut`, sums may be split. Product
-// 0 must be the one with the longer sum.
-template <class Epi>
-void planGemm(PairGemmArgs<Epi>* args, bool cut) {
+// Plans the launch for kSMs / 2 pairs. Product 0 must be the one with the
+// longer sum.
+inline void planGemm(PairGemmArgs* args) {
   PairSchedule& s = args->schedule;
   s = {};
   s.pairs = kSMs / 2;
@@ -254,21 +258,19 @@ void planGemm(PairGemmArgs<Epi>* args, bool cut) {
     s.tiles[i] = args->prob[i].tilesM * args->prob[i].tilesN;
     s.k[i] = args->prob[i].kBlocks;
   }
-  planPairs(&s, cut);
+  planPairs(&s, true);
 }
 
 // Launches the products of `args`, whose schedule is planned. Returns 0, or a
 // non-zero code without a launch.
-template <class Epi>
-int launchPairGemm(const PairGemmArgs<Epi>& args, cudaStream_t stream) {
-  auto kernel = pairGemmKernel<Epi>;
+inline int launchPairGemm(const PairGemmArgs& args, cudaStream_t stream) {
   // Opt in to the shared memory once per device (bit d of `done`).
   static std::atomic<uint64_t> done{0};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 3;
   const uint64_t bit = 1ull << dev;
   if (!(done.load(std::memory_order_acquire) & bit)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(pairGemmKernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (int)kPairSmemBytes) != cudaSuccess)
       return 3;
     done.fetch_or(bit, std::memory_order_acq_rel);
@@ -276,7 +278,7 @@ int launchPairGemm(const PairGemmArgs<Epi>& args, cudaStream_t stream) {
   const PairSchedule& s = args.schedule;
   // In a first round, pairs past the last unit have nothing to do.
   const int units = s.units(0) + s.units(1), pairs = units < s.pairs ? units : s.pairs;
-  kernel<<<2u * (unsigned)pairs, kThreads, kPairSmemBytes, stream>>>(args);
+  pairGemmKernel<<<2u * (unsigned)pairs, kThreads, kPairSmemBytes, stream>>>(args);
   return launched(cudaGetLastError());
 }
 

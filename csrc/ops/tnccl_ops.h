@@ -56,10 +56,14 @@ int tnops_bias_grad(const uint16_t* g, float* db, float* partial, int M, int N,
 int tnops_gelu_bwd_bias(const uint16_t* gy, const uint16_t* pre, uint16_t* gpre, float* db,
                         float* partial, int M, int N, cudaStream_t stream);
 int tnops_colsum_parts(int M, int N);
+// tnops_bias_grad with db in bf16 (rounded from the fp32 sum).
+int tnops_bias_grad_bf16(const uint16_t* g, uint16_t* db, float* partial, int M, int N,
+                         cudaStream_t stream);
 // tnops_gelu_bwd_bias with pre in 8-bit blocks (tnops_quantize_int8's form):
-// pre_q [M, N] 8-byte aligned, pre_e [M, ceil(N / 32)].
+// pre_q [M, N] 8-byte aligned, pre_e [M, ceil(N / 32)]; db fp32 with db_f32,
+// else bf16.
 int tnops_gelu_bwd_bias_int8(const uint16_t* gy, const uint8_t* pre_q, const uint8_t* pre_e,
-                             uint16_t* gpre, float* db, float* partial, int M, int N,
+                             uint16_t* gpre, void* db, int db_f32, float* partial, int M, int N,
                              cudaStream_t stream);
 
 // Multiplies a bf16 tensor by the fp32 scalar *scale (device memory); no-op
@@ -127,8 +131,8 @@ int tnops_linear_grads(const void* g, int64_t ldg, const void* w, const void* x,
 //    rows * width floats when piece < classes, and scratch scratch_bytes, at
 //    least tnops_linear_ce_scratch(...). A null dx or dw is left out.
 int tnops_linear_ce_parts(int classes);
-size_t tnops_linear_ce_scratch(int rows, int width, int classes, int piece, int want_dx,
-                               int want_dw);
+size_t tnops_linear_ce_scratch(int rows, int width, int classes, int vocab, int piece,
+                               int want_dx, int want_dw);
 int tnops_linear_ce_fwd(const void* x, const void* w, const int64_t* target, float* loss,
                         float* lse, float* partial, int rows, int width, int classes,
                         cudaStream_t stream);

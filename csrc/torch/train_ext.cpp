@@ -153,9 +153,11 @@ CeShape ceShape(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targ
           asInt(w.size(0), "vocabulary")};
 }
 
-// -> per-row loss, lse, and [sum or mean, 1 / rows that count]
+// -> per-row loss, lse, and (but for kNone) [sum or mean, 1 / rows that count]
+enum Reduction { kMean = 0, kSum = 1, kNone = 2 };
 std::vector<at::Tensor> linearCeFwd(const at::Tensor& x, const at::Tensor& w,
-                                    const at::Tensor& target, int64_t classes, bool mean) {
+                                    const at::Tensor& target, int64_t classes,
+                                    int64_t reduction) {
   const CeShape s = ceShape(x, w, target, classes);
   c10::cuda::CUDAGuard g(x.device());
   const auto opt = x.options().dtype(at::kFloat);
@@ -165,14 +167,15 @@ std::vector<at::Tensor> linearCeFwd(const at::Tensor& x, const at::Tensor& w,
     out.select(0, 1).fill_(1.0);
     return {loss, lse, out};
   }
-  auto out = at::empty({2}, opt);
   auto partial = at::empty({(int64_t)tnops_linear_ce_parts(s.classes), s.rows, 2}, opt);
   ok(tnops_linear_ce_fwd(x.data_ptr(), w.data_ptr(), target.data_ptr<int64_t>(),
                          loss.data_ptr<float>(), lse.data_ptr<float>(), partial.data_ptr<float>(),
                          s.rows, s.width, s.classes, streamOf(x)),
      "tnops_linear_ce_fwd");
+  if (reduction == kNone) return {loss, lse, at::Tensor()};
+  auto out = at::empty({2}, opt);
   ok(tnops_linear_ce_mean(loss.data_ptr<float>(), target.data_ptr<int64_t>(),
-                          out.data_ptr<float>(), s.rows, s.classes, mean ? 1 : 0, streamOf(x)),
+                          out.data_ptr<float>(), s.rows, s.classes, reduction == kMean ? 1 : 0, streamOf(x)),
      "tnops_linear_ce_mean");
   return {loss, lse, out};
 }
@@ -216,7 +219,7 @@ std::vector<at::Tensor> linearCeBwd(const at::Tensor& x, const at::Tensor& w,
   const int64_t piece = cePiece(s.rows, s.classes, budget);
   auto d = at::empty({(int64_t)s.rows, piece}, x.options());
   const size_t scratchBytes =
-      tnops_linear_ce_scratch(s.rows, s.width, s.classes, (int)piece, wantDx, wantDw);
+      tnops_linear_ce_scratch(s.rows, s.width, s.classes, s.vocab, (int)piece, wantDx, wantDw);
   auto scratch = scratchOf(scratchBytes, x);
   at::Tensor dxF32;
   if (wantDx && piece < s.classes) dxF32 = at::empty(x.sizes(), x.options().dtype(at::kFloat));
@@ -232,6 +235,17 @@ std::vector<at::Tensor> linearCeBwd(const at::Tensor& x, const at::Tensor& w,
 }
 
 // -- linear layers with 8-bit activations ------------------------------------------
+
+// Scratch of the column sums of an [M, N] matrix; none where one block of rows
+// is all.
+struct ColumnParts {
+  at::Tensor t;
+  operator float*() const { return t.defined() ? t.data_ptr<float>() : nullptr; }
+};
+ColumnParts columnParts(const at::Tensor& like, int M, int N) {
+  const int64_t parts = tnops_colsum_parts(M, N);
+  return {parts > 1 ? at::empty({parts * N}, like.options().dtype(at::kFloat)) : at::Tensor()};
+}
 
 // x [rows, cols] -> (q int8 [rows, cols], e uint8 [rows, ceil(cols / 32)])
 std::vector<at::Tensor> quantizeInt8(const at::Tensor& x) {
@@ -294,23 +308,27 @@ std::vector<at::Tensor> linearGeluInt8(const at::Tensor& x, const at::Tensor& w,
   return {act, q, e};
 }
 
-// g bf16 [M, N] -> db fp32 [N] (column sums)
-at::Tensor biasGradient(const at::Tensor& grad, const Opt& out) {
+// g bf16 [M, N] -> db [N] (column sums) of type st
+at::Tensor biasGradient(const at::Tensor& grad, at::ScalarType st, const Opt& out) {
   need(grad, at::kBFloat16, "grad");
   TORCH_CHECK(grad.dim() == 2 && grad.size(1) % 8 == 0, "bias_grad: want [M, N] with N % 8 == 0");
   c10::cuda::CUDAGuard g(grad.device());
   const int M = asInt(grad.size(0), "rows"), N = asInt(grad.size(1), "columns");
-  auto db = out ? *out : at::empty({N}, grad.options().dtype(at::kFloat));
-  auto part = at::empty({(int64_t)tnops_colsum_parts(M, N) * N}, grad.options().dtype(at::kFloat));
-  ok(tnops_bias_grad(static_cast<uint16_t*>(grad.data_ptr()), db.data_ptr<float>(),
-                     part.data_ptr<float>(), M, N, streamOf(grad)),
+  auto db = out ? *out : at::empty({N}, grad.options().dtype(st));
+  auto part = columnParts(grad, M, N);
+  auto* gp = static_cast<uint16_t*>(grad.data_ptr());
+  ok(st == at::kFloat
+         ? tnops_bias_grad(gp, db.data_ptr<float>(), part, M, N, streamOf(grad))
+         : tnops_bias_grad_bf16(gp, static_cast<uint16_t*>(db.data_ptr()), part, M, N,
+                                streamOf(grad)),
      "tnops_bias_grad");
   return db;
 }
 
-// gy bf16 [M, N], pre in 8-bit blocks -> (gpre bf16 [M, N], db fp32 [N])
+// gy bf16 [M, N], pre in 8-bit blocks -> (gpre bf16 [M, N], db [N] of type st)
 std::vector<at::Tensor> geluBwdBiasInt8(const at::Tensor& gy, const at::Tensor& q,
-                                        const at::Tensor& e, const Opt& dbOut) {
+                                        const at::Tensor& e, at::ScalarType st,
+                                        const Opt& dbOut) {
   need(gy, at::kBFloat16, "grad_y");
   needInt8(q, e);
   TORCH_CHECK(gy.dim() == 2 && gy.sizes() == q.sizes() && gy.size(1) % 8 == 0,
@@ -319,13 +337,11 @@ std::vector<at::Tensor> geluBwdBiasInt8(const at::Tensor& gy, const at::Tensor& 
   c10::cuda::CUDAGuard g(gy.device());
   const int M = asInt(gy.size(0), "rows"), N = asInt(gy.size(1), "columns");
   auto gpre = at::empty_like(gy);
-  auto db = dbOut ? *dbOut : at::empty({N}, gy.options().dtype(at::kFloat));
-  need(db, at::kFloat, "db_out");
-  TORCH_CHECK(db.numel() == N, "gelu_bwd_bias_int8: db_out needs N elements");
-  auto part = at::empty({(int64_t)tnops_colsum_parts(M, N) * N}, gy.options().dtype(at::kFloat));
+  auto db = dbOut ? *dbOut : at::empty({N}, gy.options().dtype(st));
+  auto part = columnParts(gy, M, N);
   ok(tnops_gelu_bwd_bias_int8(static_cast<uint16_t*>(gy.data_ptr()), bytes(q), bytes(e),
-                              static_cast<uint16_t*>(gpre.data_ptr()), db.data_ptr<float>(),
-                              part.data_ptr<float>(), M, N, streamOf(gy)),
+                              static_cast<uint16_t*>(gpre.data_ptr()), db.data_ptr(),
+                              st == at::kFloat, part, M, N, streamOf(gy)),
      "tnops_gelu_bwd_bias_int8");
   return {gpre, db};
 }
@@ -443,14 +459,12 @@ at::Tensor embedding(const at::Tensor& w, const Opt& p, const at::Tensor& idx,
   return y.view(shape);
 }
 
-enum Reduction { kMean = 0, kSum = 1, kNone = 2 };
-
 struct LinearCeFn : torch::autograd::Function<LinearCeFn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
                             const Opt& w16, const at::Tensor& target, int64_t classes,
                             int64_t reduction, bool dwDest) {
     const auto wb = bf16Copy(w, w16);
-    const auto r = linearCeFwd(x, wb, target, classes, reduction == kMean);
+    const auto r = linearCeFwd(x, wb, target, classes, reduction);
     ctx->save_for_backward({x, wb, target, r[1], r[2]});
     ctx->saved_data["w"] = w;
     ctx->saved_data["classes"] = classes;
@@ -513,15 +527,15 @@ struct LinearInt8Fn : torch::autograd::Function<LinearInt8Fn> {
     auto g = grads[0].contiguous();
     const bool wantW = ctx->needs_input_grad(1);
     const bool wantB = ctx->needs_input_grad(2);
-    const Opt dbOut =
-        wantB ? destination(b, ctx->saved_data["db"].toBool(), at::kFloat) : Opt();
+    const auto bt = b.scalar_type() == at::kBFloat16 ? at::kBFloat16 : at::kFloat;
+    const Opt dbOut = wantB ? destination(b, ctx->saved_data["db"].toBool(), bt) : Opt();
     at::Tensor db;
     if (gelu) {
-      auto r = geluBwdBiasInt8(g, s[1], s[2], dbOut);
+      auto r = geluBwdBiasInt8(g, s[1], s[2], bt, dbOut);
       g = r[0];
       if (wantB) db = r[1];
     } else if (wantB) {
-      db = biasGradient(g, dbOut);
+      db = biasGradient(g, bt, dbOut);
     }
     const auto st = w.scalar_type() == at::kFloat ? at::kFloat : at::kBFloat16;
     const auto d = linearGradsInt8(g, s[0], s[s.size() - 2], s[s.size() - 1],
@@ -554,7 +568,7 @@ void registerTrainOps(py::module_& ops) {
           py::arg("weight_bf16"), py::arg("bias_bf16"), py::arg("gelu"), py::arg("has_dw_dest"),
           py::arg("has_db_dest"));
   ops.def("linear_ce_fwd", &linearCeFwd, py::arg("x"), py::arg("weight"), py::arg("target"),
-          py::arg("classes"), py::arg("mean"));
+          py::arg("classes"), py::arg("reduction"));
   ops.def("linear_ce_piece", &cePiece, py::arg("rows"), py::arg("classes"), py::arg("budget"));
   ops.def("linear_ce_bwd", &linearCeBwd, py::arg("x"), py::arg("weight"), py::arg("target"),
           py::arg("lse"), py::arg("grad"), py::arg("share"), py::arg("classes"),

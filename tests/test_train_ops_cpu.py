@@ -57,8 +57,8 @@ def test_linear_ce_launchers_refuse(built):
                        (16, 60), (17, 0), (18, 299)])
     # The scratch of the first pieces and of the last, shorter one.
     a, b, c = (_scratch("tnops_linear_grads_scratch", 1024, n, 768, 1, 1) for n in (768, 232, 1000))
-    assert _scratch("tnops_linear_ce_scratch", 1024, 768, 1000, 768, 1, 1) == max(a, b)
-    assert _scratch("tnops_linear_ce_scratch", 1024, 768, 1000, 1024, 1, 1) == c
+    assert _scratch("tnops_linear_ce_scratch", 1024, 768, 1000, 1000, 768, 1, 1) == max(a, b)
+    assert _scratch("tnops_linear_ce_scratch", 1024, 768, 1000, 1000, 1024, 1, 1) == c
     f = _launcher("tnops_linear_ce_mean", P, P, P, I, I, I, P)
     assert f(A, A, A, 0, 5, 1, None) == 1
 
@@ -92,9 +92,12 @@ def test_int8_launchers_refuse(built):
     _refuses(f, [A, A, A, A, A, A, 4, 64, 64, None],
              [(0, A + 8), (1, A + 8), (2, A + 4), (2, None), (3, A + 16), (4, A + 8), (5, A + 2),
               (6, 0), (7, 0), (7, 60), (8, 0), (8, 60)])
-    f = _launcher("tnops_gelu_bwd_bias_int8", P, P, P, P, P, P, I, I, P)
-    _refuses(f, [A, A, A, A, A, A, 64, 768, None],
-             [(0, A + 8), (1, A + 4), (3, A + 8), (6, 0), (7, 770)])
+    f = _launcher("tnops_gelu_bwd_bias_int8", P, P, P, P, P, I, P, I, I, P)
+    for db_f32 in (0, 1):
+        _refuses(f, [A, A, A, A, A, db_f32, A, 64, 768, None],
+                 [(0, A + 8), (1, A + 4), (3, A + 8), (7, 0), (8, 770)])
+    f = _launcher("tnops_bias_grad_bf16", P, P, P, I, I, P)
+    _refuses(f, [A, A, A, 64, 768, None], [(0, A + 8), (3, 0), (4, 770)])
 
 
 def test_pair_schedule(built):
