@@ -153,12 +153,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (!(ok = warpWait(&sFull[s], (g / kPairStages) & 1u, abort, 2))) break;
         fenceAfterSync();
         const uint32_t at = base + s * kPairStage;
-        for (int h = 0; h < halves; ++h) {
+        for (int h = 0; h < 2; ++h) {
+          // Both accumulators are waited for even where the second half has no
+          // rows: its commit below must not come before the epilogue has seen
+          // the one before, or a phase of the barrier passes unseen.
           if (kb == w.kb0) {
             if (!(ok = warpWait(&sAccEmpty[h], fresh, abort, 2))) break;
             fenceAfterSync();
           }
-          if (elected) {
+          if (h < halves && elected) {
 #pragma unroll
             for (int k = 0; k < kBK / 16; ++k)
               pairMma(tmem + h * kTmemCols, pairDesc(descA, at + h * kHalf + k * stepA),

@@ -107,6 +107,14 @@ def test_pair_schedule(built):
     assert r.returncode == 0 and "pair schedule ok" in r.stdout, r.stderr
 
 
+def test_pair_pipeline_model(built):
+    """The barriers of the pair and panel products, as threads: short sums
+    behind a slow epilogue, tiles with rows in one half only, panels that
+    change."""
+    r = run([os.path.join(ROOT, "build", "bin", "pair_pipeline_model_test")], timeout=300)
+    assert r.returncode == 0 and "pair pipelines: PASS" in r.stdout, r.stdout + r.stderr
+
+
 def test_python_refusals(built):
     from tiny_nccl_b200 import ops
     w, p = torch.zeros(10, 8), torch.zeros(6, 8)

@@ -188,6 +188,8 @@ PROGRAMS = {
     "ln_plan_test": ROOT / "tests" / "cpp" / "ln_plan_test.cc",
     # which SM pair computes which part of the training operators' products
     "pair_schedule_test": ROOT / "tests" / "cpp" / "pair_schedule_test.cc",
+    # mbarrier hand-offs of those products' pipelines, as threads
+    "pair_pipeline_model_test": ROOT / "tests" / "cpp" / "pair_pipeline_model_test.cc",
     # host configuration / partition checks, built with the library's config code
     "config_test": (ROOT / "tests" / "cpp" / "config_test.cc", TNCCL_SRC / "common.cc"),
 }
