@@ -2,7 +2,7 @@
 // before the GELU left in 8 bits for the backward pass instead of in bf16:
 //
 //   pre = x w^T + bias             fp32, from the tensor cores' accumulators
-//   act = bf16(gelu_tanh(bf16(pre)))      as tnops_gemm_bias_act gives it
+//   act = bf16(gelu_tanh(pre))     rounded once, as nothing keeps pre in bf16
 //   pre_q, pre_e = pre in 8-bit blocks (int8_blocks.cuh)
 //
 // An epilogue of the CTA-pair pipeline of panel_gemm.cuh. A thread of it holds
@@ -16,6 +16,21 @@
 
 namespace tnops {
 namespace {
+
+// tanh-GELU of two numbers, x / (1 + e^(-2u)) with u = k0 (x + k1 x^3). The
+// exponent -2u log2e is held at its upper end, where 2^it would pass the fp32
+// range; at the other end the power is 0 and the result x.
+__device__ __forceinline__ uint64_t geluTanh2(uint64_t x) {
+  const float c = -2.0f * 1.4426950408889634f * 0.7978845608028654f;  // -2 log2e sqrt(2 / pi)
+  const uint64_t inner = fma2(pack2(c * 0.044715f, c * 0.044715f), mul2(x, x), pack2(c, c));
+  float a, b;
+  unpack2(mul2(x, inner), a, b);
+  unpack2(add2(pack2(ex2Approx(fminf(a, 115.0f)), ex2Approx(fminf(b, 115.0f))), pack2(1.f, 1.f)),
+          a, b);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
+  return mul2(x, pack2(a, b));
+}
 
 struct GeluInt8Epi {
   uint16_t* act;
@@ -91,8 +106,9 @@ struct GeluInt8Epi {
     uint32_t w[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const uint32_t p = packBf16(v[2 * i], v[2 * i + 1]);
-      w[i] = packBf16(geluTanh(__uint_as_float(p << 16)), geluTanh(__uint_as_float(p & 0xffff0000u)));
+      float a, b;
+      unpack2(geluTanh2(pack2(v[2 * i], v[2 * i + 1])), a, b);
+      w[i] = packBf16(a, b);
     }
     storeRow32(act + at, w, cols % 16 == 0, (cols - col0) / 8);
   }

@@ -172,7 +172,7 @@ int tnops_quantize_int8(const void* x, int x_f32, uint8_t* q, uint8_t* e, int64_
 int tnops_dequantize_int8(const uint8_t* q, const uint8_t* e, void* x, int x_f32, int64_t rows,
                           int cols, cudaStream_t stream);
 
-// act [rows, outs] (bf16) = gelu_tanh(bf16(x w^T + bias)) for x [rows, ins],
+// act [rows, outs] (bf16) = gelu_tanh(x w^T + bias) for x [rows, ins],
 // w [outs, ins], bias [outs] in bf16, and the sums before the GELU in 8-bit
 // blocks (rounded from fp32). ins, outs % 8 == 0, x, w, bias 16-byte, act
 // and pre_q 32-byte, pre_e 4-byte aligned; 1 (invalid argument) otherwise.

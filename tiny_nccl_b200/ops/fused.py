@@ -272,7 +272,8 @@ def linear_gelu(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor,
     """GELU(tanh)(x W^T + b) in bf16; the backward fuses the GELU gradient
     with the bias gradient. ``activations="int8"`` keeps x and the sums before
     the GELU for the backward pass in 8-bit blocks (see :func:`linear`); the
-    forward then always runs on the tcgen05 GEMM."""
+    GELU is then taken of the fp32 sums, where the default rounds them to bf16
+    first, and the forward always runs on the tcgen05 GEMM."""
     return _linear(x, weight, bias, True, activations)
 
 
