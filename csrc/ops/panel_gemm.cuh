@@ -37,6 +37,19 @@ struct alignas(64) PanelGemmArgs {
   Epi epi;
 };
 
+// A place in the ring and its barriers' phase, kept up by counting: a division
+// by the number of slots for each load would take the MMA warp longer than the
+// MMAs of a K block.
+struct RingAt {
+  uint32_t slot, phase;
+  __device__ __forceinline__ void next(uint32_t slots) {
+    if (++slot == slots) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
 // Epi: `State begin(row)` once per tile and thread (the thread's row of the
 // output), `chunk(state, v, row, col0)` for its 32 columns from col0 of each
 // block, `end(state, row, part)` after the last block (part: the 128 columns'
@@ -98,14 +111,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const uint32_t tmem = sTmem;
 
   if (warp == 0 && lane == 0) {
-    // Producer (both CTAs): this CTA's halves of A and B. g counts the ring's
-    // loads, panels the resident ones.
-    uint32_t g = 0, panels = 0;
+    // Producer (both CTAs): this CTA's halves of A and B.
+    RingAt at{0u, 0u};
+    uint32_t g = 0, panels = 0;  // loads through the ring, resident panels
     auto stream = [&](const CUtensorMap* map, int row, int kb) {
-      const uint32_t s = g % slots, round = g / slots;
-      if (!mbarWait(&sEmpty[s], (round & 1u) ^ 1u, abort, 1)) return false;
-      if (rank == 0) mbarExpectTx(&sFull[s], 2 * kHalf);  // both CTAs' loads
-      tmaLoadPair(ring + s * kHalf, map, kb * kBK, row, inLeader(&sFull[s]));
+      if (!mbarWait(&sEmpty[at.slot], at.phase ^ 1u, abort, 1)) return false;
+      if (rank == 0) mbarExpectTx(&sFull[at.slot], 2 * kHalf);  // both CTAs' loads
+      tmaLoadPair(ring + at.slot * kHalf, map, kb * kBK, row, inLeader(&sFull[at.slot]));
+      at.next(slots);
       ++g;
       return true;
     };
@@ -142,12 +155,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const bool elected = electOne();
     const uint64_t desc = pairDescBase(0);
     const uint32_t instr = pairInstrDesc(0, 0);
-    uint32_t g = 0, panels = 0, local = 0;
+    RingAt at{0u, 0u};
+    uint32_t panels = 0, local = 0;
+    int tileN = first % tilesN;
     bool ok = true;
     for (int t = first; ok && t < end; ++t, ++local) {
       const uint32_t b = local & 1u, use = local >> 1;
-      const int m = t / tilesN;
-      if (t == first || t == m * tilesN) {
+      if (t == first || tileN == 0) {
         if (!(ok = warpWait(&sPanelFull, panels & 1u, abort, 2))) break;
         ++panels;
       }
@@ -157,14 +171,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (int kb = 0; kb < kBlocks; ++kb) {
         uint32_t a = base + kb * kHalf, sa = 0;
         if (kb >= resident) {
-          sa = g % slots;
-          if (!(ok = warpWait(&sFull[sa], (g / slots) & 1u, abort, 2))) break;
+          sa = at.slot;
+          if (!(ok = warpWait(&sFull[sa], at.phase, abort, 2))) break;
           a = ring + sa * kHalf;
-          ++g;
+          at.next(slots);
         }
-        const uint32_t sb = g % slots;
-        if (!(ok = warpWait(&sFull[sb], (g / slots) & 1u, abort, 2))) break;
-        ++g;
+        const uint32_t sb = at.slot;
+        if (!(ok = warpWait(&sFull[sb], at.phase, abort, 2))) break;
+        at.next(slots);
         fenceAfterSync();
         const uint32_t bb = ring + sb * kHalf;
         if (elected) {
@@ -180,9 +194,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!ok) break;
       if (elected) {
         commitPair(&sAccFull[b]);
-        if (t + 1 == end || t + 1 == (m + 1) * tilesN) commitPair(&sPanelEmpty);
+        if (t + 1 == end || tileN + 1 == tilesN) commitPair(&sPanelEmpty);
       }
       __syncwarp();
+      if (++tileN == tilesN) tileN = 0;
     }
     if (elected) commitPairLocal(&sDone);
     __syncwarp();
