@@ -43,16 +43,31 @@ struct GeluInt8Epi {
     uint32_t e;
   };
   __device__ __forceinline__ State begin(int) const { return {0u}; }
-  __device__ __forceinline__ void chunk(State& st, const float (&in)[32], int row,
-                                        int col0) const {
+  // The columns' biases, zeros past the last column (cols % 8 == 0).
+  struct Bias {
+    uint4 b[4];
+  };
+  __device__ __forceinline__ Bias ahead(int col0) const {
+    Bias r;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      r.b[g] = make_uint4(0u, 0u, 0u, 0u);
+      // volatile: the load stays where it is, ahead of its use.
+      if (col0 + 8 * g < cols)
+        asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r.b[g].x), "=r"(r.b[g].y), "=r"(r.b[g].z), "=r"(r.b[g].w)
+                     : "l"(bias + col0 + 8 * g));
+    }
+    return r;
+  }
+  __device__ __forceinline__ void chunk(State& st, const float (&in)[32], const Bias& ahead,
+                                        int row, int col0) const {
     if (row >= rows || col0 >= cols) return;
     float v[32];
     uint32_t top = 0u;  // of the magnitudes' bits: a NaN's are above infinity's
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      uint4 b = make_uint4(0u, 0u, 0u, 0u);
-      const bool in8 = col0 + 8 * g < cols;  // cols % 8 == 0
-      if (in8) b = __ldg(reinterpret_cast<const uint4*>(bias + col0) + g);
+      const uint4 b = ahead.b[g];
       const uint32_t w[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {

@@ -71,7 +71,8 @@ struct StatsEpi {
   }
   // 32 logits: their maximum, then one packed FMA for two, one ex2 for each
   // and one packed addition for two.
-  __device__ __forceinline__ void chunk(State& st, const float (&in)[32], int row,
+  __device__ __forceinline__ int ahead(int) const { return 0; }
+  __device__ __forceinline__ void chunk(State& st, const float (&in)[32], int, int row,
                                         int col0) const {
     if (col0 >= classes) return;
     float v[32];
@@ -140,7 +141,8 @@ struct SoftmaxGradEpi {
     }
     return st;
   }
-  __device__ __forceinline__ void chunk(State& st, const float (&v)[32], int row,
+  __device__ __forceinline__ int ahead(int) const { return 0; }
+  __device__ __forceinline__ void chunk(State& st, const float (&v)[32], int, int row,
                                         int col0) const {
     if (row >= rows || col0 >= width) return;
     const uint64_t scale = pack2(kLog2e, kLog2e), shift = pack2(st.nb, st.nb);

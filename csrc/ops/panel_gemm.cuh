@@ -51,8 +51,8 @@ struct RingAt {
 };
 
 // Epi: `State begin(row)` once per tile and thread (the thread's row of the
-// output), `chunk(state, v, row, col0)` for its 32 columns from col0 of each
-// block, `end(state, row, part)` after the last block (part: the 128 columns'
+// output), `chunk(state, v, ahead, row, col0)` for its 32 columns from col0 of
+// each block (ahead: what `ahead(col0)` loaded while the block before was worked on), `end(state, row, part)` after the last block (part: the 128 columns'
 // number). What an epilogue writes goes straight from registers: operands in
 // and out of shared memory take its whole bandwidth here (107 of 128 bytes per
 // clock), and a staged copy of the result cost a fifth of the time.
@@ -218,11 +218,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       // The next 32 columns are on their way while these are worked on.
       uint32_t r[2][32];
       tmemIssue32(acc + (uint32_t)(half * 128), r[0]);
+      auto ahead = args.epi.ahead(tileN * 256 + half * 128);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int c = half * 128 + i * 32;
         tmemWait(r[i & 1]);
+        const auto now = ahead;
         if (i < 3) {
+          ahead = args.epi.ahead(tileN * 256 + c + 32);
           tmemIssue32(acc + (uint32_t)(c + 32), r[(i + 1) & 1]);
         } else {
           // Everything is read: the accumulator goes back before the stores.
@@ -233,7 +236,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         float v[32];
 #pragma unroll
         for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(r[i & 1][k]);
-        args.epi.chunk(st, v, row0 + lane, tileN * 256 + c);
+        args.epi.chunk(st, v, now, row0 + lane, tileN * 256 + c);
       }
       args.epi.end(st, row0 + lane, tileN * 2 + half);
     }
