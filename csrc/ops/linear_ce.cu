@@ -167,8 +167,6 @@ struct SoftmaxGradEpi {
   __device__ __forceinline__ void end(const State&, int, int) const {}
 };
 
-constexpr int kJoinWarps = 32;
-
 // (maximum, sum) of two sets; -inf and 0 stand for an empty one.
 __device__ __forceinline__ float2 joinSums(float2 a, float2 b) {
   const float m = fmaxf(a.x, b.x);
@@ -176,32 +174,38 @@ __device__ __forceinline__ float2 joinSums(float2 a, float2 b) {
   return make_float2(m, a.y * ex2Approx((a.x - m) * kLog2e) + b.y * ex2Approx((b.x - m) * kLog2e));
 }
 
-// Joins a row's partial statistics: 32 rows per CTA (one per lane), the parts
-// split over the warps, four loads in flight each; then the warps' sums in
-// order.
-__global__ void __launch_bounds__(kJoinWarps * 32)
+// Joins a row's partial statistics: eight rows per CTA, the parts dealt to 32
+// threads of each row, four loads in flight; then the threads' sums in a fixed
+// tree.
+constexpr int kJoinRows = 8, kJoinThreads = 256;
+__global__ void __launch_bounds__(kJoinThreads)
     joinStats(const float2* __restrict__ partial, const int64_t* __restrict__ target,
               const float* __restrict__ logitOfTarget, float* __restrict__ lse,
               float* __restrict__ loss, int parts, int rows, int classes) {
-  __shared__ float2 s[kJoinWarps][32];
+  __shared__ float2 s[kJoinThreads / 32][kJoinRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row = blockIdx.x * 32 + lane;
-  constexpr int U = 4;
+  const int row = blockIdx.x * kJoinRows + (lane & (kJoinRows - 1));
+  constexpr int U = 4, kStep = kJoinThreads / kJoinRows;
   float2 st = make_float2(-INFINITY, 0.f);
   if (row < rows)
-    for (int p = warp; p < parts; p += U * kJoinWarps) {
+    for (int p = threadIdx.x / kJoinRows; p < parts; p += U * kStep) {
       float2 v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        v[u] = p + u * kJoinWarps < parts ? partial[(size_t)(p + u * kJoinWarps) * rows + row]
-                                          : make_float2(-INFINITY, 0.f);
+        v[u] = p + u * kStep < parts ? partial[(size_t)(p + u * kStep) * rows + row]
+                                     : make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int u = 0; u < U; ++u) st = joinSums(st, v[u]);
     }
-  s[warp][lane] = st;
+#pragma unroll
+  for (int d = kJoinRows; d < 32; d *= 2)
+    st = joinSums(st, make_float2(__shfl_xor_sync(0xffffffffu, st.x, d),
+                                  __shfl_xor_sync(0xffffffffu, st.y, d)));
+  if (lane < kJoinRows) s[warp][lane] = st;
   __syncthreads();
-  if (warp == 0 && row < rows) {
-    for (int w = 1; w < kJoinWarps; ++w) st = joinSums(st, s[w][lane]);
+  if (threadIdx.x < kJoinRows && row < rows) {
+#pragma unroll
+    for (int w = 1; w < kJoinThreads / 32; ++w) st = joinSums(st, s[w][lane]);
     const float l = st.x + logf(st.y);
     const int64_t t = target[row];
     lse[row] = l;
@@ -270,7 +274,7 @@ extern "C" int tnops_linear_ce_fwd(const void* x, const void* w, const int64_t* 
   PanelGemmArgs<StatsEpi> args{};
   args.epi = {target, reinterpret_cast<float2*>(partial), loss, rows, classes};
   if (int rc = launchPanelGemm(args, x, w, rows, classes, width, stream)) return rc;
-  joinStats<<<(rows + 31) / 32, kJoinWarps * 32, 0, stream>>>(
+  joinStats<<<(rows + kJoinRows - 1) / kJoinRows, kJoinThreads, 0, stream>>>(
       args.epi.partial, target, loss, lse, loss, tnops_linear_ce_parts(classes), rows, classes);
   return launched(cudaGetLastError());
 }
@@ -280,6 +284,32 @@ extern "C" int tnops_linear_ce_mean(const float* loss, const int64_t* target, fl
   if (rows <= 0) return 1;
   meanLoss<<<1, kMeanThreads, 0, stream>>>(loss, target, rows, classes, mean, out2);
   return launched(cudaGetLastError());
+}
+
+// Classes per piece: whole 256-wide tiles, spread evenly over the least number
+// of pieces whose d fits the budget, or over up to five more where their
+// products leave fewer SM pairs idle (16384 rows of 50257 classes and 512 MiB:
+// six pieces instead of four, a tenth less). A piece costs about 20 K blocks
+// of launches besides.
+extern "C" int tnops_linear_ce_piece(int rows, int width, int classes, int64_t budget) {
+  if (rows <= 0 || width <= 0 || classes <= 0) return 0;
+  const int64_t tiles = ((int64_t)classes + 255) / 256;
+  int64_t most = budget / ((int64_t)rows * 512);
+  if (most < 1) most = 1;
+  const int64_t least = (tiles + most - 1) / most;
+  int64_t best = 0, bestCost = 0;
+  for (int64_t n = least; n <= tiles && n < least + 6; ++n) {
+    const int64_t piece = (tiles + n - 1) / n * 256;
+    const int whole = (int)(classes / piece), last = (int)(classes - whole * piece);
+    int64_t cost = 20 * (whole + (last > 0));
+    if (whole > 0) cost += whole * (int64_t)linearGradsCost(rows, (int)piece, width);
+    if (last > 0) cost += linearGradsCost(rows, last, width);
+    if (best == 0 || cost < bestCost) {
+      best = piece;
+      bestCost = cost;
+    }
+  }
+  return (int)best;
 }
 
 // Rows of padding after the classes that the last piece's product writes; more

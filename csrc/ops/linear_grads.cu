@@ -142,6 +142,14 @@ size_t linearGradsScratch(int rows, int outs, int padded, int ins, bool wantDx, 
   return scratchFor(args.schedule);
 }
 
+int linearGradsCost(int rows, int outs, int ins) {
+  PairGemmArgs args{};
+  bool isDx[2];
+  args.problems = shapes(rows, outs, 0, ins, true, true, args.prob, isDx);
+  planGemm(&args);
+  return planRounds(&args.schedule) + args.schedule.slots() / 2;
+}
+
 unsigned linearGradsStatus(int reset) { return readStatus(reset); }
 
 }  // namespace tnops

@@ -30,6 +30,8 @@ struct LinearGrads {
 };
 
 int linearGrads(const LinearGrads& a, cudaStream_t stream);
+// Roughly how long both products take, in K blocks of a tile.
+int linearGradsCost(int rows, int outs, int ins);
 size_t linearGradsScratch(int rows, int outs, int padded, int ins, bool wantDx, bool wantDw);
 
 // First failure code of the tensor-core kernels of linear_grads.cu,

@@ -108,16 +108,17 @@ inline int planRounds(PairSchedule* s) {
     if (s->early > most) s->early = most;
     if (s->early * len1 < len0) s->lateFirst = s->extra;
   }
+  // The late rounds give most to the first pair of their turn; the busiest
+  // pair is the first in turn among those with an extra unit or among the
+  // others.
   const int rounds0 = s->units(0) / s->pairs;
   const int late = s->units(1) - s->others() * s->early;
-  int busiest = 0;
-  for (int p = 0; p < s->pairs; ++p) {
-    const int turn = (p - s->lateFirst + s->pairs) % s->pairs;
-    int n = rounds0 * len0 + (p < s->extra ? len0 : s->early * len1);
-    if (turn < late) n += (late - turn + s->pairs - 1) / s->pairs * len1;
-    if (n > busiest) busiest = n;
-  }
-  return busiest;
+  auto lateOf = [&](int turn) { return turn < late ? (late - turn + s->pairs - 1) / s->pairs : 0; };
+  const int turnExtra = s->lateFirst == 0 ? 0 : s->others();
+  const int turnOther = s->lateFirst == 0 ? s->extra : 0;
+  const int other = s->early * len1 + lateOf(turnOther) * len1;
+  const int extra = s->extra > 0 ? len0 + lateOf(turnExtra) * len1 : 0;
+  return rounds0 * len0 + (extra > other ? extra : other);
 }
 
 // Plans the launch: sums stay whole, or with `cut` the longer product's are

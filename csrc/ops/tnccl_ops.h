@@ -130,7 +130,10 @@ int tnops_linear_grads(const void* g, int64_t ldg, const void* w, const void* x,
 //    (piece % 32 == 0); d holds rows * piece bf16 of scratch, dx_f32
 //    rows * width floats when piece < classes, and scratch scratch_bytes, at
 //    least tnops_linear_ce_scratch(...). A null dx or dw is left out.
+//  * piece: a good `piece` whose d takes at most `budget` bytes (256 classes
+//    at least).
 int tnops_linear_ce_parts(int classes);
+int tnops_linear_ce_piece(int rows, int width, int classes, int64_t budget);
 size_t tnops_linear_ce_scratch(int rows, int width, int classes, int vocab, int piece,
                                int want_dx, int want_dw);
 int tnops_linear_ce_fwd(const void* x, const void* w, const int64_t* target, float* loss,

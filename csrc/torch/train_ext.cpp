@@ -183,16 +183,6 @@ std::vector<at::Tensor> linearCeFwd(const at::Tensor& x, const at::Tensor& w,
 // Scratch for a piece of the logits' gradient.
 constexpr int64_t kCeBudget = 512ll << 20;
 
-// Classes per piece of the backward pass: as many whole 256-wide tiles as fit
-// the scratch budget, spread evenly.
-int64_t cePiece(int64_t rows, int64_t classes, int64_t budget) {
-  const int64_t tiles = (classes + 255) / 256;
-  int64_t most = budget / (rows * 512);
-  if (most < 1) most = 1;
-  const int64_t pieces = (tiles + most - 1) / most;
-  return (tiles + pieces - 1) / pieces * 256;
-}
-
 std::vector<at::Tensor> linearCeBwd(const at::Tensor& x, const at::Tensor& w,
                                     const at::Tensor& target, const at::Tensor& lse,
                                     const at::Tensor& grad, const Opt& share, int64_t classes,
@@ -216,7 +206,7 @@ std::vector<at::Tensor> linearCeBwd(const at::Tensor& x, const at::Tensor& w,
     if (s.rows == 0) dw.zero_();
   }
   if (s.rows == 0 || (!wantDx && !wantDw)) return {dx, dw};
-  const int64_t piece = cePiece(s.rows, s.classes, budget);
+  const int64_t piece = tnops_linear_ce_piece(s.rows, s.width, s.classes, budget);
   auto d = at::empty({(int64_t)s.rows, piece}, x.options());
   const size_t scratchBytes =
       tnops_linear_ce_scratch(s.rows, s.width, s.classes, s.vocab, (int)piece, wantDx, wantDw);
@@ -302,6 +292,7 @@ std::vector<at::Tensor> linearGeluInt8(const at::Tensor& x, const at::Tensor& w,
   auto act = at::empty({rows, outs}, x.options());
   auto q = at::empty({rows, outs}, x.options().dtype(at::kChar));
   auto e = at::empty({rows, (outs + 31) / 32}, x.options().dtype(at::kByte));
+  if (rows == 0) return {act, q, e};
   ok(tnops_linear_gelu_int8(x.data_ptr(), w.data_ptr(), bias.data_ptr(), act.data_ptr(), bytes(q),
                             bytes(e), rows, outs, ins, streamOf(x)),
      "tnops_linear_gelu_int8");
@@ -315,6 +306,7 @@ at::Tensor biasGradient(const at::Tensor& grad, at::ScalarType st, const Opt& ou
   c10::cuda::CUDAGuard g(grad.device());
   const int M = asInt(grad.size(0), "rows"), N = asInt(grad.size(1), "columns");
   auto db = out ? *out : at::empty({N}, grad.options().dtype(st));
+  if (M == 0) return db.zero_();
   auto part = columnParts(grad, M, N);
   auto* gp = static_cast<uint16_t*>(grad.data_ptr());
   ok(st == at::kFloat
@@ -338,6 +330,7 @@ std::vector<at::Tensor> geluBwdBiasInt8(const at::Tensor& gy, const at::Tensor& 
   const int M = asInt(gy.size(0), "rows"), N = asInt(gy.size(1), "columns");
   auto gpre = at::empty_like(gy);
   auto db = dbOut ? *dbOut : at::empty({N}, gy.options().dtype(st));
+  if (M == 0) return {gpre, db.zero_()};
   auto part = columnParts(gy, M, N);
   ok(tnops_gelu_bwd_bias_int8(static_cast<uint16_t*>(gy.data_ptr()), bytes(q), bytes(e),
                               static_cast<uint16_t*>(gpre.data_ptr()), db.data_ptr(),
@@ -371,6 +364,8 @@ std::vector<at::Tensor> linearGradsInt8(const at::Tensor& grad, const at::Tensor
     need(dw, st, "dw_out");
     TORCH_CHECK(dw.numel() == w.numel(), "linear_grads_int8: dw_out must match weight");
   }
+  if (rows == 0 && wantDw) dw.zero_();
+  if (rows == 0 || (!wantDx && !wantDw)) return {dx, dw};
   at::Tensor x;
   if (wantDw) x = dequantizeInt8(q, e, false);
   const size_t scratchBytes = tnops_linear_grads_scratch(rows, outs, ins, wantDx, wantDw);
@@ -385,10 +380,18 @@ std::vector<at::Tensor> linearGradsInt8(const at::Tensor& grad, const at::Tensor
 // -- autograd ----------------------------------------------------------------------
 //
 // The operators' autograd functions are C++: a small call's time is the host's,
-// and Python functions take several times as long on both ways.
+// and Python functions take several times as long on both ways. Where nothing
+// asks for a gradient they are passed by, and nothing is kept for one.
 
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
+
+bool wantsGradient(std::initializer_list<const at::Tensor*> inputs) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : inputs)
+    if (t != nullptr && t->requires_grad()) return true;
+  return false;
+}
 
 void onceDifferentiable(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " cannot be differentiated twice");
@@ -490,26 +493,34 @@ struct LinearCeFn : torch::autograd::Function<LinearCeFn> {
 at::Tensor linearCrossEntropy(const at::Tensor& x, const at::Tensor& w, const Opt& w16,
                               const at::Tensor& target, int64_t classes, int64_t reduction,
                               bool dwDest) {
-  auto loss = LinearCeFn::apply(x.reshape({-1, x.size(-1)}).to(at::kBFloat16).contiguous(), w, w16,
-                                target.reshape({-1}).contiguous(), classes, reduction, dwDest);
+  const auto xb = x.reshape({-1, x.size(-1)}).to(at::kBFloat16).contiguous();
+  const auto t = target.reshape({-1}).contiguous();
+  at::Tensor loss;
+  if (wantsGradient({&x, &w})) {
+    loss = LinearCeFn::apply(xb, w, w16, t, classes, reduction, dwDest);
+  } else {
+    const auto r = linearCeFwd(xb, bf16Copy(w, w16), t, classes, reduction);
+    loss = reduction == kNone ? r[0] : r[2].select(0, 0);
+  }
   return reduction == kNone ? loss.view(target.sizes()) : loss;
+}
+
+// y, and with gelu the sums before it in 8-bit blocks.
+variable_list linearInt8Out(const at::Tensor& x, const at::Tensor& w, const at::Tensor& b,
+                            bool gelu) {
+  if (gelu) return linearGeluInt8(x, w, b);
+  c10::impl::ExcludeDispatchKeyGuard guard(c10::DispatchKey::AutocastCUDA);
+  return {at::addmm(b, x, w.t())};
 }
 
 struct LinearInt8Fn : torch::autograd::Function<LinearInt8Fn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
                             const at::Tensor& b, const Opt& w16, const Opt& b16, bool gelu,
                             bool dwDest, bool dbDest) {
-    const auto wb = bf16Copy(w, w16), bb = bf16Copy(b, b16);
-    at::Tensor y;
+    const auto wb = bf16Copy(w, w16);
+    const auto out = linearInt8Out(x, wb, bf16Copy(b, b16), gelu);
     variable_list keep{wb};
-    if (gelu) {
-      auto r = linearGeluInt8(x, wb, bb);
-      y = r[0];
-      keep.insert(keep.end(), {r[1], r[2]});
-    } else {
-      c10::impl::ExcludeDispatchKeyGuard guard(c10::DispatchKey::AutocastCUDA);
-      y = at::addmm(bb, x, wb.t());
-    }
+    keep.insert(keep.end(), out.begin() + 1, out.end());
     const auto q = quantizeInt8(x);
     keep.insert(keep.end(), q.begin(), q.end());
     ctx->save_for_backward(keep);
@@ -517,7 +528,7 @@ struct LinearInt8Fn : torch::autograd::Function<LinearInt8Fn> {
     ctx->saved_data["b"] = b;
     ctx->saved_data["dw"] = dwDest;
     ctx->saved_data["db"] = dbDest;
-    return y;
+    return out[0];
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     onceDifferentiable("a linear layer with 8-bit activations");
@@ -548,8 +559,10 @@ struct LinearInt8Fn : torch::autograd::Function<LinearInt8Fn> {
 at::Tensor linearInt8(const at::Tensor& x, const at::Tensor& w, const at::Tensor& b,
                       const Opt& w16, const Opt& b16, bool gelu, bool dwDest,
                       bool dbDest) {
-  auto y = LinearInt8Fn::apply(x.reshape({-1, x.size(-1)}).to(at::kBFloat16).contiguous(), w, b,
-                               w16, b16, gelu, dwDest, dbDest);
+  const auto xb = x.reshape({-1, x.size(-1)}).to(at::kBFloat16).contiguous();
+  auto y = wantsGradient({&x, &w, &b})
+               ? LinearInt8Fn::apply(xb, w, b, w16, b16, gelu, dwDest, dbDest)
+               : linearInt8Out(xb, bf16Copy(w, w16), bf16Copy(b, b16), gelu)[0];
   auto shape = x.sizes().vec();
   shape.back() = w.size(0);
   return y.view(shape);
@@ -569,7 +582,8 @@ void registerTrainOps(py::module_& ops) {
           py::arg("has_db_dest"));
   ops.def("linear_ce_fwd", &linearCeFwd, py::arg("x"), py::arg("weight"), py::arg("target"),
           py::arg("classes"), py::arg("reduction"));
-  ops.def("linear_ce_piece", &cePiece, py::arg("rows"), py::arg("classes"), py::arg("budget"));
+  ops.def("linear_ce_piece", &tnops_linear_ce_piece, py::arg("rows"), py::arg("width"),
+          py::arg("classes"), py::arg("budget"));
   ops.def("linear_ce_bwd", &linearCeBwd, py::arg("x"), py::arg("weight"), py::arg("target"),
           py::arg("lse"), py::arg("grad"), py::arg("share"), py::arg("classes"),
           py::arg("want_dx"), py::arg("want_dw"), py::arg("dw_f32"),

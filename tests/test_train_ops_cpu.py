@@ -186,15 +186,18 @@ def test_gradient_slice_is_handed_out_once_per_backward():
 
 
 def test_cross_entropy_pieces_cover_the_classes(built):
-    """A piece is a multiple of 256 classes, fits the budget where one tile
-    does, and the pieces are even: the last is at least half of the others
-    where there are few."""
+    """A piece is a multiple of 256 classes and fits the budget where one tile
+    does; there are at most five pieces more than the budget asks for."""
     from tiny_nccl_b200._native import load
     piece = load().ops.linear_ce_piece
     for rows in (1, 7, 200, 8192, 32768, 300000):
         for classes in (1, 255, 256, 257, 1000, 50257, 200000):
-            for budget in (1 << 12, 1 << 20, 512 << 20):
-                n = piece(rows, classes, budget)
-                assert n > 0 and n % 256 == 0
-                assert n <= (classes + 255) // 256 * 256
-                assert n == 256 or n * rows * 2 <= budget
+            for width in (8, 768, 4096):
+                for budget in (1 << 12, 1 << 20, 512 << 20):
+                    n = piece(rows, width, classes, budget)
+                    tiles = (classes + 255) // 256
+                    assert n > 0 and n % 256 == 0 and n <= tiles * 256
+                    assert n == 256 or n * rows * 2 <= budget
+                    most = max(1, budget // (rows * 512))
+                    assert -(-tiles * 256 // n) <= -(-tiles // most) + 5
+    assert piece(0, 768, 100, 1 << 20) == 0
