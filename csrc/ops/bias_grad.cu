@@ -14,7 +14,8 @@
 // into one fp32 partial per block (the result, where one block is all). Pass 2 adds the partials of a column in
 // block order (colReduce, common.cuh). The summation order depends only on
 // (M, N), never on scheduling. Rounding of the GELU gradient to bf16 happens before it is
-// summed, as when the gradient tensor is materialised and then reduced.
+// summed, as when the gradient tensor is materialised and then reduced; with an
+// 8-bit pre the sum is of the fp32 products.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -154,8 +155,8 @@ __global__ void __launch_bounds__(kWarps * 32)
             unpack2(mul2(pack2(f[2 * i], f[2 * i + 1]), geluTanhGrad2(x[i])), a, b);
             const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
             o[i] = *reinterpret_cast<const uint32_t*>(&h);
-            f[2 * i] = __uint_as_float(o[i] << 16);
-            f[2 * i + 1] = __uint_as_float(o[i] & 0xffff0000u);
+            f[2 * i] = a;  // the bias gradient's sum is of the unrounded ones
+            f[2 * i + 1] = b;
           }
           *reinterpret_cast<uint4*>(gout + (size_t)r * N + col0) = make_uint4(o[0], o[1], o[2], o[3]);
         } else if (PRE == Pre::kBf16) {

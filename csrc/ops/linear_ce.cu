@@ -12,7 +12,9 @@
 // from the fp32 accumulators: no logit is rounded), and a second kernel joins
 // them. The backward pass goes over the vocabulary in pieces: a GEMM forms the
 // piece's logits again and writes d for it (bf16, the operand type of the two
-// products that follow), and one launch of linear_grads.cu forms this piece's
+// products that follow; a factor that all rows share is left to the products'
+// fp32 results: rounded into every d it would scale the whole gradient by up to
+// 2^-8), and one launch of linear_grads.cu forms this piece's
 // rows of dw and adds its share to dx (fp32 between pieces). Beyond its inputs
 // and outputs the backward pass holds one piece of d and, with more than one
 // piece, dx in fp32.
@@ -114,9 +116,8 @@ struct SoftmaxGradEpi {
   uint16_t* d;  // [rows, ld]
   const int64_t* target;
   const float* lse;
-  const float* grad;   // gradient of each row's loss, or of all with gradStep 0
-  const float* share;  // further factor (1 / rows that count), or null
-  int ld, gradStep, rows, classes, first, width;
+  const float* grad;  // gradient of each row's loss, or null for 1
+  int ld, rows, classes, first, width;
 
   // |k| exp(l - lse) = 2^(l log2e + nb) with nb = log2 |k| - lse log2e: the
   // factor costs nothing per logit; k's sign goes on the packed results.
@@ -130,10 +131,9 @@ struct SoftmaxGradEpi {
     if (row < rows) {
       const int64_t t = target[row];
       if (t >= 0 && t < classes) {
-        st.k = grad[(size_t)row * gradStep];
-        if (share != nullptr) st.k *= *share;
+        st.k = grad != nullptr ? grad[row] : 1.f;
         st.nl = -lse[row] * kLog2e;
-        st.nb = st.nl + log2f(fabsf(st.k));
+        st.nb = grad != nullptr ? st.nl + log2f(fabsf(st.k)) : st.nl;
         st.at = (int)(t - first);
         st.keep = 0xffffffffu;
         st.sign = st.k < 0.f ? 0x80008000u : 0u;
@@ -335,7 +335,7 @@ extern "C" int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* 
                                    void* scratch, size_t scratch_bytes, void* dx, void* dw, int dw_f32, int rows, int width,
                                    int classes, int vocab, cudaStream_t stream) {
   if (rows <= 0 || classes <= 0 || vocab < classes || width <= 0 || width % 8 != 0 ||
-      piece <= 0 || piece % 32 != 0 || !aligned16(x) || !aligned16(w) ||
+      piece <= 0 || piece % 32 != 0 || (grad_step != 0 && grad_step != 1) || !aligned16(x) || !aligned16(w) ||
       (reinterpret_cast<uintptr_t>(d) & 31) ||
       (dx && !aligned16(dx)) || (dw && !aligned16(dw)))
     return 1;
@@ -358,15 +358,15 @@ extern "C" int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* 
     e.ld = piece;
     e.target = target;
     e.lse = lse;
-    e.grad = grad;
-    e.share = share;
-    e.gradStep = grad_step;
+    e.grad = grad_step ? grad : nullptr;
     e.rows = rows;
     e.classes = classes;
     e.first = first;
     e.width = n;
     if (int rc = launchPanelGemm(args, x, wPiece, rows, n, width, stream)) return rc;
     LinearGrads g{};
+    g.scale[0] = grad_step ? nullptr : grad;
+    g.scale[1] = share;
     g.scratch = scratch;
     g.scratchBytes = scratch_bytes;
     g.g = d;

@@ -97,6 +97,8 @@ int linearGrads(const LinearGrads& a, cudaStream_t stream) {
     return 1;
   PairGemmArgs args{};
   bool isDx[2] = {};
+  args.scale[0] = a.scale[0];
+  args.scale[1] = a.scale[1];
   args.problems = shapes(a.rows, a.outs, a.padded, a.ins, a.dxStore != kStoreNone,
                          a.dwStore != kStoreNone, args.prob, isDx);
   if (args.problems == 0) return 0;
@@ -166,6 +168,6 @@ extern "C" int tnops_linear_grads(const void* g, int64_t ldg, const void* w, con
                                   void* scratch, size_t scratch_bytes, cudaStream_t stream) {
   if (g == nullptr || (dx && !w) || (dw && !x)) return 1;
   LinearGrads a{g, ldg, w, x, dx, dw, scratch, scratch_bytes, dx ? kStoreBf16 : kStoreNone,
-                dw ? (dw_f32 ? kStoreF32 : kStoreBf16) : kStoreNone, rows, outs, ins, 0};
+                dw ? (dw_f32 ? kStoreF32 : kStoreBf16) : kStoreNone, rows, outs, ins, 0, {nullptr, nullptr}};
   return linearGrads(a, stream);
 }

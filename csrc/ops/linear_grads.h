@@ -15,7 +15,8 @@ enum GradStore { kStoreNone = 0, kStoreBf16 = 1, kStoreF32 = 2, kAddF32 = 3 };
 // y = x w^T with y [rows, outs], x [rows, ins], w [outs, ins]; g [rows, outs]
 // (rows `ldg` elements apart) is the gradient of y. dx [rows, ins] = g w,
 // dw [outs, ins] = g^T x, each left out with kStoreNone. dw may have `padded`
-// more rows, which get zeros.
+// more rows, which get zeros. Both are multiplied by *scale[0] and *scale[1]
+// where those are given.
 struct LinearGrads {
   const void* g;
   int64_t ldg;
@@ -27,6 +28,7 @@ struct LinearGrads {
   size_t scratchBytes;
   GradStore dxStore, dwStore;
   int rows, outs, ins, padded;
+  const float* scale[2];
 };
 
 int linearGrads(const LinearGrads& a, cudaStream_t stream);

@@ -52,6 +52,7 @@ struct alignas(64) PairGemmArgs {
   int problems;
   int cols[2];             // n
   int mode[2];             // GradStore
+  const float* scale[2];   // factors of every result (null: none)
   PairSchedule schedule;
 };
 
@@ -194,6 +195,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     PairWork w;
     walk.init(schedule, pair);
     bool ok = true;
+    const float scale = (args.scale[0] ? *args.scale[0] : 1.f) *
+                        (args.scale[1] ? *args.scale[1] : 1.f);
     for (; ok && walk.next(schedule, &w); ++local) {
       const GemmProblem& p = args.prob[w.which];
       const int tileN = w.tile % p.tilesN;
@@ -222,7 +225,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 4; ++i) {
           float v[32];
 #pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(r[i][k]);
+          for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(r[i][k]) * scale;
           const int c = side * 128 + 32 * i, col0 = tileN * 256 + c;
           if (w.slot >= 0)
             storeF32(v, lane, buf, &args.mapPartial, w.slot * kPairBM + inTile, c, true, false);

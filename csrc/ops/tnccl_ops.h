@@ -60,8 +60,8 @@ int tnops_colsum_parts(int M, int N);
 int tnops_bias_grad_bf16(const uint16_t* g, uint16_t* db, float* partial, int M, int N,
                          cudaStream_t stream);
 // tnops_gelu_bwd_bias with pre in 8-bit blocks (tnops_quantize_int8's form):
-// pre_q [M, N] 8-byte aligned, pre_e [M, ceil(N / 32)]; db fp32 with db_f32,
-// else bf16.
+// pre_q [M, N] 8-byte aligned, pre_e [M, ceil(N / 32)]; db (the sum of the
+// products before their rounding to bf16) fp32 with db_f32, else bf16.
 int tnops_gelu_bwd_bias_int8(const uint16_t* gy, const uint8_t* pre_q, const uint8_t* pre_e,
                              uint16_t* gpre, void* db, int db_f32, float* partial, int M, int N,
                              cudaStream_t stream);
@@ -126,7 +126,7 @@ int tnops_linear_grads(const void* g, int64_t ldg, const void* w, const void* x,
 //    that count; out2[1] = 1 / max(1, rows that count).
 //  * bwd: dx [rows, width] (bf16) and dw [vocab, width] (fp32 with dw_f32, else
 //    bf16; rows from `classes` on are zero) of sum_r k[r] loss[r], with k[r] =
-//    grad[r * grad_step] (* *share). Works on `piece` classes at a time
+//    grad[r * grad_step] (* *share), grad_step 0 or 1. Works on `piece` classes at a time
 //    (piece % 32 == 0); d holds rows * piece bf16 of scratch, dx_f32
 //    rows * width floats when piece < classes, and scratch scratch_bytes, at
 //    least tnops_linear_ce_scratch(...). A null dx or dw is left out.

@@ -52,7 +52,7 @@ def test_linear_ce_launchers_refuse(built):
     _refuses(f, good, [(0, A + 8), (1, A + 8), (6, 0), (7, 0), (7, 60), (8, 0)])
     f = _launcher("tnops_linear_ce_bwd", P, P, P, P, P, I, P, P, I, P, P, S, P, P, I, I, I, I, I, P)
     good = [A, A, A, A, A, 0, A, A, 256, A, None, 0, A, A, 1, 4, 64, 300, 304, None]
-    _refuses(f, good, [(0, A + 8), (1, A + 8), (7, A + 16), (8, 0), (8, 264), (9, None),
+    _refuses(f, good, [(0, A + 8), (1, A + 8), (5, 2), (7, A + 16), (8, 0), (8, 264), (9, None),
                        (9, A + 4), (10, A + 8), (12, A + 8), (13, A + 4), (15, 0),
                        (16, 60), (17, 0), (18, 299)])
     # The scratch of the first pieces and of the last, shorter one.

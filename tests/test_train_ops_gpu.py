@@ -227,6 +227,24 @@ def test_linear_cross_entropy(ops, rows, width, vocab, classes, reduction):
     assert dw.dtype == torch.bfloat16 and bool((dw[classes:] == 0).all())
 
 
+def test_linear_cross_entropy_mean_does_not_scale_the_gradient(ops):
+    """1 / rows that count is no bf16 number; rounded into every entry of the
+    logits' gradient it would scale all of dx and dw. Projected onto the exact
+    gradient, the result's scale is right to a small part of a rounding: the
+    entries' own roundings are independent, and average out over
+    thousands of them."""
+    rows = 1000  # 1 / 1000 is 0.43 of a bf16 step from its neighbour
+    x, w, _ = _ce_case(rows, 128, 3000, 3000, seed=77)
+    target = torch.randint(0, 3000, (rows,), device="cuda",
+                           generator=torch.Generator(device="cuda").manual_seed(1))
+    wr = w.float().requires_grad_()
+    ops.linear_cross_entropy(x, wr, target).backward()
+    k = torch.full((rows,), 1.0 / rows, device="cuda", dtype=torch.float64)
+    _, _, ew, _, _ = _ce_exact(x, w, target, 3000, k)
+    scale = (wr.grad.double() * ew).sum() / (ew * ew).sum()
+    assert abs(float(scale) - 1) < BF16 / 8
+
+
 def test_linear_cross_entropy_fp32_weight(ops):
     """An fp32 weight is used through its bf16 copy and gets an fp32
     gradient."""
