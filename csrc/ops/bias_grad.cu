@@ -11,11 +11,12 @@
 // tiles the matrix into (256-column, rowsPer-row) blocks; each warp of a CTA
 // owns 256 columns (8 per lane, one 16-byte load per row) and every 8th row
 // of the block, 4 rows in flight; the 8 warp sums are added in warp order
-// into one fp32 partial per block (the result, where one block is all). Pass 2 adds the partials of a column in
-// block order (colReduce, common.cuh). The summation order depends only on
-// (M, N), never on scheduling. Rounding of the GELU gradient to bf16 happens before it is
-// summed, as when the gradient tensor is materialised and then reduced; with an
-// 8-bit pre the sum is of the fp32 products.
+// into one fp32 partial per block (the result, where one block is all). Pass 2
+// adds the partials of a column in block order (colReduce, common.cuh). The
+// summation order depends only on (M, N), never on scheduling. Rounding of the
+// GELU gradient to bf16 happens before it is summed, as when the gradient
+// tensor is materialised and then reduced; with an 8-bit pre the sum is of the
+// fp32 products.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -68,17 +69,25 @@ __device__ __forceinline__ float geluTanhGrad(float x) {
   return fmaf(2.0f * x * r * (e * r), du, r);
 }
 
-// The same derivative of two numbers at once, for finite ones. Only the lower
-// end of u is held: there e^(-2u) would pass the fp32 range; at the other
-// e is 0, r is 1 and the slope 1.
-__device__ __forceinline__ uint64_t geluTanhGrad2(uint64_t x) {
+// max(lo, min(x, hi)), NaN for NaN.
+__device__ __forceinline__ float within(float x, float lo, float hi) {
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(hi));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(lo));
+  return x;
+}
+// The same derivative of two numbers at once. x is held within +-9.5, where the
+// derivative is 0 or 1 to 1e-29 and nothing passes the fp32 range (further out
+// e^(-2u) would, then x^2).
+__device__ __forceinline__ uint64_t geluTanhGrad2(uint64_t in) {
   const float k0 = 0.7978845608028654f, k0k1 = 0.7978845608028654f * 0.044715f;
   const float m2log2e = -2.0f * 1.4426950408889634f;
+  float a, b;
+  unpack2(in, a, b);
+  const uint64_t x = pack2(within(a, -9.5f, 9.5f), within(b, -9.5f, 9.5f));
   const uint64_t x2 = mul2(x, x);
   const uint64_t du = fma2(pack2(3.0f * k0k1, 3.0f * k0k1), x2, pack2(k0, k0));
-  float a, b;
-  unpack2(mul2(x, fma2(pack2(k0k1, k0k1), x2, pack2(k0, k0))), a, b);
-  unpack2(mul2(pack2(fmaxf(a, -40.0f), fmaxf(b, -40.0f)), pack2(m2log2e, m2log2e)), a, b);
+  unpack2(mul2(mul2(x, fma2(pack2(k0k1, k0k1), x2, pack2(k0, k0))), pack2(m2log2e, m2log2e)), a,
+          b);
   const uint64_t e = pack2(ex2Approx(a), ex2Approx(b));
   unpack2(add2(e, pack2(1.0f, 1.0f)), a, b);
   float ra, rb;

@@ -17,15 +17,15 @@
 namespace tnops {
 namespace {
 
-// tanh-GELU of two numbers, x / (1 + e^(-2u)) with u = k0 (x + k1 x^3). The
-// exponent -2u log2e is held at its upper end, where 2^it would pass the fp32
-// range; at the other end the power is 0 and the result x.
+// tanh-GELU of two numbers, x / (1 + e^(-2u)) with u = k0 (x + k1 x^3). Where
+// the power passes the fp32 range its inverse is 0 and so is the result; at the
+// other end the power is 0 and the result x.
 __device__ __forceinline__ uint64_t geluTanh2(uint64_t x) {
   const float c = -2.0f * 1.4426950408889634f * 0.7978845608028654f;  // -2 log2e sqrt(2 / pi)
   const uint64_t inner = fma2(pack2(c * 0.044715f, c * 0.044715f), mul2(x, x), pack2(c, c));
   float a, b;
   unpack2(mul2(x, inner), a, b);
-  unpack2(add2(pack2(ex2Approx(fminf(a, 115.0f)), ex2Approx(fminf(b, 115.0f))), pack2(1.f, 1.f)),
+  unpack2(add2(pack2(ex2Approx(a), ex2Approx(b)), pack2(1.f, 1.f)),
           a, b);
   asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
   asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
@@ -152,7 +152,8 @@ extern "C" int tnops_linear_gelu_int8(const void* x, const void* w, const void* 
                                       cudaStream_t stream) {
   if (rows <= 0 || outs <= 0 || ins <= 0 || outs % 8 != 0 || ins % 8 != 0 || !aligned16(x) ||
       !aligned16(w) || !aligned16(bias) || bias == nullptr ||
-      (reinterpret_cast<uintptr_t>(act) & 31) || (reinterpret_cast<uintptr_t>(pre_q) & 31) || (reinterpret_cast<uintptr_t>(pre_e) & 3))
+      (reinterpret_cast<uintptr_t>(act) & 31) || (reinterpret_cast<uintptr_t>(pre_q) & 31) ||
+      (reinterpret_cast<uintptr_t>(pre_e) & 3))
     return 1;
   PanelGemmArgs<GeluInt8Epi> args{};
   GeluInt8Epi& epi = args.epi;

@@ -213,13 +213,13 @@ __global__ void __launch_bounds__(kJoinThreads)
   }
 }
 
-// out[0] = the sum of the losses, or their mean over the rows that count;
-// out[1] = 1 / the number of rows that count (at least one). One CTA, fixed
+// out = the sum of the losses, or their mean over the rows that count;
+// share = 1 / the number of rows that count (at least one). One CTA, fixed
 // order.
 constexpr int kMeanThreads = 1024;
 __global__ void __launch_bounds__(kMeanThreads)
     meanLoss(const float* __restrict__ loss, const int64_t* __restrict__ target, int rows,
-             int classes, int mean, float* __restrict__ out) {
+             int classes, int mean, float* __restrict__ out, float* __restrict__ share) {
   __shared__ float sSum[32];
   __shared__ int sCount[32];
   float sum = 0.f;
@@ -240,9 +240,9 @@ __global__ void __launch_bounds__(kMeanThreads)
     sum = warpSum(sSum[threadIdx.x]);
     count = __reduce_add_sync(0xffffffffu, sCount[threadIdx.x]);
     if (threadIdx.x == 0) {
-      const float share = 1.0f / (float)(count > 0 ? count : 1);
-      out[0] = mean ? sum * share : sum;
-      out[1] = share;
+      const float s = 1.0f / (float)(count > 0 ? count : 1);
+      *out = mean ? sum * s : sum;
+      *share = s;
     }
   }
 }
@@ -279,10 +279,11 @@ extern "C" int tnops_linear_ce_fwd(const void* x, const void* w, const int64_t* 
   return launched(cudaGetLastError());
 }
 
-extern "C" int tnops_linear_ce_mean(const float* loss, const int64_t* target, float* out2,
-                                    int rows, int classes, int mean, cudaStream_t stream) {
+extern "C" int tnops_linear_ce_mean(const float* loss, const int64_t* target, float* out,
+                                    float* share, int rows, int classes, int mean,
+                                    cudaStream_t stream) {
   if (rows <= 0) return 1;
-  meanLoss<<<1, kMeanThreads, 0, stream>>>(loss, target, rows, classes, mean, out2);
+  meanLoss<<<1, kMeanThreads, 0, stream>>>(loss, target, rows, classes, mean, out, share);
   return launched(cudaGetLastError());
 }
 
@@ -332,11 +333,12 @@ extern "C" size_t tnops_linear_ce_scratch(int rows, int width, int classes, int 
 extern "C" int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* target,
                                    const float* lse, const float* grad, int grad_step,
                                    const float* share, void* d, int piece, float* dx_f32,
-                                   void* scratch, size_t scratch_bytes, void* dx, void* dw, int dw_f32, int rows, int width,
-                                   int classes, int vocab, cudaStream_t stream) {
+                                   void* scratch, size_t scratch_bytes, void* dx, void* dw,
+                                   int dw_f32, int rows, int width, int classes, int vocab,
+                                   cudaStream_t stream) {
   if (rows <= 0 || classes <= 0 || vocab < classes || width <= 0 || width % 8 != 0 ||
-      piece <= 0 || piece % 32 != 0 || (grad_step != 0 && grad_step != 1) || !aligned16(x) || !aligned16(w) ||
-      (reinterpret_cast<uintptr_t>(d) & 31) ||
+      piece <= 0 || piece % 32 != 0 || (grad_step != 0 && grad_step != 1) || !aligned16(x) ||
+      !aligned16(w) || (reinterpret_cast<uintptr_t>(d) & 31) ||
       (dx && !aligned16(dx)) || (dw && !aligned16(dw)))
     return 1;
   const bool whole = classes <= piece;

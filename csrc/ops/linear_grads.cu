@@ -168,6 +168,7 @@ extern "C" int tnops_linear_grads(const void* g, int64_t ldg, const void* w, con
                                   void* scratch, size_t scratch_bytes, cudaStream_t stream) {
   if (g == nullptr || (dx && !w) || (dw && !x)) return 1;
   LinearGrads a{g, ldg, w, x, dx, dw, scratch, scratch_bytes, dx ? kStoreBf16 : kStoreNone,
-                dw ? (dw_f32 ? kStoreF32 : kStoreBf16) : kStoreNone, rows, outs, ins, 0, {nullptr, nullptr}};
+                dw ? (dw_f32 ? kStoreF32 : kStoreBf16) : kStoreNone, rows, outs, ins, 0,
+                {nullptr, nullptr}};
   return linearGrads(a, stream);
 }

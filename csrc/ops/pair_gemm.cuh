@@ -1,7 +1,6 @@
-// pair_gemm.cuh - the matrix products behind the training operators: one
-// persistent CTA-pair pipeline (tcgen05 cta_group::2, 256 x 256 tiles, fp32
-// accumulators in TMEM) whose operands may lie either way round in memory and
-// whose epilogue is the caller's.
+// pair_gemm.cuh - the matrix products behind the backward passes of the
+// training operators: one persistent CTA-pair pipeline (tcgen05 cta_group::2,
+// fp32 accumulators in TMEM) whose operands may lie either way round in memory.
 //
 //   D[m, n] = sum_k A(m, k) B(n, k)
 //

@@ -118,16 +118,16 @@ int tnops_linear_grads(const void* g, int64_t ldg, const void* w, const void* x,
 // Softmax cross-entropy of l = x w^T without the logits in memory: x
 // [rows, width], w [vocab, width] in bf16, of which the first `classes` rows
 // are classes. A row whose target is outside [0, classes) does not count
-// (zero loss, zero gradient). width % 8 == 0, x, w, dx, dw 16-byte, d 32-byte aligned;
-// 1 (invalid argument) without a launch otherwise.
+// (zero loss, zero gradient). width % 8 == 0, x, w, dx, dw 16-byte, d 32-byte
+// aligned; 1 (invalid argument) without a launch otherwise.
 //  * fwd: loss[r] and lse[r] (fp32); partial holds
 //    2 * rows * tnops_linear_ce_parts(classes) floats of scratch.
-//  * mean: out2[0] = the losses' sum, or with `mean` their mean over the rows
-//    that count; out2[1] = 1 / max(1, rows that count).
+//  * mean: *out = the losses' sum, or with `mean` their mean over the rows that
+//    count; *share = 1 / max(1, rows that count).
 //  * bwd: dx [rows, width] (bf16) and dw [vocab, width] (fp32 with dw_f32, else
 //    bf16; rows from `classes` on are zero) of sum_r k[r] loss[r], with k[r] =
-//    grad[r * grad_step] (* *share), grad_step 0 or 1. Works on `piece` classes at a time
-//    (piece % 32 == 0); d holds rows * piece bf16 of scratch, dx_f32
+//    grad[r * grad_step] (* *share), grad_step 0 or 1. Works on `piece` classes
+//    at a time (piece % 32 == 0); d holds rows * piece bf16 of scratch, dx_f32
 //    rows * width floats when piece < classes, and scratch scratch_bytes, at
 //    least tnops_linear_ce_scratch(...). A null dx or dw is left out.
 //  * piece: a good `piece` whose d takes at most `budget` bytes (256 classes
@@ -139,12 +139,13 @@ size_t tnops_linear_ce_scratch(int rows, int width, int classes, int vocab, int 
 int tnops_linear_ce_fwd(const void* x, const void* w, const int64_t* target, float* loss,
                         float* lse, float* partial, int rows, int width, int classes,
                         cudaStream_t stream);
-int tnops_linear_ce_mean(const float* loss, const int64_t* target, float* out2, int rows,
-                         int classes, int mean, cudaStream_t stream);
+int tnops_linear_ce_mean(const float* loss, const int64_t* target, float* out, float* share,
+                         int rows, int classes, int mean, cudaStream_t stream);
 int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* target, const float* lse,
                         const float* grad, int grad_step, const float* share, void* d, int piece,
-                        float* dx_f32, void* scratch, size_t scratch_bytes, void* dx, void* dw, int dw_f32, int rows, int width,
-                        int classes, int vocab, cudaStream_t stream);
+                        float* dx_f32, void* scratch, size_t scratch_bytes, void* dx, void* dw,
+                        int dw_f32, int rows, int width, int classes, int vocab,
+                        cudaStream_t stream);
 
 // Token and position embedding: y[r] = scale * w[token[r]] + p[position[r]]
 // for w [vocab, cols] and p [context, cols] (both fp32 with w_f32, else bf16;

@@ -153,7 +153,8 @@ CeShape ceShape(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targ
           asInt(w.size(0), "vocabulary")};
 }
 
-// -> per-row loss, lse, and (but for kNone) [sum or mean, 1 / rows that count]
+// -> per-row loss, lse, and (but for kNone) the sum or mean, 1 / rows that count.
+// The last two are tensors of their own: the loss may be changed in place.
 enum Reduction { kMean = 0, kSum = 1, kNone = 2 };
 std::vector<at::Tensor> linearCeFwd(const at::Tensor& x, const at::Tensor& w,
                                     const at::Tensor& target, int64_t classes,
@@ -163,21 +164,20 @@ std::vector<at::Tensor> linearCeFwd(const at::Tensor& x, const at::Tensor& w,
   const auto opt = x.options().dtype(at::kFloat);
   auto loss = at::empty({s.rows}, opt), lse = at::empty({s.rows}, opt);
   if (s.rows == 0) {
-    auto out = at::zeros({2}, opt);
-    out.select(0, 1).fill_(1.0);
-    return {loss, lse, out};
+    return {loss, lse, at::zeros({}, opt), at::ones({}, opt)};
   }
   auto partial = at::empty({(int64_t)tnops_linear_ce_parts(s.classes), s.rows, 2}, opt);
   ok(tnops_linear_ce_fwd(x.data_ptr(), w.data_ptr(), target.data_ptr<int64_t>(),
                          loss.data_ptr<float>(), lse.data_ptr<float>(), partial.data_ptr<float>(),
                          s.rows, s.width, s.classes, streamOf(x)),
      "tnops_linear_ce_fwd");
-  if (reduction == kNone) return {loss, lse, at::Tensor()};
-  auto out = at::empty({2}, opt);
+  if (reduction == kNone) return {loss, lse, at::Tensor(), at::Tensor()};
+  auto out = at::empty({}, opt), share = at::empty({}, opt);
   ok(tnops_linear_ce_mean(loss.data_ptr<float>(), target.data_ptr<int64_t>(),
-                          out.data_ptr<float>(), s.rows, s.classes, reduction == kMean ? 1 : 0, streamOf(x)),
+                          out.data_ptr<float>(), share.data_ptr<float>(), s.rows, s.classes,
+                          reduction == kMean ? 1 : 0, streamOf(x)),
      "tnops_linear_ce_mean");
-  return {loss, lse, out};
+  return {loss, lse, out, share};
 }
 
 // Scratch for a piece of the logits' gradient.
@@ -409,15 +409,27 @@ Opt destination(const at::Tensor& p, bool has, at::ScalarType st) {
       py::module_::import("tiny_nccl_b200.ops.fused").attr("grad_destination")(p);
   if (d.is_none()) return c10::nullopt;
   const auto t = d.cast<at::Tensor>();
-  if (t.scalar_type() != st || !t.is_contiguous()) return c10::nullopt;
+  if (t.scalar_type() != st || !t.is_contiguous() ||
+      reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0)
+    return c10::nullopt;
   return t.detach();
 }
 Opt savedOpt(AutogradContext* ctx, const char* key) {
   const auto& v = ctx->saved_data[key];
   return v.isNone() ? Opt() : Opt(v.toTensor());
 }
+// The products read 16-byte pieces: a tensor that is not contiguous, or starts
+// off that boundary, is copied.
+at::Tensor packed(const at::Tensor& t) {
+  const auto c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
 at::Tensor bf16Copy(const at::Tensor& p, const Opt& copy) {
-  return (copy ? *copy : p.detach().to(at::kBFloat16)).contiguous();
+  return packed(copy ? *copy : p.detach().to(at::kBFloat16));
+}
+// x [*, width] as bf16 rows.
+at::Tensor bf16Rows(const at::Tensor& x) {
+  return packed(x.reshape({-1, x.size(-1)}).to(at::kBFloat16));
 }
 
 struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
@@ -456,7 +468,8 @@ at::Tensor embedding(const at::Tensor& w, const Opt& p, const at::Tensor& idx,
                      const Opt& positions, int64_t seq, double scale, bool outF32,
                      bool dwDest, bool dpDest) {
   auto flat = [](const at::Tensor& t) { return t.reshape({-1}).to(at::kLong).contiguous(); };
-  auto y = EmbeddingFn::apply(w, p, flat(idx), positions ? Opt(flat(*positions)) : Opt(), seq, scale, outF32, dwDest, dpDest);
+  auto y = EmbeddingFn::apply(w, p, flat(idx), positions ? Opt(flat(*positions)) : Opt(), seq,
+                              scale, outF32, dwDest, dpDest);
   auto shape = idx.sizes().vec();
   shape.push_back(w.size(1));
   return y.view(shape);
@@ -468,12 +481,12 @@ struct LinearCeFn : torch::autograd::Function<LinearCeFn> {
                             int64_t reduction, bool dwDest) {
     const auto wb = bf16Copy(w, w16);
     const auto r = linearCeFwd(x, wb, target, classes, reduction);
-    ctx->save_for_backward({x, wb, target, r[1], r[2]});
+    ctx->save_for_backward({x, wb, target, r[1], r[3]});
     ctx->saved_data["w"] = w;
     ctx->saved_data["classes"] = classes;
     ctx->saved_data["mean"] = reduction == kMean;
     ctx->saved_data["dw"] = dwDest;
-    return reduction == kNone ? r[0] : r[2].select(0, 0);
+    return reduction == kNone ? r[0] : r[2];
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     onceDifferentiable("linear_cross_entropy");
@@ -483,7 +496,7 @@ struct LinearCeFn : torch::autograd::Function<LinearCeFn> {
     const auto g = grads[0].reshape({-1}).to(at::kFloat).contiguous();
     const bool wantW = ctx->needs_input_grad(1);
     const auto d = linearCeBwd(
-        s[0], s[1], s[2], s[3], g, ctx->saved_data["mean"].toBool() ? Opt(s[4].slice(0, 1)) : Opt(),
+        s[0], s[1], s[2], s[3], g, ctx->saved_data["mean"].toBool() ? Opt(s[4]) : Opt(),
         ctx->saved_data["classes"].toInt(), ctx->needs_input_grad(0), wantW, st == at::kFloat,
         wantW ? destination(w, ctx->saved_data["dw"].toBool(), st) : Opt(), kCeBudget);
     return {d[0], d[1], {}, {}, {}, {}, {}};
@@ -493,14 +506,14 @@ struct LinearCeFn : torch::autograd::Function<LinearCeFn> {
 at::Tensor linearCrossEntropy(const at::Tensor& x, const at::Tensor& w, const Opt& w16,
                               const at::Tensor& target, int64_t classes, int64_t reduction,
                               bool dwDest) {
-  const auto xb = x.reshape({-1, x.size(-1)}).to(at::kBFloat16).contiguous();
+  const auto xb = bf16Rows(x);
   const auto t = target.reshape({-1}).contiguous();
   at::Tensor loss;
   if (wantsGradient({&x, &w})) {
     loss = LinearCeFn::apply(xb, w, w16, t, classes, reduction, dwDest);
   } else {
     const auto r = linearCeFwd(xb, bf16Copy(w, w16), t, classes, reduction);
-    loss = reduction == kNone ? r[0] : r[2].select(0, 0);
+    loss = reduction == kNone ? r[0] : r[2];
   }
   return reduction == kNone ? loss.view(target.sizes()) : loss;
 }
@@ -535,7 +548,7 @@ struct LinearInt8Fn : torch::autograd::Function<LinearInt8Fn> {
     const auto s = ctx->get_saved_variables();
     const bool gelu = s.size() == 5;
     const at::Tensor w = ctx->saved_data["w"].toTensor(), b = ctx->saved_data["b"].toTensor();
-    auto g = grads[0].contiguous();
+    auto g = packed(grads[0]);
     const bool wantW = ctx->needs_input_grad(1);
     const bool wantB = ctx->needs_input_grad(2);
     const auto bt = b.scalar_type() == at::kBFloat16 ? at::kBFloat16 : at::kFloat;
@@ -549,9 +562,9 @@ struct LinearInt8Fn : torch::autograd::Function<LinearInt8Fn> {
       db = biasGradient(g, bt, dbOut);
     }
     const auto st = w.scalar_type() == at::kFloat ? at::kFloat : at::kBFloat16;
-    const auto d = linearGradsInt8(g, s[0], s[s.size() - 2], s[s.size() - 1],
-                                   ctx->needs_input_grad(0), wantW, st == at::kFloat,
-                                   wantW ? destination(w, ctx->saved_data["dw"].toBool(), st) : Opt());
+    const auto d = linearGradsInt8(
+        g, s[0], s[s.size() - 2], s[s.size() - 1], ctx->needs_input_grad(0), wantW,
+        st == at::kFloat, wantW ? destination(w, ctx->saved_data["dw"].toBool(), st) : Opt());
     return {d[0], d[1], db, {}, {}, {}, {}, {}};
   }
 };
@@ -559,7 +572,12 @@ struct LinearInt8Fn : torch::autograd::Function<LinearInt8Fn> {
 at::Tensor linearInt8(const at::Tensor& x, const at::Tensor& w, const at::Tensor& b,
                       const Opt& w16, const Opt& b16, bool gelu, bool dwDest,
                       bool dbDest) {
-  const auto xb = x.reshape({-1, x.size(-1)}).to(at::kBFloat16).contiguous();
+  TORCH_CHECK(w.dim() == 2 && b.dim() == 1 && b.size(0) == w.size(0) && x.dim() > 0 &&
+                  x.size(-1) == w.size(1),
+              "linear_int8: want x [*, ins], weight [outs, ins], bias [outs]");
+  TORCH_CHECK(w.size(0) % 8 == 0 && w.size(1) % 8 == 0,
+              "linear_int8: the layer's sizes must be multiples of 8");
+  const auto xb = bf16Rows(x);
   auto y = wantsGradient({&x, &w, &b})
                ? LinearInt8Fn::apply(xb, w, b, w16, b16, gelu, dwDest, dbDest)
                : linearInt8Out(xb, bf16Copy(w, w16), bf16Copy(b, b16), gelu)[0];

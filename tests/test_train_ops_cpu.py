@@ -59,8 +59,8 @@ def test_linear_ce_launchers_refuse(built):
     a, b, c = (_scratch("tnops_linear_grads_scratch", 1024, n, 768, 1, 1) for n in (768, 232, 1000))
     assert _scratch("tnops_linear_ce_scratch", 1024, 768, 1000, 1000, 768, 1, 1) == max(a, b)
     assert _scratch("tnops_linear_ce_scratch", 1024, 768, 1000, 1000, 1024, 1, 1) == c
-    f = _launcher("tnops_linear_ce_mean", P, P, P, I, I, I, P)
-    assert f(A, A, A, 0, 5, 1, None) == 1
+    f = _launcher("tnops_linear_ce_mean", P, P, P, P, I, I, I, P)
+    assert f(A, A, A, A, 0, 5, 1, None) == 1
 
 
 def test_embedding_launchers_refuse(built):
@@ -151,6 +151,13 @@ def test_python_refusals(built):
     for f in (ops.linear, ops.linear_gelu):
         with pytest.raises(ValueError):
             f(x, w, torch.zeros(10), activations="int4")
+        # Sizes are refused before anything is computed, not in the backward pass.
+        with pytest.raises(RuntimeError, match="multiples of 8"):
+            f(x, w, torch.zeros(10), activations="int8")
+        with pytest.raises(RuntimeError, match="bias"):
+            f(x, w[:8], torch.zeros(10), activations="int8")
+        with pytest.raises(RuntimeError, match="weight"):
+            f(x[:, :4], w[:8], torch.zeros(8), activations="int8")
 
 
 def test_gradient_slice_is_handed_out_once_per_backward():

@@ -265,9 +265,9 @@ def test_linear_cross_entropy_pieces(ops, budget_tiles):
     rows belong to one piece each), and dx up to the fp32 sums' order."""
     from tiny_nccl_b200._native import load
     x, w, target = _ce_case(200, 136, 1500, 1437, seed=21)
-    loss, lse, out = load().ops.linear_ce_fwd(x, w, target, 1437, 0)
+    loss, lse, _, share = load().ops.linear_ce_fwd(x, w, target, 1437, 0)
     one = torch.ones(1, device="cuda")
-    args = (x, w, target, lse, one, out[1:], 1437, True, True, True, None)
+    args = (x, w, target, lse, one, share, 1437, True, True, True, None)
     dx, dw = load().ops.linear_ce_bwd(*args, 512 << 20)
     px, pw = load().ops.linear_ce_bwd(*args, budget_tiles * 200 * 512)
     status_ok()
@@ -612,6 +612,75 @@ def test_strided_and_misaligned_inputs(ops):
     b = ops.linear_cross_entropy(x[:, ::2].contiguous(), hw, t)
     assert torch.equal(a, b)
     assert torch.equal(ops.quantize_int8(x.t())[0], ops.quantize_int8(x.t().contiguous())[0])
+
+
+def test_misaligned_gradients_and_parameters(ops):
+    """A gradient, an input and parameters that start off a 16-byte boundary
+    give the bits of aligned ones."""
+    def off(t):  # the same values, one element past a boundary
+        base = torch.empty(t.numel() + 1, device="cuda", dtype=t.dtype)
+        return base[1:].view(t.shape).copy_(t)
+    x = _normal(40, 64, seed=1, dtype=torch.bfloat16)
+    w, b = _normal(48, 64, seed=2, dtype=torch.bfloat16), _normal(48, seed=3, dtype=torch.bfloat16)
+    t = torch.arange(40, device="cuda")
+    flat = torch.cat([torch.zeros(3, device="cuda"), _normal(40 * 48, seed=4)])
+    gy = flat[3:].view(40, 48).to(torch.bfloat16)
+    for f in (lambda *a: ops.linear(*a, activations="int8"),
+              lambda *a: ops.linear_gelu(*a, activations="int8"),
+              lambda x, w, b: ops.linear_cross_entropy(x, w, t, reduction="none")):
+        out = []
+        for move in (lambda v: v, off):
+            leaves = [move(v).requires_grad_() for v in (x, w, b)]
+            y = f(*leaves)
+            # The gradient that arrives is a view of the joined tensor's.
+            joined = torch.cat([torch.zeros(3 if move is off else 0, device="cuda", dtype=y.dtype),
+                                y.flatten()])
+            g = flat.to(joined.dtype)[3 if move is not off else 0:][:joined.numel()]
+            out.append([y, *torch.autograd.grad(joined, leaves, g, allow_unused=True)])
+        for a, c in zip(*out):
+            assert (a is None and c is None) or torch.equal(a, c)
+    status_ok()
+
+
+def test_loss_may_be_changed_in_place(ops):
+    x = _normal(40, 64, seed=1, dtype=torch.bfloat16).requires_grad_()
+    w = _normal(100, 64, seed=2).requires_grad_()
+    t = torch.arange(40, device="cuda")
+    for reduction in ("mean", "sum"):
+        want = torch.autograd.grad(ops.linear_cross_entropy(x, w, t, reduction=reduction) * 0.5,
+                                   [x, w])
+        loss = ops.linear_cross_entropy(x, w, t, reduction=reduction)
+        loss.mul_(0.5)
+        for a, b in zip(torch.autograd.grad(loss, [x, w]), want):
+            assert torch.equal(a, b)
+
+
+def test_linear_gelu_int8_far_from_zero(ops):
+    """Sums of any size: the GELU is 0 or its argument, the slope 0 or 1, and a
+    sum that is no number gives none."""
+    values = [20.0, -20.0, 1e12, -1e12, 1e20, -1e20, 3e38, -3e38]
+    b = torch.tensor(values, device="cuda").repeat_interleave(32).to(torch.bfloat16)
+    x = torch.zeros(5, 64, device="cuda", dtype=torch.bfloat16)
+    w = _normal(256, 64, seed=1)
+    b.requires_grad_()
+    y = ops.linear_gelu(x, w, b, activations="int8")
+    gy = _normal(5, 256, seed=2, dtype=torch.bfloat16)
+    (db,) = torch.autograd.grad(y, [b], gy)
+    up = b.detach() > 0
+    assert torch.equal(y[:, up], b.detach()[up].expand(5, -1))
+    assert bool((y[:, ~up].abs() <= 1e-30).all())
+    g64 = gy.double()
+    _within(db[up], g64.sum(0)[up], BF16 * g64.sum(0)[up].abs() * 1.01
+            + 5 * F32 * g64.abs().sum(0)[up])
+    assert bool((db[~up].abs() <= 1e-25).all())
+    with torch.no_grad():
+        b[40] = float("nan")
+    y = ops.linear_gelu(x, w, b, activations="int8")
+    (db,) = torch.autograd.grad(y, [b], gy)
+    assert bool(y[:, 40].isnan().all()) and not bool(y[:, :40].isnan().any())
+    # 8-bit blocks lose a number's neighbours with it, and no others.
+    assert bool(db[32:64].isnan().all()) and not bool(db[:32].isnan().any())
+    assert not bool(db[64:].isnan().any())
 
 
 def test_refuses_to_be_differentiated_twice(ops):
