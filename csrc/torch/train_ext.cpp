@@ -7,6 +7,7 @@
 #include <torch/extension.h>
 
 #include <climits>
+#include <string>
 #include <vector>
 
 #include "tnccl_ops.h"
@@ -414,6 +415,11 @@ Opt destination(const at::Tensor& p, bool has, at::ScalarType st) {
     return c10::nullopt;
   return t.detach();
 }
+// Whether p may have one: an attribute of the parameter's Python object.
+bool hasDestination(const at::Tensor& p) {
+  const py::object t = py::cast(p);
+  return py::hasattr(t, "_tn_grad_dest") && !t.attr("_tn_grad_dest").is_none();
+}
 Opt savedOpt(AutogradContext* ctx, const char* key) {
   const auto& v = ctx->saved_data[key];
   return v.isNone() ? Opt() : Opt(v.toTensor());
@@ -464,12 +470,50 @@ struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
   }
 };
 
-at::Tensor embedding(const at::Tensor& w, const Opt& p, const at::Tensor& idx,
-                     const Opt& positions, int64_t seq, double scale, bool outF32,
-                     bool dwDest, bool dpDest) {
-  auto flat = [](const at::Tensor& t) { return t.reshape({-1}).to(at::kLong).contiguous(); };
-  auto y = EmbeddingFn::apply(w, p, flat(idx), positions ? Opt(flat(*positions)) : Opt(), seq,
-                              scale, outF32, dwDest, dpDest);
+// The checks that Python callers see as TypeError and ValueError stand here as
+// well: in Python they take a third of a decoding step's call.
+at::Tensor embedding(const at::Tensor& idx, const at::Tensor& weight, const Opt& posWeight,
+                     const Opt& positions, double scale, c10::optional<at::ScalarType> outType) {
+  auto floating = [](at::ScalarType t, const char* name) {
+    if (t != at::kFloat && t != at::kBFloat16)
+      throw py::type_error(std::string(name) + " must be float32 or bfloat16, not " +
+                           c10::toString(t));
+  };
+  auto index = [](const at::Tensor& t, const char* name) {
+    if (t.scalar_type() != at::kLong && t.scalar_type() != at::kInt)
+      throw py::type_error(std::string(name) + " must be int64 or int32, not " +
+                           c10::toString(t.scalar_type()));
+  };
+  floating(weight.scalar_type(), "weight");
+  if (weight.dim() != 2) throw py::value_error("weight must be [vocab, width]");
+  if (posWeight) {
+    if (posWeight->dim() != 2 || posWeight->size(1) != weight.size(1))
+      throw py::value_error("pos_weight must be [context, width], of weight's width");
+    if (posWeight->scalar_type() != weight.scalar_type())
+      throw py::type_error("weight and pos_weight must have one dtype");
+  }
+  if (outType) floating(*outType, "out_dtype");
+  index(idx, "idx");
+  if (positions) {
+    if (!posWeight) throw py::value_error("positions without pos_weight");
+    if (positions->sizes() != idx.sizes())
+      throw py::value_error("positions must have idx's shape");
+    index(*positions, "positions");
+  }
+  const auto w = weight.contiguous();
+  const Opt p = posWeight ? Opt(posWeight->contiguous()) : Opt();
+  auto flat = [](const at::Tensor& t) {
+    return (t.dim() == 1 ? t : t.reshape({-1})).to(at::kLong).contiguous();
+  };
+  const auto token = flat(idx);
+  const Opt position = positions ? Opt(flat(*positions)) : Opt();
+  const int64_t seq = idx.dim() > 0 ? idx.size(-1) : 1;
+  const bool outF32 = outType.value_or(w.scalar_type()) == at::kFloat;
+  auto y = wantsGradient({&w, p ? &*p : nullptr})
+               ? EmbeddingFn::apply(w, p, token, position, seq, scale, outF32,
+                                    hasDestination(w), p && hasDestination(*p))
+               : embeddingFwd(token, position, w, p, seq, scale, outF32);
+  if (idx.dim() == 1) return y;
   auto shape = idx.sizes().vec();
   shape.push_back(w.size(1));
   return y.view(shape);
@@ -504,13 +548,12 @@ struct LinearCeFn : torch::autograd::Function<LinearCeFn> {
 };
 
 at::Tensor linearCrossEntropy(const at::Tensor& x, const at::Tensor& w, const Opt& w16,
-                              const at::Tensor& target, int64_t classes, int64_t reduction,
-                              bool dwDest) {
+                              const at::Tensor& target, int64_t classes, int64_t reduction) {
   const auto xb = bf16Rows(x);
   const auto t = target.reshape({-1}).contiguous();
   at::Tensor loss;
   if (wantsGradient({&x, &w})) {
-    loss = LinearCeFn::apply(xb, w, w16, t, classes, reduction, dwDest);
+    loss = LinearCeFn::apply(xb, w, w16, t, classes, reduction, hasDestination(w));
   } else {
     const auto r = linearCeFwd(xb, bf16Copy(w, w16), t, classes, reduction);
     loss = reduction == kNone ? r[0] : r[2];
@@ -570,8 +613,7 @@ struct LinearInt8Fn : torch::autograd::Function<LinearInt8Fn> {
 };
 
 at::Tensor linearInt8(const at::Tensor& x, const at::Tensor& w, const at::Tensor& b,
-                      const Opt& w16, const Opt& b16, bool gelu, bool dwDest,
-                      bool dbDest) {
+                      const Opt& w16, const Opt& b16, bool gelu) {
   TORCH_CHECK(w.dim() == 2 && b.dim() == 1 && b.size(0) == w.size(0) && x.dim() > 0 &&
                   x.size(-1) == w.size(1),
               "linear_int8: want x [*, ins], weight [outs, ins], bias [outs]");
@@ -579,7 +621,8 @@ at::Tensor linearInt8(const at::Tensor& x, const at::Tensor& w, const at::Tensor
               "linear_int8: the layer's sizes must be multiples of 8");
   const auto xb = bf16Rows(x);
   auto y = wantsGradient({&x, &w, &b})
-               ? LinearInt8Fn::apply(xb, w, b, w16, b16, gelu, dwDest, dbDest)
+               ? LinearInt8Fn::apply(xb, w, b, w16, b16, gelu, hasDestination(w),
+                                     hasDestination(b))
                : linearInt8Out(xb, bf16Copy(w, w16), bf16Copy(b, b16), gelu)[0];
   auto shape = x.sizes().vec();
   shape.back() = w.size(0);
@@ -589,15 +632,12 @@ at::Tensor linearInt8(const at::Tensor& x, const at::Tensor& w, const at::Tensor
 }  // namespace
 
 void registerTrainOps(py::module_& ops) {
-  ops.def("embedding", &embedding, py::arg("weight"), py::arg("pos_weight"), py::arg("idx"),
-          py::arg("positions"), py::arg("seq"), py::arg("scale"), py::arg("out_f32"),
-          py::arg("has_dw_dest"), py::arg("has_dp_dest"));
+  ops.def("embedding", &embedding, py::arg("idx"), py::arg("weight"), py::arg("pos_weight"),
+          py::arg("positions"), py::arg("scale"), py::arg("out_dtype"));
   ops.def("linear_cross_entropy", &linearCrossEntropy, py::arg("x"), py::arg("weight"),
-          py::arg("weight_bf16"), py::arg("target"), py::arg("classes"), py::arg("reduction"),
-          py::arg("has_dw_dest"));
+          py::arg("weight_bf16"), py::arg("target"), py::arg("classes"), py::arg("reduction"));
   ops.def("linear_int8", &linearInt8, py::arg("x"), py::arg("weight"), py::arg("bias"),
-          py::arg("weight_bf16"), py::arg("bias_bf16"), py::arg("gelu"), py::arg("has_dw_dest"),
-          py::arg("has_db_dest"));
+          py::arg("weight_bf16"), py::arg("bias_bf16"), py::arg("gelu"));
   ops.def("linear_ce_fwd", &linearCeFwd, py::arg("x"), py::arg("weight"), py::arg("target"),
           py::arg("classes"), py::arg("reduction"));
   ops.def("linear_ce_piece", &tnops_linear_ce_piece, py::arg("rows"), py::arg("width"),

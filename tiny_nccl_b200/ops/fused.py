@@ -115,13 +115,6 @@ def bf16_weight(p: torch.Tensor) -> torch.Tensor:
     return c if c is not None else p.to(torch.bfloat16)
 
 
-def has_destination(p: torch.Tensor | None) -> bool:
-    """Whether p's gradient may have a place in a flat gradient buffer. The
-    native backward functions then ask :func:`grad_destination` when they
-    run."""
-    return getattr(p, "_tn_grad_dest", None) is not None
-
-
 def grad_destination(p: torch.Tensor):
     """Where the gradient of parameter p can be written directly: its slice
     of a flat gradient buffer (FlatGradReducer sets ``p._tn_grad_dest``), as
@@ -242,8 +235,7 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 
 def _linear(x, weight, bias, gelu, activations):
     if activations == "int8":
-        return _ops().linear_int8(x, weight, bias, current_copy(weight), current_copy(bias), gelu,
-                                  has_destination(weight), has_destination(bias))
+        return _ops().linear_int8(x, weight, bias, current_copy(weight), current_copy(bias), gelu)
     if activations != "bf16":
         raise ValueError(f"activations must be 'bf16' or 'int8', not {activations!r}")
     y = (_LinearGelu if gelu else _LinearBias).apply(_rows(x), weight, bias)

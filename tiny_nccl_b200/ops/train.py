@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import torch
 
-from .fused import _ops, current_copy, has_destination
+from .fused import _ops, current_copy
 
 
 def _needs_float(name: str, t: torch.Tensor) -> None:
@@ -31,32 +31,7 @@ def embedding(idx: torch.Tensor, weight: torch.Tensor, pos_weight: torch.Tensor 
 
     The gradients of both tables are fp32 sums in row order, bit-identical
     from run to run; a row that no token names gets zero."""
-    for name, t in (("weight", weight), ("pos_weight", pos_weight)):
-        if t is not None:
-            _needs_float(name, t)
-            if t.dim() != 2 or t.shape[1] != weight.shape[1]:
-                raise ValueError(f"{name} must be [rows, {weight.shape[-1]}], not "
-                                 f"{tuple(t.shape)}")
-            if t.dtype != weight.dtype:
-                raise TypeError("weight and pos_weight must have one dtype")
-    out_dtype = weight.dtype if out_dtype is None else out_dtype
-    if out_dtype not in (torch.float32, torch.bfloat16):
-        raise TypeError(f"out_dtype must be float32 or bfloat16, not {out_dtype}")
-    if idx.dtype not in (torch.int64, torch.int32):
-        raise TypeError(f"idx must be int64 or int32, not {idx.dtype}")
-    seq = idx.shape[-1] if idx.dim() else 1
-    if positions is not None:
-        if pos_weight is None:
-            raise ValueError("positions without pos_weight")
-        if positions.shape != idx.shape:
-            raise ValueError(f"positions must have idx's shape {tuple(idx.shape)}, not "
-                             f"{tuple(positions.shape)}")
-        if positions.dtype not in (torch.int64, torch.int32):
-            raise TypeError(f"positions must be int64 or int32, not {positions.dtype}")
-    return _ops().embedding(weight.contiguous(),
-                            None if pos_weight is None else pos_weight.contiguous(), idx,
-                            positions, seq, scale, out_dtype == torch.float32,
-                            has_destination(weight), has_destination(pos_weight))
+    return _ops().embedding(idx, weight, pos_weight, positions, scale, out_dtype)
 
 
 _REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
@@ -88,8 +63,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     if target.numel() * x.shape[-1] != x.numel():
         raise ValueError("target must have one entry per row of x")
     return _ops().linear_cross_entropy(x, weight, current_copy(weight), target,
-                                       int(classes) or weight.shape[0], _REDUCTIONS[reduction],
-                                       has_destination(weight))
+                                       int(classes) or weight.shape[0], _REDUCTIONS[reduction])
 
 
 def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
