@@ -481,6 +481,25 @@ __device__ __forceinline__ Cols<4> sumBlocks(const float* partial, int from, int
   return acc;
 }
 
+// The first block at or past b0 whose follower does not begin with k, + 1, by
+// the whole warp: each load narrows the blocks to a 33rd (65536 rows with one
+// token in ten alike: the kernel takes 14.4 us, 17 with a binary search).
+__device__ __forceinline__ int runEnd(const Table& t, int k, int b0) {
+  const int lane = threadIdx.x & 31;
+  int lo = b0, hi = t.blocks - 1;  // the block is in [lo, hi]: the last has no follower
+  while (lo < hi) {
+    const int step = (hi - lo + 32) / 33;
+    const int b = lo + (lane + 1) * step - 1;
+    const bool ends = b >= hi || t.key((b + 1) * t.block) != k;
+    const uint32_t votes = __ballot_sync(0xffffffffu, ends);
+    const int n = votes ? __ffs(votes) - 1 : 32;  // probes that go on
+    const int from = lo + n * step;
+    if (votes) hi = min(hi, from + step - 1);
+    lo = min(from, hi);
+  }
+  return lo + 1;
+}
+
 template <class W, bool FAST>
 __global__ void __launch_bounds__(kJoinWarps * 32, 3)
     joinRuns(const __grid_constant__ TableGradArgs a, int firstTable) {
@@ -506,8 +525,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3)
       const int b = block + 1 + lane;
       const bool ends = b >= t.blocks - 1 || t.key((b + 1) * t.block) != k;
       const uint32_t votes = __ballot_sync(0xffffffffu, ends);
-      end = votes ? block + 1 + __ffs(votes)
-                  : (lowerBound(t, a.rows, k + 1) - 1) / t.block + 1;
+      end = votes ? block + 1 + __ffs(votes) : runEnd(t, k, block + 33);
     }
   }
   const bool isLong = token >= 0 && end - block > kLongRun;
