@@ -7,13 +7,16 @@
 // An index outside its table contributes nothing: zero to y, and no gradient.
 //
 // The gradient, deterministic whatever the launch:
-//   1. sortChunks    a CTA sorts 1024 (or 4096) tokens with their row in the
-//                    chunk in shared memory;
+//   1. sortChunk     a CTA sorts 1024 to 4096 tokens with their row in the
+//                    chunk. These CTAs belong to the forward pass's launch,
+//                    which is bound by memory and hides most of them (65536 rows:
+//                    5 us are seen of 13 as a launch of their own), and leave the
+//                    sorted chunks for the backward pass;
 //   2. mergeRanks    a token's place in the whole order is its place in its
 //                    chunk plus the number of smaller ones in every other
 //                    chunk (equal ones count in chunks before its own), found
-//                    by binary searches: a stable sort in two launches, one
-//                    when a single chunk holds all rows;
+//                    by binary searches. Not needed when a single chunk holds
+//                    all rows;
 //   3. tableGrads    the sorted rows in blocks of 16 to 64: a group of threads,
 //                    one per 16 bytes of a row, adds the gradients of each run
 //                    of equal tokens in row order and writes the table row of
@@ -24,6 +27,8 @@
 // Without explicit positions the second table's order is known (row r has
 // position r % seq) and skips the sort; both tables share the launches of 3
 // and 4. Sums are fp32, rounded once to the table's type.
+#include <type_traits>
+
 #include "common.cuh"
 #include "tnccl_ops.h"
 
@@ -143,18 +148,167 @@ __device__ __forceinline__ Cols<N> scaled(const Cols<N>& a, float s) {
   return r;
 }
 
+// -- sorting ---------------------------------------------------------------------
+
+// Sort keys are (token << bits | row in the chunk), bits = log2(chunk), so
+// they differ and the order of equal tokens is the rows'. A token outside the
+// table takes the value `vocab`, after all others; padding follows it.
+// Keys take 32 bits where token and place in the chunk fit.
+constexpr int kSmallChunk = 1024, kChunk = 2048, kLargeChunk = 4096;
+
+template <int CHUNK>
+__host__ __device__ __forceinline__ constexpr int chunkBits() {
+  return CHUNK == kSmallChunk ? 10 : CHUNK == kChunk ? 11 : 12;
+}
+
+// Chunks of 1024, 2048 or 4096 rows: small ones are sorted quickly, large ones
+// leave the merge fewer searches per row (one in every other chunk). Forward and
+// backward pass in us (width 768, fp32 below, bf16 from 65536 rows on):
+//   rows          20480   32768   65536   131072   262144 (width 256)
+//   chunk 1024       74      95     129      246      519
+//   chunk 2048       78      92     120      208      366
+//   chunk 4096        -       -     126     189      281
+struct SortPlan {
+  int chunk, chunks;
+  bool wide;  // 64-bit keys
+};
+__host__ inline SortPlan sortPlan(int rows, int vocab) {
+  SortPlan p;
+  p.chunk = rows <= 24 * 1024 ? kSmallChunk : rows <= 96 * 1024 ? kChunk : kLargeChunk;
+  p.chunks = (rows + p.chunk - 1) / p.chunk;
+  p.wide = (int64_t)(vocab + 1ll) * p.chunk >= (1ll << 32);
+  return p;
+}
+
+// What a list of indices is sorted into: the chunks' keys, or with one chunk
+// the sorted indices and their rows (`second`, at the next 16 bytes).
+struct SortList {
+  const int64_t* index;
+  void* first;
+  int* second;
+  int vocab, wide;
+};
+
+// The steps of a bitonic sort from (SIZE, D) on, for E neighbouring keys per
+// thread: steps at a distance inside a thread's keys need no exchange, those
+// inside a warp shuffle, and longer ones go through shared memory. Recursion,
+// not loops: the compiler unrolls only some of the 78 steps of 4096 keys, and
+// the keys then lie in memory (a forward pass of 65536 rows with chunks of 4096:
+// 62 us, 51 like this).
+template <int SIZE, int D, int CHUNK, int E, class Key>
+__device__ __forceinline__ void sortSteps(Key (&k)[E], Key* s) {
+  const int t0 = threadIdx.x * E;
+  if constexpr (D < E) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      if (j & D) continue;
+      const bool up = ((t0 + j) & SIZE) == 0;
+      const Key lo = min(k[j], k[j | D]), hi = max(k[j], k[j | D]);
+      k[j] = up ? lo : hi;
+      k[j | D] = up ? hi : lo;
+    }
+  } else {
+    // The partner of key i is key i ^ D, held by thread ^ (D / E).
+    const bool takeMin = ((t0 & SIZE) == 0) == ((t0 & D) == 0);
+    if constexpr (D >= 32 * E) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < E; ++j) s[j * kThreads + threadIdx.x] = k[j];
+      __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      Key other;
+      if constexpr (D >= 32 * E)
+        other = s[j * kThreads + (threadIdx.x ^ (D / E))];
+      else
+        other = __shfl_xor_sync(0xffffffffu, k[j], D / E);
+      k[j] = takeMin ? min(k[j], other) : max(k[j], other);
+    }
+  }
+  if constexpr (D > 1)
+    sortSteps<SIZE, D / 2, CHUNK>(k, s);
+  else if constexpr (SIZE < CHUNK)
+    sortSteps<2 * SIZE, SIZE, CHUNK>(k, s);
+}
+
+// Sorts one chunk of a list, CHUNK / 256 keys per thread.
+template <class Key, int CHUNK>
+__device__ __noinline__ void sortChunk(const SortList& list, int rows, int chunk, bool one, Key* s) {
+  constexpr int bits = chunkBits<CHUNK>();
+  constexpr int E = CHUNK / kThreads;
+  const int64_t* __restrict__ token = list.index;
+  const int vocab = list.vocab;
+  const int64_t base = (int64_t)chunk * CHUNK;
+  const int t0 = threadIdx.x * E;
+  Key k[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    const int64_t r = base + t0 + j;
+    k[j] = ~(Key)0;
+    if (r < rows) {
+      const int64_t t = token[r];
+      k[j] = ((Key)(t >= 0 && t < vocab ? t : vocab) << bits) | (Key)(t0 + j);
+    }
+  }
+  sortSteps<2, 1, CHUNK>(k, s);
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    const int64_t r = base + t0 + j;
+    if (r >= rows) continue;
+    if (one) {
+      static_cast<int*>(list.first)[r] = (int)(k[j] >> bits);
+      list.second[r] = (int)(k[j] & (CHUNK - 1));
+    } else {
+      static_cast<Key*>(list.first)[r] = k[j];
+    }
+  }
+}
+
+// -- forward -----------------------------------------------------------------------
+
 // A CTA takes `per` rows: their indices first, then the rows' pieces of N
 // columns in turn, so that several loads per thread are in flight whatever the
-// width. Bound by memory: a row of each table read, one written.
+// width. Bound by memory: a row of each table read, one written. With SORT the
+// first CTAs sort the chunks of the lists.
 constexpr int kFwdMaxRows = 16;
-template <class W, class Y, bool FAST, int N>
+struct SortLists {
+  SortList list[2];
+  int lists, chunk, chunks;
+};
+template <class W, class Y, bool FAST, int N, bool SORT>
 __global__ void __launch_bounds__(kThreads, 4)
     embeddingFwd(const int64_t* __restrict__ token, const int64_t* __restrict__ position,
                  const W* __restrict__ w, const W* __restrict__ p, Y* __restrict__ y, int rows,
-                 int seq, int vocab, int context, int cols, float scale, int per) {
+                 int seq, int vocab, int context, int cols, float scale, int per,
+                 const __grid_constant__ SortLists sort) {
+  int cta = blockIdx.x;
+  if (SORT) {
+    __shared__ __align__(16) uint64_t sKeys[kLargeChunk];
+    if (cta < sort.lists * sort.chunks) {
+      const bool second = cta >= sort.chunks, one = sort.chunks == 1;
+      const SortList& list = sort.list[second ? 1 : 0];
+      const int chunk = second ? cta - sort.chunks : cta;
+      auto run = [&](auto* keys) {
+        using Key = std::remove_pointer_t<decltype(keys)>;
+        if (sort.chunk == kSmallChunk)
+          sortChunk<Key, kSmallChunk>(list, rows, chunk, one, keys);
+        else if (sort.chunk == kChunk)
+          sortChunk<Key, kChunk>(list, rows, chunk, one, keys);
+        else
+          sortChunk<Key, kLargeChunk>(list, rows, chunk, one, keys);
+      };
+      if (list.wide)
+        run(sKeys);
+      else
+        run(reinterpret_cast<uint32_t*>(sKeys));
+      return;
+    }
+    cta -= sort.lists * sort.chunks;
+  }
   __shared__ const W* sW[kFwdMaxRows];
   __shared__ const W* sP[kFwdMaxRows];
-  const int64_t first = (int64_t)blockIdx.x * per;
+  const int64_t first = (int64_t)cta * per;
   const int n = (int)min((int64_t)per, rows - first);
   if (threadIdx.x < n) {
     const int64_t r = first + threadIdx.x, t = token[r];
@@ -189,87 +343,7 @@ __global__ void __launch_bounds__(kThreads, 4)
   }
 }
 
-// -- sorting ---------------------------------------------------------------------
-
-// Sort keys are (token << bits | row in the chunk), bits = log2(chunk), so
-// they differ and the order of equal tokens is the rows'. A token outside the
-// table takes the value `vocab`, after all others; padding follows it.
-constexpr int kSmallChunk = 1024, kLargeChunk = 4096;
-constexpr int kSortThreads = 1024;
-
-template <class Key, int CHUNK>
-__device__ __forceinline__ constexpr int chunkBits() {
-  return CHUNK == 1024 ? 10 : 12;
-}
-
-// Bitonic sort of CHUNK keys, CHUNK / 1024 neighbouring ones per thread: steps
-// at a distance inside a thread's keys need no exchange, those inside a warp
-// shuffle, and only the 15 at longer distances go through shared memory. With
-// one chunk the result goes straight to `skey` / `perm`.
-template <class Key, int CHUNK>
-__global__ void __launch_bounds__(kSortThreads)
-    sortChunks(const int64_t* __restrict__ token, Key* __restrict__ sorted,
-               int* __restrict__ skey, int* __restrict__ perm, int rows, int vocab) {
-  constexpr int bits = chunkBits<Key, CHUNK>();
-  constexpr int E = CHUNK / kSortThreads;
-  __shared__ Key s[CHUNK];
-  const int64_t base = (int64_t)blockIdx.x * CHUNK;
-  const int t0 = threadIdx.x * E;
-  Key k[E];
-#pragma unroll
-  for (int j = 0; j < E; ++j) {
-    const int64_t r = base + t0 + j;
-    k[j] = ~(Key)0;
-    if (r < rows) {
-      const int64_t t = token[r];
-      k[j] = ((Key)(t >= 0 && t < vocab ? t : vocab) << bits) | (Key)(t0 + j);
-    }
-  }
-#pragma unroll
-  for (int size = 2; size <= CHUNK; size <<= 1) {
-#pragma unroll
-    for (int d = size >> 1; d > 0; d >>= 1) {
-      if (d < E) {
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-          if (j & d) continue;
-          const bool up = ((t0 + j) & size) == 0;
-          const Key a = k[j], b = k[j | d];
-          const bool swap = (a > b) == up;
-          k[j] = swap ? b : a;
-          k[j | d] = swap ? a : b;
-        }
-      } else {
-        // The partner of key i is key i ^ d, held by thread ^ (d / E).
-        const bool up = (t0 & size) == 0, low = (t0 & d) == 0;
-        if (d >= 32 * E) {
-          __syncthreads();
-#pragma unroll
-          for (int j = 0; j < E; ++j) s[t0 + j] = k[j];
-          __syncthreads();
-        }
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-          const Key other = d >= 32 * E ? s[(t0 + j) ^ d]
-                                        : __shfl_xor_sync(0xffffffffu, k[j], (d / E) & 31);
-          const bool takeMin = low == up;
-          k[j] = (other < k[j]) == takeMin ? other : k[j];
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < E; ++j) {
-    const int64_t r = base + t0 + j;
-    if (r >= rows) continue;
-    if (gridDim.x == 1) {
-      skey[r] = (int)(k[j] >> bits);
-      perm[r] = (int)(k[j] & (CHUNK - 1));
-    } else {
-      sorted[r] = k[j];
-    }
-  }
-}
+// -- merging -----------------------------------------------------------------------
 
 // Several chunks at a time in shared memory (128 KiB), one search in each
 // going on side by side.
@@ -282,7 +356,7 @@ __global__ void __launch_bounds__(kMergeThreads)
                int rows) {
   extern __shared__ __align__(16) uint8_t smem[];
   Key* s = reinterpret_cast<Key*>(smem);
-  constexpr int bits = chunkBits<Key, CHUNK>();
+  constexpr int bits = chunkBits<CHUNK>();
   constexpr int at1 = kMergeSmem / (CHUNK * sizeof(Key));  // chunks at a time
   constexpr int side = 4;                                  // searches side by side
   const int64_t at = (int64_t)blockIdx.x * kMergeThreads + threadIdx.x;  // CHUNK % 512 == 0
@@ -296,7 +370,7 @@ __global__ void __launch_bounds__(kMergeThreads)
     const int64_t from = (int64_t)c0 * CHUNK;
     const int n = (int)min((int64_t)at1 * CHUNK, rows - from);
     __syncthreads();
-    // 16-byte pieces; the last may run past n, into scratch that follows.
+    // 16-byte pieces; the last may run past n, within the rounded-up buffer.
     for (int i = threadIdx.x; i < (int)((n * sizeof(Key) + 15) / 16); i += kMergeThreads)
       reinterpret_cast<uint4*>(smem)[i] =
           __ldg(reinterpret_cast<const uint4*>(sorted + from) + i);
@@ -574,28 +648,28 @@ bool pieces(const void* p, int valueBytes, int cols, int n) {
 
 template <class W, class Y>
 int fwd(const int64_t* token, const int64_t* position, const void* w, const void* p, void* y,
-        int rows, int seq, int vocab, int context, int cols, float scale, cudaStream_t stream) {
+        int rows, int seq, int vocab, int context, int cols, float scale, const SortLists& sort,
+        cudaStream_t stream) {
   constexpr int N = 16 / sizeof(W);  // 16-byte loads
   const bool fast = pieces(w, sizeof(W), cols, N) && pieces(p, sizeof(W), cols, N) &&
                     pieces(y, sizeof(Y), cols, N);
   // Few rows spread over the SMs; many take 16 to a CTA.
   int per = (rows + kSMs * 4 - 1) / (kSMs * 4);
   if (per > kFwdMaxRows) per = kFwdMaxRows;
-  auto kernel = fast ? embeddingFwd<W, Y, true, N> : embeddingFwd<W, Y, false, 4>;
-  kernel<<<(unsigned)((rows + per - 1) / per), kThreads, 0, stream>>>(
-      token, position, static_cast<const W*>(w), static_cast<const W*>(p), static_cast<Y*>(y),
-      rows, seq, vocab, context, cols, scale, per);
+  auto kernel = sort.lists == 0 ? (fast ? embeddingFwd<W, Y, true, N, false>
+                                        : embeddingFwd<W, Y, false, 4, false>)
+                                : (fast ? embeddingFwd<W, Y, true, N, true>
+                                        : embeddingFwd<W, Y, false, 4, true>);
+  const unsigned ctas = (unsigned)((rows + per - 1) / per) + (unsigned)(sort.lists * sort.chunks);
+  kernel<<<ctas, kThreads, 0, stream>>>(token, position, static_cast<const W*>(w),
+                                        static_cast<const W*>(p), static_cast<Y*>(y), rows, seq,
+                                        vocab, context, cols, scale, per, sort);
   return launched(cudaGetLastError());
 }
 
 template <class Key, int CHUNK>
-int sortTokens(const int64_t* token, void* sorted, int* skey, int* perm, int rows, int vocab,
-               cudaStream_t stream) {
-  const int chunks = (rows + CHUNK - 1) / CHUNK;
-  sortChunks<Key, CHUNK><<<chunks, kSortThreads, 0, stream>>>(token, static_cast<Key*>(sorted),
-                                                              skey, perm, rows, vocab);
-  if (int rc = launched(cudaGetLastError())) return rc;
-  if (chunks == 1) return 0;
+int mergeChunks(const void* sorted, int* skey, int* perm, int rows, int chunks,
+                cudaStream_t stream) {
   auto merge = mergeRanks<Key, CHUNK>;
   static std::atomic<uint64_t> done{0};  // devices (bit d) with the shared memory opted in
   int dev = 0;
@@ -606,27 +680,22 @@ int sortTokens(const int64_t* token, void* sorted, int* skey, int* perm, int row
     if (e != cudaSuccess) return (int)e;
     done.fetch_or(1ull << dev, std::memory_order_acq_rel);
   }
-  const uint32_t bytes = (uint32_t)chunks * CHUNK * sizeof(Key);
+  const uint64_t bytes = (uint64_t)chunks * CHUNK * sizeof(Key);
   merge<<<(rows + kMergeThreads - 1) / kMergeThreads, kMergeThreads,
           bytes < kMergeSmem ? bytes : kMergeSmem, stream>>>(static_cast<const Key*>(sorted), skey,
                                                             perm, rows);
   return launched(cudaGetLastError());
 }
-// Chunks of 1024 up to 16384 rows (the sort's one CTA per chunk is what takes
-// the time), of 4096 above (there each row's searches do, one per chunk: 65536
-// rows take 13 + 12 us to sort and merge in chunks of 4096, 4 + 27 in chunks of
-// 1024). Keys
-// take 32 bits where token and place in the chunk fit.
-int sortTokens(const int64_t* token, void* sorted, int* skey, int* perm, int rows, int vocab,
-               cudaStream_t stream) {
-  if (rows <= 16 * kSmallChunk) {
-    if (vocab < (1 << 22) - 1)
-      return sortTokens<uint32_t, kSmallChunk>(token, sorted, skey, perm, rows, vocab, stream);
-    return sortTokens<uint64_t, kSmallChunk>(token, sorted, skey, perm, rows, vocab, stream);
-  }
-  if (vocab < (1 << 20) - 1)
-    return sortTokens<uint32_t, kLargeChunk>(token, sorted, skey, perm, rows, vocab, stream);
-  return sortTokens<uint64_t, kLargeChunk>(token, sorted, skey, perm, rows, vocab, stream);
+int mergeChunks(const SortPlan& p, const void* sorted, int* skey, int* perm, int rows,
+                cudaStream_t stream) {
+  auto pick = [&](auto key) {
+    using Key = decltype(key);
+    return p.chunk == kSmallChunk ? mergeChunks<Key, kSmallChunk>
+           : p.chunk == kChunk    ? mergeChunks<Key, kChunk>
+                                  : mergeChunks<Key, kLargeChunk>;
+  };
+  auto f = p.wide ? pick(uint64_t{}) : pick(uint32_t{});
+  return f(sorted, skey, perm, rows, p.chunks, stream);
 }
 
 // Sorted rows per block: 16, or 32 where there are many rows (half the partial
@@ -679,9 +748,12 @@ int tableGradients(const void* g, const TableGradArgs& args, cudaStream_t stream
   return launched(cudaGetLastError());
 }
 
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+constexpr int64_t kMostRows = INT32_MAX - kLargeChunk;
+
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
-// Scratch of one table: sort keys, sorted keys and rows, partial sums.
-size_t sortBytes(int64_t rows) { return round16(8 * rows) + 2 * round16(4 * rows); }
+// Scratch of one table: sorted keys and their rows, partial sums.
+size_t sortBytes(int64_t rows) { return 2 * round16(4 * rows); }
 size_t partialBytes(int64_t rows, int cols) {
   return round16(sizeof(float) * 2 * ((rows + 15) / 16) * cols);
 }
@@ -691,58 +763,84 @@ size_t partialBytes(int64_t rows, int cols) {
 
 using namespace tnops;
 
+extern "C" size_t tnops_embedding_order_bytes(int64_t rows, int size) {
+  if (rows <= 0 || rows > kMostRows || size <= 0 || size == INT32_MAX) return 0;
+  const SortPlan p = sortPlan((int)rows, size);
+  return p.chunks == 1 ? 2 * round16(4 * rows) : round16((p.wide ? 8 : 4) * rows);
+}
+
 extern "C" int tnops_embedding_fwd(const int64_t* token, const int64_t* position, const void* w,
                                    const void* p, int w_f32, void* y, int y_f32, int64_t rows,
                                    int seq, int vocab, int context, int cols, float scale,
-                                   cudaStream_t stream) {
-  if (rows <= 0 || rows > INT32_MAX || seq <= 0 || vocab <= 0 || cols <= 0 || (p && context <= 0))
+                                   void* token_order, void* position_order, cudaStream_t stream) {
+  if (rows <= 0 || rows > kMostRows || seq <= 0 || vocab <= 0 || cols <= 0 ||
+      (p && context <= 0) || (token_order && vocab == INT32_MAX) || !aligned16(token_order) ||
+      (position_order && (!position || context <= 0 || context == INT32_MAX)) ||
+      !aligned16(position_order))
     return 1;
+  SortLists sort{};
+  auto add = [&](const int64_t* index, void* order, int size) {
+    if (order == nullptr) return;
+    const SortPlan plan = sortPlan((int)rows, size);
+    sort.chunk = plan.chunk;
+    sort.chunks = plan.chunks;
+    sort.list[sort.lists++] = {
+        index, order, reinterpret_cast<int*>(static_cast<char*>(order) + round16(4 * rows)), size,
+        plan.wide};
+  };
+  add(token, token_order, vocab);
+  add(position, position_order, context);
   auto f = w_f32 ? (y_f32 ? fwd<float, float> : fwd<float, uint16_t>)
                  : (y_f32 ? fwd<uint16_t, float> : fwd<uint16_t, uint16_t>);
-  return f(token, position, w, p, y, (int)rows, seq, vocab, context, cols, scale, stream);
+  return f(token, position, w, p, y, (int)rows, seq, vocab, context, cols, scale, sort, stream);
 }
 
 extern "C" size_t tnops_embedding_grad_scratch(int64_t rows, int cols, int tables) {
   return rows <= 0 || cols <= 0 ? 0 : tables * (sortBytes(rows) + partialBytes(rows, cols));
 }
 
-extern "C" int tnops_embedding_grad(const void* g, int g_f32, const int64_t* token, void* dw,
-                                    int vocab, float scale, const int64_t* position, int seq,
+extern "C" int tnops_embedding_grad(const void* g, int g_f32, const void* token_order, void* dw,
+                                    int vocab, float scale, const void* position_order, int seq,
                                     void* dp, int context, int d_f32, int64_t rows, int cols,
                                     void* scratch, cudaStream_t stream) {
-  if (rows <= 0 || rows > INT32_MAX - kLargeChunk || cols <= 0 || (!dw && !dp) ||
-      (dw && (!token || vocab <= 0 || vocab == INT32_MAX)) ||
-      (dp && (context <= 0 || context == INT32_MAX || (!position && (seq <= 0 || rows % seq)))) ||
-      scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 15))
+  if (rows <= 0 || rows > kMostRows || cols <= 0 || (!dw && !dp) ||
+      (dw && (!token_order || vocab <= 0 || vocab == INT32_MAX)) || !aligned16(token_order) ||
+      (dp && (context <= 0 || context == INT32_MAX ||
+              (!position_order && (seq <= 0 || rows % seq)))) ||
+      !aligned16(position_order) || scratch == nullptr || !aligned16(scratch))
     return 1;
   TableGradArgs a{};
   a.rows = (int)rows;
   a.cols = cols;
   char* at = static_cast<char*>(scratch);
-  auto add = [&](const int64_t* index, void* out, int n, float s) {
+  auto add = [&](const void* order, void* out, int n, float s) {
     Table& t = a.table[a.tables++];
     t.out = out;
     t.vocab = n;
     t.scale = s;
     t.seq = seq;
-    t.batch = index ? 1 : (int)(rows / seq);
+    t.batch = order ? 1 : (int)(rows / seq);
     t.partial = reinterpret_cast<float*>(at);
     at += partialBytes(rows, cols);
-    if (index == nullptr) return 0;
-    void* sorted = at;
-    at += round16(8 * rows);
+    if (order == nullptr) return 0;
+    const SortPlan plan = sortPlan((int)rows, n);
+    if (plan.chunks == 1) {
+      t.skey = static_cast<const int*>(order);
+      t.perm = reinterpret_cast<const int*>(static_cast<const char*>(order) + round16(4 * rows));
+      return 0;
+    }
     int* skey = reinterpret_cast<int*>(at);
     at += round16(4 * rows);
     int* perm = reinterpret_cast<int*>(at);
     at += round16(4 * rows);
     t.skey = skey;
     t.perm = perm;
-    return sortTokens(index, sorted, skey, perm, (int)rows, n, stream);
+    return mergeChunks(plan, order, skey, perm, (int)rows, stream);
   };
   if (dw)
-    if (int rc = add(token, dw, vocab, scale)) return rc;
+    if (int rc = add(token_order, dw, vocab, scale)) return rc;
   if (dp)
-    if (int rc = add(position, dp, context, 1.0f)) return rc;
+    if (int rc = add(position_order, dp, context, 1.0f)) return rc;
   auto f = g_f32 ? (d_f32 ? tableGradients<float, float> : tableGradients<float, uint16_t>)
                  : (d_f32 ? tableGradients<uint16_t, float> : tableGradients<uint16_t, uint16_t>);
   return f(g, a, stream);

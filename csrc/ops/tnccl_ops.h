@@ -151,20 +151,26 @@ int tnops_linear_ce_bwd(const void* x, const void* w, const int64_t* target, con
 // for w [vocab, cols] and p [context, cols] (both fp32 with w_f32, else bf16;
 // p may be null), y [rows, cols] (fp32 with y_f32, else bf16). A null
 // `position` stands for r % seq. An index outside its table adds nothing.
+// token_order and position_order (or null): for the gradient of w and, where
+// positions are given, of p; tnops_embedding_order_bytes(rows, vocab or
+// context) bytes each, 16-byte aligned.
+size_t tnops_embedding_order_bytes(int64_t rows, int size);
 int tnops_embedding_fwd(const int64_t* token, const int64_t* position, const void* w,
                         const void* p, int w_f32, void* y, int y_f32, int64_t rows, int seq,
-                        int vocab, int context, int cols, float scale, cudaStream_t stream);
+                        int vocab, int context, int cols, float scale, void* token_order,
+                        void* position_order, cudaStream_t stream);
 // Gradients of the tables for g [rows, cols] (fp32 with g_f32, else bf16), dw
 // and dp of one type (fp32 with d_f32, else bf16); a null dw or dp is left
 // out. dw[v] = scale * the sum of g[r] over the rows with token[r] = v, for
 // every v (rows without a token: zero); dp alike over positions, without the
-// scale (a null `position` stands for r % seq; rows must then be a multiple of
-// seq). Bit-identical from run to run. scratch: 16-byte aligned,
+// scale (a null position_order stands for r % seq; rows must then be a multiple
+// of seq). The orders are the forward pass's, of the same rows and table sizes;
+// they are only read. Bit-identical from run to run. scratch: 16-byte aligned,
 // tnops_embedding_grad_scratch(rows, cols, 1 or 2 tables) bytes. Returns 1
 // (invalid argument) without a launch for anything else.
 size_t tnops_embedding_grad_scratch(int64_t rows, int cols, int tables);
-int tnops_embedding_grad(const void* g, int g_f32, const int64_t* token, void* dw, int vocab,
-                         float scale, const int64_t* position, int seq, void* dp, int context,
+int tnops_embedding_grad(const void* g, int g_f32, const void* token_order, void* dw, int vocab,
+                         float scale, const void* position_order, int seq, void* dp, int context,
                          int d_f32, int64_t rows, int cols, void* scratch, cudaStream_t stream);
 
 // x [rows, cols] (fp32 with x_f32, else bf16) in 8-bit blocks: q [rows, cols]

@@ -55,8 +55,11 @@ uint8_t* bytes(const at::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr())
 
 // -- embedding -----------------------------------------------------------------
 
+// orderW and orderP (or null) receive what the gradients of w and p need to
+// know of token and position.
 at::Tensor embeddingFwd(const at::Tensor& token, const Opt& position, const at::Tensor& w,
-                        const Opt& p, int64_t seq, double scale, bool outF32) {
+                        const Opt& p, int64_t seq, double scale, bool outF32,
+                        at::Tensor* orderW = nullptr, at::Tensor* orderP = nullptr) {
   need(token, at::kLong, "idx");
   need(w, "weight");
   TORCH_CHECK(w.dim() == 2, "weight must be [vocab, width]");
@@ -76,33 +79,35 @@ at::Tensor embeddingFwd(const at::Tensor& token, const Opt& position, const at::
   const int64_t rows = token.numel();
   auto y = at::empty({rows, w.size(1)}, w.options().dtype(outF32 ? at::kFloat : at::kBFloat16));
   if (y.numel() == 0) return y;
+  auto order = [&](at::Tensor* out, const at::Tensor& table) -> void* {
+    if (out == nullptr) return nullptr;
+    *out = scratchOf(tnops_embedding_order_bytes(rows, asInt(table.size(0), "table size")), w);
+    TORCH_CHECK(out->defined(), "embedding: too many rows, or a table without rows");
+    return out->data_ptr();
+  };
+  void* tokenOrder = order(orderW, w);
+  void* positionOrder = p && position ? order(orderP, *p) : nullptr;
   ok(tnops_embedding_fwd(token.data_ptr<int64_t>(),
                          position ? position->data_ptr<int64_t>() : nullptr, w.data_ptr(),
                          p ? p->data_ptr() : nullptr, wF32, y.data_ptr(), outF32 ? 1 : 0, rows,
                          asInt(seq, "sequence length"), asInt(w.size(0), "vocabulary"),
                          p ? asInt(p->size(0), "context") : 0, asInt(w.size(1), "width"),
-                         (float)scale, streamOf(token)),
+                         (float)scale, tokenOrder, positionOrder, streamOf(token)),
      "tnops_embedding_fwd");
   return y;
 }
 
-// grad [rows, width]; token and position (or none for row % seq) [rows] -> the
-// gradients of the [vocab, width] and [context, width] tables; one with no
-// rows (vocab or context 0) is left out.
-std::vector<at::Tensor> embeddingGrad(const at::Tensor& grad, const at::Tensor& token,
-                                      const Opt& position, int64_t seq, int64_t vocab,
-                                      int64_t context, double scale, bool outF32, const Opt& dwOut,
+// grad [rows, width]; the forward pass's orders of token and position
+// (undefined for row % seq) -> the gradients of the [vocab, width] and
+// [context, width] tables; one with no rows (vocab or context 0) is left out.
+std::vector<at::Tensor> embeddingGrad(const at::Tensor& grad, const at::Tensor& tokenOrder,
+                                      const at::Tensor& positionOrder, int64_t seq,
+                                      int64_t vocab, int64_t context, double scale, bool outF32, const Opt& dwOut,
                                       const Opt& dpOut) {
   need(grad, "grad");
   TORCH_CHECK(grad.dim() == 2, "embedding_grad: want grad [rows, width]");
   const int gF32 = f32(grad, "grad");
   const int64_t rows = grad.size(0), width = grad.size(1);
-  for (const at::Tensor* t : {&token, position ? &*position : nullptr}) {
-    if (t == nullptr) continue;
-    need(*t, at::kLong, "an index");
-    TORCH_CHECK(t->numel() == rows, "embedding_grad: one index per row of grad");
-    sameDevice(grad, *t, "an index");
-  }
   TORCH_CHECK(seq > 0 ? rows % seq == 0 : rows == 0, "embedding_grad: rows must be whole sequences");
   c10::cuda::CUDAGuard g(grad.device());
   const auto opt = grad.options().dtype(outF32 ? at::kFloat : at::kBFloat16);
@@ -121,12 +126,10 @@ std::vector<at::Tensor> embeddingGrad(const at::Tensor& grad, const at::Tensor& 
   auto scratch = at::empty(
       {(int64_t)tnops_embedding_grad_scratch(rows, cols, (vocab > 0) + (context > 0))},
       grad.options().dtype(at::kByte));
-  ok(tnops_embedding_grad(grad.data_ptr(), gF32, token.data_ptr<int64_t>(),
-                          dw.defined() ? dw.data_ptr() : nullptr, asInt(vocab, "vocabulary"),
-                          (float)scale, position ? position->data_ptr<int64_t>() : nullptr,
-                          asInt(seq, "sequence length"), dp.defined() ? dp.data_ptr() : nullptr,
-                          asInt(context, "context"), outF32 ? 1 : 0, rows, cols,
-                          scratch.data_ptr(), streamOf(grad)),
+  ok(tnops_embedding_grad(grad.data_ptr(), gF32, orNull(tokenOrder), orNull(dw),
+                          asInt(vocab, "vocabulary"), (float)scale, orNull(positionOrder),
+                          asInt(seq, "sequence length"), orNull(dp), asInt(context, "context"),
+                          outF32 ? 1 : 0, rows, cols, scratch.data_ptr(), streamOf(grad)),
      "tnops_embedding_grad");
   return {dw, dp};
 }
@@ -442,7 +445,6 @@ struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& w, const Opt& p,
                             const at::Tensor& idx, const Opt& positions, int64_t seq, double scale,
                             bool outF32, bool dwDest, bool dpDest) {
-    ctx->save_for_backward({idx, positions ? *positions : at::Tensor()});
     // The parameters themselves, for what their gradients look like: their
     // values are not needed, so they may change before the backward pass.
     ctx->saved_data["w"] = w;
@@ -451,7 +453,12 @@ struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["dw"] = dwDest;
     ctx->saved_data["dp"] = dpDest;
-    return embeddingFwd(idx, positions, w, p, seq, scale, outF32);
+    at::Tensor orderW, orderP;
+    auto y = embeddingFwd(idx, positions, w, p, seq, scale, outF32,
+                          w.requires_grad() ? &orderW : nullptr,
+                          p && p->requires_grad() ? &orderP : nullptr);
+    ctx->save_for_backward({orderW, orderP});
+    return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     onceDifferentiable("embedding");
@@ -462,7 +469,7 @@ struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
     const auto st = w.scalar_type();
     const auto g = grads[0].contiguous();
     const auto d = embeddingGrad(
-        g, saved[0], saved[1].defined() ? Opt(saved[1]) : Opt(), ctx->saved_data["seq"].toInt(),
+        g, saved[0], saved[1], ctx->saved_data["seq"].toInt(),
         wantW ? w.size(0) : 0, wantP ? p->size(0) : 0, ctx->saved_data["scale"].toDouble(),
         st == at::kFloat, wantW ? destination(w, ctx->saved_data["dw"].toBool(), st) : Opt(),
         wantP ? destination(*p, ctx->saved_data["dp"].toBool(), st) : Opt());

@@ -64,13 +64,14 @@ def test_linear_ce_launchers_refuse(built):
 
 
 def test_embedding_launchers_refuse(built):
-    f = _launcher("tnops_embedding_fwd", P, P, P, P, I, P, I, L, I, I, I, I, F, P)
-    good = [A, None, A, A, 1, A, 1, 8, 4, 100, 16, 64, 1.0, None]
-    _refuses(f, good, [(7, 0), (7, 1 << 31), (8, 0), (9, 0), (10, 0), (11, 0)])
+    f = _launcher("tnops_embedding_fwd", P, P, P, P, I, P, I, L, I, I, I, I, F, P, P, P)
+    good = [A, None, A, A, 1, A, 1, 8, 4, 100, 16, 64, 1.0, A, None, None]
+    _refuses(f, good, [(7, 0), (7, 1 << 31), (8, 0), (9, 0), (10, 0), (11, 0), (13, A + 8),
+                       (9, (1 << 31) - 1), (14, A)])  # an order of positions that are not given
     f = _launcher("tnops_embedding_grad", P, I, P, P, I, F, P, I, P, I, I, L, I, P, P)
     good = [A, 1, A, A, 100, 1.0, None, 4, A, 50, 1, 8, 64, A, None]
     _refuses(f, good, [(2, None), (4, 0), (7, 0), (7, 3), (9, 0), (11, 0), (11, 1 << 31),
-                       (12, 0), (13, None), (13, A + 8)])
+                       (12, 0), (13, None), (13, A + 8), (2, A + 8), (6, A + 8)])
     assert f(A, 1, A, None, 100, 1.0, None, 4, None, 50, 1, 8, 64, A, None) == 1
 
 
@@ -78,9 +79,22 @@ def test_embedding_scratch_grows_with_its_parts(built):
     f = _launcher("tnops_embedding_grad_scratch", L, I, I)
     f.restype = ctypes.c_size_t
     assert f(0, 64, 2) == 0 and f(1, 1, 1) % 16 == 0
-    # Sort keys and rows of 16 bytes a row, and two rows of fp32 partial sums
-    # for each 16 rows.
-    assert f(65536, 1024, 2) == 2 * (16 * 65536 + 8 * 4096 * 1024)
+    # Sorted keys and their rows, 8 bytes a row, and two rows of fp32 partial
+    # sums for each 16 rows.
+    assert f(65536, 1024, 2) == 2 * (8 * 65536 + 8 * 4096 * 1024)
+
+
+def test_embedding_order_bytes(built):
+    """One chunk: sorted indices and rows; more: a key per row, of 64 bits where
+    index and place do not fit 32."""
+    f = _launcher("tnops_embedding_order_bytes", L, I)
+    f.restype = ctypes.c_size_t
+    assert [f(n, 50304) for n in (0, 1, 1023, 1024, 1025, 16384, 16385, 1 << 31)] == [
+        0, 32, 2 * 4096, 2 * 4096, 4112, 65536, 65552, 0]
+    assert f(2000, (1 << 22) - 2) == 8000 and f(2000, (1 << 22) - 1) == 16000
+    assert f(30000, (1 << 21) - 2) == 120000 and f(30000, (1 << 21) - 1) == 240000
+    assert f(100000, (1 << 20) - 2) == 400000 and f(100000, (1 << 20) - 1) == 800000
+    assert f(20000, 0) == 0 and f(20000, (1 << 31) - 1) == 0
 
 
 def test_int8_launchers_refuse(built):

@@ -80,6 +80,9 @@ def _embedding_sums(idx, gy, vocab, scale):
     (33, 2048, 70000, 2048, 36, False, ""),  # many chunks of the sort
     (3, 700, 4200000, 700, 4, True, ""),     # 64-bit sort keys
     (17, 1024, 1050000, 1024, 4, False, "few"),
+    (30, 1000, 2100000, 1000, 4, True, ""),  # chunks of 2048, one list's keys of 64 bits
+    (101, 1000, 1050000, 1000, 4, True, "few"),  # chunks of 4096
+    (101, 1000, 5000, 1000, 12, True, ""),
     (16, 4096, 11, 4096, 40, False, "one"),  # a run of thousands of blocks
 ])
 def test_embedding(ops, dtype, batch, seq, vocab, context, width, positions, repeat):
