@@ -91,8 +91,9 @@ struct StatsEpi {
 #pragma unroll
     for (int i = 4; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], v[i]);
     const float m = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), st.m);
-    if (m == -INFINITY) return;
-    const float nm = -m * kLog2e;
+    // fmaxf passes over NaNs: with none but those and -inf so far the maximum is
+    // -inf, and the sum is taken all the same, from 0, so that a NaN stays in it.
+    const float nm = m == -INFINITY ? 0.f : -m * kLog2e;
     const uint64_t scale = pack2(kLog2e, kLog2e), shift = pack2(nm, nm);
     uint64_t s[4] = {pack2(st.s * ex2Approx(fmaf(st.m, kLog2e, nm)), 0.f), 0ull, 0ull, 0ull};
 #pragma unroll

@@ -1,0 +1,74 @@
+"""The training operators at their edges: values that are no number, logits of
+hundreds, forward-mode differentiation, parameters that are frozen, very many
+rows, and the 8-bit sums of the fused GELU bit by bit.
+
+As in test_train_ops_gpu.py, tolerances count roundings: half a step is eps / 2
+of a type relative to the value (bf16 2^-8, fp32 2^-24).
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = 2.0 ** -8, 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def ops(built):
+    import tiny_nccl_b200.ops as o
+    return o
+
+
+def _normal(*shape, seed, std=1.0, dtype=torch.float32):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (std * torch.randn(*shape, device="cuda", generator=g)).to(dtype)
+
+
+# -- cross-entropy: values that are no number ---------------------------------------
+
+
+@pytest.mark.parametrize("first,count,classes", [
+    (0, 32, 300),     # a whole block of 32 classes, the first of its 128
+    (128, 32, 300),
+    (128, 128, 400),  # all 128
+    (128, 1, 129),    # the only class of its block
+    (256, 1, 257),    # ... and of its tile
+    (5, 1, 300),
+    (32, 32, 300),
+])
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+def test_nan_logits_reach_the_loss(ops, first, count, classes, reduction):
+    """A class whose logits are NaN makes every loss that counts NaN, wherever
+    the class stands; a row that does not count stays 0."""
+    x, w = _normal(20, 64, seed=1, dtype=torch.bfloat16), _normal(classes, 64, seed=2, std=0.2)
+    w[first:first + count] = float("nan")
+    target = torch.full((20,), 100, device="cuda")  # a class that is a number
+    target[3] = -100
+    with torch.no_grad():
+        loss = ops.linear_cross_entropy(x, w, target, reduction=reduction)
+    if reduction == "mean":
+        assert bool(loss.isnan())
+    else:
+        counts = target >= 0
+        assert bool(loss[counts].isnan().all()) and bool((loss[~counts] == 0).all())
+
+
+@pytest.mark.parametrize("first,count,classes", [(0, 32, 300), (128, 128, 400), (256, 1, 257),
+                                                 (0, 299, 300)])
+def test_classes_at_minus_infinity_are_absent(ops, first, count, classes):
+    """Logits of -inf add nothing: the losses are those of the other classes,
+    bit for bit where their blocks are the same."""
+    x, w = _normal(20, 64, seed=1, dtype=torch.bfloat16), _normal(classes, 64, seed=2, std=0.2)
+    x[:, 0] = 1.0
+    w[first:first + count, 0] = float("-inf")
+    keep = torch.ones(classes, dtype=torch.bool, device="cuda")
+    keep[first:first + count] = False
+    target = torch.full((20,), int(keep.nonzero()[-1]), device="cuda")
+    with torch.no_grad():
+        loss = ops.linear_cross_entropy(x, w, target, reduction="none")
+    logits = x.double() @ w[keep].to(torch.bfloat16).double().t()
+    want = torch.logsumexp(logits, 1) - logits[:, int(keep[:target[0]].sum())]
+    # 64 fp32 products and sums a logit, ex2's and the sums' 2^-20.
+    size = x.double().abs() @ w[keep].to(torch.bfloat16).double().abs().t()
+    off = 2 * 65 * F32 * size.amax(1) + 2.0 ** -20 + 4 * F32 * logits.abs().amax(1)
+    assert bool(((loss.double() - want).abs() <= off).all())
