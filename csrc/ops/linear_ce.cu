@@ -71,8 +71,12 @@ struct StatsEpi {
   __device__ __forceinline__ State begin(int row) const {
     return {-INFINITY, 0.f, row < rows ? target[row] : -1};
   }
-  // 32 logits: their maximum, then one packed FMA for two, one ex2 for each
-  // and one packed addition for two.
+  // 32 logits: their maximum, then its difference to two of them and that times
+  // log2 e in one packed instruction each, one ex2 for each and one packed
+  // addition for two. The difference comes first: it is exact where it counts,
+  // the largest logit adds exactly 1 and an unchanged maximum leaves the sum as
+  // it is, so that lse is never below a logit. (One FMA with -maximum log2 e
+  // scales every term by that product's rounding, up to 2^-14 of them at logits of 1000.)
   __device__ __forceinline__ int ahead(int) const { return 0; }
   __device__ __forceinline__ void chunk(State& st, const float (&in)[32], int, int row,
                                         int col0) const {
@@ -93,13 +97,13 @@ struct StatsEpi {
     const float m = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), st.m);
     // fmaxf passes over NaNs: with none but those and -inf so far the maximum is
     // -inf, and the sum is taken all the same, from 0, so that a NaN stays in it.
-    const float nm = m == -INFINITY ? 0.f : -m * kLog2e;
+    const float nm = m == -INFINITY ? 0.f : -m;
     const uint64_t scale = pack2(kLog2e, kLog2e), shift = pack2(nm, nm);
-    uint64_t s[4] = {pack2(st.s * ex2Approx(fmaf(st.m, kLog2e, nm)), 0.f), 0ull, 0ull, 0ull};
+    uint64_t s[4] = {pack2(st.s * ex2Approx((st.m + nm) * kLog2e), 0.f), 0ull, 0ull, 0ull};
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float a, b;
-      unpack2(fma2(pack2(v[2 * i], v[2 * i + 1]), scale, shift), a, b);
+      unpack2(mul2(add2(pack2(v[2 * i], v[2 * i + 1]), shift), scale), a, b);
       s[i & 3] = add2(s[i & 3], pack2(ex2Approx(a), ex2Approx(b)));
     }
     float a, b;
@@ -121,9 +125,12 @@ struct SoftmaxGradEpi {
   int ld, rows, classes, first, width;
 
   // |k| exp(l - lse) = 2^(l log2e + nb) with nb = log2 |k| - lse log2e: the
-  // factor costs nothing per logit; k's sign goes on the packed results.
+  // factor costs nothing per logit; k's sign goes on the packed results. The
+  // rounding of nb scales a row's d by up to 2^-14 at logits of 1000, less than
+  // bf16's 2^-8, but p - 1 of a sure row would be all error: the target's own
+  // takes the difference first.
   struct State {
-    float nb, nl, k;      // nl = -lse log2e
+    float nb, lse, k;
     int at;               // the target's column in this piece (any other value: none)
     uint32_t keep, sign;  // masks of a pair of bf16: all or nothing, k's sign
   };
@@ -133,8 +140,9 @@ struct SoftmaxGradEpi {
       const int64_t t = target[row];
       if (t >= 0 && t < classes) {
         st.k = grad != nullptr ? grad[row] : 1.f;
-        st.nl = -lse[row] * kLog2e;
-        st.nb = grad != nullptr ? st.nl + log2f(fabsf(st.k)) : st.nl;
+        st.lse = lse[row];
+        st.nb = -st.lse * kLog2e;
+        if (grad != nullptr) st.nb += log2f(fabsf(st.k));
         st.at = (int)(t - first);
         st.keep = 0xffffffffu;
         st.sign = st.k < 0.f ? 0x80008000u : 0u;
@@ -159,7 +167,7 @@ struct SoftmaxGradEpi {
     if (at >= 0 && at < 32) {
       // The target's own: k (p - 1), rounded once.
       const float l = valueAt(v, at);
-      const float d = st.k * (ex2Approx(fmaf(l, kLog2e, st.nl)) - 1.f);
+      const float d = st.k * (ex2Approx((l - st.lse) * kLog2e) - 1.f);
       putBf16(w, at, f2bf(d));
     }
     // Whole: d's rows are `ld` apart, a multiple of 32 at or past the width.

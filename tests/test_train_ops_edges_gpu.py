@@ -72,3 +72,37 @@ def test_classes_at_minus_infinity_are_absent(ops, first, count, classes):
     size = x.double().abs() @ w[keep].to(torch.bfloat16).double().abs().t()
     off = 2 * 65 * F32 * size.amax(1) + 2.0 ** -20 + 4 * F32 * logits.abs().amax(1)
     assert bool(((loss.double() - want).abs() <= off).all())
+
+
+# -- cross-entropy: rows that are sure ------------------------------------------------
+
+
+@pytest.mark.parametrize("at", [0, 31, 32, 127, 130, 299])
+def test_sure_rows_have_no_loss_and_no_gradient(ops, at):
+    """Logits in the hundreds that fp32 holds exactly, the target's above all
+    others by more than exp's range: the softmax is exactly the target's, so
+    that loss and gradients are exactly 0, not a rounding of the logits (lse's
+    half step is 3e-5 at 1000)."""
+    a = torch.arange(129, 256, 2, device="cuda")  # bf16 holds whole numbers to 256
+    x = torch.zeros(len(a), 64, device="cuda")
+    x[:, 0] = a
+    w = torch.zeros(300, 64, device="cuda")
+    w[:, 0] = 1.0
+    w[at, 0] = 4.0  # the target's logit is 4 a, the others' are a
+    w[:, 1:] = _normal(300, 63, seed=1)  # seen by no row, but by dx
+    xr, wr = x.requires_grad_(), w.requires_grad_()
+    target = torch.full((len(a),), at, device="cuda")
+    loss = ops.linear_cross_entropy(xr, wr, target, reduction="none")
+    dx, dw = torch.autograd.grad(loss, [xr, wr], torch.ones_like(loss))
+    assert bool((loss == 0).all()), loss
+    assert not bool(dx.any()) and not bool(dw.any())
+
+
+def test_loss_is_never_negative(ops):
+    """lse is at least the target's logit, in the kernel's arithmetic too."""
+    x = _normal(512, 64, seed=3, std=40.0, dtype=torch.bfloat16)
+    w = _normal(700, 64, seed=4, dtype=torch.bfloat16)
+    target = (x.double() @ w.double().t()).argmax(1)
+    with torch.no_grad():
+        loss = ops.linear_cross_entropy(x, w, target, reduction="none")
+    assert bool((loss >= 0).all()), float(loss.min())
