@@ -385,15 +385,19 @@ std::vector<at::Tensor> linearGradsInt8(const at::Tensor& grad, const at::Tensor
 //
 // The operators' autograd functions are C++: a small call's time is the host's,
 // and Python functions take several times as long on both ways. Where nothing
-// asks for a gradient they are passed by, and nothing is kept for one.
+// asks for a derivative they are passed by, and nothing is kept for one. They
+// have no forward mode and refuse an input with a tangent, also under no_grad;
+// passed by, it would come back without one.
 
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-bool wantsGradient(std::initializer_list<const at::Tensor*> inputs) {
-  if (!at::GradMode::is_enabled()) return false;
+bool wantsDerivative(std::initializer_list<const at::Tensor*> inputs) {
+  const bool backward = at::GradMode::is_enabled();
   for (const at::Tensor* t : inputs)
-    if (t != nullptr && t->requires_grad()) return true;
+    if (t != nullptr &&
+        ((backward && t->requires_grad()) || t->_fw_grad(/*level=*/0).defined()))
+      return true;
   return false;
 }
 
@@ -516,7 +520,7 @@ at::Tensor embedding(const at::Tensor& idx, const at::Tensor& weight, const Opt&
   const Opt position = positions ? Opt(flat(*positions)) : Opt();
   const int64_t seq = idx.dim() > 0 ? idx.size(-1) : 1;
   const bool outF32 = outType.value_or(w.scalar_type()) == at::kFloat;
-  auto y = wantsGradient({&w, p ? &*p : nullptr})
+  auto y = wantsDerivative({&w, p ? &*p : nullptr})
                ? EmbeddingFn::apply(w, p, token, position, seq, scale, outF32,
                                     hasDestination(w), p && hasDestination(*p))
                : embeddingFwd(token, position, w, p, seq, scale, outF32);
@@ -559,7 +563,7 @@ at::Tensor linearCrossEntropy(const at::Tensor& x, const at::Tensor& w, const Op
   const auto xb = bf16Rows(x);
   const auto t = target.reshape({-1}).contiguous();
   at::Tensor loss;
-  if (wantsGradient({&x, &w})) {
+  if (wantsDerivative({&x, &w})) {
     loss = LinearCeFn::apply(xb, w, w16, t, classes, reduction, hasDestination(w));
   } else {
     const auto r = linearCeFwd(xb, bf16Copy(w, w16), t, classes, reduction);
@@ -627,7 +631,7 @@ at::Tensor linearInt8(const at::Tensor& x, const at::Tensor& w, const at::Tensor
   TORCH_CHECK(w.size(0) % 8 == 0 && w.size(1) % 8 == 0,
               "linear_int8: the layer's sizes must be multiples of 8");
   const auto xb = bf16Rows(x);
-  auto y = wantsGradient({&x, &w, &b})
+  auto y = wantsDerivative({&x, &w, &b})
                ? LinearInt8Fn::apply(xb, w, b, w16, b16, gelu, hasDestination(w),
                                      hasDestination(b))
                : linearInt8Out(xb, bf16Copy(w, w16), bf16Copy(b, b16), gelu)[0];

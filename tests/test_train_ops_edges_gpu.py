@@ -106,3 +106,34 @@ def test_loss_is_never_negative(ops):
     with torch.no_grad():
         loss = ops.linear_cross_entropy(x, w, target, reduction="none")
     assert bool((loss >= 0).all()), float(loss.min())
+
+
+# -- what is asked for ------------------------------------------------------------------
+
+
+def _small_calls(ops):
+    """(call, its differentiable inputs) for each operator, small."""
+    idx = torch.arange(6, device="cuda")
+    w, p = _normal(10, 64, seed=1), _normal(8, 64, seed=2)
+    x, b = _normal(6, 64, seed=3), _normal(24, seed=4)
+    x16, lw = x.to(torch.bfloat16), _normal(24, 64, seed=5)
+    return [(lambda w, p: ops.embedding(idx, w, p), (w, p)),
+            (lambda x, w: ops.linear_cross_entropy(x, w, idx), (x, w)),
+            (lambda x, w: ops.linear_cross_entropy(x, w, idx, reduction="none"), (x16, w)),
+            (lambda x, w, b: ops.linear(x, w, b, activations="int8"), (x, lw, b)),
+            (lambda x, w, b: ops.linear_gelu(x, w, b, activations="int8"), (x16, lw, b))]
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(ops, grad):
+    """A dual tensor among the inputs raises, as it does in every other
+    autograd function here: the result would come back without its tangent."""
+    from torch.autograd import forward_ad
+    for call, inputs in _small_calls(ops):
+        for i, t in enumerate(inputs):
+            with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+                dual = forward_ad.make_dual(t, torch.ones_like(t))
+                with pytest.raises(RuntimeError):
+                    call(*inputs[:i], dual, *inputs[i + 1:])
+        with torch.no_grad():
+            call(*inputs)
