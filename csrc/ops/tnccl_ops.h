@@ -184,8 +184,9 @@ int tnops_dequantize_int8(const uint8_t* q, const uint8_t* e, void* x, int x_f32
 
 // act [rows, outs] (bf16) = gelu_tanh(x w^T + bias) for x [rows, ins],
 // w [outs, ins], bias [outs] in bf16, and the sums before the GELU in 8-bit
-// blocks (rounded from fp32). ins, outs % 8 == 0, x, w, bias 16-byte, act
-// and pre_q 32-byte, pre_e 4-byte aligned; 1 (invalid argument) otherwise.
+// blocks (rounded from fp32), left out where pre_q and pre_e are null. ins,
+// outs % 8 == 0, x, w, bias 16-byte, act and pre_q 32-byte, pre_e 4-byte
+// aligned; 1 (invalid argument) otherwise.
 int tnops_linear_gelu_int8(const void* x, const void* w, const void* bias, void* act,
                            uint8_t* pre_q, uint8_t* pre_e, int rows, int outs, int ins,
                            cudaStream_t stream);

@@ -278,9 +278,9 @@ at::Tensor dequantizeInt8(const at::Tensor& q, const at::Tensor& e, bool outF32)
 }
 
 // x bf16 [rows, ins], w bf16 [outs, ins], bias bf16 [outs] -> (act bf16, and
-// the sums before the GELU in 8-bit blocks)
+// with `keep` the sums before the GELU in 8-bit blocks, else two undefined tensors)
 std::vector<at::Tensor> linearGeluInt8(const at::Tensor& x, const at::Tensor& w,
-                                       const at::Tensor& bias) {
+                                       const at::Tensor& bias, bool keep) {
   need(x, at::kBFloat16, "x");
   need(w, at::kBFloat16, "weight");
   need(bias, at::kBFloat16, "bias");
@@ -294,11 +294,15 @@ std::vector<at::Tensor> linearGeluInt8(const at::Tensor& x, const at::Tensor& w,
   const int rows = asInt(x.size(0), "rows"), outs = asInt(w.size(0), "outputs"),
             ins = asInt(w.size(1), "inputs");
   auto act = at::empty({rows, outs}, x.options());
-  auto q = at::empty({rows, outs}, x.options().dtype(at::kChar));
-  auto e = at::empty({rows, (outs + 31) / 32}, x.options().dtype(at::kByte));
+  at::Tensor q, e;
+  if (keep) {
+    q = at::empty({rows, outs}, x.options().dtype(at::kChar));
+    e = at::empty({rows, (outs + 31) / 32}, x.options().dtype(at::kByte));
+  }
   if (rows == 0) return {act, q, e};
-  ok(tnops_linear_gelu_int8(x.data_ptr(), w.data_ptr(), bias.data_ptr(), act.data_ptr(), bytes(q),
-                            bytes(e), rows, outs, ins, streamOf(x)),
+  ok(tnops_linear_gelu_int8(x.data_ptr(), w.data_ptr(), bias.data_ptr(), act.data_ptr(),
+                            static_cast<uint8_t*>(orNull(q)), static_cast<uint8_t*>(orNull(e)),
+                            rows, outs, ins, streamOf(x)),
      "tnops_linear_gelu_int8");
   return {act, q, e};
 }
@@ -572,10 +576,10 @@ at::Tensor linearCrossEntropy(const at::Tensor& x, const at::Tensor& w, const Op
   return reduction == kNone ? loss.view(target.sizes()) : loss;
 }
 
-// y, and with gelu the sums before it in 8-bit blocks.
+// y, and with gelu and `keep` the sums before it in 8-bit blocks.
 variable_list linearInt8Out(const at::Tensor& x, const at::Tensor& w, const at::Tensor& b,
-                            bool gelu) {
-  if (gelu) return linearGeluInt8(x, w, b);
+                            bool gelu, bool keep) {
+  if (gelu) return linearGeluInt8(x, w, b, keep);
   c10::impl::ExcludeDispatchKeyGuard guard(c10::DispatchKey::AutocastCUDA);
   return {at::addmm(b, x, w.t())};
 }
@@ -585,7 +589,7 @@ struct LinearInt8Fn : torch::autograd::Function<LinearInt8Fn> {
                             const at::Tensor& b, const Opt& w16, const Opt& b16, bool gelu,
                             bool dwDest, bool dbDest) {
     const auto wb = bf16Copy(w, w16);
-    const auto out = linearInt8Out(x, wb, bf16Copy(b, b16), gelu);
+    const auto out = linearInt8Out(x, wb, bf16Copy(b, b16), gelu, true);
     variable_list keep{wb};
     keep.insert(keep.end(), out.begin() + 1, out.end());
     const auto q = quantizeInt8(x);
@@ -634,7 +638,7 @@ at::Tensor linearInt8(const at::Tensor& x, const at::Tensor& w, const at::Tensor
   auto y = wantsDerivative({&x, &w, &b})
                ? LinearInt8Fn::apply(xb, w, b, w16, b16, gelu, hasDestination(w),
                                      hasDestination(b))
-               : linearInt8Out(xb, bf16Copy(w, w16), bf16Copy(b, b16), gelu)[0];
+               : linearInt8Out(xb, bf16Copy(w, w16), bf16Copy(b, b16), gelu, false)[0];
   auto shape = x.sizes().vec();
   shape.back() = w.size(0);
   return y.view(shape);

@@ -137,3 +137,28 @@ def test_forward_mode_is_refused(ops, grad):
                     call(*inputs[:i], dual, *inputs[i + 1:])
         with torch.no_grad():
             call(*inputs)
+
+
+def _peak(call):
+    """Bytes that a call has on the device at once, beyond what it found."""
+    call()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    call()
+    return torch.cuda.max_memory_allocated() - before
+
+
+@pytest.mark.parametrize("rows,ins,outs", [(300, 72, 264), (2048, 256, 1024)])
+def test_gelu_keeps_no_8_bit_sums_without_a_gradient(ops, rows, ins, outs):
+    """Inference forms the activations alone, the same bits."""
+    x = _normal(rows, ins, seed=1, dtype=torch.bfloat16)
+    w, b = _normal(outs, ins, seed=2, dtype=torch.bfloat16), _normal(outs, seed=3, dtype=torch.bfloat16)
+    want = ops.linear_gelu(x, w.clone().requires_grad_(), b, activations="int8").detach()
+    with torch.no_grad():
+        assert torch.equal(ops.linear_gelu(x, w, b, activations="int8"), want)
+        peak = _peak(lambda: ops.linear_gelu(x, w, b, activations="int8"))
+    # The activations in bf16, and less than the byte for each of them that the
+    # 8-bit sums would take.
+    assert 2 * rows * outs <= peak < 2 * rows * outs + rows * outs // 2
