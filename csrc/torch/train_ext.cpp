@@ -347,20 +347,24 @@ std::vector<at::Tensor> geluBwdBiasInt8(const at::Tensor& gy, const at::Tensor& 
   return {gpre, db};
 }
 
-// g [rows, outs], w [outs, ins], x in 8-bit blocks [rows, ins] -> (dx bf16, dw)
-std::vector<at::Tensor> linearGradsInt8(const at::Tensor& grad, const at::Tensor& w,
-                                        const at::Tensor& q, const at::Tensor& e, bool wantDx,
-                                        bool wantDw, bool dwF32, const Opt& dwOut) {
+// g [rows, outs], w [outs, ins], x in 8-bit blocks [rows, ins] (none: no dw)
+// -> (dx bf16, dw)
+std::vector<at::Tensor> linearGradsInt8(const at::Tensor& grad, const at::Tensor& w, const Opt& q,
+                                        const Opt& e, bool wantDx, bool dwF32, const Opt& dwOut) {
   need(grad, at::kBFloat16, "grad");
   need(w, at::kBFloat16, "weight");
-  needInt8(q, e);
-  TORCH_CHECK(grad.dim() == 2 && w.dim() == 2 && grad.size(1) == w.size(0) &&
-                  q.size(0) == grad.size(0) && q.size(1) == w.size(1),
-              "linear_grads_int8: want grad [rows, outs], weight [outs, ins], q [rows, ins]");
+  TORCH_CHECK(grad.dim() == 2 && w.dim() == 2 && grad.size(1) == w.size(0),
+              "linear_grads_int8: want grad [rows, outs], weight [outs, ins]");
   TORCH_CHECK(w.size(0) % 8 == 0 && w.size(1) % 8 == 0,
               "linear_grads_int8: the layer's sizes must be multiples of 8");
   sameDevice(grad, w, "weight");
-  sameDevice(grad, q, "q");
+  const bool wantDw = q.has_value();
+  if (wantDw) {
+    needInt8(*q, *e);
+    TORCH_CHECK(q->size(0) == grad.size(0) && q->size(1) == w.size(1),
+                "linear_grads_int8: want q [rows, ins]");
+    sameDevice(grad, *q, "q");
+  }
   c10::cuda::CUDAGuard g(grad.device());
   const int rows = asInt(grad.size(0), "rows"), outs = asInt(w.size(0), "outputs"),
             ins = asInt(w.size(1), "inputs");
@@ -375,7 +379,7 @@ std::vector<at::Tensor> linearGradsInt8(const at::Tensor& grad, const at::Tensor
   if (rows == 0 && wantDw) dw.zero_();
   if (rows == 0 || (!wantDx && !wantDw)) return {dx, dw};
   at::Tensor x;
-  if (wantDw) x = dequantizeInt8(q, e, false);
+  if (wantDw) x = dequantizeInt8(*q, *e, false);
   const size_t scratchBytes = tnops_linear_grads_scratch(rows, outs, ins, wantDx, wantDw);
   auto scratch = scratchOf(scratchBytes, grad);
   ok(tnops_linear_grads(grad.data_ptr(), outs, w.data_ptr(), orNull(x), orNull(dx), orNull(dw),
@@ -592,7 +596,8 @@ struct LinearInt8Fn : torch::autograd::Function<LinearInt8Fn> {
     const auto out = linearInt8Out(x, wb, bf16Copy(b, b16), gelu, true);
     variable_list keep{wb};
     keep.insert(keep.end(), out.begin() + 1, out.end());
-    const auto q = quantizeInt8(x);
+    // The inputs are read by the weight's gradient alone.
+    const auto q = w.requires_grad() ? quantizeInt8(x) : variable_list(2);
     keep.insert(keep.end(), q.begin(), q.end());
     ctx->save_for_backward(keep);
     ctx->saved_data["w"] = w;
@@ -620,8 +625,9 @@ struct LinearInt8Fn : torch::autograd::Function<LinearInt8Fn> {
       db = biasGradient(g, bt, dbOut);
     }
     const auto st = w.scalar_type() == at::kFloat ? at::kFloat : at::kBFloat16;
+    const at::Tensor &q = s[s.size() - 2], &e = s[s.size() - 1];
     const auto d = linearGradsInt8(
-        g, s[0], s[s.size() - 2], s[s.size() - 1], ctx->needs_input_grad(0), wantW,
+        g, s[0], wantW ? Opt(q) : Opt(), wantW ? Opt(e) : Opt(), ctx->needs_input_grad(0),
         st == at::kFloat, wantW ? destination(w, ctx->saved_data["dw"].toBool(), st) : Opt());
     return {d[0], d[1], db, {}, {}, {}, {}, {}};
   }

@@ -162,3 +162,28 @@ def test_gelu_keeps_no_8_bit_sums_without_a_gradient(ops, rows, ins, outs):
     # The activations in bf16, and less than the byte for each of them that the
     # 8-bit sums would take.
     assert 2 * rows * outs <= peak < 2 * rows * outs + rows * outs // 2
+
+
+def _launches(ops, call):
+    before = ops.launch_count()
+    out = call()
+    return ops.launch_count() - before, out
+
+
+def test_frozen_weight_keeps_no_inputs(ops):
+    """Only the weight's gradient reads the inputs: a frozen weight (the rest
+    trained) forms no 8-bit copy of them, and the other gradients are the same."""
+    x = _normal(300, 128, seed=1, dtype=torch.bfloat16)
+    w, b = _normal(264, 128, seed=2), _normal(264, seed=3).requires_grad_()
+    gy = _normal(300, 264, seed=4, dtype=torch.bfloat16)
+    for f in (ops.linear, ops.linear_gelu):
+        launches, res = [], []
+        for frozen in (False, True):
+            xr = x.clone().requires_grad_()
+            wr = w.clone().requires_grad_(not frozen)
+            n, y = _launches(ops, lambda: f(xr, wr, b, activations="int8"))
+            launches.append(n)
+            res.append((y.detach(), *torch.autograd.grad(y, [xr, b], gy)))
+        assert launches[1] == launches[0] - 1  # the quantizing kernel
+        for one, other in zip(*res):
+            assert torch.equal(one, other)
