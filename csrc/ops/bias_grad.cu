@@ -112,7 +112,7 @@ __device__ __forceinline__ void int8x4Pairs(uint32_t q, uint64_t step, uint64_t&
 enum class Pre { kNone, kBf16, kInt8 };
 
 // T: what the sums are written as (fp32 partial sums, or the result itself
-// where one block of rows is all).
+// where one block of rows is all); null: no sums.
 template <Pre PRE, class T>
 __global__ void __launch_bounds__(kWarps * 32)
     colsumPartial(const uint16_t* __restrict__ gy, const void* __restrict__ pre,
@@ -187,6 +187,7 @@ __global__ void __launch_bounds__(kWarps * 32)
       }
     }
   }
+  if (partial == nullptr) return;
 #pragma unroll
   for (int e = 0; e < 8; ++e) sAcc[w][lane * 8 + e] = acc[e];
   __syncthreads();
@@ -216,7 +217,7 @@ template <class T>
 static int launchColsum(Pre kind, const uint16_t* gy, const void* pre, const uint8_t* preExp,
                         uint16_t* gout, T* db, float* partial, int M, int N,
                         cudaStream_t stream) {
-  if (M <= 0 || N <= 0 || N % 8 != 0) return 1;
+  if (M <= 0 || N <= 0 || N % 8 != 0 || (db == nullptr && gout == nullptr)) return 1;
   // 16-byte pieces of every row (8-byte ones of an 8-bit pre): N % 8 == 0
   // keeps the rows on the boundary when the base pointers are.
   const uintptr_t preMask = kind == Pre::kInt8 ? 7 : 15;
@@ -233,10 +234,11 @@ static int launchColsum(Pre kind, const uint16_t* gy, const void* pre, const uin
                                        : colsumPartial<Pre::kInt8, S>;
     kernel<<<grid, kWarps * 32, 0, stream>>>(gy, pre, preExp, gout, sums, M, N, rowsPer);
   };
-  if (parts == 1) {
+  if (parts == 1 || db == nullptr) {
     run(db);
     return launched(cudaGetLastError()) == 0 ? 0 : 2;
   }
+  if (partial == nullptr) return 1;
   run(partial);
   colReduce<T><<<(N + 31) / 32, kColReduceWarps * 32, 0, stream>>>(partial, parts, N, N, N, db,
                                                                    static_cast<T*>(nullptr));

@@ -61,7 +61,8 @@ int tnops_bias_grad_bf16(const uint16_t* g, uint16_t* db, float* partial, int M,
                          cudaStream_t stream);
 // tnops_gelu_bwd_bias with pre in 8-bit blocks (tnops_quantize_int8's form):
 // pre_q [M, N] 8-byte aligned, pre_e [M, ceil(N / 32)]; db (the sum of the
-// products before their rounding to bf16) fp32 with db_f32, else bf16.
+// products before their rounding to bf16) fp32 with db_f32, else bf16, or null
+// (partial may then be null too).
 int tnops_gelu_bwd_bias_int8(const uint16_t* gy, const uint8_t* pre_q, const uint8_t* pre_e,
                              uint16_t* gpre, void* db, int db_f32, float* partial, int M, int N,
                              cudaStream_t stream);

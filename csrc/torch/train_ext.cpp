@@ -325,9 +325,10 @@ at::Tensor biasGradient(const at::Tensor& grad, at::ScalarType st, const Opt& ou
   return db;
 }
 
-// gy bf16 [M, N], pre in 8-bit blocks -> (gpre bf16 [M, N], db [N] of type st)
+// gy bf16 [M, N], pre in 8-bit blocks -> (gpre bf16 [M, N], db [N] of type st, or
+// undefined where it is not wanted)
 std::vector<at::Tensor> geluBwdBiasInt8(const at::Tensor& gy, const at::Tensor& q,
-                                        const at::Tensor& e, at::ScalarType st,
+                                        const at::Tensor& e, bool wantDb, at::ScalarType st,
                                         const Opt& dbOut) {
   need(gy, at::kBFloat16, "grad_y");
   needInt8(q, e);
@@ -337,11 +338,16 @@ std::vector<at::Tensor> geluBwdBiasInt8(const at::Tensor& gy, const at::Tensor& 
   c10::cuda::CUDAGuard g(gy.device());
   const int M = asInt(gy.size(0), "rows"), N = asInt(gy.size(1), "columns");
   auto gpre = at::empty_like(gy);
-  auto db = dbOut ? *dbOut : at::empty({N}, gy.options().dtype(st));
-  if (M == 0) return {gpre, db.zero_()};
-  auto part = columnParts(gy, M, N);
+  at::Tensor db;
+  ColumnParts part;
+  if (wantDb) {
+    db = dbOut ? *dbOut : at::empty({N}, gy.options().dtype(st));
+    if (M == 0) db.zero_();
+    part = columnParts(gy, M, N);
+  }
+  if (M == 0) return {gpre, db};
   ok(tnops_gelu_bwd_bias_int8(static_cast<uint16_t*>(gy.data_ptr()), bytes(q), bytes(e),
-                              static_cast<uint16_t*>(gpre.data_ptr()), db.data_ptr(),
+                              static_cast<uint16_t*>(gpre.data_ptr()), orNull(db),
                               st == at::kFloat, part, M, N, streamOf(gy)),
      "tnops_gelu_bwd_bias_int8");
   return {gpre, db};
@@ -618,9 +624,9 @@ struct LinearInt8Fn : torch::autograd::Function<LinearInt8Fn> {
     const Opt dbOut = wantB ? destination(b, ctx->saved_data["db"].toBool(), bt) : Opt();
     at::Tensor db;
     if (gelu) {
-      auto r = geluBwdBiasInt8(g, s[1], s[2], bt, dbOut);
+      auto r = geluBwdBiasInt8(g, s[1], s[2], wantB, bt, dbOut);
       g = r[0];
-      if (wantB) db = r[1];
+      db = r[1];
     } else if (wantB) {
       db = biasGradient(g, bt, dbOut);
     }

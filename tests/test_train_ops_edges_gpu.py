@@ -187,3 +187,26 @@ def test_frozen_weight_keeps_no_inputs(ops):
         assert launches[1] == launches[0] - 1  # the quantizing kernel
         for one, other in zip(*res):
             assert torch.equal(one, other)
+
+
+def test_frozen_bias_is_not_summed(ops):
+    """A frozen bias: no column sums behind the GELU's gradient, the other
+    gradients the same."""
+    rows, outs = 2000, 264
+    x = _normal(rows, 128, seed=1, dtype=torch.bfloat16)
+    w, b = _normal(outs, 128, seed=2).requires_grad_(), _normal(outs, seed=3)
+    gy = _normal(rows, outs, seed=4, dtype=torch.bfloat16)
+    launches, res = [], []
+    for frozen in (False, True):
+        xr, br = x.clone().requires_grad_(), b.clone().requires_grad_(not frozen)
+        y = ops.linear_gelu(xr, w, br, activations="int8")
+        n, d = _launches(ops, lambda: torch.autograd.grad(y, [xr, w], gy, retain_graph=True))
+        launches.append(n)
+        res.append(d)
+        if not frozen:
+            n, d = _launches(ops, lambda: torch.autograd.grad(y, [xr, w, br], gy))
+            launches.append(n)
+    # Asked for or not makes the difference, not whether the bias is frozen.
+    assert launches[0] == launches[2] == launches[1] - 1, launches
+    for one, other in zip(*res):
+        assert torch.equal(one, other)
