@@ -16,7 +16,9 @@
 //                    chunk plus the number of smaller ones in every other
 //                    chunk (equal ones count in chunks before its own), found
 //                    by binary searches. Not needed when a single chunk holds
-//                    all rows;
+//                    all rows; more than 131072 rows are merged that many
+//                    at a time, then the sorted parts two and two (mergePairs),
+//                    so that the work grows with rows log rows;
 //   3. tableGrads    the sorted rows in blocks of 16 to 64: a group of threads,
 //                    one per 16 bytes of a row, adds the gradients of each run
 //                    of equal tokens in row order and writes the table row of
@@ -164,10 +166,10 @@ __host__ __device__ __forceinline__ constexpr int chunkBits() {
 // Chunks of 1024, 2048 or 4096 rows: small ones are sorted quickly, large ones
 // leave the merge fewer searches per row (one in every other chunk). Forward and
 // backward pass in us (width 768, fp32 below, bf16 from 65536 rows on):
-//   rows          20480   32768   65536   131072   262144 (width 256)
-//   chunk 1024       74      95     129      246      519
-//   chunk 2048       78      92     120      208      366
-//   chunk 4096        -       -     126     189      281
+//   rows          20480   32768   65536   131072
+//   chunk 1024       74      95     129      246
+//   chunk 2048       78      92     120      208
+//   chunk 4096        -       -     126     189
 struct SortPlan {
   int chunk, chunks;
   bool wide;  // 64-bit keys
@@ -349,6 +351,12 @@ __global__ void __launch_bounds__(kThreads, 4)
 // going on side by side.
 constexpr int kMergeThreads = 512;
 constexpr uint32_t kMergeSmem = 128 * 1024;
+// Rows whose chunks are merged at once. Forward and backward pass in us, bf16:
+//   rows (width)    262144 (256)  524288 (256)  1048576 (256)  4194304 (64)  16777216 (4)
+//   131072               214           397            771          2380         10540
+//   262144               282           519           1012          3320         14370
+//   1048576              282           756           2495          9230         37620
+constexpr int kMergeRows = 128 * 1024;
 
 template <class Key, int CHUNK>
 __global__ void __launch_bounds__(kMergeThreads)
@@ -361,14 +369,17 @@ __global__ void __launch_bounds__(kMergeThreads)
   constexpr int side = 4;                                  // searches side by side
   const int64_t at = (int64_t)blockIdx.x * kMergeThreads + threadIdx.x;  // CHUNK % 512 == 0
   const int own = (int)((int64_t)blockIdx.x * kMergeThreads / CHUNK);
-  const int chunks = (rows + CHUNK - 1) / CHUNK;
+  constexpr int together = kMergeRows / CHUNK;
+  const int chunk0 = own / together * together;
+  const int chunks = min((rows + CHUNK - 1) / CHUNK, chunk0 + together);
+  const int64_t end = min((int64_t)rows, (int64_t)chunks * CHUNK);
   const bool has = at < rows;
   const Key key = has ? sorted[at] : 0;
   const Key token = key >> bits;
-  int rank = (int)(at - (int64_t)own * CHUNK);
-  for (int c0 = 0; c0 < chunks; c0 += at1) {
+  int rank = (int)(at - (int64_t)(own - chunk0) * CHUNK);
+  for (int c0 = chunk0; c0 < chunks; c0 += at1) {
     const int64_t from = (int64_t)c0 * CHUNK;
-    const int n = (int)min((int64_t)at1 * CHUNK, rows - from);
+    const int n = (int)min((int64_t)at1 * CHUNK, end - from);
     __syncthreads();
     // 16-byte pieces; the last may run past n, within the rounded-up buffer.
     for (int i = threadIdx.x; i < (int)((n * sizeof(Key) + 15) / 16); i += kMergeThreads)
@@ -403,6 +414,30 @@ __global__ void __launch_bounds__(kMergeThreads)
     skey[rank] = (int)token;
     perm[rank] = own * CHUNK + (int)(key & (CHUNK - 1));
   }
+}
+
+// Sorted parts of `len` places, two and two: a place's new one is its own in its
+// part plus the number of smaller tokens in the other (equal ones count in the
+// first part), found by a binary search. Neighbouring threads have neighbouring
+// tokens, so that a warp's searches read the same few lines.
+__global__ void __launch_bounds__(kThreads)
+    mergePairs(const int* __restrict__ skey, const int* __restrict__ perm,
+               int* __restrict__ skeyOut, int* __restrict__ permOut, int rows, int64_t len) {
+  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (at >= rows) return;
+  const int64_t part = at / len, from = min((part ^ 1) * len, (int64_t)rows);
+  const int key = skey[at], limit = key + (int)(part & 1);
+  int64_t lo = from, hi = min(from + len, (int64_t)rows);
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (skey[mid] < limit)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  const int64_t to = at - (part & 1) * len + lo - from;
+  skeyOut[to] = key;
+  permOut[to] = perm[at];
 }
 
 // -- gradients of the tables -------------------------------------------------------
@@ -686,8 +721,15 @@ int mergeChunks(const void* sorted, int* skey, int* perm, int rows, int chunks,
                                                             perm, rows);
   return launched(cudaGetLastError());
 }
-int mergeChunks(const SortPlan& p, const void* sorted, int* skey, int* perm, int rows,
-                cudaStream_t stream) {
+
+size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+// Two lists, sorted tokens and their rows; a pass of mergePairs needs two more.
+size_t listsBytes(int64_t rows) { return 2 * round16(4 * rows); }
+size_t sortBytes(int64_t rows) { return (rows > kMergeRows ? 2 : 1) * listsBytes(rows); }
+
+// Sorts whole from sorted chunks; lists in `at`, sortBytes(rows) of scratch.
+int mergeChunks(const SortPlan& p, const void* sorted, char* at, int rows, const int** skey,
+                const int** perm, cudaStream_t stream) {
   auto pick = [&](auto key) {
     using Key = decltype(key);
     return p.chunk == kSmallChunk ? mergeChunks<Key, kSmallChunk>
@@ -695,7 +737,27 @@ int mergeChunks(const SortPlan& p, const void* sorted, int* skey, int* perm, int
                                   : mergeChunks<Key, kLargeChunk>;
   };
   auto f = p.wide ? pick(uint64_t{}) : pick(uint32_t{});
-  return f(sorted, skey, perm, rows, p.chunks, stream);
+  auto lists = [&](bool second, int** k, int** r) {
+    char* base = at + (second ? listsBytes(rows) : 0);
+    *k = reinterpret_cast<int*>(base);
+    *r = reinterpret_cast<int*>(base + listsBytes(rows) / 2);
+  };
+  int *k, *r, *k2, *r2;
+  bool second = false;
+  lists(second, &k, &r);
+  if (int rc = f(sorted, k, r, rows, p.chunks, stream)) return rc;
+  for (int64_t len = kMergeRows; len < rows; len *= 2) {
+    second = !second;
+    lists(second, &k2, &r2);
+    mergePairs<<<(unsigned)(((int64_t)rows + kThreads - 1) / kThreads), kThreads, 0, stream>>>(
+        k, r, k2, r2, rows, len);
+    if (int rc = launched(cudaGetLastError())) return rc;
+    k = k2;
+    r = r2;
+  }
+  *skey = k;
+  *perm = r;
+  return 0;
 }
 
 // Sorted rows per block: 16, or 32 where there are many rows (half the partial
@@ -751,9 +813,7 @@ int tableGradients(const void* g, const TableGradArgs& args, cudaStream_t stream
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 constexpr int64_t kMostRows = INT32_MAX - kLargeChunk;
 
-size_t round16(size_t n) { return (n + 15) / 16 * 16; }
-// Scratch of one table: sorted keys and their rows, partial sums.
-size_t sortBytes(int64_t rows) { return 2 * round16(4 * rows); }
+// Scratch of one table beside its sortBytes.
 size_t partialBytes(int64_t rows, int cols) {
   return round16(sizeof(float) * 2 * ((rows + 15) / 16) * cols);
 }
@@ -829,13 +889,9 @@ extern "C" int tnops_embedding_grad(const void* g, int g_f32, const void* token_
       t.perm = reinterpret_cast<const int*>(static_cast<const char*>(order) + round16(4 * rows));
       return 0;
     }
-    int* skey = reinterpret_cast<int*>(at);
-    at += round16(4 * rows);
-    int* perm = reinterpret_cast<int*>(at);
-    at += round16(4 * rows);
-    t.skey = skey;
-    t.perm = perm;
-    return mergeChunks(plan, order, skey, perm, (int)rows, stream);
+    char* lists = at;
+    at += sortBytes(rows);
+    return mergeChunks(plan, order, lists, (int)rows, &t.skey, &t.perm, stream);
   };
   if (dw)
     if (int rc = add(token_order, dw, vocab, scale)) return rc;

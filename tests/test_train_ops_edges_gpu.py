@@ -210,3 +210,69 @@ def test_frozen_bias_is_not_summed(ops):
     assert launches[0] == launches[2] == launches[1] - 1, launches
     for one, other in zip(*res):
         assert torch.equal(one, other)
+
+
+# -- embedding: very many rows ------------------------------------------------------------
+
+
+def _embedding_grad_ms(ops, rows):
+    g = torch.Generator(device="cuda").manual_seed(1)
+    idx = torch.randint(0, 50000, (rows,), device="cuda", generator=g)
+    w = torch.zeros(50000, 4, device="cuda", requires_grad=True)
+    gy = torch.ones(rows, 4, device="cuda")
+    y = ops.embedding(idx, w)
+    times = []
+    for _ in range(4):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        torch.autograd.grad(y, [w], gy, retain_graph=True)
+        b.record()
+        b.synchronize()
+        times.append(a.elapsed_time(b))
+    return min(times)
+
+
+def test_embedding_gradient_grows_with_the_rows(ops):
+    """Eight times the rows take about eight times as long (twice that is
+    allowed), where searching every chunk for every row would take 64 times."""
+    assert _embedding_grad_ms(ops, 1 << 22) < 16 * _embedding_grad_ms(ops, 1 << 19)
+
+
+@pytest.mark.parametrize("rows,vocab", [
+    (1 << 17, 1000),             # as many chunks as are merged at once
+    ((1 << 17) + 1, 1000),       # ... and one row
+    ((1 << 18) + 4097, 50000),
+    (3 * (1 << 17), 7),          # an odd number of sorted parts
+    (1300001, 2100000),          # 64-bit sort keys
+    (1300001, 1),                # one run
+])
+def test_embedding_of_very_many_rows(ops, rows, vocab):
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    idx = torch.randint(-1, vocab + 1, (rows,), device="cuda", generator=g)
+    at = torch.randint(0, 300, (rows,), device="cuda", generator=g)
+    w = torch.zeros(vocab, 3, device="cuda", requires_grad=True)
+    p = torch.zeros(300, 3, device="cuda", requires_grad=True)
+    gy = torch.randint(-2, 3, (rows, 3), device="cuda", generator=g).float()
+    dw, dp = torch.autograd.grad(ops.embedding(idx, w, p, positions=at), [w, p], gy)
+    # Whole numbers whose sums stay below 2^24: exact in any order.
+    keep = (idx >= 0) & (idx < vocab)
+    assert torch.equal(dw, torch.zeros_like(w).index_add_(0, idx[keep], gy[keep]))
+    assert torch.equal(dp, torch.zeros_like(p).index_add_(0, at, gy))
+
+
+def test_embedding_of_very_many_rows_adds_in_row_order(ops):
+    """The order of equal tokens is the rows': a run's first block is added in
+    fp32 in that order, so that a sum of values far apart shows any other."""
+    rows = (1 << 17) + 30000
+    g = torch.Generator(device="cuda").manual_seed(5)
+    idx = torch.randperm(rows // 16 * 16, device="cuda", generator=g) // 16
+    vocab = int(idx.max()) + 1
+    gy = _normal(len(idx), 4, seed=6) * 10.0 ** torch.randint(-4, 5, (len(idx), 1), device="cuda",
+                                                               generator=g)
+    w = torch.zeros(vocab, 4, device="cuda", requires_grad=True)
+    (dw,) = torch.autograd.grad(ops.embedding(idx, w), [w], gy)
+    by_token = gy[torch.sort(idx, stable=True)[1]].view(vocab, 16, 4)
+    want = torch.zeros(vocab, 4, device="cuda")
+    for i in range(16):  # sixteen rows each: every run lies within its block
+        want += by_token[:, i]
+    assert torch.equal(dw, want)
