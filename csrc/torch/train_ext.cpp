@@ -665,6 +665,8 @@ void registerTrainOps(py::module_& ops) {
           py::arg("weight_bf16"), py::arg("target"), py::arg("classes"), py::arg("reduction"));
   ops.def("linear_int8", &linearInt8, py::arg("x"), py::arg("weight"), py::arg("bias"),
           py::arg("weight_bf16"), py::arg("bias_bf16"), py::arg("gelu"));
+  ops.def("linear_gelu_int8", &linearGeluInt8, py::arg("x"), py::arg("weight"), py::arg("bias"),
+          py::arg("keep") = true);
   ops.def("linear_ce_fwd", &linearCeFwd, py::arg("x"), py::arg("weight"), py::arg("target"),
           py::arg("classes"), py::arg("reduction"));
   ops.def("linear_ce_piece", &tnops_linear_ce_piece, py::arg("rows"), py::arg("width"),

@@ -276,3 +276,90 @@ def test_embedding_of_very_many_rows_adds_in_row_order(ops):
     for i in range(16):  # sixteen rows each: every run lies within its block
         want += by_token[:, i]
     assert torch.equal(dw, want)
+
+
+# -- the fused GELU's 8-bit sums, bit by bit ------------------------------------------------
+
+
+def _int8_exponent(top):
+    """The exponent byte of a block whose largest magnitude is top: the least
+    e >= 0 with round(top / 2^(e - 133)) <= 127, in 64 bits."""
+    e = (torch.frexp(top).exponent.long() - 9 + 133).clamp(min=0) * (top > 0)
+    for _ in range(4):
+        e = torch.where(torch.round(top / _step64(e)) > 127, e + 1, e)
+    return e
+
+
+def _step64(e):
+    return ((e - 133 + 1023) << 52).view(torch.float64)  # 2^(e - 133), exactly
+
+
+def _gelu_slope64(x):
+    k0, k1 = (2.0 / torch.pi) ** 0.5, 0.044715
+    r = 1 / (1 + torch.exp(-2 * k0 * (x + k1 * x ** 3)))
+    return r + 2 * x * r * (1 - r) * k0 * (1 + 3 * k1 * x ** 2)
+
+
+def _off_by(q, lo, hi):
+    return int(((q < lo) | (q > hi)).sum())
+
+
+GELU_SHAPES = [(1, 8, 8), (33, 128, 512), (130, 72, 264), (300, 520, 136), (70, 64, 40),
+               (257, 1600, 1032), (1000, 200, 776)]
+
+
+@pytest.mark.parametrize("rows,ins,outs", GELU_SHAPES)
+def test_gelu_int8_sums_bit_by_bit(ops, rows, ins, outs):
+    """q and e of the sums before the GELU: the fp32 sum is off by at most
+    (ins + 1) half steps of its magnitudes' sum, and between the whole numbers
+    that both ends of that range round to nothing is allowed. Then the gradients
+    from these q and e, whose only roundings are the GELU gradient's to bf16 and
+    the results'."""
+    from tiny_nccl_b200._native import load
+    x = _normal(rows, ins, seed=rows, dtype=torch.bfloat16)
+    w = _normal(outs, ins, seed=rows + 1, std=ins ** -0.5, dtype=torch.bfloat16)
+    b = _normal(outs, seed=rows + 2, std=0.1, dtype=torch.bfloat16)
+    # Blocks of every size, and one of zeros.
+    w *= (2.0 ** (torch.arange(outs, device="cuda") // 32 % 40 - 20))[:, None].to(torch.bfloat16)
+    w[:32] = 0.0
+    b[:32] = 0.0
+    act, q, e = load().ops.linear_gelu_int8(x, w, b)
+    x64, w64, b64 = x.double(), w.double(), b.double()
+    pre = x64 @ w64.t() + b64
+    err = (ins + 1) * F32 * (x64.abs() @ w64.abs().t() + b64.abs())
+    pad = -outs % 32
+    block = lambda t: torch.nn.functional.pad(t, (0, pad)).view(rows, -1, 32)  # noqa: E731
+    size, eb = block(pre.abs()), block(err)
+    lo = _int8_exponent((size - eb).clamp(min=0).amax(2))
+    hi = _int8_exponent((size + eb).amax(2))
+    assert _off_by(e.long(), lo, hi) == 0
+    step = _step64(e.long()).repeat_interleave(32, 1)[:, :outs]
+    qlo, qhi = (torch.round(t / step).clamp(-127, 127) for t in (pre - err, pre + err))
+    assert _off_by(q.double(), qlo, qhi) == 0
+    # Most values leave no choice. Where the weights are small a sum is its bf16
+    # bias and a little: with eight significant bits against q's seven, half of
+    # the values in a block's top binade lie next to a tie; elsewhere the range
+    # is 2 (ins + 1) 2^-24 0.64 sqrt(ins) of a value near 1, a sixth of the step
+    # 2^-5 at 1600 inputs.
+    assert float((qlo == qhi).double().mean()) > 0.5
+    back = q.double() * step
+    assert torch.equal(load().ops.dequantize_int8(q, e, True).double(), back)
+
+    xr, wr, br = x.clone().requires_grad_(), w.float().requires_grad_(), b.float().requires_grad_()
+    y = ops.linear_gelu(xr, wr, br, activations="int8")
+    assert torch.equal(y, act)
+    gy = _normal(rows, outs, seed=rows + 3, dtype=torch.bfloat16)
+    dx, dw, db = torch.autograd.grad(y, [xr, wr, br], gy)
+    g = gy.double() * _gelu_slope64(back)
+    # The slope: ex2, a reciprocal and fp32 products, 2^-20 of at most 1.13; g's
+    # bf16 rounding, then fp32 sums, then the result's rounding (dx bf16).
+    slope = 2.0 ** -20 * gy.double().abs()
+    each = BF16 * g.abs() + slope * (1 + BF16)
+    xq = load().ops.dequantize_int8(*ops.quantize_int8(x), True).double()
+    ex, ew, es = g @ w64, g.t() @ xq, g.sum(0)
+    off = (each + (outs + 2) * F32 * g.abs()) @ w64.abs() + BF16 * ex.abs() * 1.01 + 1e-30
+    assert bool(((dx.double() - ex).abs() <= off).all())
+    off = (each + (rows + 2) * F32 * g.abs()).t() @ xq.abs() + 1e-30
+    assert bool(((dw.double() - ew).abs() <= off).all())
+    off = (slope + (rows + 2) * F32 * g.abs()).sum(0) + 1e-30
+    assert bool(((db.double() - es).abs() <= off).all())
