@@ -68,7 +68,8 @@ int shapes(int rows, int outs, int padded, int ins, bool wantDx, bool wantDw, Ge
   int n = 0;
   auto add = [&](bool dx) {
     GemmProblem& p = prob[n];
-    p.rows = dx ? rows : outs + padded;  // past the last of g's columns A reads zero
+    p.real = dx ? rows : outs;
+    p.rows = dx ? rows : outs + padded;
     p.tilesM = (p.rows + kPairBM - 1) / kPairBM;
     p.tilesN = (ins + 255) / 256;
     p.kBlocks = ((dx ? outs : rows) + kBK - 1) / kBK;

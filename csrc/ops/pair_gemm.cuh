@@ -41,6 +41,7 @@ struct alignas(64) GemmProblem {
   CUtensorMap mapA, mapB;
   int tilesM, tilesN, kBlocks;
   int rows;  // m
+  int real;  // rows of A; results of those behind are zero, whatever B holds
   int aMn, bMn;
 };
 
@@ -214,6 +215,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 4; ++i) tmemIssue32(acc + (uint32_t)(side * 128 + 32 * i), r[i]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) tmemWait(r[i]);
+          if (row0 + 32 > p.real && row0 + lane >= p.real) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int k = 0; k < 32; ++k) r[i][k] = 0u;
+          }
         }
         fenceBeforeSync();
         __syncwarp();

@@ -363,3 +363,17 @@ def test_gelu_int8_sums_bit_by_bit(ops, rows, ins, outs):
     assert bool(((dw.double() - ew).abs() <= off).all())
     off = (slope + (rows + 2) * F32 * g.abs()).sum(0) + 1e-30
     assert bool(((db.double() - es).abs() <= off).all())
+
+
+@pytest.mark.parametrize("classes,vocab", [(480, 500), (480, 1000), (700, 704), (1000, 1001)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_padding_rows_get_zero_whatever_x_holds(ops, classes, vocab, dtype):
+    """The rows of weight behind the classes have a zero gradient also where
+    a row of x is no number."""
+    x = _normal(600, 64, seed=1, dtype=torch.bfloat16)
+    x[5, 3], x[7, 0] = float("nan"), float("inf")
+    w = _normal(vocab, 64, seed=2, dtype=dtype).requires_grad_()
+    target = torch.arange(600, device="cuda") % classes
+    (dw,) = torch.autograd.grad(ops.linear_cross_entropy(x, w, target, classes=classes), [w])
+    assert bool((dw[classes:] == 0).all())
+    assert bool(dw[:classes].isnan().any())
