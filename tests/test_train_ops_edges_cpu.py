@@ -1,5 +1,8 @@
 """Host side of the training operators at their edges, without a GPU: what the
 C launchers refuse before any CUDA call."""
+import pytest
+import torch
+
 from test_train_ops_cpu import A, I, P, _launcher, _refuses
 
 
@@ -17,3 +20,12 @@ def test_gelu_gradient_launcher_with_and_without_a_bias_gradient(built):
     _refuses(f, [A, A, A, A, A, 1, A, 6400, 768, None], [(6, None)])  # sums without scratch
     f = _launcher("tnops_bias_grad", P, P, P, I, I, P)
     _refuses(f, [A, A, A, 64, 768, None], [(1, None)])
+
+
+def test_int8_blocks_need_a_dimension(built):
+    from tiny_nccl_b200 import ops
+    x = torch.zeros(())
+    with pytest.raises(ValueError):
+        ops.quantize_int8(x)
+    with pytest.raises(ValueError):
+        ops.dequantize_int8(x.to(torch.int8), torch.zeros(1, dtype=torch.uint8))

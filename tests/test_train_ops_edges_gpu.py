@@ -377,3 +377,11 @@ def test_padding_rows_get_zero_whatever_x_holds(ops, classes, vocab, dtype):
     (dw,) = torch.autograd.grad(ops.linear_cross_entropy(x, w, target, classes=classes), [w])
     assert bool((dw[classes:] == 0).all())
     assert bool(dw[:classes].isnan().any())
+
+
+def test_int8_blocks_without_values(ops):
+    for shape in [(5, 0), (0, 40), (0, 0), (3, 0, 64), (3, 2, 0)]:
+        x = torch.empty(shape, device="cuda")
+        q, e = ops.quantize_int8(x)
+        assert q.shape == shape and e.shape == (*shape[:-1], -(-shape[-1] // 32))
+        assert ops.dequantize_int8(q, e).shape == shape

@@ -16,6 +16,12 @@ def _needs_float(name: str, t: torch.Tensor) -> None:
         raise TypeError(f"{name} must be float32 or bfloat16, not {t.dtype}")
 
 
+def _as_rows(name: str, t: torch.Tensor) -> torch.Tensor:
+    if t.dim() == 0:
+        raise ValueError(f"{name} must have at least one dimension")
+    return t.reshape(t.shape[:-1].numel(), t.shape[-1]).contiguous()
+
+
 def embedding(idx: torch.Tensor, weight: torch.Tensor, pos_weight: torch.Tensor | None = None,
               positions: torch.Tensor | None = None, scale: float = 1.0,
               out_dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -73,8 +79,7 @@ def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     block's largest magnitude; a block with an infinity or a NaN reads back as
     NaN."""
     _needs_float("x", x)
-    cols = x.shape[-1]
-    q, e = _ops().quantize_int8(x.reshape(-1, cols).contiguous())
+    q, e = _ops().quantize_int8(_as_rows("x", x))
     return q.view(x.shape), e.view(*x.shape[:-1], e.shape[1])
 
 
@@ -84,6 +89,5 @@ def dequantize_int8(q: torch.Tensor, e: torch.Tensor,
     float32)."""
     if dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"dtype must be float32 or bfloat16, not {dtype}")
-    x = _ops().dequantize_int8(q.reshape(-1, q.shape[-1]).contiguous(),
-                               e.reshape(-1, e.shape[-1]).contiguous(), dtype == torch.float32)
+    x = _ops().dequantize_int8(_as_rows("q", q), _as_rows("e", e), dtype == torch.float32)
     return x.view(q.shape)
