@@ -195,10 +195,17 @@ std::vector<at::Tensor> linearCeBwd(const at::Tensor& x, const at::Tensor& w,
   const CeShape s = ceShape(x, w, target, classes);
   need(lse, at::kFloat, "lse");
   need(grad, at::kFloat, "grad");
+  TORCH_CHECK(lse.numel() == s.rows, "linear_cross_entropy: want one lse per row");
   TORCH_CHECK(grad.numel() == 1 || grad.numel() == s.rows,
               "linear_cross_entropy: want one gradient, or one per row");
+  sameDevice(x, lse, "lse");
+  sameDevice(x, grad, "grad");
   TORCH_CHECK(budget > 0, "linear_cross_entropy: the scratch budget must be positive");
-  if (share) need(*share, at::kFloat, "share");
+  if (share) {
+    need(*share, at::kFloat, "share");
+    TORCH_CHECK(share->numel() == 1, "linear_cross_entropy: want one share");
+    sameDevice(x, *share, "share");
+  }
   c10::cuda::CUDAGuard g(x.device());
   at::Tensor dx, dw;
   if (wantDx) dx = at::empty_like(x);
@@ -207,6 +214,7 @@ std::vector<at::Tensor> linearCeBwd(const at::Tensor& x, const at::Tensor& w,
     dw = dwOut ? *dwOut : at::empty({s.vocab, s.width}, w.options().dtype(st));
     need(dw, st, "dw_out");
     TORCH_CHECK(dw.numel() == w.numel(), "linear_cross_entropy: dw_out must match weight");
+    sameDevice(x, dw, "dw_out");
     if (s.rows == 0) dw.zero_();
   }
   if (s.rows == 0 || (!wantDx && !wantDw)) return {dx, dw};
@@ -239,6 +247,12 @@ struct ColumnParts {
 ColumnParts columnParts(const at::Tensor& like, int M, int N) {
   const int64_t parts = tnops_colsum_parts(M, N);
   return {parts > 1 ? at::empty({parts * N}, like.options().dtype(at::kFloat)) : at::Tensor()};
+}
+
+void needSums(const at::Tensor& grad, const at::Tensor& db, at::ScalarType st, int N) {
+  need(db, st, "db_out");
+  TORCH_CHECK(db.numel() == N, "db_out must have one value per column");
+  sameDevice(grad, db, "db_out");
 }
 
 // x [rows, cols] -> (q int8 [rows, cols], e uint8 [rows, ceil(cols / 32)])
@@ -314,6 +328,7 @@ at::Tensor biasGradient(const at::Tensor& grad, at::ScalarType st, const Opt& ou
   c10::cuda::CUDAGuard g(grad.device());
   const int M = asInt(grad.size(0), "rows"), N = asInt(grad.size(1), "columns");
   auto db = out ? *out : at::empty({N}, grad.options().dtype(st));
+  needSums(grad, db, st, N);
   if (M == 0) return db.zero_();
   auto part = columnParts(grad, M, N);
   auto* gp = static_cast<uint16_t*>(grad.data_ptr());
@@ -342,6 +357,7 @@ std::vector<at::Tensor> geluBwdBiasInt8(const at::Tensor& gy, const at::Tensor& 
   ColumnParts part;
   if (wantDb) {
     db = dbOut ? *dbOut : at::empty({N}, gy.options().dtype(st));
+    needSums(gy, db, st, N);
     if (M == 0) db.zero_();
     part = columnParts(gy, M, N);
   }
@@ -381,6 +397,7 @@ std::vector<at::Tensor> linearGradsInt8(const at::Tensor& grad, const at::Tensor
     dw = dwOut ? *dwOut : at::empty({outs, ins}, w.options().dtype(st));
     need(dw, st, "dw_out");
     TORCH_CHECK(dw.numel() == w.numel(), "linear_grads_int8: dw_out must match weight");
+    sameDevice(grad, dw, "dw_out");
   }
   if (rows == 0 && wantDw) dw.zero_();
   if (rows == 0 || (!wantDx && !wantDw)) return {dx, dw};

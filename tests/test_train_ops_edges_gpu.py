@@ -385,3 +385,22 @@ def test_int8_blocks_without_values(ops):
         q, e = ops.quantize_int8(x)
         assert q.shape == shape and e.shape == (*shape[:-1], -(-shape[-1] // 32))
         assert ops.dequantize_int8(q, e).shape == shape
+
+
+def test_binding_refuses_sizes_that_do_not_match(ops):
+    """What the backward pass of the cross-entropy reads has the sizes of its
+    forward pass."""
+    from tiny_nccl_b200._native import load
+    x, w = _normal(40, 64, seed=1, dtype=torch.bfloat16), _normal(300, 64, seed=2, dtype=torch.bfloat16)
+    target = torch.arange(40, device="cuda")
+    _, lse, _, share = load().ops.linear_ce_fwd(x, w, target, 300, 0)
+    one = torch.ones(1, device="cuda")
+    good = dict(x=x, weight=w, target=target, lse=lse, grad=one, share=share, classes=300,
+                want_dx=True, want_dw=True, dw_f32=True)
+    load().ops.linear_ce_bwd(**good)
+    for bad in (dict(lse=lse[:39]), dict(lse=lse.cpu()), dict(grad=torch.ones(39, device="cuda")),
+                dict(grad=one.cpu()), dict(share=torch.empty(0, device="cuda")),
+                dict(share=share.cpu()), dict(target=target[:39]),
+                dict(dw_out=torch.empty(299, 64, device="cuda"))):
+        with pytest.raises(RuntimeError):
+            load().ops.linear_ce_bwd(**{**good, **bad})
