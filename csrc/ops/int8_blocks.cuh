@@ -4,8 +4,10 @@
 //
 //   value = q 2^(e - 133),  e = 0 .. 254 one byte per block, 255: not a number
 //
-// e is the least with round(max / 2^(e - 133)) <= 127, so a value is off by
-// at most half a step, 2^-7 of the block's largest value. Multiplying by a
+// e is the least with round(max / 2^(e - 133)) <= 127, so the largest value of a
+// block is at least 63.75 steps and a value is off by at most half a step, 1 / 127.5
+// of the block's largest (but for blocks below 2^-127, whose step stays 2^-133, and
+// the last half step below 2^128, which keeps 127 steps). Multiplying by a
 // power of two is exact, so the only rounding is the one to whole numbers
 // (nearest, ties to even), and a value read back has seven significant bits:
 // it is a bf16 number, whatever the block. A block that holds an infinity or
@@ -19,9 +21,9 @@ namespace {
 
 constexpr int kInt8Block = 32;
 
-// Exponent byte of a block from its largest magnitude. Adding 2^16 to the
-// fp32 bits carries into the exponent when the mantissa is at least 127/64
-// steps of 64, i.e. when 127.5 steps or more would be needed.
+// Exponent byte of a block from its largest magnitude: with a step that makes it
+// 64 to 128 steps, 127.5 or more (a mantissa of at least 127.5 / 64) would round
+// to 128. Adding 2^16 to the fp32 bits carries into the exponent from there on.
 __device__ __forceinline__ uint32_t int8Exponent(float top) {
   const uint32_t u = __float_as_uint(top);
   if (u >= 0x7f800000u) return 255u;

@@ -404,3 +404,19 @@ def test_binding_refuses_sizes_that_do_not_match(ops):
                 dict(dw_out=torch.empty(299, 64, device="cuda"))):
         with pytest.raises(RuntimeError):
             load().ops.linear_ce_bwd(**{**good, **bad})
+
+
+def test_int8_blocks_bound(ops):
+    """Half a step is at most 1 / 127.5 of a block's largest magnitude, reached
+    where 127.5 steps become 63.75; 2^-7 does not hold there."""
+    x = torch.zeros(2, 32, device="cuda")
+    x[0, 0], x[0, 1] = 127.5 / 64, 1 / 64   # 63.75 steps of 2^-5, and half a step
+    x[1, 0], x[1, 1] = 127.0 / 64, 1 / 128  # 127 steps of 2^-6, and half a step
+    back = ops.dequantize_int8(*ops.quantize_int8(x), torch.float32)
+    off = (back.double() - x.double()).abs().amax(1) / x.double().amax(1)
+    assert off[0] == 1 / 127.5 and off[0] > 2.0 ** -7 > off[1]
+    for seed in range(4):
+        x = _normal(500, 96, seed=seed) * 2.0 ** (torch.arange(500, device="cuda")[:, None] % 60 - 30)
+        back = ops.dequantize_int8(*ops.quantize_int8(x), torch.float32)
+        top = x.double().view(500, 3, 32).abs().amax(2).repeat_interleave(32, 1)
+        assert bool(((back.double() - x.double()).abs() <= top / 127.5).all())

@@ -75,9 +75,9 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
 def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """x (float32 or bfloat16) as (q, e): whole numbers in [-127, 127] (int8,
     x's shape) and one exponent byte for each 32 neighbours of the last
-    dimension (uint8); value = q * 2^(e - 133). Off by at most 2^-7 of the
-    block's largest magnitude; a block with an infinity or a NaN reads back as
-    NaN."""
+    dimension (uint8); value = q * 2^(e - 133). Off by at most half a step, 1/127.5
+    of the block's largest magnitude (magnitudes below 2^-127 have steps of
+    2^-133); a block with an infinity or a NaN reads back as NaN."""
     _needs_float("x", x)
     q, e = _ops().quantize_int8(_as_rows("x", x))
     return q.view(x.shape), e.view(*x.shape[:-1], e.shape[1])
