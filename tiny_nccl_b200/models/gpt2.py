@@ -14,11 +14,15 @@ Two implementations share one parameter layout:
 * ``impl="torch"``: the same math in stock PyTorch ops; it is the fp32
   numerics reference for the fused kernels and the path the CPU tests use.
 
-The fused implementation has three options, each the default's math on other
+The fused implementation has three options, each the default's layers on other
 kernels: ``embedding="fused"`` (token + position embedding and the gradients of
-both tables by sorted tokens), ``head="pieces"`` (LM head and loss without the
-logits in memory), ``activations="int8"`` (the blocks' linear layers keep
-what their backward pass reads in 8 bits).
+both tables by sorted tokens; an index outside its table adds nothing),
+``head="pieces"`` (LM head and loss without the logits in memory),
+``activations="int8"`` (the blocks' linear layers keep what their backward pass
+reads in 8 bits). Where targets are ignored (outside the classes, such as -100)
+the losses differ by a factor: ``head="pieces"`` and ``impl="torch"`` take the
+mean over the rows that count, ``head="logits"`` of the fused implementation
+divides by all rows.
 
 The reference (tiny-nccl) has no model; this is the workload of the
 "GPT-2 small DP tokens/s" headline metric.

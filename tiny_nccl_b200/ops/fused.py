@@ -87,7 +87,9 @@ def cross_entropy(logits: torch.Tensor, target: torch.Tensor,
                   reuse_logits: bool = True, classes: int = 0) -> torch.Tensor:
     """Mean cross-entropy of [rows, ld] logits against int64 targets, over the
     first ``classes`` columns (all columns when 0; the rest is vocabulary
-    padding, excluded from the softmax and given zero gradient).
+    padding, excluded from the softmax and given zero gradient). A target
+    outside the classes gives its row zero loss and gradient; the mean is over
+    all rows, these included (``linear_cross_entropy`` leaves them out).
 
     With ``reuse_logits`` (the default, used for the model's temporary logits)
     the gradient is written into the logits storage during the forward pass,
