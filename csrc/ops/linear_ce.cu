@@ -185,12 +185,12 @@ __device__ __forceinline__ float2 joinSums(float2 a, float2 b) {
 
 // Joins a row's partial statistics: eight rows per CTA, the parts dealt to 32
 // threads of each row, four loads in flight; then the threads' sums in a fixed
-// tree.
+// tree. loss comes in with the targets' logits.
 constexpr int kJoinRows = 8, kJoinThreads = 256;
 __global__ void __launch_bounds__(kJoinThreads)
     joinStats(const float2* __restrict__ partial, const int64_t* __restrict__ target,
-              const float* __restrict__ logitOfTarget, float* __restrict__ lse,
-              float* __restrict__ loss, int parts, int rows, int classes) {
+              float* __restrict__ lse, float* __restrict__ loss, int parts, int rows,
+              int classes) {
   __shared__ float2 s[kJoinThreads / 32][kJoinRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.x * kJoinRows + (lane & (kJoinRows - 1));
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     const float l = st.x + logf(st.y);
     const int64_t t = target[row];
     lse[row] = l;
-    loss[row] = t >= 0 && t < classes ? l - logitOfTarget[row] : 0.f;
+    loss[row] = t >= 0 && t < classes ? l - loss[row] : 0.f;
   }
 }
 
@@ -284,7 +284,7 @@ extern "C" int tnops_linear_ce_fwd(const void* x, const void* w, const int64_t* 
   args.epi = {target, reinterpret_cast<float2*>(partial), loss, rows, classes};
   if (int rc = launchPanelGemm(args, x, w, rows, classes, width, stream)) return rc;
   joinStats<<<(rows + kJoinRows - 1) / kJoinRows, kJoinThreads, 0, stream>>>(
-      args.epi.partial, target, loss, lse, loss, tnops_linear_ce_parts(classes), rows, classes);
+      args.epi.partial, target, lse, loss, tnops_linear_ce_parts(classes), rows, classes);
   return launched(cudaGetLastError());
 }
 
