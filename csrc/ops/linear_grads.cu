@@ -74,7 +74,6 @@ int shapes(int rows, int outs, int padded, int ins, bool wantDx, bool wantDw, Ge
     p.tilesN = (ins + 255) / 256;
     p.kBlocks = ((dx ? outs : rows) + kBK - 1) / kBK;
     p.aMn = dx ? 0 : 1;
-    p.bMn = 1;
     isDx[n++] = dx;
   };
   const bool dxFirst = outs >= rows;

@@ -1,12 +1,12 @@
 // pair_gemm.cuh - the matrix products behind the backward passes of the
 // training operators: one persistent CTA-pair pipeline (tcgen05 cta_group::2,
-// fp32 accumulators in TMEM) whose operands may lie either way round in memory.
+// fp32 accumulators in TMEM).
 //
 //   D[m, n] = sum_k A(m, k) B(n, k)
 //
-// Either operand may be K-major or MN-major (pair_parts.cuh): with both, the
-// products of a backward pass (dX = G W, dW = G^T X) read G, W and X as they
-// lie, without a transposed copy.
+// A may be K-major or MN-major, B is MN-major (pair_parts.cuh): the products of
+// a backward pass (dX = G W, dW = G^T X) read G, W and X as they lie, without a
+// transposed copy.
 //
 // The pipeline is that of the GEMM with the bias epilogue (gemm_tcgen05.cu)
 // with tiles of 512 x 256: each CTA of a pair stages, per 64-wide K block, 128
@@ -35,14 +35,14 @@ constexpr uint32_t kPairStage = 3 * kHalf;  // two halves of A, one of B
 constexpr uint32_t kPairSmemBytes = kPairStages * kPairStage + kEpiBytes + 1024;
 
 // One product of a launch. The tensor maps' boxes are {64 k, 128 rows} for a
-// K-major operand and {64 m, 64 k} for an MN-major one; out-of-range rows and
+// K-major A and {64 m, 64 k} for an MN-major operand; out-of-range rows and
 // columns read zero, so K, M and N need no padding.
 struct alignas(64) GemmProblem {
   CUtensorMap mapA, mapB;
   int tilesM, tilesN, kBlocks;
   int rows;  // m
   int real;  // rows of A; results of those behind are zero, whatever B holds
-  int aMn, bMn;
+  int aMn;
 };
 
 struct alignas(64) PairGemmArgs {
@@ -112,14 +112,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int m0 = (w.tile / p.tilesN) * kPairBM + (int)rank * 128;
       const bool both = (w.tile / p.tilesN) * kPairBM + 256 < p.rows;  // the second half has rows
       const int n0 = (w.tile % p.tilesN) * 256 + (int)rank * 128;
-      const int aMn = p.aMn, bMn = p.bMn;
+      const int aMn = p.aMn;
       for (int kb = w.kb0; kb < w.kb1; ++kb, ++g) {
         const uint32_t s = g % kPairStages, round = g / kPairStages;
         if (!mbarWait(&sEmpty[s], (round & 1u) ^ 1u, abort, 1)) break;
         if (rank == 0) mbarExpectTx(&sFull[s], (both ? 6 : 4) * kHalf);  // both CTAs' loads
         const uint32_t bar = inLeader(&sFull[s]), at = base + s * kPairStage;
         loadHalf(at, &p.mapA, aMn, m0, kb * kBK, bar);
-        loadHalf(at + 2 * kHalf, &p.mapB, bMn, n0, kb * kBK, bar);
+        loadHalf(at + 2 * kHalf, &p.mapB, 1, n0, kb * kBK, bar);
         if (both) loadHalf(at + kHalf, &p.mapA, aMn, m0 + 256, kb * kBK, bar);
       }
     }
@@ -144,9 +144,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (; ok && walk.next(schedule, &w); ++local) {
       const GemmProblem& p = args.prob[w.which];
-      const uint64_t descA = pairDescBase(p.aMn), descB = pairDescBase(p.bMn);
-      const uint32_t stepA = p.aMn ? 2048 : 32, stepB = p.bMn ? 2048 : 32;
-      const uint32_t instr = pairInstrDesc(p.aMn, p.bMn);
+      const uint64_t descA = pairDescBase(p.aMn), descB = pairDescBase(1);
+      const uint32_t stepA = p.aMn ? 2048 : 32, stepB = 2048;
+      const uint32_t instr = pairInstrDesc(p.aMn, 1);
       const int halves = (w.tile / p.tilesN) * kPairBM + 256 < p.rows ? 2 : 1;
       const uint32_t fresh = (local & 1u) ^ 1u;  // phase of an accumulator handed back
       for (int kb = w.kb0; kb < w.kb1; ++kb, ++g) {
