@@ -420,3 +420,84 @@ def test_int8_blocks_bound(ops):
         back = ops.dequantize_int8(*ops.quantize_int8(x), torch.float32)
         top = x.double().view(500, 3, 32).abs().amax(2).repeat_interleave(32, 1)
         assert bool(((back.double() - x.double()).abs() <= top / 127.5).all())
+
+
+# -- sizes past the tiles ------------------------------------------------------------------
+
+
+def _blocks64(x):
+    """x as its 8-bit blocks hold it, in 64 bits."""
+    pad = torch.nn.functional.pad(x.double(), (0, -x.shape[1] % 32)).view(len(x), -1, 32)
+    step = _step64(_int8_exponent(pad.abs().amax(2)))[..., None]
+    return (torch.round(pad / step).clamp(-127, 127) * step).view(len(x), -1)[:, :x.shape[1]]
+
+
+@pytest.mark.parametrize("rows,ins,outs", [
+    (300, 1600, 2560),   # as wide as a layer is timed
+    (700, 4096, 1024),   # 64 K blocks
+    (2048, 768, 2304),   # few tiles for the SM pairs
+    (9001, 776, 264),    # 141 K blocks of dW in few tiles: its sums are cut
+])
+def test_linear_int8_wide(ops, rows, ins, outs):
+    x = _normal(rows, ins, seed=1, dtype=torch.bfloat16).requires_grad_()
+    w = _normal(outs, ins, seed=2, std=ins ** -0.5).requires_grad_()
+    b = _normal(outs, seed=3, std=0.1).requires_grad_()
+    gy = _normal(rows, outs, seed=4, dtype=torch.bfloat16)
+    y = ops.linear(x, w, b, activations="int8")
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], gy)
+    x64, w64, g64 = x.detach().double(), w.detach().to(torch.bfloat16).double(), gy.double()
+    xq = _blocks64(x.detach())
+    size = x64.abs() @ w64.abs().t() + 1.0
+    b64 = b.detach().to(torch.bfloat16).double()
+    # fp32 sums of exact products, then the results' rounding.
+    for got, want, off in ((y.detach(), x64 @ w64.t() + b64, (ins + 1) * F32 * size),
+                           (dx, g64 @ w64, outs * F32 * (g64.abs() @ w64.abs())),
+                           (dw, g64.t() @ xq, rows * F32 * (g64.abs().t() @ xq.abs())),
+                           (db, g64.sum(0), rows * F32 * g64.abs().sum(0))):
+        half = BF16 if got.dtype == torch.bfloat16 else F32
+        assert bool(((got.double() - want).abs() <= off + half * 1.01 * want.abs()).all())
+
+
+@pytest.mark.parametrize("rows,width,classes,vocab", [
+    (300, 1600, 2000, 2048),    # a wide head
+    (20001, 128, 20000, 20000),  # the logits' gradient in several pieces by the rule itself
+])
+def test_linear_cross_entropy_wide(ops, rows, width, classes, vocab):
+    from tiny_nccl_b200._native import load
+    if rows > 10000:
+        assert load().ops.linear_ce_piece(rows, width, classes, 512 << 20) < classes
+    x = _normal(rows, width, seed=1, dtype=torch.bfloat16)
+    w = _normal(vocab, width, seed=2, std=2.0 * width ** -0.5)
+    target = torch.arange(rows, device="cuda") * 7919 % classes
+    target[::9] = -1
+    xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = ops.linear_cross_entropy(xr, wr, target, classes=classes)
+    dx, dw = torch.autograd.grad(loss, [xr, wr])
+    wc = w.to(torch.bfloat16).double()[:classes]
+    keep = target >= 0
+    total = 0.0
+    ew, sw = torch.zeros_like(wc), torch.zeros_like(wc)
+    n = int(keep.sum())
+    # A logit's fp32 sum: `width` half steps of its magnitudes; the exponential
+    # and the sums 2^-20; d's rounding to bf16.
+    logit = 0.0
+    for at in range(0, rows, 4096):
+        xs, t, k = x[at:at + 4096].double(), target[at:at + 4096].clamp(min=0), keep[at:at + 4096]
+        logit = max(logit, width * F32 * float((xs.abs() @ wc.abs().t()).max()))
+        logits = xs @ wc.t()
+        lse = torch.logsumexp(logits, 1)
+        i = torch.arange(len(t), device="cuda")
+        total += float((lse - logits[i, t])[k].sum())
+        d = torch.exp(logits - lse[:, None])
+        d[i, t] -= 1
+        d *= k[:, None] / n
+        ew += d.t() @ xs
+        sw += d.abs().t() @ xs.abs()
+        off = BF16 + 3 * logit + 2.0 ** -20 + 2 * classes * F32
+        ex, sx = d @ wc, d.abs() @ wc.abs()
+        got = dx[at:at + 4096].double()
+        assert bool(((got - ex).abs() <= off * sx + 1.01 * BF16 * ex.abs()).all())
+    off = BF16 + 3 * logit + 2.0 ** -20 + 2 * rows * F32
+    assert bool(((dw[:classes].double() - ew).abs() <= off * sw + 1.01 * F32 * ew.abs()).all())
+    assert not bool(dw[classes:].any())
+    assert abs(loss.item() - total / n) <= 2 * logit + 2.0 ** -20 + (rows + 4) * F32 * total / n
