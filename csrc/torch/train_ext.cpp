@@ -647,7 +647,7 @@ struct LinearInt8Fn : torch::autograd::Function<LinearInt8Fn> {
     } else if (wantB) {
       db = biasGradient(g, bt, dbOut);
     }
-    const auto st = w.scalar_type() == at::kFloat ? at::kFloat : at::kBFloat16;
+    const auto st = w.scalar_type() == at::kBFloat16 ? at::kBFloat16 : at::kFloat;
     const at::Tensor &q = s[s.size() - 2], &e = s[s.size() - 1];
     const auto d = linearGradsInt8(
         g, s[0], wantW ? Opt(q) : Opt(), wantW ? Opt(e) : Opt(), ctx->needs_input_grad(0),

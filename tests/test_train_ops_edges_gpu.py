@@ -501,3 +501,19 @@ def test_linear_cross_entropy_wide(ops, rows, width, classes, vocab):
     assert bool(((dw[:classes].double() - ew).abs() <= off * sw + 1.01 * F32 * ew.abs()).all())
     assert not bool(dw[classes:].any())
     assert abs(loss.item() - total / n) <= 2 * logit + 2.0 ** -20 + (rows + 4) * F32 * total / n
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float16])
+def test_linear_int8_gradients_of_other_types(ops, dtype):
+    """Parameters of other types are used through bf16 copies, as in the default
+    linear layers; their gradients come from fp32 sums, not from bf16 results."""
+    x = _normal(300, 128, seed=1, dtype=torch.bfloat16)
+    w, b = _normal(264, 128, seed=2, dtype=torch.bfloat16), _normal(264, seed=3, dtype=torch.bfloat16)
+    gy = _normal(300, 264, seed=4, dtype=torch.bfloat16)
+    for f in (ops.linear, ops.linear_gelu):
+        res = []
+        for t in (torch.float32, dtype):
+            wt, bt = w.to(t).requires_grad_(), b.to(t).requires_grad_()
+            res.append(torch.autograd.grad(f(x, wt, bt, activations="int8"), [wt, bt], gy))
+        for fp32, other in zip(*res):
+            assert other.dtype == dtype and torch.equal(fp32.to(dtype), other)
