@@ -167,7 +167,8 @@ __global__ void __launch_bounds__(kWarps * 32)
             f[2 * i] = a;  // the bias gradient's sum is of the unrounded ones
             f[2 * i + 1] = b;
           }
-          *reinterpret_cast<uint4*>(gout + (size_t)r * N + col0) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(gout + (size_t)r * N + col0) =
+              make_uint4(o[0], o[1], o[2], o[3]);
         } else if (PRE == Pre::kBf16) {
           float x[8];
           bf16x8ToF(p[u], x);
@@ -180,7 +181,8 @@ __global__ void __launch_bounds__(kWarps * 32)
             f[2 * i] = bf2f(lo);
             f[2 * i + 1] = bf2f(hi);
           }
-          *reinterpret_cast<uint4*>(gout + (size_t)r * N + col0) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(gout + (size_t)r * N + col0) =
+              make_uint4(o[0], o[1], o[2], o[3]);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] += f[e];

@@ -236,7 +236,8 @@ __device__ __forceinline__ void sortSteps(Key (&k)[E], Key* s) {
 
 // Sorts one chunk of a list, CHUNK / 256 keys per thread.
 template <class Key, int CHUNK>
-__device__ __noinline__ void sortChunk(const SortList& list, int rows, int chunk, bool one, Key* s) {
+__device__ __noinline__ void sortChunk(const SortList& list, int rows, int chunk, bool one,
+                                       Key* s) {
   constexpr int bits = chunkBits<CHUNK>();
   constexpr int E = CHUNK / kThreads;
   const int64_t* __restrict__ token = list.index;

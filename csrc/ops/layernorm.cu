@@ -525,8 +525,8 @@ extern "C" int tnops_ln_bwd(const uint16_t* gy, const float* g_res, const float*
               : bwdGroup<1>(gy, g_res, x_out, w, mean, rstd, dx, dx_bf16, partial, rows, C,
                             &nparts, stream);
     if (launched(e) != 0) return (int)e;
-    colReduce<float><<<(2 * C + 31) / 32, kColReduceWarps * 32, 0, stream>>>(partial, nparts, 2 * C,
-                                                                      2 * C, C, dw, db);
+    colReduce<float><<<(2 * C + 31) / 32, kColReduceWarps * 32, 0, stream>>>(
+        partial, nparts, 2 * C, 2 * C, C, dw, db);
     return launched(cudaGetLastError());
   }
   cudaError_t e;
@@ -541,8 +541,8 @@ extern "C" int tnops_ln_bwd(const uint16_t* gy, const float* g_res, const float*
   int nparts = (rows + kWarpsPerBlock - 1) / kWarpsPerBlock;
   if (nparts > kPartialRows) nparts = kPartialRows;
   // dw = column sums of the first C partial columns, db of the next C.
-  colReduce<float><<<(2 * C + 31) / 32, kColReduceWarps * 32, 0, stream>>>(partial, nparts, 2 * C,
-                                                                    2 * C, C, dw, db);
+  colReduce<float><<<(2 * C + 31) / 32, kColReduceWarps * 32, 0, stream>>>(
+      partial, nparts, 2 * C, 2 * C, C, dw, db);
   return launched(cudaGetLastError());
 }
 

@@ -11,8 +11,9 @@
 // Pairs that work at the same time so have neighbouring units, which read the
 // same rows of an operand in the same order: one read from memory serves them
 // all. (An even cut of the K blocks over the pairs, which also keeps all of
-// them busy, lets every pair read at a place of its own: on a 65536 x 1024 x
-// 4096 layer the two products took 995 us that way and 830 us in turns.)
+// them busy, lets every pair read at a place of its own: with tiles of 256 x 256
+// the two products of a 65536 x 1024 x 4096 layer took 995 us that way and 830
+// us in turns; tiles of 512 x 256, in turns, take 740.)
 //
 // Units of a cut tile leave partial sums, one slot per unit, which a second
 // kernel adds in the order of the sum.

@@ -52,7 +52,8 @@ struct RingAt {
 
 // Epi: `State begin(row)` once per tile and thread (the thread's row of the
 // output), `chunk(state, v, ahead, row, col0)` for its 32 columns from col0 of
-// each block (ahead: what `ahead(col0)` loaded while the block before was worked on), `end(state, row, part)` after the last block (part: the 128 columns'
+// each block (ahead: what `ahead(col0)` loaded while the block before was worked
+// on), `end(state, row, part)` after the last block (part: the 128 columns'
 // number). What an epilogue writes goes straight from registers: operands in
 // and out of shared memory take its whole bandwidth here (107 of 128 bytes per
 // clock), and a staged copy of the result cost a fifth of the time.

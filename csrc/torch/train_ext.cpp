@@ -102,13 +102,14 @@ at::Tensor embeddingFwd(const at::Tensor& token, const Opt& position, const at::
 // [context, width] tables; one with no rows (vocab or context 0) is left out.
 std::vector<at::Tensor> embeddingGrad(const at::Tensor& grad, const at::Tensor& tokenOrder,
                                       const at::Tensor& positionOrder, int64_t seq,
-                                      int64_t vocab, int64_t context, double scale, bool outF32, const Opt& dwOut,
-                                      const Opt& dpOut) {
+                                      int64_t vocab, int64_t context, double scale, bool outF32,
+                                      const Opt& dwOut, const Opt& dpOut) {
   need(grad, "grad");
   TORCH_CHECK(grad.dim() == 2, "embedding_grad: want grad [rows, width]");
   const int gF32 = f32(grad, "grad");
   const int64_t rows = grad.size(0), width = grad.size(1);
-  TORCH_CHECK(seq > 0 ? rows % seq == 0 : rows == 0, "embedding_grad: rows must be whole sequences");
+  TORCH_CHECK(seq > 0 ? rows % seq == 0 : rows == 0,
+              "embedding_grad: rows must be whole sequences");
   c10::cuda::CUDAGuard g(grad.device());
   const auto opt = grad.options().dtype(outF32 ? at::kFloat : at::kBFloat16);
   auto table = [&](int64_t n, const Opt& out) {

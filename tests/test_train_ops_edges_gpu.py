@@ -154,7 +154,8 @@ def _peak(call):
 def test_gelu_keeps_no_8_bit_sums_without_a_gradient(ops, rows, ins, outs):
     """Inference forms the activations alone, the same bits."""
     x = _normal(rows, ins, seed=1, dtype=torch.bfloat16)
-    w, b = _normal(outs, ins, seed=2, dtype=torch.bfloat16), _normal(outs, seed=3, dtype=torch.bfloat16)
+    w = _normal(outs, ins, seed=2, dtype=torch.bfloat16)
+    b = _normal(outs, seed=3, dtype=torch.bfloat16)
     want = ops.linear_gelu(x, w.clone().requires_grad_(), b, activations="int8").detach()
     with torch.no_grad():
         assert torch.equal(ops.linear_gelu(x, w, b, activations="int8"), want)
@@ -391,7 +392,8 @@ def test_binding_refuses_sizes_that_do_not_match(ops):
     """What the backward pass of the cross-entropy reads has the sizes of its
     forward pass."""
     from tiny_nccl_b200._native import load
-    x, w = _normal(40, 64, seed=1, dtype=torch.bfloat16), _normal(300, 64, seed=2, dtype=torch.bfloat16)
+    x = _normal(40, 64, seed=1, dtype=torch.bfloat16)
+    w = _normal(300, 64, seed=2, dtype=torch.bfloat16)
     target = torch.arange(40, device="cuda")
     _, lse, _, share = load().ops.linear_ce_fwd(x, w, target, 300, 0)
     one = torch.ones(1, device="cuda")
@@ -416,7 +418,8 @@ def test_int8_blocks_bound(ops):
     off = (back.double() - x.double()).abs().amax(1) / x.double().amax(1)
     assert off[0] == 1 / 127.5 and off[0] > 2.0 ** -7 > off[1]
     for seed in range(4):
-        x = _normal(500, 96, seed=seed) * 2.0 ** (torch.arange(500, device="cuda")[:, None] % 60 - 30)
+        scale = 2.0 ** (torch.arange(500, device="cuda")[:, None] % 60 - 30)
+        x = _normal(500, 96, seed=seed) * scale
         back = ops.dequantize_int8(*ops.quantize_int8(x), torch.float32)
         top = x.double().view(500, 3, 32).abs().amax(2).repeat_interleave(32, 1)
         assert bool(((back.double() - x.double()).abs() <= top / 127.5).all())
@@ -508,7 +511,8 @@ def test_linear_int8_gradients_of_other_types(ops, dtype):
     """Parameters of other types are used through bf16 copies, as in the default
     linear layers; their gradients come from fp32 sums, not from bf16 results."""
     x = _normal(300, 128, seed=1, dtype=torch.bfloat16)
-    w, b = _normal(264, 128, seed=2, dtype=torch.bfloat16), _normal(264, seed=3, dtype=torch.bfloat16)
+    w = _normal(264, 128, seed=2, dtype=torch.bfloat16)
+    b = _normal(264, seed=3, dtype=torch.bfloat16)
     gy = _normal(300, 264, seed=4, dtype=torch.bfloat16)
     for f in (ops.linear, ops.linear_gelu):
         res = []

@@ -177,7 +177,11 @@ class _LinearBias(torch.autograd.Function):
 # pairs, cta_group::2), persistent (one CTA per SM) or 1 (one tile per CTA);
 # 0 selects cuBLAS and a separate GELU kernel. The persistent variants
 # assume they get (nearly) every SM: in training they run in the forward
-# pass, when no gradient all-reduce is in flight.
+# pass, when no gradient all-reduce is in flight. The products behind
+# activations="int8" and linear_cross_entropy are persistent as well and run in
+# the backward pass: beside an all-reduce on some of the SMs their share of the
+# work waits for the others', so a product may take up to about twice as
+# long. They were timed on one GPU only.
 _TCGEN05 = os.environ.get("TNCCL_TCGEN05_GEMM", "pair")
 _TCGEN05_VARIANT = {"1": 0, "persistent": 1, "pair": 2}.get(_TCGEN05, 0)
 
@@ -250,8 +254,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor,
 
     ``activations="int8"`` keeps x for the backward pass in 8-bit blocks
     (:func:`quantize_int8`, half the memory): the forward result stays the
-    same, dW = gy^T x is formed from the 8-bit x. Both sizes of the layer must
-    then be multiples of 8."""
+    same, dW = gy^T x is formed from the 8-bit x; a weight that requires no
+    gradient keeps none. Both sizes of the layer must then be multiples of 8."""
     return _linear(x, weight, bias, False, activations)
 
 
@@ -267,7 +271,9 @@ def linear_gelu(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor,
     with the bias gradient. ``activations="int8"`` keeps x and the sums before
     the GELU for the backward pass in 8-bit blocks (see :func:`linear`); the
     GELU is then taken of the fp32 sums, where the default rounds them to bf16
-    first, and the forward always runs on the tcgen05 GEMM."""
+    first, and the forward always runs on the tcgen05 GEMM. In both forms the
+    GELU's gradient is rounded to bf16 before dX and dW, the operand type of
+    their products."""
     return _linear(x, weight, bias, True, activations)
 
 

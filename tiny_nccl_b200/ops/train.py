@@ -1,6 +1,7 @@
 """Training operators (csrc/ops): token and position embedding, linear layer +
 softmax cross-entropy in pieces of the vocabulary, and 8-bit activation
-blocks. Their autograd functions are native too (csrc/torch/train_ext.cpp).
+blocks. Their autograd functions are native too (csrc/torch/train_ext.cpp); a
+second differentiation and forward-mode inputs (dual tensors) raise.
 Like :mod:`.fused`, every function calls the native kernels; a missing
 extension or an unsupported argument raises.
 """
@@ -35,8 +36,9 @@ def embedding(idx: torch.Tensor, weight: torch.Tensor, pos_weight: torch.Tensor 
     positions are int64 (int32 is converted). An index outside its table, such
     as a negative one for padding, adds nothing and gets no gradient.
 
-    The gradients of both tables are fp32 sums in row order, bit-identical
-    from run to run; a row that no token names gets zero."""
+    The gradients of both tables are fp32 sums over the rows sorted by token (in
+    row order within blocks, which are then added), bit-identical from run to
+    run; a row that no token names gets zero."""
     return _ops().embedding(idx, weight, pos_weight, positions, scale, out_dtype)
 
 
@@ -57,8 +59,11 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     or "none" for fp32 losses of target's shape.
 
     Backward: the gradient of x is bf16, that of weight has weight's type; the
-    gradient of the logits is rounded to bf16 between the products, a piece of
-    the vocabulary of at most 512 MiB at a time. width must be a multiple of 8."""
+    gradient of the logits is rounded to bf16 between the products (a factor
+    that all rows share is not), a piece of the vocabulary of at most 512 MiB
+    (or 256 classes) at a time. A row of x that is not finite makes the weight's
+    gradient NaN also where its target does not count (its share is 0 x), but
+    no other row's loss or gradient. width must be a multiple of 8."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', not {reduction!r}")
     _needs_float("weight", weight)
